@@ -421,6 +421,76 @@ int b200c_fps_large_segment(const void *src, int64_t seg_lo, int64_t seg_points,
                             int64_t *out, void *workspace, size_t workspace_bytes,
                             int32_t *status, b200c_stream_t stream);
 
+/* ---- What a network does next with the same batch vectors, coordinates and edges -----------------------------
+ * These have no counterpart in the reference.  Types: B200C_F32, B200C_F16, B200C_BF16; sums, softmax statistics
+ * and norms are held in 32 bits and each result is rounded once. */
+
+/* Rows by index, scaled: out[e] = scale * x[index[e]] (x [rows, channels], out [edges, channels], contiguous).  An
+ * index outside [0, rows) is padding, as the -1 of b200c_knn's padded form is: it gives a row of zeros. */
+int b200c_gather_rows(const void *x, const int64_t *index, int64_t rows, int64_t edges, int64_t channels, float scale,
+                      int dtype, void *out, b200c_stream_t stream);
+/* Its gradient: dx[r] = scale * (sum of dout[e] over index[e] == r), zeros for rows that no index names.  The sum
+ * of a row is taken in ascending order of e, in pieces, without atomics: the same bits every time.
+ * At most 2^31 - 1 edges.  workspace: b200c_gather_rows_workspace_bytes(...) bytes. */
+size_t b200c_gather_rows_workspace_bytes(int64_t rows, int64_t edges, int64_t channels);
+int b200c_gather_rows_backward(const void *dout, const int64_t *index, int64_t rows, int64_t edges, int64_t channels,
+                               float scale, int dtype, void *dx, void *workspace, size_t workspace_bytes,
+                               b200c_stream_t stream);
+
+/* RMS norm of every head's row and its rotation by the row's coordinates, for queries and keys in one launch:
+ *   u = weight * x / sqrt(mean(x^2) + eps),  a_p = sum_d pos[d] * freq[d][p]  (p < channels / 2, in 64 bits),
+ *   y[p] = u[p] cos a_p - u[p + channels/2] sin a_p,  y[p + channels/2] = u[p + channels/2] cos a_p + u[p] sin a_p.
+ * channels: even, at most 256.  A side with rows == 0 is left out. */
+typedef struct {
+  const void *x;                   /* [rows, heads, channels]; channels contiguous, other strides in elements */
+  int64_t rows, row_stride, head_stride;
+  int heads;
+  const void *pos;                 /* [rows, dims] f32, or f64 with pos_f64 */
+  const float *weight;             /* [channels], NULL: ones */
+  void *y;                         /* [rows, heads, channels] contiguous; forward */
+  const void *dy;                  /* the same; backward */
+  void *dx;                        /* the same; backward */
+  float *dweight;                  /* [channels], NULL: not wanted; backward */
+} b200c_norm_rotate_side_t;
+int b200c_norm_rotate(const b200c_norm_rotate_side_t *q, const b200c_norm_rotate_side_t *k, const void *freq,
+                      int dims, int channels, int pos_f64, int freq_f64, float eps, int dtype, b200c_stream_t stream);
+size_t b200c_norm_rotate_workspace_bytes(int channels); /* of the backward pass */
+int b200c_norm_rotate_backward(const b200c_norm_rotate_side_t *q, const b200c_norm_rotate_side_t *k, const void *freq,
+                               int dims, int channels, int pos_f64, int freq_f64, float eps, int dtype,
+                               void *workspace, size_t workspace_bytes, b200c_stream_t stream);
+
+/* Softmax attention inside the examples of a ragged batch: row i of q sees the rows j of k and v of the same segment,
+ *   z_ij = t_ij - slope[h] |pos_q[i] - pos_k[j]|,  t_ij = scale q_i.k_j, or cap tanh(scale q_i.k_j / cap) with cap > 0,
+ *   out_i = sum_j softmax_j(z_ij) v_j.
+ * Query head h reads key/value head h / (heads / groups).  Rows without keys (empty segments, rows outside every
+ * segment) and rows whose scores are all -inf give zeros.  What stands in one segment, NaN and infinities included,
+ * does not reach another. */
+typedef struct {
+  const void *q, *k, *v;           /* [m, heads, channels], [n, groups, channels] x 2; channels contiguous */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* strides in elements */
+  const int64_t *ptr_q, *ptr_k;    /* [num_segments + 1], ascending; NULL: one segment */
+  int64_t num_segments;
+  const float *pos_q, *pos_k;      /* [m, dims], [n, dims]; used when dims > 0 */
+  const float *slope;              /* [heads]; used when dims > 0 */
+  int64_t m, n;
+  int heads, groups, channels;     /* heads a multiple of groups; channels 1 .. 128 */
+  int dims;                        /* 0 .. 8 */
+  float scale, cap;                /* cap <= 0: none */
+  int dtype;
+} b200c_attention_t;
+/* out [m, heads, channels] contiguous; lse (may be NULL) [heads, m]: log2 of the sum of exp(z), +inf where out is
+ * zero by the rules above; the backward pass needs it.  workspace: b200c_attention_workspace_bytes(a) bytes (may be 0).
+ * The backward pass takes out, lse and the gradient dout [m, heads, channels] (contiguous) and writes dq [m, heads,
+ * channels] and dk, dv [n, groups, channels] (contiguous; dq or both of dk and dv may be NULL).  Positions and slopes are
+ * constants.  No atomics: the same bits every time. */
+size_t b200c_attention_workspace_bytes(const b200c_attention_t *a);
+int b200c_attention_forward(const b200c_attention_t *a, void *out, float *lse, void *workspace,
+                            size_t workspace_bytes, b200c_stream_t stream);
+size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a);
+int b200c_attention_backward(const b200c_attention_t *a, const void *out, const float *lse, const void *dout,
+                             void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                             b200c_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -124,6 +124,27 @@ def cabi() -> ctypes.CDLL:
     lib.b200c_fps_large_segment_workspace_bytes.restype = sz
     lib.b200c_fps_large_segment.argtypes = [p, i64, i64, i64, i64, i64, i32, p, p, sz, p, p]
     lib.b200c_fps_large_segment.restype = i32
+    f32 = ctypes.c_float
+    lib.b200c_gather_rows.argtypes = [p, p, i64, i64, i64, f32, i32, p, p]
+    lib.b200c_gather_rows.restype = i32
+    lib.b200c_gather_rows_workspace_bytes.argtypes = [i64, i64, i64]
+    lib.b200c_gather_rows_workspace_bytes.restype = sz
+    lib.b200c_gather_rows_backward.argtypes = [p, p, i64, i64, i64, f32, i32, p, p, sz, p]
+    lib.b200c_gather_rows_backward.restype = i32
+    lib.b200c_norm_rotate.argtypes = [p, p, p, i32, i32, i32, i32, f32, i32, p]
+    lib.b200c_norm_rotate.restype = i32
+    lib.b200c_norm_rotate_workspace_bytes.argtypes = [i32]
+    lib.b200c_norm_rotate_workspace_bytes.restype = sz
+    lib.b200c_norm_rotate_backward.argtypes = [p, p, p, i32, i32, i32, i32, f32, i32, p, sz, p]
+    lib.b200c_norm_rotate_backward.restype = i32
+    lib.b200c_attention_workspace_bytes.argtypes = [p]
+    lib.b200c_attention_workspace_bytes.restype = sz
+    lib.b200c_attention_forward.argtypes = [p, p, p, p, sz, p]
+    lib.b200c_attention_forward.restype = i32
+    lib.b200c_attention_backward_workspace_bytes.argtypes = [p]
+    lib.b200c_attention_backward_workspace_bytes.restype = sz
+    lib.b200c_attention_backward.argtypes = [p, p, p, p, p, p, p, p, sz, p]
+    lib.b200c_attention_backward.restype = i32
     for name in ("b200c_segment_ptr", "b200c_exclusive_scan", "b200c_exclusive_scan_static", "b200c_knn", "b200c_knn_compact", "b200c_knn_graph_tail_count", "b200c_knn_graph_tail_write",
                  "b200c_radius_count", "b200c_radius_fill"):
         getattr(lib, name).restype = i32

@@ -3,7 +3,7 @@
 ``libb200cluster.so``   the C ABI of ``include/b200_cluster.h``: hand-written sm_100a CUDA
                         kernels, compiled by nvcc with
                         ``-gencode arch=compute_100a,code=sm_100a``; no torch dependency.
-``_torch_ops.so``       the torch operator layer (``torch_cluster::knn`` / ``radius``),
+``_torch_ops.so``       the torch operator layer (``torch_cluster::knn`` / ``radius`` and the others),
                         compiled by g++ against libtorch and linked to the first.
 
 ``python pytorch_cluster_b200/build.py`` builds both (incremental by mtime).  Run it as a script:
@@ -74,15 +74,24 @@ def build_ops(force: bool = False, verbose: bool = False) -> str:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    deps = [src, os.path.join(INCLUDE, "b200_cluster.h"), os.path.join(INCLUDE, "b200_cluster_torch.h"), LIB_CABI]
+    sources = sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
+    deps = sources + [os.path.join(INCLUDE, "b200_cluster.h"), os.path.join(INCLUDE, "b200_cluster_torch.h"), LIB_CABI]
     if not force and _newer(LIB_OPS, deps):
         return LIB_OPS
     lib_dir = ce.library_paths()[0]
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wno-sign-compare", src, "-o", LIB_OPS,
-           f"-I{INCLUDE}", f"-I{os.path.join(_cuda_home(), 'include')}"]
-    cmd += [f"-I{p}" for p in ce.include_paths()]
-    cmd += [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    flags = ["-std=c++17", "-O2", "-fPIC", "-Wno-sign-compare", f"-I{INCLUDE}",
+             f"-I{os.path.join(_cuda_home(), 'include')}"]
+    flags += [f"-I{p}" for p in ce.include_paths()]
+    flags += [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    jobs, objs = [], []
+    for s in sources:
+        o = os.path.join(OBJ_DIR, os.path.basename(s)[:-4] + ".cpp.o")
+        objs.append(o)
+        jobs.append(["g++"] + flags + ["-c", s, "-o", o])
+    with ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
+        list(ex.map(lambda c: _run(c, verbose), jobs))
+    cmd = ["g++", "-shared"] + objs + ["-o", LIB_OPS]
     cmd += [f"-L{PKG}", "-lb200cluster", "-Wl,-rpath,$ORIGIN", f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}",
             "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ldl"]
     _run(cmd, verbose)

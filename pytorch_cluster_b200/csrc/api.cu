@@ -21,7 +21,7 @@ void set_error(const char *fmt, ...) {
 
 // The kernels are built for sm_100a only; refuse other devices with a clear message instead of
 // a launch failure.
-static int check_device() {
+int check_device() {
   static thread_local int checked_device = -1;
   int dev = 0;
   B200C_CUDA(cudaGetDevice(&dev));

@@ -1,0 +1,70 @@
+// Softmax attention inside the examples of a ragged batch (shared by the attention_*.cu kernels).
+//
+// For query i (row of q, head h) and every key j of the same example (segment of ptr_q / ptr_k):
+//   t_ij = scale q_i . k_j           with a cap: t_ij = cap tanh(scale q_i . k_j / cap)
+//   z_ij = t_ij - slope_h |pos_i - pos_j|
+//   o_i  = sum_j p_ij v_j,  p_ij = exp(z_ij) / sum_j exp(z_ij)
+// Head h reads key/value head h / (heads / groups).  A row without keys (its example has none, or it belongs
+// to no example) and a row whose scores are all -inf give zeros.
+//
+// Backward, with D_i = do_i . o_i:  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - D_i) (1 - (t_ij / cap)^2),
+//   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,
+// the sums over i running over all heads of the key's group.  p is formed again from the forward pass's
+//   lse_i = log2 sum_j exp(z_ij)      (+inf for rows that give zeros, so that p = 0),
+// stored [heads, m].  Scores are kept in units of log 2: exp(z) = 2^(z log2 e).
+#pragma once
+
+#include "common.cuh"
+
+namespace b200c {
+
+constexpr float AT_LOG2E = 1.4426950408889634f;
+constexpr int AT_MAX_CHANNELS = 128;
+constexpr int AT_MAX_DIMS = 8;
+
+struct AttnArgs {
+  b200c_attention_t p;
+  void *out = nullptr;           // [m, heads, channels]
+  float *lse = nullptr;          // [heads, m]; forward: may be null
+  const void *dout = nullptr;    // [m, heads, channels]
+  const float *delta = nullptr;  // [heads, m]: D_i
+  void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // [m, heads, channels], [n, groups, channels] x 2
+  int *error = nullptr;          // set when a bounded wait ran out
+  cudaStream_t stream = nullptr;
+};
+
+template <typename T>
+__device__ __forceinline__ float at_float(T v) { return (float)v; }
+template <>
+__device__ __forceinline__ float at_float<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float at_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T at_round(float v) { return (T)v; }
+template <>
+__device__ __forceinline__ __half at_round<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 at_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Rows [lo, hi) of one side that belong to segment b, clipped to the rows there are: an unsorted batch vector gives
+// wrong segments, never an access out of range.
+__device__ __forceinline__ void at_segment(const int64_t *__restrict__ ptr, int64_t rows, int64_t b, int64_t &lo,
+                                           int64_t &hi) {
+  lo = 0;
+  hi = rows;
+  if (ptr == nullptr) return;
+  lo = ptr[b];
+  hi = ptr[b + 1];
+  if (lo < 0) lo = 0;
+  if (hi > rows) hi = rows;
+  if (hi < lo) hi = lo;
+}
+
+int launch_attention_plain_forward(const AttnArgs &a);
+int launch_attention_plain_backward(const AttnArgs &a);
+int launch_attention_delta(const AttnArgs &a, float *delta);
+int attention_few_splits(const b200c_attention_t &p);  // 0: not for this call
+size_t attention_few_workspace_bytes(const b200c_attention_t &p);
+int launch_attention_few(const AttnArgs &a, int splits, void *workspace);
+
+}  // namespace b200c

@@ -1,0 +1,470 @@
+// Attention for every type and channel count, on the FP32 pipe (see attention.cuh for the formulas).
+//
+// A block of 256 threads owns 64 rows of one head and walks the other side's rows of the same example in tiles of
+// 64: one pass over the keys with the running maximum and sum of the softmax.  Operands are widened to fp32 and kept
+// transposed in shared memory ([channel][row], rows padded to 68 so that the 16-byte reads of both products are
+// free of bank conflicts); a thread holds a 4 x 4 tile of the scores and 4 x channels/16 of the result.
+// Tiles hold rows of several examples where examples are short; those are processed one example after the other, so
+// that a NaN in one example never meets another one's zeros.
+// The backward pass is two kernels of the same shape: one owns 64 queries and sums dq over the keys, one owns 64 keys and
+// sums dk and dv over the queries of all heads of its group.  Scores are formed twice, but nothing is
+// added atomically: the result does not depend on the order of the blocks.
+#include "attention.cuh"
+
+namespace b200c {
+
+constexpr int AP_T = 64;        // rows and columns of a tile
+constexpr int AP_LD = AP_T + 4;
+constexpr int AP_THREADS = 256;
+
+// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]
+template <typename T>
+__device__ __forceinline__ void ap_load(float *dst, const T *__restrict__ src, int64_t row_stride, int64_t row0,
+                                        int64_t lo, int64_t hi, int channels, int padded, int tid) {
+  for (int i = tid; i < AP_T * padded; i += AP_THREADS) {
+    const int r = i / padded, c = i - r * padded;
+    const int64_t row = row0 + r;
+    dst[c * AP_LD + r] = (row >= lo && row < hi && c < channels) ? at_float(src[row * row_stride + c]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void ap_load_pos(float *dst, const float *__restrict__ src, int dims, int64_t row0,
+                                            int64_t lo, int64_t hi, int tid) {
+  for (int i = tid; i < AP_T * dims; i += AP_THREADS) {
+    const int r = i / dims, d = i - r * dims;
+    const int64_t row = row0 + r;
+    dst[d * AP_LD + r] = (row >= lo && row < hi) ? src[row * dims + d] : 0.f;
+  }
+}
+
+// acc[i][j] += sum_c a[c][4 ty + i] b[c][4 tx + j]
+__device__ __forceinline__ void ap_scores(const float *a, const float *b, int channels, int ty, int tx,
+                                          float (&acc)[4][4]) {
+#pragma unroll 4
+  for (int c = 0; c < channels; ++c) {
+    const float4 x = *reinterpret_cast<const float4 *>(a + c * AP_LD + 4 * ty);
+    const float4 y = *reinterpret_cast<const float4 *>(b + c * AP_LD + 4 * tx);
+    const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
+  }
+}
+
+// acc[i][n] += sum_j w[4 ty + i][j] b[tx + 16 n][j]
+template <int NC>
+__device__ __forceinline__ void ap_accumulate(const float *w, const float *b, int ty, int tx, float (&acc)[4][NC]) {
+  for (int j = 0; j < AP_T; j += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(w + (4 * ty + i) * AP_LD + j);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const float4 y = *reinterpret_cast<const float4 *>(b + (tx + 16 * n) * AP_LD + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[i][n] = fmaf(x[i].x, y.x, fmaf(x[i].y, y.y, fmaf(x[i].z, y.z, fmaf(x[i].w, y.w, acc[i][n]))));
+    }
+  }
+}
+
+// log2 e (t - slope |pos_a - pos_b|) of the 4 x 4 tile; bend[i][j] = 1 - (t / cap)^2
+template <bool BEND>
+__device__ __forceinline__ void ap_logits(float (&s)[4][4], float (&bend)[4][4], const float *pa, const float *pb,
+                                          int dims, int ty, int tx, float scale, float cap, float slope) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float t = s[i][j] * scale;
+      if (BEND) bend[i][j] = 1.f;
+      if (cap > 0.f) {
+        const float u = tanhf(t / cap);
+        t = cap * u;
+        if (BEND) bend[i][j] = 1.f - u * u;
+      }
+      if (dims > 0) {
+        float d2 = 0.f;
+        for (int d = 0; d < dims; ++d) {
+          const float df = pa[d * AP_LD + 4 * ty + i] - pb[d * AP_LD + 4 * tx + j];
+          d2 = fmaf(df, df, d2);
+        }
+        t = fmaf(-slope, sqrtf(d2), t);
+      }
+      s[i][j] = t * AT_LOG2E;
+    }
+}
+
+__device__ __forceinline__ float ap_max16(float v) {
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL_MASK, v, o));
+  return v;
+}
+__device__ __forceinline__ float ap_sum16(float v) {
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+  return v;
+}
+
+template <int CP>
+struct ApSmem {
+  static constexpr int TILE = CP * AP_LD, W = AP_T * AP_LD, POS = AT_MAX_DIMS * AP_LD;
+};
+
+template <typename T, int CP>
+__global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(AttnArgs a) {
+  constexpr int NC = CP / 16;
+  using S = ApSmem<CP>;
+  extern __shared__ __align__(16) float ap_smem[];
+  float *sq = ap_smem, *sk = sq + S::TILE, *sv = sk + S::TILE, *sw = sv + S::TILE, *spq = sw + S::W,
+        *spk = spq + S::POS;
+  const b200c_attention_t &p = a.p;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int head = blockIdx.y, group = head / (p.heads / p.groups);
+  const T *q = (const T *)p.q + (int64_t)head * p.q_head;
+  const T *k = (const T *)p.k + (int64_t)group * p.k_head;
+  const T *v = (const T *)p.v + (int64_t)group * p.v_head;
+  const float slope = p.dims > 0 ? p.slope[head] : 0.f;
+  const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
+  T *out = (T *)a.out;
+
+  ap_load(sq, q, p.q_row, t0, t0, t1, p.channels, CP, tid);
+  if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, t0, t0, t1, tid);
+  // rows of no example stay at zero
+  for (int64_t row = t0; row < t1; ++row) {
+    const int b = segment_of(p.ptr_q, p.num_segments, row);
+    int64_t lo, hi;
+    at_segment(p.ptr_q, p.m, b, lo, hi);
+    if (row >= lo && row < hi) {
+      row = hi - 1;
+      continue;
+    }
+    for (int c = tid; c < p.channels; c += AP_THREADS) out[(row * p.heads + head) * p.channels + c] = at_round<T>(0.f);
+    if (a.lse && tid == 0) a.lse[(int64_t)head * p.m + row] = pos_inf<float>();
+  }
+  const int b_first = segment_of(p.ptr_q, p.num_segments, t0), b_last = segment_of(p.ptr_q, p.num_segments, t1 - 1);
+  for (int b = b_first; b <= b_last; ++b) {
+    int64_t q_lo, q_hi, k_lo, k_hi;
+    at_segment(p.ptr_q, p.m, b, q_lo, q_hi);
+    at_segment(p.ptr_k, p.n, b, k_lo, k_hi);
+    if (q_lo < t0) q_lo = t0;
+    if (q_hi > t1) q_hi = t1;
+    if (q_lo >= q_hi) continue;
+    float o[4][NC] = {}, top[4], sum[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = -pos_inf<float>();
+    for (int64_t c0 = k_lo; c0 < k_hi; c0 += AP_T) {
+      __syncthreads();
+      ap_load(sk, k, p.k_row, c0, k_lo, k_hi, p.channels, CP, tid);
+      ap_load(sv, v, p.v_row, c0, k_lo, k_hi, p.channels, CP, tid);
+      if (p.dims > 0) ap_load_pos(spk, p.pos_k, p.dims, c0, k_lo, k_hi, tid);
+      __syncthreads();
+      float s[4][4] = {}, unused[4][4];
+      ap_scores(sq, sk, p.channels, ty, tx, s);
+      ap_logits<false>(s, unused, spq, spk, p.dims, ty, tx, p.scale, p.cap, slope);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float m = top[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (c0 + 4 * tx + j >= k_hi) s[i][j] = -pos_inf<float>();
+          m = fmaxf(m, s[i][j]);
+        }
+        m = ap_max16(m);
+        const float base = m == -pos_inf<float>() ? 0.f : m;
+        const float shrink = exp2f(top[i] - base);
+        top[i] = m;
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = exp2f(s[i][j] - base);
+          part += s[i][j];
+        }
+        sum[i] = fmaf(sum[i], shrink, ap_sum16(part));
+#pragma unroll
+        for (int n = 0; n < NC; ++n) o[i][n] *= shrink;
+        *reinterpret_cast<float4 *>(sw + (4 * ty + i) * AP_LD + 4 * tx) =
+            make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+      }
+      __syncwarp();  // a row of the weights is written and read by the same half warp
+      ap_accumulate<NC>(sw, sv, ty, tx, o);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = t0 + 4 * ty + i;
+      if (row < q_lo || row >= q_hi) continue;
+      const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];  // NaN sums stay NaN
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int c = tx + 16 * n;
+        if (c < p.channels) out[(row * p.heads + head) * p.channels + c] = at_round<T>(o[i][n] * inv);
+      }
+      if (a.lse && tx == 0)
+        a.lse[(int64_t)head * p.m + row] = sum[i] == 0.f ? pos_inf<float>() : top[i] + log2f(sum[i]);
+    }
+  }
+}
+
+// dq of 64 queries of one head
+template <typename T, int CP>
+__global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs a) {
+  constexpr int NC = CP / 16;
+  using S = ApSmem<CP>;
+  extern __shared__ __align__(16) float ap_smem[];
+  float *sq = ap_smem, *sdo = sq + S::TILE, *sk = sdo + S::TILE, *sv = sk + S::TILE, *sw = sv + S::TILE,
+        *spq = sw + S::W, *spk = spq + S::POS;
+  const b200c_attention_t &p = a.p;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int head = blockIdx.y, group = head / (p.heads / p.groups);
+  const int64_t qrow = (int64_t)p.heads * p.channels;
+  const T *q = (const T *)p.q + (int64_t)head * p.q_head;
+  const T *k = (const T *)p.k + (int64_t)group * p.k_head;
+  const T *v = (const T *)p.v + (int64_t)group * p.v_head;
+  const T *dout = (const T *)a.dout + (int64_t)head * p.channels;
+  T *dq = (T *)a.dq + (int64_t)head * p.channels;
+  const float slope = p.dims > 0 ? p.slope[head] : 0.f;
+  const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
+
+  ap_load(sq, q, p.q_row, t0, t0, t1, p.channels, CP, tid);
+  ap_load(sdo, dout, qrow, t0, t0, t1, p.channels, CP, tid);
+  if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, t0, t0, t1, tid);
+  for (int64_t row = t0; row < t1; ++row) {
+    const int b = segment_of(p.ptr_q, p.num_segments, row);
+    int64_t lo, hi;
+    at_segment(p.ptr_q, p.m, b, lo, hi);
+    if (row >= lo && row < hi) {
+      row = hi - 1;
+      continue;
+    }
+    for (int c = tid; c < p.channels; c += AP_THREADS) dq[row * qrow + c] = at_round<T>(0.f);
+  }
+  float lse[4], delta[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = t0 + 4 * ty + i;
+    lse[i] = row < t1 ? a.lse[(int64_t)head * p.m + row] : pos_inf<float>();
+    delta[i] = row < t1 ? a.delta[(int64_t)head * p.m + row] : 0.f;
+  }
+  const int b_first = segment_of(p.ptr_q, p.num_segments, t0), b_last = segment_of(p.ptr_q, p.num_segments, t1 - 1);
+  for (int b = b_first; b <= b_last; ++b) {
+    int64_t q_lo, q_hi, k_lo, k_hi;
+    at_segment(p.ptr_q, p.m, b, q_lo, q_hi);
+    at_segment(p.ptr_k, p.n, b, k_lo, k_hi);
+    if (q_lo < t0) q_lo = t0;
+    if (q_hi > t1) q_hi = t1;
+    if (q_lo >= q_hi) continue;
+    float acc[4][NC] = {};
+    for (int64_t c0 = k_lo; c0 < k_hi; c0 += AP_T) {
+      __syncthreads();
+      ap_load(sk, k, p.k_row, c0, k_lo, k_hi, p.channels, CP, tid);
+      ap_load(sv, v, p.v_row, c0, k_lo, k_hi, p.channels, CP, tid);
+      if (p.dims > 0) ap_load_pos(spk, p.pos_k, p.dims, c0, k_lo, k_hi, tid);
+      __syncthreads();
+      float s[4][4] = {}, dp[4][4] = {}, bend[4][4];
+      ap_scores(sq, sk, p.channels, ty, tx, s);
+      ap_scores(sdo, sv, p.channels, ty, tx, dp);
+      ap_logits<true>(s, bend, spq, spk, p.dims, ty, tx, p.scale, p.cap, slope);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool there = c0 + 4 * tx + j < k_hi && lse[i] < pos_inf<float>();
+          const float w = exp2f(s[i][j] - lse[i]) * (dp[i][j] - delta[i]) * bend[i][j];
+          s[i][j] = there || lse[i] != lse[i] ? w : 0.f;
+          if (c0 + 4 * tx + j >= k_hi) s[i][j] = 0.f;
+        }
+        *reinterpret_cast<float4 *>(sw + (4 * ty + i) * AP_LD + 4 * tx) =
+            make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+      }
+      __syncwarp();
+      ap_accumulate<NC>(sw, sk, ty, tx, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = t0 + 4 * ty + i;
+      if (row < q_lo || row >= q_hi) continue;
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int c = tx + 16 * n;
+        if (c < p.channels) dq[row * qrow + c] = at_round<T>(acc[i][n] * p.scale);
+      }
+    }
+  }
+}
+
+// dk and dv of 64 keys of one group
+template <typename T, int CP>
+__global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArgs a) {
+  constexpr int NC = CP / 16;
+  using S = ApSmem<CP>;
+  extern __shared__ __align__(16) float ap_smem[];
+  float *sk = ap_smem, *sv = sk + S::TILE, *sq = sv + S::TILE, *sdo = sq + S::TILE, *sw = sdo + S::TILE,
+        *spq = sw + S::W, *spk = spq + S::POS, *slse = spk + S::POS, *sdelta = slse + AP_T;
+  const b200c_attention_t &p = a.p;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int group = blockIdx.y, per_group = p.heads / p.groups;
+  const int64_t qrow = (int64_t)p.heads * p.channels, krow = (int64_t)p.groups * p.channels;
+  const T *k = (const T *)p.k + (int64_t)group * p.k_head;
+  const T *v = (const T *)p.v + (int64_t)group * p.v_head;
+  T *dk = (T *)a.dk + (int64_t)group * p.channels, *dv = (T *)a.dv + (int64_t)group * p.channels;
+  const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.n ? t0 + AP_T : p.n;
+
+  ap_load(sk, k, p.k_row, t0, t0, t1, p.channels, CP, tid);
+  ap_load(sv, v, p.v_row, t0, t0, t1, p.channels, CP, tid);
+  if (p.dims > 0) ap_load_pos(spk, p.pos_k, p.dims, t0, t0, t1, tid);
+  for (int64_t row = t0; row < t1; ++row) {
+    const int b = segment_of(p.ptr_k, p.num_segments, row);
+    int64_t lo, hi;
+    at_segment(p.ptr_k, p.n, b, lo, hi);
+    if (row >= lo && row < hi) {
+      row = hi - 1;
+      continue;
+    }
+    for (int c = tid; c < p.channels; c += AP_THREADS) dk[row * krow + c] = dv[row * krow + c] = at_round<T>(0.f);
+  }
+  const int b_first = segment_of(p.ptr_k, p.num_segments, t0), b_last = segment_of(p.ptr_k, p.num_segments, t1 - 1);
+  for (int b = b_first; b <= b_last; ++b) {
+    int64_t q_lo, q_hi, k_lo, k_hi;
+    at_segment(p.ptr_q, p.m, b, q_lo, q_hi);
+    at_segment(p.ptr_k, p.n, b, k_lo, k_hi);
+    if (k_lo < t0) k_lo = t0;
+    if (k_hi > t1) k_hi = t1;
+    if (k_lo >= k_hi) continue;
+    float gk[4][NC] = {}, gv[4][NC] = {};
+    for (int e = 0; e < per_group; ++e) {
+      const int head = group * per_group + e;
+      const float slope = p.dims > 0 ? p.slope[head] : 0.f;
+      for (int64_t c0 = q_lo; c0 < q_hi; c0 += AP_T) {
+        __syncthreads();
+        ap_load(sq, (const T *)p.q + (int64_t)head * p.q_head, p.q_row, c0, q_lo, q_hi, p.channels, CP, tid);
+        ap_load(sdo, (const T *)a.dout + (int64_t)head * p.channels, qrow, c0, q_lo, q_hi, p.channels, CP, tid);
+        if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, c0, q_lo, q_hi, tid);
+        if (tid < AP_T) {
+          const bool there = c0 + tid < q_hi;
+          slse[tid] = there ? a.lse[(int64_t)head * p.m + c0 + tid] : pos_inf<float>();
+          sdelta[tid] = there ? a.delta[(int64_t)head * p.m + c0 + tid] : 0.f;
+        }
+        __syncthreads();
+        float s[4][4] = {}, dp[4][4] = {}, bend[4][4];
+        ap_scores(sk, sq, p.channels, ty, tx, s);
+        ap_scores(sv, sdo, p.channels, ty, tx, dp);
+        ap_logits<true>(s, bend, spk, spq, p.dims, ty, tx, p.scale, p.cap, slope);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lse = slse[4 * tx + j], delta = sdelta[4 * tx + j];
+          const bool none = lse == pos_inf<float>();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[i][j] = none ? 0.f : exp2f(s[i][j] - lse);
+            dp[i][j] = none ? 0.f : s[i][j] * (dp[i][j] - delta) * bend[i][j];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4 *>(sw + (4 * ty + i) * AP_LD + 4 * tx) =
+              make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        __syncwarp();
+        ap_accumulate<NC>(sw, sdo, ty, tx, gv);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4 *>(sw + (4 * ty + i) * AP_LD + 4 * tx) =
+              make_float4(dp[i][0], dp[i][1], dp[i][2], dp[i][3]);
+        __syncwarp();
+        ap_accumulate<NC>(sw, sq, ty, tx, gk);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = t0 + 4 * ty + i;
+      if (row < k_lo || row >= k_hi) continue;
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int c = tx + 16 * n;
+        if (c < p.channels) {
+          dk[row * krow + c] = at_round<T>(gk[i][n] * p.scale);
+          dv[row * krow + c] = at_round<T>(gv[i][n]);
+        }
+      }
+    }
+  }
+}
+
+// D_i = do_i . o_i, one warp per (row, head)
+template <typename T>
+__global__ void __launch_bounds__(256) attention_delta_kernel(const T *__restrict__ dout, const T *__restrict__ out,
+                                                              int64_t m, int heads, int channels,
+                                                              float *__restrict__ delta) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (i >= m * heads) return;
+  float s = 0.f;
+  for (int c = lane; c < channels; c += 32) s = fmaf(at_float(dout[i * channels + c]), at_float(out[i * channels + c]), s);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
+  if (lane == 0) delta[(i % heads) * m + i / heads] = s;
+}
+
+template <typename T, int CP>
+static int ap_forward(const AttnArgs &a) {
+  constexpr size_t smem = (3 * ApSmem<CP>::TILE + ApSmem<CP>::W + 2 * ApSmem<CP>::POS) * 4;
+  static unsigned long long configured = 0ull;
+  B200C_CUDA(opt_in_shared_memory(attention_plain_forward_kernel<T, CP>, smem, configured));
+  const dim3 grid((unsigned)((a.p.m + AP_T - 1) / AP_T), (unsigned)a.p.heads);
+  attention_plain_forward_kernel<T, CP><<<grid, AP_THREADS, smem, a.stream>>>(a);
+  B200C_LAUNCH_CHECK("attention_plain_forward_kernel");
+  return B200C_OK;
+}
+
+template <typename T, int CP>
+static int ap_backward(const AttnArgs &a) {
+  constexpr size_t smem = (4 * ApSmem<CP>::TILE + ApSmem<CP>::W + 2 * ApSmem<CP>::POS + 2 * AP_T) * 4;
+  static_assert(smem <= 227 * 1024, "shared memory of a block");
+  static unsigned long long configured_q = 0ull, configured_kv = 0ull;
+  if (a.dq && a.p.m > 0) {
+    B200C_CUDA(opt_in_shared_memory(attention_plain_dq_kernel<T, CP>, smem, configured_q));
+    const dim3 grid((unsigned)((a.p.m + AP_T - 1) / AP_T), (unsigned)a.p.heads);
+    attention_plain_dq_kernel<T, CP><<<grid, AP_THREADS, smem, a.stream>>>(a);
+    B200C_LAUNCH_CHECK("attention_plain_dq_kernel");
+  }
+  if (a.dk && a.p.n > 0) {
+    B200C_CUDA(opt_in_shared_memory(attention_plain_dkv_kernel<T, CP>, smem, configured_kv));
+    const dim3 grid((unsigned)((a.p.n + AP_T - 1) / AP_T), (unsigned)a.p.groups);
+    attention_plain_dkv_kernel<T, CP><<<grid, AP_THREADS, smem, a.stream>>>(a);
+    B200C_LAUNCH_CHECK("attention_plain_dkv_kernel");
+  }
+  return B200C_OK;
+}
+
+template <typename T>
+static int ap_dispatch(const AttnArgs &a, bool forward) {
+  if (a.p.channels <= 32) return forward ? ap_forward<T, 32>(a) : ap_backward<T, 32>(a);
+  if (a.p.channels <= 64) return forward ? ap_forward<T, 64>(a) : ap_backward<T, 64>(a);
+  return forward ? ap_forward<T, 128>(a) : ap_backward<T, 128>(a);
+}
+
+static int ap_any(const AttnArgs &a, bool forward) {
+  if (a.p.dtype == B200C_F32) return ap_dispatch<float>(a, forward);
+  if (a.p.dtype == B200C_F16) return ap_dispatch<__half>(a, forward);
+  return ap_dispatch<__nv_bfloat16>(a, forward);
+}
+
+int launch_attention_plain_forward(const AttnArgs &a) { return ap_any(a, true); }
+int launch_attention_plain_backward(const AttnArgs &a) { return ap_any(a, false); }
+
+int launch_attention_delta(const AttnArgs &a, float *delta) {
+  const int64_t rows = a.p.m * a.p.heads;
+  if (rows == 0) return B200C_OK;
+  const unsigned blocks = (unsigned)((rows + 7) / 8);
+  if (a.p.dtype == B200C_F32)
+    attention_delta_kernel<float><<<blocks, 256, 0, a.stream>>>((const float *)a.dout, (const float *)a.out, a.p.m,
+                                                                a.p.heads, a.p.channels, delta);
+  else if (a.p.dtype == B200C_F16)
+    attention_delta_kernel<__half><<<blocks, 256, 0, a.stream>>>((const __half *)a.dout, (const __half *)a.out, a.p.m,
+                                                                 a.p.heads, a.p.channels, delta);
+  else
+    attention_delta_kernel<__nv_bfloat16><<<blocks, 256, 0, a.stream>>>(
+        (const __nv_bfloat16 *)a.dout, (const __nv_bfloat16 *)a.out, a.p.m, a.p.heads, a.p.channels, delta);
+  B200C_LAUNCH_CHECK("attention_delta_kernel");
+  return B200C_OK;
+}
+
+}  // namespace b200c

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "b200_cluster.h"
+
 namespace b200c {
 
 struct KnnArgs {
@@ -96,5 +98,27 @@ size_t knn_spatial_workspace_bytes(int64_t n, int64_t m, int dim, int64_t num_se
 int launch_knn_spatial_f32(const KnnArgs &a, void *workspace, int64_t max_segment_rows);
 int knn_spatial_scan_timing(int enable);  // record CUDA events around the scan kernel of later calls
 float knn_spatial_last_scan_ms();         // duration of the last timed scan kernel (waits for it), -1 if none
+
+// Rows by index and their gradient (gather_rows.cu)
+size_t gather_rows_workspace_bytes(int64_t rows, int64_t edges, int64_t channels);
+int launch_gather_rows(const void *x, const int64_t *index, int64_t rows, int64_t edges, int64_t channels, float scale,
+                       int dtype, void *out, cudaStream_t stream);
+int launch_gather_rows_backward(const void *dout, const int64_t *index, int64_t rows, int64_t edges, int64_t channels,
+                                float scale, int dtype, void *dx, void *workspace, cudaStream_t stream);
+
+// Norm and rotation of queries and keys (norm_rotate.cu)
+struct NormRotateArgs {
+  b200c_norm_rotate_side_t side[2];
+  const void *freq;
+  int dims, half;  // half = channels / 2
+  int pos_f64, freq_f64;
+  float eps;
+  int dtype;
+  int joint;  // both sides have the same positions: one set of angles serves them
+  float *dweight[2];
+  cudaStream_t stream;
+};
+size_t norm_rotate_workspace_bytes(int64_t channels);
+int launch_norm_rotate(const NormRotateArgs &a, bool forward, float *parts);
 
 }  // namespace b200c

@@ -1,0 +1,204 @@
+// extern "C" entry points of gather_rows, norm_rotate and attention: argument checks and kernel selection.
+#include "attention.cuh"
+#include "common.cuh"
+#include "launchers.h"
+
+namespace b200c {
+
+int check_device();  // api.cu
+
+static bool is_network_type(int dtype) { return dtype == B200C_F32 || dtype == B200C_F16 || dtype == B200C_BF16; }
+static size_t elem_bytes(int dtype) { return dtype == B200C_F32 ? 4 : 2; }
+constexpr int64_t MOST_ROWS = 0x7fffffffLL;
+
+static int check_gather(const void *in, const int64_t *index, int64_t rows, int64_t edges, int64_t channels, int dtype,
+                        const void *out) {
+  B200C_CHECK_ARG(is_network_type(dtype), "unsupported dtype");
+  B200C_CHECK_ARG(rows >= 0 && edges >= 0 && channels >= 1, "Input mismatch");
+  B200C_CHECK_ARG(rows <= MOST_ROWS && edges <= MOST_ROWS, "more than 2^31-1 rows or edges are not supported");
+  B200C_CHECK_ARG(channels <= 65536, "more than 65536 channels are not supported");
+  B200C_CHECK_ARG((edges == 0 || index != nullptr) && (rows == 0 || edges == 0 || (in != nullptr && out != nullptr)),
+                  "null pointer");
+  const uintptr_t mask = elem_bytes(dtype) - 1;
+  B200C_CHECK_ARG(((uintptr_t)in & mask) == 0 && ((uintptr_t)out & mask) == 0, "misaligned pointer");
+  return check_device();
+}
+
+static int check_rotate(const b200c_norm_rotate_side_t *q, const b200c_norm_rotate_side_t *k, const void *freq, int dims,
+                        int channels, int pos_f64, int freq_f64, float eps, int dtype, bool forward,
+                        cudaStream_t stream, NormRotateArgs &a) {
+  B200C_CHECK_ARG(q != nullptr && k != nullptr && freq != nullptr, "null pointer");
+  B200C_CHECK_ARG(is_network_type(dtype), "unsupported dtype");
+  B200C_CHECK_ARG(channels >= 2 && channels <= 256 && channels % 2 == 0, "channels must be even and at most 256");
+  B200C_CHECK_ARG(dims >= 1 && dims <= 8, "1 to 8 coordinates are supported");
+  const b200c_norm_rotate_side_t *sides[2] = {q, k};
+  for (int i = 0; i < 2; ++i) {
+    const b200c_norm_rotate_side_t &s = *sides[i];
+    B200C_CHECK_ARG(s.rows >= 0 && s.rows <= MOST_ROWS, "more than 2^31-1 rows are not supported");
+    B200C_CHECK_ARG(s.heads >= 1 && s.heads <= 1024, "1 to 1024 heads are supported");
+    if (s.rows > 0) {
+      B200C_CHECK_ARG(s.x && s.pos, "null pointer");
+      B200C_CHECK_ARG(forward ? s.y != nullptr : (s.dy && s.dx), "null pointer");
+    }
+    a.side[i] = s;
+    if (s.rows == 0) a.side[i].x = a.side[i].y = a.side[i].dx = nullptr, a.side[i].dy = nullptr;
+    a.dweight[i] = forward ? nullptr : s.dweight;
+  }
+  a.freq = freq;
+  a.dims = dims;
+  a.half = channels / 2;
+  a.pos_f64 = pos_f64;
+  a.freq_f64 = freq_f64;
+  a.eps = eps;
+  a.dtype = dtype;
+  a.joint = q->rows == k->rows && q->pos == k->pos;
+  a.stream = stream;
+  return check_device();
+}
+
+static int check_attention(const b200c_attention_t *a) {
+  B200C_CHECK_ARG(a != nullptr, "null pointer");
+  B200C_CHECK_ARG(is_network_type(a->dtype), "unsupported dtype");
+  B200C_CHECK_ARG(a->m >= 0 && a->n >= 0 && a->m <= MOST_ROWS && a->n <= MOST_ROWS,
+                  "more than 2^31-1 rows are not supported");
+  B200C_CHECK_ARG(a->channels >= 1 && a->channels <= AT_MAX_CHANNELS, "1 to 128 channels are supported");
+  B200C_CHECK_ARG(a->groups >= 1 && a->heads >= a->groups && a->heads % a->groups == 0 && a->heads <= 1024,
+                  "heads must be a multiple of the key heads, at most 1024");
+  B200C_CHECK_ARG(a->dims >= 0 && a->dims <= AT_MAX_DIMS, "0 to 8 coordinates are supported");
+  B200C_CHECK_ARG(a->m * a->heads <= (1ll << 33), "more than 2^33 rows of all heads are not supported");
+  B200C_CHECK_ARG((a->ptr_q == nullptr) == (a->ptr_k == nullptr), "Input mismatch");
+  B200C_CHECK_ARG(a->ptr_q == nullptr ? a->num_segments == 1 : (a->num_segments >= 1 && a->num_segments <= MOST_ROWS),
+                  "Input mismatch");
+  B200C_CHECK_ARG(a->m == 0 || a->q, "null pointer");
+  B200C_CHECK_ARG(a->n == 0 || (a->k && a->v), "null pointer");
+  B200C_CHECK_ARG(a->dims == 0 || (a->slope && (a->m == 0 || a->pos_q) && (a->n == 0 || a->pos_k)), "null pointer");
+  B200C_CHECK_ARG(a->scale == a->scale && a->cap == a->cap, "scale and cap must be numbers");
+  const uintptr_t mask = elem_bytes(a->dtype) - 1;
+  B200C_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & mask) == 0, "misaligned pointer");
+  return B200C_OK;
+}
+
+}  // namespace b200c
+
+using namespace b200c;
+
+extern "C" int b200c_gather_rows(const void *x, const int64_t *index, int64_t rows, int64_t edges, int64_t channels,
+                                 float scale, int dtype, void *out, b200c_stream_t stream) {
+  const int st = check_gather(x, index, rows, edges, channels, dtype, out);
+  if (st != B200C_OK || edges == 0) return st;
+  B200C_CHECK_ARG(out != nullptr, "null pointer");
+  return launch_gather_rows(x, index, rows, edges, channels, scale, dtype, out, (cudaStream_t)stream);
+}
+
+extern "C" size_t b200c_gather_rows_workspace_bytes(int64_t rows, int64_t edges, int64_t channels) {
+  return gather_rows_workspace_bytes(rows, edges, channels);
+}
+
+extern "C" int b200c_gather_rows_backward(const void *dout, const int64_t *index, int64_t rows, int64_t edges,
+                                          int64_t channels, float scale, int dtype, void *dx, void *workspace,
+                                          size_t workspace_bytes, b200c_stream_t stream) {
+  const int st = check_gather(dout, index, rows, edges, channels, dtype, dx);
+  if (st != B200C_OK || rows == 0) return st;
+  B200C_CHECK_ARG(dx != nullptr, "null pointer");
+  if (edges == 0) {
+    B200C_CUDA(cudaMemsetAsync(dx, 0, (size_t)rows * channels * elem_bytes(dtype), (cudaStream_t)stream));
+    return B200C_OK;
+  }
+  const size_t need = gather_rows_workspace_bytes(rows, edges, channels);
+  if (workspace == nullptr || workspace_bytes < need) {
+    set_error("gather_rows workspace too small: %zu < %zu", workspace_bytes, need);
+    return B200C_ERR_WORKSPACE;
+  }
+  return launch_gather_rows_backward(dout, index, rows, edges, channels, scale, dtype, dx, workspace,
+                                     (cudaStream_t)stream);
+}
+
+extern "C" int b200c_norm_rotate(const b200c_norm_rotate_side_t *q, const b200c_norm_rotate_side_t *k, const void *freq,
+                                 int dims, int channels, int pos_f64, int freq_f64, float eps, int dtype,
+                                 b200c_stream_t stream) {
+  NormRotateArgs a{};
+  const int st = check_rotate(q, k, freq, dims, channels, pos_f64, freq_f64, eps, dtype, true, (cudaStream_t)stream, a);
+  if (st != B200C_OK || (q->rows == 0 && k->rows == 0)) return st;
+  return launch_norm_rotate(a, true, nullptr);
+}
+
+extern "C" size_t b200c_norm_rotate_workspace_bytes(int channels) { return norm_rotate_workspace_bytes(channels); }
+
+extern "C" int b200c_norm_rotate_backward(const b200c_norm_rotate_side_t *q, const b200c_norm_rotate_side_t *k,
+                                          const void *freq, int dims, int channels, int pos_f64, int freq_f64, float eps,
+                                          int dtype, void *workspace, size_t workspace_bytes, b200c_stream_t stream) {
+  NormRotateArgs a{};
+  const int st = check_rotate(q, k, freq, dims, channels, pos_f64, freq_f64, eps, dtype, false, (cudaStream_t)stream, a);
+  if (st != B200C_OK) return st;
+  const size_t need = norm_rotate_workspace_bytes(channels);
+  if ((a.dweight[0] || a.dweight[1]) && (workspace == nullptr || workspace_bytes < need)) {
+    set_error("norm_rotate workspace too small: %zu < %zu", workspace_bytes, need);
+    return B200C_ERR_WORKSPACE;
+  }
+  if (q->rows == 0 && k->rows == 0) {
+    for (float *dw : a.dweight)
+      if (dw) B200C_CUDA(cudaMemsetAsync(dw, 0, (size_t)channels * 4, a.stream));
+    return B200C_OK;
+  }
+  return launch_norm_rotate(a, false, (float *)workspace);
+}
+
+static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+extern "C" size_t b200c_attention_workspace_bytes(const b200c_attention_t *a) {
+  if (check_attention(a) != B200C_OK) return 0;
+  return attention_few_workspace_bytes(*a);
+}
+
+extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, float *lse, void *workspace,
+                                       size_t workspace_bytes, b200c_stream_t stream) {
+  int st = check_attention(p);
+  if (st != B200C_OK) return st;
+  if ((st = check_device()) != B200C_OK || p->m == 0) return st;
+  B200C_CHECK_ARG(out != nullptr, "null output pointer");
+  const size_t need = b200c_attention_workspace_bytes(p);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    set_error("attention workspace too small: %zu < %zu", workspace_bytes, need);
+    return B200C_ERR_WORKSPACE;
+  }
+  AttnArgs a;
+  a.p = *p;
+  a.out = out;
+  a.lse = lse;
+  a.stream = (cudaStream_t)stream;
+  const int splits = attention_few_splits(*p);
+  if (splits > 0) return launch_attention_few(a, splits, workspace);
+  return launch_attention_plain_forward(a);
+}
+
+extern "C" size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a) {
+  if (check_attention(a) != B200C_OK) return 0;
+  return align256((size_t)a->m * a->heads * 4);
+}
+
+extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const float *lse, const void *dout,
+                                        void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                                        b200c_stream_t stream) {
+  int st = check_attention(p);
+  if (st != B200C_OK) return st;
+  if ((st = check_device()) != B200C_OK) return st;
+  B200C_CHECK_ARG(p->m == 0 || (out && lse && dout), "null pointer");
+  B200C_CHECK_ARG((dk == nullptr) == (dv == nullptr), "dk and dv come together");
+  const size_t need = b200c_attention_backward_workspace_bytes(p);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
+    set_error("attention workspace too small: %zu < %zu", workspace_bytes, need);
+    return B200C_ERR_WORKSPACE;
+  }
+  AttnArgs a;
+  a.p = *p;
+  a.out = (void *)out;
+  a.lse = (float *)lse;
+  a.dout = dout;
+  a.delta = (const float *)workspace;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.stream = (cudaStream_t)stream;
+  if ((st = launch_attention_delta(a, (float *)workspace)) != B200C_OK) return st;
+  return launch_attention_plain_backward(a);
+}

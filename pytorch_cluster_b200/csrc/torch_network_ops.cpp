@@ -1,0 +1,320 @@
+// Torch operators of gather_rows, norm_rotate and attention: tensor checks, output and workspace allocation, the
+// caller's current stream.  Forward and backward are operators of their own; the Python layer joins them into
+// differentiable functions.  No CPU branch.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/script.h>
+#include <nvtx3/nvToolsExt.h>
+
+#include <tuple>
+#include <vector>
+
+#include "b200_cluster.h"
+
+namespace {
+
+#define CHECK_CUDA(x) TORCH_CHECK(x.device().is_cuda(), #x " must be CUDA tensor")
+#define CHECK_INPUT(x) TORCH_CHECK(x, "Input mismatch")
+
+using OptTensor = std::optional<torch::Tensor>;
+
+struct OpRange {
+  explicit OpRange(const char *name) { nvtxRangePushA(name); }
+  ~OpRange() { nvtxRangePop(); }
+  OpRange(const OpRange &) = delete;
+  OpRange &operator=(const OpRange &) = delete;
+};
+
+void check_status(int status) { TORCH_CHECK(status == B200C_OK, "b200_cluster: ", b200c_last_error()); }
+
+int dtype_code(const torch::Tensor &t, const char *op) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return B200C_F32;
+    case at::kHalf: return B200C_F16;
+    case at::kBFloat16: return B200C_BF16;
+    default: TORCH_CHECK(false, op, " covers float, half and bfloat16 tensors, got ", t.scalar_type());
+  }
+  return -1;
+}
+
+torch::Tensor workspace(size_t bytes, const torch::Tensor &like) {
+  return torch::empty({(int64_t)bytes}, like.options().dtype(torch::kByte));
+}
+
+// rows whose channels are contiguous are taken as they stand (a slice of a joint projection), others are copied
+torch::Tensor rows_of(const torch::Tensor &t) {
+  return t.numel() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+
+// ---- gather_rows -------------------------------------------------------------------------------------------------
+
+torch::Tensor gather_rows(torch::Tensor x, torch::Tensor index, double scale) {
+  OpRange range("torch_cluster::gather_rows");
+  CHECK_CUDA(x);
+  CHECK_CUDA(index);
+  CHECK_INPUT(x.dim() == 2 && index.dim() == 1);
+  CHECK_INPUT(x.get_device() == index.get_device());
+  TORCH_CHECK(index.scalar_type() == at::kLong, "index must be an int64 tensor");
+  const int dtype = dtype_code(x, "gather_rows");
+  c10::cuda::CUDAGuard guard(x.device());
+  x = x.contiguous();
+  index = index.contiguous();
+  auto out = torch::empty({index.numel(), x.size(1)}, x.options());
+  if (out.numel() == 0) return out;
+  if (x.size(0) == 0) return out.zero_();
+  check_status(b200c_gather_rows(x.data_ptr(), index.data_ptr<int64_t>(), x.size(0), index.numel(), x.size(1),
+                                 (float)scale, dtype, out.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
+torch::Tensor gather_rows_backward(torch::Tensor dout, torch::Tensor index, int64_t rows, double scale) {
+  OpRange range("torch_cluster::gather_rows_backward");
+  CHECK_CUDA(dout);
+  CHECK_CUDA(index);
+  CHECK_INPUT(dout.dim() == 2 && index.dim() == 1 && dout.size(0) == index.numel() && rows >= 0);
+  CHECK_INPUT(dout.get_device() == index.get_device());
+  TORCH_CHECK(index.scalar_type() == at::kLong, "index must be an int64 tensor");
+  const int dtype = dtype_code(dout, "gather_rows");
+  c10::cuda::CUDAGuard guard(dout.device());
+  dout = dout.contiguous();
+  index = index.contiguous();
+  const int64_t edges = index.numel(), channels = dout.size(1);
+  auto dx = torch::empty({rows, channels}, dout.options());
+  if (dx.numel() == 0) return dx;
+  const size_t bytes = b200c_gather_rows_workspace_bytes(rows, edges, channels);
+  auto ws = workspace(bytes, dout);
+  check_status(b200c_gather_rows_backward(dout.data_ptr(), index.data_ptr<int64_t>(), rows, edges, channels,
+                                          (float)scale, dtype, dx.data_ptr(), ws.data_ptr(), bytes,
+                                          at::cuda::getCurrentCUDAStream().stream()));
+  return dx;
+}
+
+// ---- norm_rotate -------------------------------------------------------------------------------------------------
+
+struct Rotation {
+  torch::Tensor x[2], pos[2], freq;
+  OptTensor weight[2];
+  b200c_norm_rotate_side_t side[2];
+  int dims = 0, channels = 0, pos_f64 = 0, freq_f64 = 0, dtype = 0;
+};
+
+void prepare_rotation(Rotation &r, const torch::Tensor &q, const torch::Tensor &k, const torch::Tensor &pos_q,
+                      const torch::Tensor &pos_k, const torch::Tensor &freq, const OptTensor &weight_q,
+                      const OptTensor &weight_k) {
+  const torch::Tensor in[2] = {q, k}, pos[2] = {pos_q, pos_k};
+  const OptTensor weight[2] = {weight_q, weight_k};
+  CHECK_CUDA(freq);
+  CHECK_INPUT(freq.dim() == 2);
+  TORCH_CHECK(freq.scalar_type() == at::kFloat || freq.scalar_type() == at::kDouble, "freq must be float or double");
+  r.freq = freq.contiguous();
+  r.freq_f64 = freq.scalar_type() == at::kDouble;
+  r.dims = (int)freq.size(0);
+  r.channels = (int)q.size(-1);
+  r.dtype = dtype_code(q, "norm_rotate");
+  CHECK_INPUT(q.dim() == 3 && k.dim() == 3 && q.size(2) == k.size(2) && q.scalar_type() == k.scalar_type());
+  TORCH_CHECK(q.size(2) % 2 == 0 && q.size(2) >= 2 && q.size(2) <= 256, "channels must be even and at most 256");
+  TORCH_CHECK(freq.size(1) * 2 == q.size(2), "freq must be [coordinates, channels / 2]");
+  TORCH_CHECK(freq.size(0) >= 1 && freq.size(0) <= 8, "1 to 8 coordinates are supported");
+  CHECK_INPUT(pos_q.scalar_type() == pos_k.scalar_type());
+  TORCH_CHECK(pos_q.scalar_type() == at::kFloat || pos_q.scalar_type() == at::kDouble,
+              "positions must be float or double");
+  r.pos_f64 = pos_q.scalar_type() == at::kDouble;
+  const bool same = pos_q.is_same(pos_k);
+  for (int i = 0; i < 2; ++i) {
+    TORCH_CHECK(in[i].is_cuda(), i == 0 ? "q" : "k", " must be CUDA tensor");
+    TORCH_CHECK(pos[i].is_cuda(), i == 0 ? "pos_q" : "pos_k", " must be CUDA tensor");
+    CHECK_INPUT(pos[i].dim() == 2 && pos[i].size(0) == in[i].size(0) && pos[i].size(1) == freq.size(0));
+    CHECK_INPUT(in[i].get_device() == q.get_device() && pos[i].get_device() == q.get_device() &&
+                freq.get_device() == q.get_device());
+    CHECK_INPUT(in[i].size(1) >= 1);
+    r.x[i] = rows_of(in[i]);
+    r.pos[i] = i == 1 && same ? r.pos[0] : pos[i].contiguous();
+    if (weight[i].has_value()) {
+      const torch::Tensor &w = weight[i].value();
+      CHECK_INPUT(w.is_cuda() && w.get_device() == q.get_device() && w.dim() == 1 && w.size(0) == q.size(2) &&
+                  w.scalar_type() == at::kFloat);
+      r.weight[i] = w.contiguous();
+    }
+    b200c_norm_rotate_side_t &s = r.side[i];
+    s = {};
+    s.x = r.x[i].data_ptr();
+    s.rows = in[i].size(0);
+    s.row_stride = r.x[i].stride(0);
+    s.head_stride = r.x[i].stride(1);
+    s.heads = (int)in[i].size(1);
+    s.pos = r.pos[i].data_ptr();
+    s.weight = r.weight[i].has_value() ? r.weight[i].value().data_ptr<float>() : nullptr;
+  }
+}
+
+std::tuple<torch::Tensor, torch::Tensor> norm_rotate(torch::Tensor q, torch::Tensor k, torch::Tensor pos_q,
+                                                     torch::Tensor pos_k, torch::Tensor freq, OptTensor weight_q,
+                                                     OptTensor weight_k, double eps) {
+  OpRange range("torch_cluster::norm_rotate");
+  CHECK_CUDA(q);
+  CHECK_INPUT(q.dim() == 3);
+  c10::cuda::CUDAGuard guard(q.device());
+  Rotation r;
+  prepare_rotation(r, q, k, pos_q, pos_k, freq, weight_q, weight_k);
+  auto yq = torch::empty(q.sizes(), q.options()), yk = torch::empty(k.sizes(), k.options());
+  r.side[0].y = yq.data_ptr();
+  r.side[1].y = yk.data_ptr();
+  check_status(b200c_norm_rotate(&r.side[0], &r.side[1], r.freq.data_ptr(), r.dims, r.channels, r.pos_f64, r.freq_f64,
+                                 (float)eps, r.dtype, at::cuda::getCurrentCUDAStream().stream()));
+  return {yq, yk};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> norm_rotate_backward(
+    torch::Tensor dyq, torch::Tensor dyk, torch::Tensor q, torch::Tensor k, torch::Tensor pos_q, torch::Tensor pos_k,
+    torch::Tensor freq, OptTensor weight_q, OptTensor weight_k, double eps) {
+  OpRange range("torch_cluster::norm_rotate_backward");
+  CHECK_CUDA(q);
+  CHECK_INPUT(q.dim() == 3);
+  CHECK_INPUT(dyq.sizes() == q.sizes() && dyk.sizes() == k.sizes() && dyq.scalar_type() == q.scalar_type() &&
+              dyk.scalar_type() == k.scalar_type() && dyq.device() == q.device() && dyk.device() == q.device());
+  c10::cuda::CUDAGuard guard(q.device());
+  Rotation r;
+  prepare_rotation(r, q, k, pos_q, pos_k, freq, weight_q, weight_k);
+  dyq = dyq.contiguous();
+  dyk = dyk.contiguous();
+  auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
+  const auto fopts = q.options().dtype(torch::kFloat);
+  auto dwq = torch::empty({weight_q.has_value() ? r.channels : 0}, fopts);
+  auto dwk = torch::empty({weight_k.has_value() ? r.channels : 0}, fopts);
+  r.side[0].dy = dyq.data_ptr();
+  r.side[1].dy = dyk.data_ptr();
+  r.side[0].dx = dq.data_ptr();
+  r.side[1].dx = dk.data_ptr();
+  r.side[0].dweight = weight_q.has_value() ? dwq.data_ptr<float>() : nullptr;
+  r.side[1].dweight = weight_k.has_value() ? dwk.data_ptr<float>() : nullptr;
+  const size_t bytes = weight_q.has_value() || weight_k.has_value() ? b200c_norm_rotate_workspace_bytes(r.channels) : 0;
+  auto ws = workspace(bytes, q);
+  check_status(b200c_norm_rotate_backward(&r.side[0], &r.side[1], r.freq.data_ptr(), r.dims, r.channels, r.pos_f64,
+                                          r.freq_f64, (float)eps, r.dtype, bytes ? ws.data_ptr() : nullptr, bytes,
+                                          at::cuda::getCurrentCUDAStream().stream()));
+  return {dq, dk, dwq, dwk};
+}
+
+// ---- attention -----------------------------------------------------------------------------------------------------
+
+struct Attention {
+  torch::Tensor q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope;
+  b200c_attention_t a{};
+};
+
+void prepare_attention(Attention &t, const torch::Tensor &q, const torch::Tensor &k, const torch::Tensor &v,
+                       const OptTensor &ptr_q, const OptTensor &ptr_k, const OptTensor &pos_q, const OptTensor &pos_k,
+                       const OptTensor &slope, double scale, double cap) {
+  CHECK_CUDA(q);
+  CHECK_CUDA(k);
+  CHECK_CUDA(v);
+  CHECK_INPUT(q.dim() == 3 && k.dim() == 3 && v.dim() == 3);
+  CHECK_INPUT(k.sizes() == v.sizes() && q.size(2) == k.size(2));
+  CHECK_INPUT(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type());
+  CHECK_INPUT(q.get_device() == k.get_device() && q.get_device() == v.get_device());
+  b200c_attention_t &a = t.a;
+  a.dtype = dtype_code(q, "attention");
+  TORCH_CHECK(q.size(2) >= 1 && q.size(2) <= 128, "attention covers 1 to 128 channels per head, got ", q.size(2));
+  TORCH_CHECK(k.size(1) >= 1 && q.size(1) >= 1 && q.size(1) % k.size(1) == 0 && q.size(1) <= 1024,
+              "the heads of q must be a multiple of the heads of k and v, at most 1024");
+  t.q = rows_of(q);
+  t.k = rows_of(k);
+  t.v = rows_of(v);
+  a.q = t.q.data_ptr();
+  a.k = t.k.data_ptr();
+  a.v = t.v.data_ptr();
+  a.q_row = t.q.stride(0), a.q_head = t.q.stride(1);
+  a.k_row = t.k.stride(0), a.k_head = t.k.stride(1);
+  a.v_row = t.v.stride(0), a.v_head = t.v.stride(1);
+  a.m = q.size(0), a.n = k.size(0);
+  a.heads = (int)q.size(1), a.groups = (int)k.size(1), a.channels = (int)q.size(2);
+  a.scale = (float)scale, a.cap = (float)cap;
+  a.num_segments = 1;
+  CHECK_INPUT(ptr_q.has_value() == ptr_k.has_value());
+  if (ptr_q.has_value()) {
+    t.ptr_q = ptr_q.value().contiguous();
+    t.ptr_k = ptr_k.value().contiguous();
+    CHECK_INPUT(t.ptr_q.is_cuda() && t.ptr_k.is_cuda() && t.ptr_q.get_device() == q.get_device() &&
+                t.ptr_k.get_device() == q.get_device());
+    CHECK_INPUT(t.ptr_q.dim() == 1 && t.ptr_k.dim() == 1 && t.ptr_q.numel() == t.ptr_k.numel() && t.ptr_q.numel() >= 2);
+    TORCH_CHECK(t.ptr_q.scalar_type() == at::kLong && t.ptr_k.scalar_type() == at::kLong,
+                "ptr_q and ptr_k must be int64 tensors");
+    a.ptr_q = t.ptr_q.data_ptr<int64_t>();
+    a.ptr_k = t.ptr_k.data_ptr<int64_t>();
+    a.num_segments = t.ptr_q.numel() - 1;
+  }
+  CHECK_INPUT(pos_q.has_value() == pos_k.has_value() && pos_q.has_value() == slope.has_value());
+  if (pos_q.has_value()) {
+    t.pos_q = pos_q.value().contiguous();
+    t.pos_k = pos_k.value().contiguous();
+    t.slope = slope.value().contiguous();
+    for (const auto &p : {t.pos_q, t.pos_k, t.slope})
+      CHECK_INPUT(p.is_cuda() && p.get_device() == q.get_device() && p.scalar_type() == at::kFloat);
+    CHECK_INPUT(t.pos_q.dim() == 2 && t.pos_k.dim() == 2 && t.pos_q.size(0) == a.m && t.pos_k.size(0) == a.n &&
+                t.pos_q.size(1) == t.pos_k.size(1));
+    TORCH_CHECK(t.pos_q.size(1) >= 1 && t.pos_q.size(1) <= 8, "1 to 8 coordinates are supported");
+    CHECK_INPUT(t.slope.dim() == 1 && t.slope.size(0) == a.heads);
+    a.dims = (int)t.pos_q.size(1);
+    a.pos_q = t.pos_q.data_ptr<float>();
+    a.pos_k = t.pos_k.data_ptr<float>();
+    a.slope = t.slope.data_ptr<float>();
+  }
+}
+
+std::tuple<torch::Tensor, torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                                           OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q,
+                                                           OptTensor pos_k, OptTensor slope, double scale, double cap,
+                                                           bool with_lse) {
+  OpRange range("torch_cluster::attention_forward");
+  CHECK_CUDA(q);
+  c10::cuda::CUDAGuard guard(q.device());
+  Attention t;
+  prepare_attention(t, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap);
+  auto out = torch::empty(q.sizes(), q.options());
+  auto lse = torch::empty({with_lse ? t.a.heads : 0, t.a.m}, q.options().dtype(torch::kFloat));
+  const size_t bytes = b200c_attention_workspace_bytes(&t.a);
+  auto ws = workspace(bytes, q);
+  check_status(b200c_attention_forward(&t.a, out.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr,
+                                       bytes ? ws.data_ptr() : nullptr, bytes,
+                                       at::cuda::getCurrentCUDAStream().stream()));
+  return {out, lse};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
+    torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
+    OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q, OptTensor pos_k, OptTensor slope, double scale, double cap,
+    bool need_q, bool need_kv) {
+  OpRange range("torch_cluster::attention_backward");
+  CHECK_CUDA(q);
+  c10::cuda::CUDAGuard guard(q.device());
+  Attention t;
+  prepare_attention(t, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap);
+  CHECK_INPUT(dout.sizes() == q.sizes() && out.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&
+              out.scalar_type() == q.scalar_type() && dout.device() == q.device() && out.device() == q.device());
+  CHECK_INPUT(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.dim() == 2 &&
+              lse.size(0) == q.size(1) && lse.size(1) == q.size(0));
+  dout = dout.contiguous();
+  out = out.contiguous();
+  lse = lse.contiguous();
+  auto none = torch::empty({0}, q.options());
+  auto dq = need_q ? torch::empty(q.sizes(), q.options()) : none;
+  auto dk = need_kv ? torch::empty(k.sizes(), k.options()) : none;
+  auto dv = need_kv ? torch::empty(v.sizes(), v.options()) : none;
+  const size_t bytes = b200c_attention_backward_workspace_bytes(&t.a);
+  auto ws = workspace(bytes, q);
+  check_status(b200c_attention_backward(&t.a, out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(),
+                                        need_q ? dq.data_ptr() : nullptr, need_kv ? dk.data_ptr() : nullptr,
+                                        need_kv ? dv.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
+                                        at::cuda::getCurrentCUDAStream().stream()));
+  return {dq, dk, dv};
+}
+
+}  // namespace
+
+static auto registry = torch::RegisterOperators()
+                           .op("torch_cluster::gather_rows", &gather_rows)
+                           .op("torch_cluster::gather_rows_backward", &gather_rows_backward)
+                           .op("torch_cluster::norm_rotate", &norm_rotate)
+                           .op("torch_cluster::norm_rotate_backward", &norm_rotate_backward)
+                           .op("torch_cluster::attention_forward", &attention_forward)
+                           .op("torch_cluster::attention_backward", &attention_backward);
