@@ -478,17 +478,19 @@ typedef struct {
   float scale, cap;                /* cap <= 0: none */
   int dtype;
 } b200c_attention_t;
-/* out [m, heads, channels] contiguous; lse (may be NULL) [heads, m]: log2 of the sum of exp(z), +inf where out is
+/* out [m, heads, channels] contiguous; rest (may be NULL): the same shape and type, what rounding took from out, which
+ * sharpens the gradients of 16-bit types; lse (may be NULL) [heads, m]: log2 of the sum of exp(z), +inf where out is
  * zero by the rules above; the backward pass needs it.  workspace: b200c_attention_workspace_bytes(a) bytes (may be 0).
- * The backward pass takes out, lse and the gradient dout [m, heads, channels] (contiguous) and writes dq [m, heads,
+ * The backward pass takes out, rest, lse and the gradient dout [m, heads, channels] (contiguous) and writes dq [m, heads,
  * channels] and dk, dv [n, groups, channels] (contiguous; dq or both of dk and dv may be NULL).  Positions and slopes are
- * constants.  No atomics: the same bits every time. */
+ * constants.  Sums take no atomics: the same bits every time.  The tensor-core kernels' waits are bounded; if one ever ran
+ * out, its block's rows would be NaN. */
 size_t b200c_attention_workspace_bytes(const b200c_attention_t *a);
-int b200c_attention_forward(const b200c_attention_t *a, void *out, float *lse, void *workspace,
+int b200c_attention_forward(const b200c_attention_t *a, void *out, void *rest, float *lse, void *workspace,
                             size_t workspace_bytes, b200c_stream_t stream);
 size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a);
-int b200c_attention_backward(const b200c_attention_t *a, const void *out, const float *lse, const void *dout,
-                             void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+int b200c_attention_backward(const b200c_attention_t *a, const void *out, const void *rest, const float *lse,
+                             const void *dout, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
                              b200c_stream_t stream);
 
 #ifdef __cplusplus

@@ -139,11 +139,11 @@ def cabi() -> ctypes.CDLL:
     lib.b200c_norm_rotate_backward.restype = i32
     lib.b200c_attention_workspace_bytes.argtypes = [p]
     lib.b200c_attention_workspace_bytes.restype = sz
-    lib.b200c_attention_forward.argtypes = [p, p, p, p, sz, p]
+    lib.b200c_attention_forward.argtypes = [p, p, p, p, p, sz, p]
     lib.b200c_attention_forward.restype = i32
     lib.b200c_attention_backward_workspace_bytes.argtypes = [p]
     lib.b200c_attention_backward_workspace_bytes.restype = sz
-    lib.b200c_attention_backward.argtypes = [p, p, p, p, p, p, p, p, sz, p]
+    lib.b200c_attention_backward.argtypes = [p, p, p, p, p, p, p, p, p, sz, p]
     lib.b200c_attention_backward.restype = i32
     for name in ("b200c_segment_ptr", "b200c_exclusive_scan", "b200c_exclusive_scan_static", "b200c_knn", "b200c_knn_compact", "b200c_knn_graph_tail_count", "b200c_knn_graph_tail_write",
                  "b200c_radius_count", "b200c_radius_fill"):

@@ -9,19 +9,18 @@ from torch.autograd.function import once_differentiable
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap):
-        out, lse = torch.ops.torch_cluster.attention_forward(q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap,
-                                                             True)
-        ctx.save_for_backward(q, k, v, out, lse, ptr_q, ptr_k, pos_q, pos_k, slope)
+        out, rest, lse = torch.ops.torch_cluster.attention_forward(q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale,
+                                                                   cap, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, ptr_q, ptr_k, pos_q, pos_k, slope)
         ctx.scale, ctx.cap = scale, cap
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, *rest = ctx.saved_tensors
+        tensors = ctx.saved_tensors
         need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq, dk, dv = torch.ops.torch_cluster.attention_backward(dout, q, k, v, out, lse, *rest, ctx.scale, ctx.cap,
-                                                                need_q, need_kv)
+        dq, dk, dv = torch.ops.torch_cluster.attention_backward(dout, *tensors, ctx.scale, ctx.cap, need_q, need_kv)
         return (dq if need_q else None, dk if ctx.needs_input_grad[1] else None,
                 dv if ctx.needs_input_grad[2] else None, None, None, None, None, None, None, None)
 

@@ -11,7 +11,8 @@
 //   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,
 // the sums over i running over all heads of the key's group.  p is formed again from the forward pass's
 //   lse_i = log2 sum_j exp(z_ij)      (+inf for rows that give zeros, so that p = 0),
-// stored [heads, m].  Scores are kept in units of log 2: exp(z) = 2^(z log2 e).
+// stored [heads, m].  D is a small difference of what the rounded outputs give where few keys share the weight, so the
+// forward pass of a training step also keeps what rounding took from out, in out's type.  Scores are kept in units of log 2: exp(z) = 2^(z log2 e).
 #pragma once
 
 #include "common.cuh"
@@ -26,10 +27,11 @@ struct AttnArgs {
   b200c_attention_t p;
   void *out = nullptr;           // [m, heads, channels]
   float *lse = nullptr;          // [heads, m]; forward: may be null
+  void *rest = nullptr;          // [m, heads, channels]: what rounding took from out, in out's type; may be null
   const void *dout = nullptr;    // [m, heads, channels]
   const float *delta = nullptr;  // [heads, m]: D_i
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // [m, heads, channels], [n, groups, channels] x 2
-  int *error = nullptr;          // set when a bounded wait ran out
+  const float *norms = nullptr;  // fp16: the largest |do|^2 and |v|^2 of a row
   cudaStream_t stream = nullptr;
 };
 
@@ -62,7 +64,10 @@ __device__ __forceinline__ void at_segment(const int64_t *__restrict__ ptr, int6
 
 int launch_attention_plain_forward(const AttnArgs &a);
 int launch_attention_plain_backward(const AttnArgs &a);
-int launch_attention_delta(const AttnArgs &a, float *delta);
+int launch_attention_delta(const AttnArgs &a, float *delta, float *norms);
+bool attention_tensor_applicable(const b200c_attention_t &p);
+int launch_attention_tensor_forward(const AttnArgs &a);
+int launch_attention_tensor_backward(const AttnArgs &a);
 int attention_few_splits(const b200c_attention_t &p);  // 0: not for this call
 size_t attention_few_workspace_bytes(const b200c_attention_t &p);
 int launch_attention_few(const AttnArgs &a, int splits, void *workspace);

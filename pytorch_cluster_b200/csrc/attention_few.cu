@@ -245,7 +245,9 @@ __global__ void __launch_bounds__(256) attention_few_join_kernel(AttnArgs a, int
     if (inside)
       for (int s = 0; s < splits; ++s)
         acc = fmaf(src[(int64_t)s * width + 2 + c], exp2f(src[(int64_t)s * width] - base), acc);
-    out[c] = at_round<T>(acc * inv);
+    const T r = at_round<T>(acc * inv);
+    out[c] = r;
+    if (a.rest) ((T *)a.rest)[i * p.channels + c] = at_round<T>(acc * inv - at_float(r));
   }
   if (a.lse && lane == 0) a.lse[(int64_t)head * p.m + row] = l == 0.f ? pos_inf<float>() : m + log2f(l);
 }

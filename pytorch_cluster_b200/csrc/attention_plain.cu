@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
   const T *v = (const T *)p.v + (int64_t)group * p.v_head;
   const float slope = p.dims > 0 ? p.slope[head] : 0.f;
   const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
-  T *out = (T *)a.out;
+  T *out = (T *)a.out, *rest = (T *)a.rest;
 
   ap_load(sq, q, p.q_row, t0, t0, t1, p.channels, CP, tid);
   if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, t0, t0, t1, tid);
@@ -138,7 +138,10 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
       row = hi - 1;
       continue;
     }
-    for (int c = tid; c < p.channels; c += AP_THREADS) out[(row * p.heads + head) * p.channels + c] = at_round<T>(0.f);
+    for (int c = tid; c < p.channels; c += AP_THREADS) {
+      out[(row * p.heads + head) * p.channels + c] = at_round<T>(0.f);
+      if (rest) rest[(row * p.heads + head) * p.channels + c] = at_round<T>(0.f);
+    }
     if (a.lse && tid == 0) a.lse[(int64_t)head * p.m + row] = pos_inf<float>();
   }
   const int b_first = segment_of(p.ptr_q, p.num_segments, t0), b_last = segment_of(p.ptr_q, p.num_segments, t1 - 1);
@@ -196,7 +199,10 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         const int c = tx + 16 * n;
-        if (c < p.channels) out[(row * p.heads + head) * p.channels + c] = at_round<T>(o[i][n] * inv);
+        if (c >= p.channels) continue;
+        const T r = at_round<T>(o[i][n] * inv);
+        out[(row * p.heads + head) * p.channels + c] = r;
+        if (rest) rest[(row * p.heads + head) * p.channels + c] = at_round<T>(o[i][n] * inv - at_float(r));
       }
       if (a.lse && tx == 0)
         a.lse[(int64_t)head * p.m + row] = sum[i] == 0.f ? pos_inf<float>() : top[i] + log2f(sum[i]);
@@ -389,18 +395,49 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
   }
 }
 
-// D_i = do_i . o_i, one warp per (row, head)
+// D_i = do_i . o_i, one warp per (row, head); norms[0] rises to the largest |do_i|^2
 template <typename T>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const T *__restrict__ dout, const T *__restrict__ out,
-                                                              int64_t m, int heads, int channels,
-                                                              float *__restrict__ delta) {
+                                                              const T *__restrict__ rest, int64_t m, int heads,
+                                                              int channels, float *__restrict__ delta,
+                                                              float *__restrict__ norms) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (i >= m * heads) return;
-  float s = 0.f;
-  for (int c = lane; c < channels; c += 32) s = fmaf(at_float(dout[i * channels + c]), at_float(out[i * channels + c]), s);
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL_MASK, s, o);
-  if (lane == 0) delta[(i % heads) * m + i / heads] = s;
+  float s = 0.f, sq = 0.f;
+  for (int c = lane; c < channels; c += 32) {
+    const float g = at_float(dout[i * channels + c]);
+    float o = at_float(out[i * channels + c]);
+    if (rest) o += at_float(rest[i * channels + c]);
+    s = fmaf(g, o, s);
+    sq = fmaf(g, g, sq);
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(FULL_MASK, s, o);
+    sq += __shfl_xor_sync(FULL_MASK, sq, o);
+  }
+  if (lane == 0) {
+    delta[(i % heads) * m + i / heads] = s;
+    // non-negative floats order like their bits; a maximum does not depend on the order
+    if (norms && __float_as_uint(sq) > __float_as_uint(*(volatile float *)norms))
+      atomicMax((unsigned *)norms, __float_as_uint(sq));
+  }
+}
+
+// norms[1] rises to the largest |v_j|^2
+template <typename T>
+__global__ void __launch_bounds__(256) attention_value_norm_kernel(const T *__restrict__ v, int64_t n, int groups,
+                                                                   int channels, int64_t row_stride,
+                                                                   int64_t head_stride, float *__restrict__ norms) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (i >= n * groups) return;
+  const T *row = v + (i / groups) * row_stride + (i % groups) * head_stride;
+  float sq = 0.f;
+  for (int c = lane; c < channels; c += 32) sq = fmaf(at_float(row[c]), at_float(row[c]), sq);
+  for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(FULL_MASK, sq, o);
+  if (lane == 0 && __float_as_uint(sq) > __float_as_uint(*(volatile float *)(norms + 1)))
+    atomicMax((unsigned *)(norms + 1), __float_as_uint(sq));
 }
 
 template <typename T, int CP>
@@ -450,21 +487,28 @@ static int ap_any(const AttnArgs &a, bool forward) {
 int launch_attention_plain_forward(const AttnArgs &a) { return ap_any(a, true); }
 int launch_attention_plain_backward(const AttnArgs &a) { return ap_any(a, false); }
 
-int launch_attention_delta(const AttnArgs &a, float *delta) {
-  const int64_t rows = a.p.m * a.p.heads;
-  if (rows == 0) return B200C_OK;
-  const unsigned blocks = (unsigned)((rows + 7) / 8);
-  if (a.p.dtype == B200C_F32)
-    attention_delta_kernel<float><<<blocks, 256, 0, a.stream>>>((const float *)a.dout, (const float *)a.out, a.p.m,
-                                                                a.p.heads, a.p.channels, delta);
-  else if (a.p.dtype == B200C_F16)
-    attention_delta_kernel<__half><<<blocks, 256, 0, a.stream>>>((const __half *)a.dout, (const __half *)a.out, a.p.m,
-                                                                 a.p.heads, a.p.channels, delta);
-  else
-    attention_delta_kernel<__nv_bfloat16><<<blocks, 256, 0, a.stream>>>(
-        (const __nv_bfloat16 *)a.dout, (const __nv_bfloat16 *)a.out, a.p.m, a.p.heads, a.p.channels, delta);
-  B200C_LAUNCH_CHECK("attention_delta_kernel");
+template <typename T>
+static int ap_delta(const AttnArgs &a, float *delta, float *norms) {
+  const b200c_attention_t &p = a.p;
+  const int64_t rows = p.m * p.heads, values = p.n * p.groups;
+  if (norms) B200C_CUDA(cudaMemsetAsync(norms, 0, 8, a.stream));
+  if (rows > 0) {
+    attention_delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, a.stream>>>(
+        (const T *)a.dout, (const T *)a.out, (const T *)a.rest, p.m, p.heads, p.channels, delta, norms);
+    B200C_LAUNCH_CHECK("attention_delta_kernel");
+  }
+  if (norms && values > 0) {
+    attention_value_norm_kernel<T><<<(unsigned)((values + 7) / 8), 256, 0, a.stream>>>(
+        (const T *)p.v, p.n, p.groups, p.channels, p.v_row, p.v_head, norms);
+    B200C_LAUNCH_CHECK("attention_value_norm_kernel");
+  }
   return B200C_OK;
+}
+
+int launch_attention_delta(const AttnArgs &a, float *delta, float *norms) {
+  if (a.p.dtype == B200C_F32) return ap_delta<float>(a, delta, nullptr);
+  if (a.p.dtype == B200C_F16) return ap_delta<__half>(a, delta, norms);
+  return ap_delta<__nv_bfloat16>(a, delta, nullptr);
 }
 
 }  // namespace b200c

@@ -150,7 +150,7 @@ extern "C" size_t b200c_attention_workspace_bytes(const b200c_attention_t *a) {
   return attention_few_workspace_bytes(*a);
 }
 
-extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, float *lse, void *workspace,
+extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, void *rest, float *lse, void *workspace,
                                        size_t workspace_bytes, b200c_stream_t stream) {
   int st = check_attention(p);
   if (st != B200C_OK) return st;
@@ -164,20 +164,23 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, fl
   AttnArgs a;
   a.p = *p;
   a.out = out;
+  a.rest = rest;
   a.lse = lse;
   a.stream = (cudaStream_t)stream;
   const int splits = attention_few_splits(*p);
   if (splits > 0) return launch_attention_few(a, splits, workspace);
+  if (attention_tensor_applicable(*p) && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0)
+    return launch_attention_tensor_forward(a);
   return launch_attention_plain_forward(a);
 }
 
 extern "C" size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a) {
   if (check_attention(a) != B200C_OK) return 0;
-  return align256((size_t)a->m * a->heads * 4);
+  return align256((size_t)a->m * a->heads * 4) + 256;  // D, and the largest norms
 }
 
-extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const float *lse, const void *dout,
-                                        void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const void *rest, const float *lse,
+                                        const void *dout, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
                                         b200c_stream_t stream) {
   int st = check_attention(p);
   if (st != B200C_OK) return st;
@@ -192,6 +195,7 @@ extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *
   AttnArgs a;
   a.p = *p;
   a.out = (void *)out;
+  a.rest = (void *)rest;
   a.lse = (float *)lse;
   a.dout = dout;
   a.delta = (const float *)workspace;
@@ -199,6 +203,11 @@ extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *
   a.dk = dk;
   a.dv = dv;
   a.stream = (cudaStream_t)stream;
-  if ((st = launch_attention_delta(a, (float *)workspace)) != B200C_OK) return st;
+  float *norms = (float *)((char *)workspace + align256((size_t)p->m * p->heads * 4));
+  a.norms = norms;
+  if ((st = launch_attention_delta(a, (float *)workspace, norms)) != B200C_OK) return st;
+  if (attention_tensor_applicable(*p) &&
+      (((uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0)
+    return launch_attention_tensor_backward(a);
   return launch_attention_plain_backward(a);
 }

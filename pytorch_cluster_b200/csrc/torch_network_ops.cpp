@@ -261,28 +261,31 @@ void prepare_attention(Attention &t, const torch::Tensor &q, const torch::Tensor
   }
 }
 
-std::tuple<torch::Tensor, torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                                                           OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q,
-                                                           OptTensor pos_k, OptTensor slope, double scale, double cap,
-                                                           bool with_lse) {
+// training: also the statistics and, for 16-bit types, what rounding took from the output
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_forward(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q,
+    OptTensor pos_k, OptTensor slope, double scale, double cap, bool training) {
   OpRange range("torch_cluster::attention_forward");
   CHECK_CUDA(q);
   c10::cuda::CUDAGuard guard(q.device());
   Attention t;
   prepare_attention(t, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap);
   auto out = torch::empty(q.sizes(), q.options());
-  auto lse = torch::empty({with_lse ? t.a.heads : 0, t.a.m}, q.options().dtype(torch::kFloat));
+  auto lse = torch::empty({training ? t.a.heads : 0, t.a.m}, q.options().dtype(torch::kFloat));
+  const bool keep = training && t.a.dtype != B200C_F32;
+  auto rest = keep ? torch::empty(q.sizes(), q.options()) : torch::empty({0}, q.options());
   const size_t bytes = b200c_attention_workspace_bytes(&t.a);
   auto ws = workspace(bytes, q);
-  check_status(b200c_attention_forward(&t.a, out.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr,
+  check_status(b200c_attention_forward(&t.a, out.data_ptr(), keep ? rest.data_ptr() : nullptr,
+                                       training ? lse.data_ptr<float>() : nullptr,
                                        bytes ? ws.data_ptr() : nullptr, bytes,
                                        at::cuda::getCurrentCUDAStream().stream()));
-  return {out, lse};
+  return {out, rest, lse};
 }
 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
-    torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
-    OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q, OptTensor pos_k, OptTensor slope, double scale, double cap,
+    torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor rest,
+    torch::Tensor lse, OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q, OptTensor pos_k, OptTensor slope, double scale, double cap,
     bool need_q, bool need_kv) {
   OpRange range("torch_cluster::attention_backward");
   CHECK_CUDA(q);
@@ -296,13 +299,16 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
   dout = dout.contiguous();
   out = out.contiguous();
   lse = lse.contiguous();
+  const bool kept = rest.numel() > 0;
+  CHECK_INPUT(!kept || (rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() && rest.device() == q.device()));
+  rest = rest.contiguous();
   auto none = torch::empty({0}, q.options());
   auto dq = need_q ? torch::empty(q.sizes(), q.options()) : none;
   auto dk = need_kv ? torch::empty(k.sizes(), k.options()) : none;
   auto dv = need_kv ? torch::empty(v.sizes(), v.options()) : none;
   const size_t bytes = b200c_attention_backward_workspace_bytes(&t.a);
   auto ws = workspace(bytes, q);
-  check_status(b200c_attention_backward(&t.a, out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(),
+  check_status(b200c_attention_backward(&t.a, out.data_ptr(), kept ? rest.data_ptr() : nullptr, lse.data_ptr<float>(), dout.data_ptr(),
                                         need_q ? dq.data_ptr() : nullptr, need_kv ? dk.data_ptr() : nullptr,
                                         need_kv ? dv.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
                                         at::cuda::getCurrentCUDAStream().stream()));

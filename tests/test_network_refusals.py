@@ -68,12 +68,12 @@ def test_attention_argument_checks(changes, message):
 
     lib = _native.cabi()
     a = attention_args(**changes)
-    for call in (lambda: lib.b200c_attention_forward(ctypes.byref(a), 1 << 20, None, None, 0, None),
-                 lambda: lib.b200c_attention_backward(ctypes.byref(a), 1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20,
+    for call in (lambda: lib.b200c_attention_forward(ctypes.byref(a), 1 << 20, None, None, None, 0, None),
+                 lambda: lib.b200c_attention_backward(ctypes.byref(a), 1 << 20, None, 1 << 20, 1 << 20, 1 << 20, 1 << 20,
                                                       1 << 20, None, 0, None)):
         assert call() == 1 and message in lib.b200c_last_error()
     assert lib.b200c_attention_workspace_bytes(ctypes.byref(a)) == 0
-    assert lib.b200c_attention_forward(None, 1 << 20, None, None, 0, None) == 1
+    assert lib.b200c_attention_forward(None, 1 << 20, None, None, None, 0, None) == 1
 
 
 class Side(ctypes.Structure):
