@@ -191,6 +191,11 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
         if (s < steps) {
           const uint32_t g = it + s, st = g % F::STAGES, nb = g % F::NB;
           ok = __all_sync(FULL_MASK, t5_mbar_wait(&full[st], (g / F::STAGES) & 1, failed));
+          // the accumulators hold the weights of NB steps ago: products of different accumulators are not ordered
+          if (ok && s >= F::NB) {
+            const uint32_t b = g - F::NB;
+            ok = __all_sync(FULL_MASK, t5_mbar_wait(&empty[b % F::STAGES], (b / F::STAGES) & 1, failed));
+          }
           if (!ok) break;
           t5_fence_after();
           if (lane == 0) {
@@ -264,7 +269,8 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           float x[32], dp[32], u[CAP ? 32 : 1];
           t5_ld32(t_s, x);
           t5_ld32(t_dp, dp);
-          t5_wait_ld();
+          t5_wait_ld32(x);
+          t5_wait_ld32(dp);
           at_logits<DIM, CAP, CAP>(x, u, sd, pos, slope2, pre, post);
           const bool whole = __all_sync(FULL_MASK, lo <= base && hi >= base + 32);
 #pragma unroll
@@ -348,7 +354,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           float o[32];
           if (steps > 0 && ok) {
             t5_ld32(t_acc + (KV && half ? CP : 0) + lane_base + cc, o);
-            t5_wait_ld();
+            t5_wait_ld32(o);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;

@@ -39,7 +39,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   unsigned char *sq = smem;
   unsigned char *stages = smem + F::Q_BYTES;
   float *spos = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[2], p_ready[2], o_done, drained;
+  __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[2], p_ready[2], o_done, done, drained;
   __shared__ uint32_t tmem_s;
   __shared__ int failed_s, bad_s;
   volatile int *failed = &failed_s;
@@ -61,6 +61,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       t5_mbar_init(&p_ready[i], AT_ROWS);
     }
     t5_mbar_init(&o_done, 1);
+    t5_mbar_init(&done, 1);
     t5_mbar_init(&drained, 1);
     failed_s = 0;
     bad_s = 0;
@@ -104,6 +105,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   AtPass pass = tile.all();
   const bool mixed = tile.b_first != tile.b_last;
   uint32_t it = 0;      // steps so far, over all passes
+  uint32_t passes = 0;  // passes with steps
   uint32_t issued = 0;  // copy warp: steps whose copies were issued
   bool ok = true;
   if (warp == 5) ok = __all_sync(FULL_MASK, t5_mbar_wait(&q_full, 0, failed));
@@ -144,6 +146,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         if (s < steps) {
           const uint32_t g = it + s, st = g % F::STAGES;
           ok = __all_sync(FULL_MASK, t5_mbar_wait(&full[st], (g / F::STAGES) & 1, failed));
+          // the accumulator holds the weights of two steps ago: products of different accumulators are not ordered
+          if (ok && s > 1) ok = __all_sync(FULL_MASK, t5_mbar_wait(&o_done, (g - 2) & 1, failed));
           if (!ok) break;
           t5_fence_after();
           if (lane == 0) {
@@ -171,6 +175,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
                         s > 1 || ks > 0);
             t5_commit(&empty[st]);
             t5_commit(&o_done);
+            if (s == steps) t5_commit(&done);
           }
           __syncwarp();
         }
@@ -202,7 +207,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           float x[AT_COLS];
           t5_ld32(t_s, x);
           t5_ld32(t_s + 32, x + 32);
-          t5_wait_ld();
+          t5_wait_ld32(x);
+          t5_wait_ld32(x + 32);
           const float *cp = spos + st * (AT_MAX_DIMS * AT_COLS);
           at_logits<DIM, CAP, false>(x, nullptr, cp, pos, slope2, pre, post);
           at_logits<DIM, CAP, false>(x + 32, nullptr, cp + 32, pos, slope2, pre, post);
@@ -235,7 +241,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
               for (int c = 0; c < CP; c += 32) {
                 float o[32];
                 t5_ld32(t_o + lane_base + c, o);
-                t5_wait_ld();
+                t5_wait_ld32(o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] *= shrink;
                 t5_st32(t_o + lane_base + c, reinterpret_cast<const uint32_t *>(o));
@@ -266,7 +272,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         t5_mbar_arrive(&p_ready[g & 1]);
       }
       if (ok && steps > 0) {
-        ok = __all_sync(FULL_MASK, t5_mbar_wait(&o_done, (it + steps - 1) & 1, failed));
+        ok = __all_sync(FULL_MASK, t5_mbar_wait(&done, passes & 1, failed));
         t5_fence_after();
       }
       if (bad) bad_s = 1;
@@ -285,7 +291,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           float o[32];
           if (steps > 0 && ok) {
             t5_ld32(t_o + lane_base + c, o);
-            t5_wait_ld();
+            t5_wait_ld32(o);
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -313,6 +319,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       }
     }
     it += steps;
+    if (steps > 0) ++passes;
     t5_fence_before();
     __syncthreads();
     t5_fence_after();

@@ -28,9 +28,10 @@ __device__ __forceinline__ bool t5_mbar_try(uint64_t *bar, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-constexpr int T5_SPIN_LIMIT = 1 << 24;  // polls of a wait, each suspended for a while by the hardware: seconds
-// Waits for the phase of the given parity; gives up after T5_SPIN_LIMIT polls, or when another thread of the block did
-// (*failed), and says so.
+constexpr int T5_SPIN_LIMIT = 1 << 22;  // polls of a wait of some ten nanoseconds each; a step takes a microsecond or two
+// Waits for the phase of the given parity.  A parity tells two neighbouring phases apart, no more: a caller must know that
+// the phase before is over and that the one after cannot end before it has gone on.  Gives up after T5_SPIN_LIMIT polls,
+// or when another thread of the block did (*failed), and says so.
 __device__ __forceinline__ bool t5_mbar_wait(uint64_t *bar, uint32_t parity, volatile int *failed) {
   if (t5_mbar_try(bar, parity)) return true;
   for (int i = 0; i < T5_SPIN_LIMIT; ++i) {
@@ -51,7 +52,6 @@ __device__ __forceinline__ void t5_tma_3d(void *dst, const CUtensorMap *map, int
 
 __device__ __forceinline__ void t5_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void t5_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void t5_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void t5_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void t5_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(t5_smem(bar))
@@ -88,17 +88,27 @@ __device__ __forceinline__ void t5_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       : "memory");
 }
 
-// 32 columns of the thread's lane; the caller waits (t5_wait_ld) before it reads v
-__device__ __forceinline__ void t5_ld32(uint32_t taddr, float *v) {
-  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+// Waits for the thread's loads from tensor memory.  The values pass through the instruction, so that no use of them can be
+// moved ahead of it.
+__device__ __forceinline__ void t5_wait_ld32(float *v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]),"+f"(v[1]),"+f"(v[2]),"+f"(v[3]),"+f"(v[4]),"+f"(v[5]),"+f"(v[6]),"+f"(v[7]),
+                 "+f"(v[8]),"+f"(v[9]),"+f"(v[10]),"+f"(v[11]),"+f"(v[12]),"+f"(v[13]),"+f"(v[14]),"+f"(v[15]),
+                 "+f"(v[16]),"+f"(v[17]),"+f"(v[18]),"+f"(v[19]),"+f"(v[20]),"+f"(v[21]),"+f"(v[22]),"+f"(v[23]),
+                 "+f"(v[24]),"+f"(v[25]),"+f"(v[26]),"+f"(v[27]),"+f"(v[28]),"+f"(v[29]),"+f"(v[30]),"+f"(v[31])
+               ::"memory");
+}
+
+// 32 columns of the thread's lane; the caller waits (t5_wait_ld32) before it reads v
+__device__ __forceinline__ void t5_ld32(uint32_t taddr, float *r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
       "%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(taddr));
 }
 __device__ __forceinline__ void t5_st32(uint32_t taddr, const uint32_t *r) {

@@ -619,3 +619,26 @@ def test_a_layer_on_the_graph(dtype):
     # well below 16 of them
     for a, z in zip(got, want):
         assert (a.double() - z.double()).norm() <= 16 * half_step(dtype) * z.double().norm()
+
+
+def test_attention_long_examples_same_bits():
+    """Every wait of the tensor-core kernels counts here: thousands of steps, slow and fast ones."""
+    import pytorch_cluster_b200 as pc
+
+    g = gen(30)
+    lens = [2515, 1594, 2290, 1852]
+    n, b = sum(lens), ids(lens)
+    for channels, dims, cap in ((64, 3, None), (64, 0, None), (32, 8, 4.0), (128, 2, None), (128, 0, 4.0)):
+        ts = [rand(g, n, 4, channels, dtype=torch.bfloat16).requires_grad_() for _ in range(3)]
+        extra = {}
+        if dims:
+            pos = rand(g, n, dims, dtype=torch.float32)
+            extra = dict(pos_q=pos, pos_k=pos, slope=torch.tensor([1.0, 0.5, 0.1, 0.0], device="cuda"))
+        do = rand(g, n, 4, channels, dtype=torch.bfloat16)
+        first = None
+        for _ in range(6):
+            out = pc.attention(*ts, b, b, cap=cap, batch_size=4, **extra)
+            got = [out.detach(), *torch.autograd.grad(out, ts, do)]
+            first = first or got
+            assert all(torch.equal(x, y) for x, y in zip(first, got))
+        assert all(torch.isfinite(x).all() for x in first)
