@@ -2,9 +2,8 @@
 // over the keys, KV = true sums dk and dv of 128 keys of a group over the queries of all its heads.
 //
 // Forming the scores once per direction costs two products more than one kernel for both would, which the tensor
-// cores have to spare here (exponentials and roots bound these kernels); in return no sum is shared
-// between blocks, so there are no atomics.  The statistics of the softmax are known, so a row's columns need no
-// reduction: two groups of four warps take 32 columns of a step each.
+// cores have to spare here; in return no sum is shared between blocks, so there are no atomics.  The statistics of the
+// softmax are known, so the groups' steps need nothing of one another and share one accumulator.
 // P and dS enter the second products in the 16-bit type.  In fp16, whose range is small, P is kept times 2^12 and dS times a
 // power of two that brings the largest value that |do| and |v| allow to 2^14; both are taken out of the fp32 sums.
 #pragma once
@@ -13,19 +12,22 @@
 
 namespace b200c {
 
-template <int CP>
+template <int CP, bool KV>
 struct AtBackward {
-  static constexpr int EL_WARPS = 8;
-  static constexpr int THREADS = 32 * (EL_WARPS + 2);
-  static constexpr int EL_THREADS = 32 * EL_WARPS;
-  static constexpr int NB = CP == 64 ? 1 : 2;      // score accumulators
-  static constexpr int BLOCKS = CP == 64 ? 2 : 1;  // resident blocks per SM: tensor memory and shared memory
-  static constexpr int STAGES = CP == 64 ? 3 : 4;
+  // groups and resident blocks per SM, as tensor memory allows: 16 warps per SM, 8 where two results of 128 channels fill it
+  static constexpr int BLOCKS = CP == 64 && !KV ? 2 : 1;
+  static constexpr int G = CP == 64 && !KV ? 2 : CP == 128 && KV ? 2 : 4;
+  static constexpr int EL_WARPS = 4 * G, EL_THREADS = 32 * EL_WARPS;
+  static constexpr int THREADS = EL_THREADS + 64;
+  static constexpr int STAGES = BLOCKS == 2 ? 3 : 4;
   static constexpr int ROW_BYTES = AT_ROWS * CP * 2, TILE_BYTES = AT_COLS * CP * 2;
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-  static constexpr int SIDE_FLOATS = (AT_MAX_DIMS + 2) * AT_COLS;  // coordinates, lse, D of a step's columns
+  static constexpr int SIDE_FLOATS = (AT_MAX_DIMS + 2) * AT_COLS;  // coordinates, lse, D of a stage's columns
   static constexpr int SMEM = 2 * ROW_BYTES + STAGES * (STAGE_BYTES + SIDE_FLOATS * 4) + 1024;
-  static constexpr int TMEM = CP == 64 ? 256 : 512;
+  static constexpr int GROUP_COLS = 2 * AT_SUB + (KV ? 2 : 1) * (AT_SUB / 2);  // S, dP, dS, P
+  static constexpr int TMEM = BLOCKS == 2 ? 256 : 512;
+  static_assert(G * GROUP_COLS + (KV ? 2 : 1) * CP <= TMEM, "tensor memory");
+  static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 
 struct AtBackwardMaps {
@@ -45,24 +47,26 @@ __device__ __forceinline__ float at_sigma(const float *norms) {
 }
 
 template <typename T, int CP, int DIM, bool CAP, bool KV>
-__global__ void __launch_bounds__(AtBackward<CP>::THREADS, AtBackward<CP>::BLOCKS)
+__global__ void __launch_bounds__(AtBackward<CP, KV>::THREADS, AtBackward<CP, KV>::BLOCKS)
 attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __grid_constant__ AttnArgs a,
                           const float *__restrict__ norms) {
-  using F = AtBackward<CP>;
+  using F = AtBackward<CP, KV>;
   using A = AtType<T>;
-  constexpr int ATOMS = CP / 64;
+  constexpr int ATOMS = CP / 64, G = F::G, COPY = F::EL_WARPS, PRODUCT = F::EL_WARPS + 1;
   extern __shared__ unsigned char at_raw[];
   unsigned char *smem = at_raw + ((1024u - (t5_smem(at_raw) & 1023u)) & 1023u);
   unsigned char *rows0 = smem, *rows1 = smem + F::ROW_BYTES, *stages = smem + 2 * F::ROW_BYTES;
   float *side = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  __shared__ __align__(8) uint64_t r_full, full[F::STAGES], empty[F::STAGES], s_full[F::NB], w_ready[F::NB], done,
-      drained;
+  // s_full / s_free: a group's scores are in / have been read; w_ready: its weights are in; a_done: its second product is
+  __shared__ __align__(8) uint64_t r_full, full[F::STAGES], empty[F::STAGES], s_full[G], s_free[G], w_ready[G],
+      a_done[G], done, drained;
   __shared__ uint32_t tmem_s;
   __shared__ int failed_s, bad_s;
+  __shared__ AtTileShared shared_tile;
   volatile int *failed = &failed_s;
 
   const b200c_attention_t &p = a.p;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = t5_warp(), lane = tid & 31;
   const int per_group = p.heads / p.groups;
   const int head0 = KV ? (int)blockIdx.y * per_group : (int)blockIdx.y;
   const int group = KV ? (int)blockIdx.y : head0 / per_group;
@@ -73,15 +77,17 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   else
     tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
 
-  if (tid == 0) {
+  if (tid == 64) {
     t5_mbar_init(&r_full, 1);
     for (int i = 0; i < F::STAGES; ++i) {
       t5_mbar_init(&full[i], 1);
       t5_mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < F::NB; ++i) {
+    for (int i = 0; i < G; ++i) {
       t5_mbar_init(&s_full[i], 1);
-      t5_mbar_init(&w_ready[i], F::EL_THREADS);
+      t5_mbar_init(&s_free[i], 4);
+      t5_mbar_init(&w_ready[i], 4);
+      t5_mbar_init(&a_done[i], 1);
     }
     t5_mbar_init(&done, 1);
     t5_mbar_init(&drained, 1);
@@ -89,22 +95,36 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
     bad_s = 0;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == F::EL_WARPS) t5_alloc(&tmem_s, F::TMEM);
+  if (warp == COPY) t5_alloc(&tmem_s, F::TMEM);
+  tile.search(shared_tile, warp, lane);
   t5_fence_before();
   __syncthreads();
   t5_fence_after();
   const uint32_t tmem = tmem_s;
-  const uint32_t t_acc = tmem + F::NB * 2 * AT_COLS;  // dq, or dv and dk side by side
+  const uint32_t t_acc = tmem + G * F::GROUP_COLS;  // dq, or dv and dk side by side
+  if (warp == COPY && lane == 0) {
+    t5_mbar_expect(&r_full, 2 * F::ROW_BYTES);
+    for (int at = 0; at < ATOMS; ++at) {
+      t5_tma_3d(rows0 + at * (AT_ROWS * 128), &maps.row0, at * 64, KV ? group : head0, (int)tile.t0, &r_full);
+      t5_tma_3d(rows1 + at * (AT_ROWS * 128), &maps.row1, at * 64, KV ? group : head0, (int)tile.t0, &r_full);
+    }
+    t5_mbar_arrive(&r_full);
+  }
+  tile.found(shared_tile);
+  if (tile.listed()) {
+    if (tid <= tile.b_last - tile.b_first) shared_tile.ends[tid] = tile.ptr_r[tile.b_first + 1 + tid];
+    __syncthreads();
+  }
 
-  // element threads: a row and half of a step's columns each
+  // element threads: a row each
   const bool element = warp < F::EL_WARPS;
-  const int half = warp >> 2;
-  const int64_t row = tile.t0 + (tid & (AT_ROWS - 1));
+  const int grp = warp >> 2, lrow = tid & (AT_ROWS - 1);
+  const int64_t row = tile.t0 + lrow;
   int64_t row_lo = 0, row_hi = 0;
   int row_segment = -1;
   float pos[DIM == 0 ? 1 : DIM], lse = 0.f, delta = 0.f;
   if (element && row < tile.t1) {
-    row_segment = segment_of(tile.ptr_r, tile.segments, row);
+    row_segment = tile.segment(shared_tile, row);
     int64_t lo, hi;
     at_segment(tile.ptr_r, tile.rows, row_segment, lo, hi);
     if (row >= lo && row < hi) at_segment(tile.ptr_c, tile.cols, row_segment, row_lo, row_hi);
@@ -122,36 +142,40 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   const float sigma = at_sigma<T>(norms);
   const float sig = A::BF16 ? 1.f : sigma * (1.f / 4096.f);  // P carries 2^SHIFT already
 
-  if (warp == F::EL_WARPS && lane == 0) {
-    t5_mbar_expect(&r_full, 2 * F::ROW_BYTES);
-    for (int at = 0; at < ATOMS; ++at) {
-      t5_tma_3d(rows0 + at * (AT_ROWS * 128), &maps.row0, at * 64, KV ? group : head0, (int)tile.t0, &r_full);
-      t5_tma_3d(rows1 + at * (AT_ROWS * 128), &maps.row1, at * 64, KV ? group : head0, (int)tile.t0, &r_full);
-    }
-    t5_mbar_arrive(&r_full);
-  }
-
   bool by_example = false;
   int64_t next_row = tile.t0;
   AtPass pass = tile.all();
   const bool mixed = tile.b_first != tile.b_last;
-  uint32_t it = 0, issued = 0, passes = 0;
+  uint32_t step0 = 0, stage0 = 0, passes = 0, issued = 0;
   bool ok = true;
-  if (warp == F::EL_WARPS + 1) ok = __all_sync(FULL_MASK, t5_mbar_wait(&r_full, 0, failed));
+  if (warp == PRODUCT) ok = t5_mbar_wait_warp(&r_full, 0, failed);
 
   for (;;) {
     const int64_t count = pass.c_hi - pass.c_lo;
-    const uint32_t each = (uint32_t)((count + AT_COLS - 1) / AT_COLS);  // steps per head
-    const uint32_t steps = each * heads;
-    if (warp == F::EL_WARPS) {
+    const AtWalk walk(count, heads);
+    if (warp == COPY) {
       // ---- copies
+      AtRing<F::STAGES> ring(stage0);
       uint32_t e = 0, c = 0;
-      for (uint32_t s = 0; s < steps && ok; ++s) {
-        const uint32_t g = it + s, st = g % F::STAGES, round = g / F::STAGES;
-        if (round > 0) ok = __all_sync(FULL_MASK, t5_mbar_wait(&empty[st], (round - 1) & 1, failed));
-        if (!ok) break;
+      for (uint32_t g = stage0; g < stage0 + walk.all_stages() && ok; ++g, ring.next()) {
+        const uint32_t st = ring.st;
         const int64_t c0 = pass.c_lo + (int64_t)c * AT_COLS;
         const int head = KV ? head0 + (int)e : group;
+        // what the columns bring beside the operands is on its way while the stage is waited for
+        float place[DIM == 0 ? 1 : 2 * DIM], col_lse[2], col_delta[2];
+        at_fetch_places<DIM>(place, KV ? p.pos_q : p.pos_k, p.dims, c0, pass.c_hi, lane);
+        if constexpr (KV) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const bool there = c0 + n * 32 + lane < pass.c_hi;
+            const int64_t at = (int64_t)head * p.m + c0 + n * 32 + lane;
+            col_lse[n] = there ? a.lse[at] - A::SHIFT : pos_inf<float>();
+            col_delta[n] = there ? a.delta[at] : 0.f;
+          }
+        }
+        // the stage's round before this one is through
+        if (g >= F::STAGES) ok = t5_mbar_wait_warp(&empty[st], ring.parity ^ 1u, failed);
+        if (!ok) break;
         unsigned char *dst = stages + st * F::STAGE_BYTES;
         if (lane == 0) {
           t5_mbar_expect(&full[st], F::STAGE_BYTES);
@@ -161,130 +185,131 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           }
         }
         float *sd = side + st * F::SIDE_FLOATS;
-        if constexpr (DIM > 0) {
-          const float *src = KV ? p.pos_q : p.pos_k;
-          for (int i = lane; i < AT_COLS * DIM; i += 32) {
-            const int j = i / DIM, d = i - j * DIM;
-            sd[d * AT_COLS + j] = c0 + j < pass.c_hi && d < p.dims ? src[(c0 + j) * p.dims + d] : 0.f;
-          }
-        }
+        at_put_places<DIM>(sd, place, lane);
         if constexpr (KV) {
-          for (int j = lane; j < AT_COLS; j += 32) {
-            const bool there = c0 + j < pass.c_hi;
-            sd[AT_MAX_DIMS * AT_COLS + j] = there ? a.lse[(int64_t)head * p.m + c0 + j] - A::SHIFT : pos_inf<float>();
-            sd[(AT_MAX_DIMS + 1) * AT_COLS + j] = there ? a.delta[(int64_t)head * p.m + c0 + j] : 0.f;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            sd[AT_MAX_DIMS * AT_COLS + n * 32 + lane] = col_lse[n];
+            sd[(AT_MAX_DIMS + 1) * AT_COLS + n * 32 + lane] = col_delta[n];
           }
         }
         __syncwarp();
         if (lane == 0) t5_mbar_arrive(&full[st]);
         issued = g + 1;
-        if (++c == each) {
+        if (++c == walk.stages) {
           c = 0;
           ++e;
         }
       }
-    } else if (warp == F::EL_WARPS + 1) {
-      // ---- products
-      const uint32_t id_s = t5_idesc(A::BF16, AT_COLS, false), id_a = t5_idesc(A::BF16, CP, true);
-      constexpr uint32_t LAG = F::NB - 1;
-      for (uint32_t s = 0; s < steps + LAG && steps > 0 && ok; ++s) {
-        if (s < steps) {
-          const uint32_t g = it + s, st = g % F::STAGES, nb = g % F::NB;
-          ok = __all_sync(FULL_MASK, t5_mbar_wait(&full[st], (g / F::STAGES) & 1, failed));
-          // the accumulators hold the weights of NB steps ago: products of different accumulators are not ordered
-          if (ok && s >= F::NB) {
-            const uint32_t b = g - F::NB;
-            ok = __all_sync(FULL_MASK, t5_mbar_wait(&empty[b % F::STAGES], (b / F::STAGES) & 1, failed));
-          }
+    } else if (warp == PRODUCT) {
+      // ---- products: the scores of step i + G, then the second products of step i
+      const uint32_t id_s = t5_idesc(A::BF16, AT_SUB, false), id_a = t5_idesc(A::BF16, CP, true);
+      const uint64_t d_r0 = t5_desc(t5_smem(rows0)), d_r1 = t5_desc(t5_smem(rows1)), d_c0 = t5_desc(t5_smem(stages)),
+                     d_c1 = t5_desc(t5_smem(stages + F::TILE_BYTES)),
+                     d_m0 = t5_desc(t5_smem(stages), AT_COLS * 128),
+                     d_m1 = t5_desc(t5_smem(stages + F::TILE_BYTES), AT_COLS * 128);
+      const uint32_t total = walk.all_steps();
+      AtRing<F::STAGES> ring_s(stage0), ring_a(stage0);
+      AtAt at_s, at_a;
+      uint32_t js = 0;  // steps whose scores were issued
+      for (uint32_t ja = 0; ja < total && ok; ++ja) {
+        for (; js < total && js <= ja + G && ok; ++js) {
+          const uint32_t i = step0 + js, gr = i % G, k = i / G;
+          if (at_s.half() == 0) ok = t5_mbar_wait_warp(&full[ring_s.st], ring_s.parity, failed);
+          if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[gr], (k - 1) & 1, failed);
           if (!ok) break;
           t5_fence_after();
-          if (lane == 0) {
-            const uint32_t c0 = t5_smem(stages + st * F::STAGE_BYTES), c1 = c0 + F::TILE_BYTES;
+          const uint32_t off = (ring_s.st * F::STAGE_BYTES + at_s.half() * (AT_SUB * 128)) / 16;
+          const uint32_t t_s = tmem + gr * F::GROUP_COLS;
+          if (t5_elect()) {
 #pragma unroll
-            for (int ks = 0; ks < CP / 16; ++ks) {
-              const uint32_t ro = (ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32, co = (ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32;
-              t5_mma_ss(tmem + nb * 2 * AT_COLS, t5_desc(t5_smem(rows0) + ro), t5_desc(c0 + co), id_s, ks > 0);
-            }
+          for (int ks = 0; ks < CP / 16; ++ks)
+            t5_mma_ss(t_s, d_r0 + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
+                      d_c0 + off + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
 #pragma unroll
-            for (int ks = 0; ks < CP / 16; ++ks) {
-              const uint32_t ro = (ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32, co = (ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32;
-              t5_mma_ss(tmem + nb * 2 * AT_COLS + AT_COLS, t5_desc(t5_smem(rows1) + ro), t5_desc(c1 + co), id_s, ks > 0);
-            }
-            t5_commit(&s_full[nb]);
+          for (int ks = 0; ks < CP / 16; ++ks)
+            t5_mma_ss(t_s + AT_SUB, d_r1 + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
+                      d_c1 + off + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
+          t5_commit(&s_full[gr]);
           }
           __syncwarp();
+          if (at_s.last_of_stage(walk)) ring_s.next();
+          at_s.move(walk, 1);
         }
-        if (s >= LAG) {
-          const uint32_t g = it + s - LAG, st = g % F::STAGES, nb = g % F::NB;
-          ok = __all_sync(FULL_MASK, t5_mbar_wait(&w_ready[nb], (g / F::NB) & 1, failed));
-          if (!ok) break;
-          t5_fence_after();
-          if (lane == 0) {
-            const uint32_t c0 = t5_smem(stages + st * F::STAGE_BYTES), c1 = c0 + F::TILE_BYTES;
-            const uint32_t w = tmem + nb * 2 * AT_COLS;
-            const bool more = s > LAG;
+        if (!ok) break;
+        const uint32_t i = step0 + ja, gr = i % G, k = i / G;
+        ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
+        if (!ok) break;
+        t5_fence_after();
+        const uint32_t off = (ring_a.st * F::STAGE_BYTES + at_a.half() * (AT_SUB * 128)) / 16;
+        const uint32_t w = tmem + gr * F::GROUP_COLS + 2 * AT_SUB;
+        const bool last = at_a.last_of_stage(walk);
+        if (t5_elect()) {
 #pragma unroll
-            for (int ks = 0; ks < AT_COLS / 16; ++ks) {
-              const uint32_t wo = (ks >> 1) * 32 + (ks & 1) * 8;
-              if constexpr (KV) {
-                t5_mma_ts(t_acc, w + wo, t5_desc(c1 + ks * 2048, AT_COLS * 128), id_a, more || ks > 0);
-                t5_mma_ts(t_acc + CP, w + AT_COLS + wo, t5_desc(c0 + ks * 2048, AT_COLS * 128), id_a, more || ks > 0);
-              } else {
-                t5_mma_ts(t_acc, w + AT_COLS + wo, t5_desc(c0 + ks * 2048, AT_COLS * 128), id_a, more || ks > 0);
-              }
-            }
-            t5_commit(&empty[st]);
-            if (s == steps + LAG - 1) t5_commit(&done);
-          }
-          __syncwarp();
+        for (int ks = 0; ks < AT_SUB / 16; ++ks) {
+          if constexpr (KV)
+            t5_mma_ts(t_acc, w + AT_SUB / 2 + ks * 8, d_m1 + off + ks * (2048 / 16), id_a, ja > 0 || ks > 0);
+          t5_mma_ts(t_acc + (KV ? CP : 0), w + ks * 8, d_m0 + off + ks * (2048 / 16), id_a, ja > 0 || ks > 0);
         }
+        t5_commit(&a_done[gr]);
+        if (last) t5_commit(&empty[ring_a.st]);
+        if (ja + 1 == total) t5_commit(&done);
+        }
+        __syncwarp();
+        if (last) ring_a.next();
+        at_a.move(walk, 1);
       }
     } else {
       // ---- elements
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t t_s = tmem + grp * F::GROUP_COLS + lane_base, t_w = t_s + 2 * AT_SUB;
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
       const int64_t lo64 = mine ? row_lo - pass.c_lo : 0, hi64 = mine ? row_hi - pass.c_lo : 0;
       const int lo = (int)(lo64 < 0 ? 0 : lo64 > count ? count : lo64), hi = (int)(hi64 < 0 ? 0 : hi64 > count ? count : hi64);
-      uint32_t bad = 0u, e = 0, c = 0;
-      for (uint32_t s = 0; s < steps && ok; ++s) {
-        const uint32_t g = it + s, st = g % F::STAGES, nb = g % F::NB;
-        const int step_base = (int)(c * AT_COLS), base = step_base + half * 32;
-        const bool last = step_base + AT_COLS > (int)count;
-        unsigned char *stage = stages + st * F::STAGE_BYTES;
-        const float *sd = side + st * F::SIDE_FLOATS + half * 32;
+      const bool scan = mixed && !by_example;
+      uint32_t bad = 0u;
+      AtAt at;
+      const uint32_t j0 = (grp + G - step0 % G) % G, total = walk.all_steps();  // the group's first step
+      at.move(walk, j0);
+      for (uint32_t j = j0; j < total && ok; j += G, at.move(walk, G)) {
+        const uint32_t g = stage0 + at.stage(walk), st = g % F::STAGES, k = (step0 + j) / G;
+        const int base = at.base();
+        const bool tail = base + AT_SUB > (int)count;
+        unsigned char *stage = stages + st * F::STAGE_BYTES + at.half() * (AT_SUB * 128);
+        const float *sd = side + st * F::SIDE_FLOATS + at.half() * AT_SUB;
         float slope2 = 0.f;
-        if constexpr (DIM > 0) slope2 = __ldg(p.slope + head0 + e) * AT_LOG2E;
-        ok = __all_sync(FULL_MASK, t5_mbar_wait(&full[st], (g / F::STAGES) & 1, failed));
-        if (mixed && !by_example && ok) {
-          bad |= at_scan<T, CP>(stage, tid, F::EL_THREADS);
-          if constexpr (KV) bad |= at_scan<T, CP>(stage + F::TILE_BYTES, tid, F::EL_THREADS);
+        if constexpr (DIM > 0) slope2 = __ldg(p.slope + head0 + at.e) * AT_LOG2E;
+        ok = t5_mbar_wait_warp(&full[st], (g / F::STAGES) & 1, failed);
+        if (scan && ok) {
+          bad |= at_scan<T, CP>(stage, lrow);
+          if constexpr (KV) bad |= at_scan<T, CP>(stage + F::TILE_BYTES, lrow);
         }
-        if (ok) ok = __all_sync(FULL_MASK, t5_mbar_wait(&s_full[nb], (g / F::NB) & 1, failed));
+        if (ok) ok = t5_mbar_wait_warp(&s_full[grp], k & 1, failed);
         if (!ok) break;
         t5_fence_after();
-        const uint32_t t_s = tmem + nb * 2 * AT_COLS + half * 32 + lane_base, t_dp = t_s + AT_COLS;
-        uint32_t w[16], wp[KV ? 16 : 1];
-        const bool any = __any_sync(FULL_MASK, hi > base && lo < base + 32 && lo < hi);
+        uint32_t w[AT_SUB / 2], wp[KV ? AT_SUB / 2 : 1];
+        const bool any = __any_sync(FULL_MASK, hi > base && lo < base + AT_SUB && lo < hi);
         if (any) {
-          float x[32], dp[32], u[CAP ? 32 : 1];
+          float x[AT_SUB], dp[AT_SUB], u[CAP ? AT_SUB : 1];
           t5_ld32(t_s, x);
-          t5_ld32(t_dp, dp);
+          t5_ld32(t_s + AT_SUB, dp);
           t5_wait_ld32(x);
           t5_wait_ld32(dp);
-          at_logits<DIM, CAP, CAP>(x, u, sd, pos, slope2, pre, post);
-          const bool whole = __all_sync(FULL_MASK, lo <= base && hi >= base + 32);
+          t5_fence_before();
+          __syncwarp();
+          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
+          at_logits<DIM, CAP, CAP, KV>(x, u, sd, pos, slope2, pre, post, lse, sd + AT_MAX_DIMS * AT_COLS);
+          const bool whole = __all_sync(FULL_MASK, lo <= base && hi >= base + AT_SUB);
 #pragma unroll
-          for (int j4 = 0; j4 < 32; j4 += 4) {
-            float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta};
+          for (int j4 = 0; j4 < AT_SUB; j4 += 4) {
+            float de[4] = {delta, delta, delta, delta};
             if constexpr (KV) {
-              const float4 l4 = *reinterpret_cast<const float4 *>(sd + AT_MAX_DIMS * AT_COLS + j4);
               const float4 d4 = *reinterpret_cast<const float4 *>(sd + (AT_MAX_DIMS + 1) * AT_COLS + j4);
-              ls[0] = l4.x, ls[1] = l4.y, ls[2] = l4.z, ls[3] = l4.w;
               de[0] = d4.x, de[1] = d4.y, de[2] = d4.z, de[3] = d4.w;
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float pr = t5_ex2(x[j4 + j] - ls[j]);
+              const float pr = t5_ex2(x[j4 + j]);
               float ds = pr * (dp[j4 + j] - de[j]);
               if constexpr (CAP) ds *= fmaf(-u[j4 + j], u[j4 + j], 1.f);
               if constexpr (!A::BF16) ds *= sig;
@@ -294,70 +319,66 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           }
           if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < AT_SUB; ++j)
               if (base + j < lo || base + j >= hi) x[j] = dp[j] = 0.f;
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < AT_SUB / 2; ++j) {
             w[j] = A::pack(dp[2 * j], dp[2 * j + 1]);
             if constexpr (KV) wp[j] = A::pack(x[2 * j], x[2 * j + 1]);
           }
         } else {
+          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < AT_SUB / 2; ++j) {
             w[j] = 0u;
             if constexpr (KV) wp[j] = 0u;
           }
         }
-        t5_st16(t_dp, w);
-        if constexpr (KV) t5_st16(t_s, wp);
+        // the weights of the group's step before have been taken
+        if (j >= G) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
+        if (!ok) break;
+        t5_fence_after();
+        t5_st16(t_w, w);
+        if constexpr (KV) t5_st16(t_w + AT_SUB / 2, wp);
         t5_wait_st();
-        if (last) {
-          at_clear<CP>(stage, (int)count - step_base, tid, F::EL_THREADS);
-          if constexpr (KV) at_clear<CP>(stage + F::TILE_BYTES, (int)count - step_base, tid, F::EL_THREADS);
+        if (tail) {
+          at_clear<CP>(stage, (int)count - base, lrow);
+          if constexpr (KV) at_clear<CP>(stage + F::TILE_BYTES, (int)count - base, lrow);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         t5_fence_before();
-        t5_mbar_arrive(&w_ready[nb]);
-        if (++c == each) {
-          c = 0;
-          ++e;
-        }
+        __syncwarp();
+        if (lane == 0) t5_mbar_arrive(&w_ready[grp]);
       }
-      if (ok && steps > 0) {
-        ok = __all_sync(FULL_MASK, t5_mbar_wait(&done, passes & 1, failed));
+      if (ok && count > 0) {
+        ok = t5_mbar_wait_warp(&done, passes & 1, failed);
         t5_fence_after();
       }
       if (bad) bad_s = 1;
-      const bool redo = mixed && !by_example;
-      if (redo) asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (!(redo && *(volatile int *)&bad_s)) {
+      if (scan) asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
+      if (!(scan && *(volatile int *)&bad_s)) {
         const bool store = mine && row < tile.t1;
         const float nan = __int_as_float(0x7fffffff);
-        // the first half of the warps takes dv (or the first channels of dq), the second dk (or the others)
-        T *dst;
-        float times;
-        int c_first, c_count;
-        if constexpr (KV) {
-          dst = (half == 0 ? (T *)a.dv : (T *)a.dk) + (row * p.groups + group) * p.channels;
-          times = half == 0 ? (A::BF16 ? 1.f : 1.f / 4096.f) : p.scale / sigma;
-          c_first = 0;
-          c_count = CP;
-        } else {
-          dst = (T *)a.dq + (row * p.heads + head0) * p.channels;
-          times = p.scale / sigma;
-          c_first = half * (CP / 2);
-          c_count = CP / 2;
-        }
-        if (!ok) times = nan;
-        for (int cc = c_first; cc < c_first + c_count; cc += 32) {
-          float o[32];
-          if (steps > 0 && ok) {
-            t5_ld32(t_acc + (KV && half ? CP : 0) + lane_base + cc, o);
-            t5_wait_ld32(o);
+        // the results' channels in chunks of 32, dealt out to the groups
+        constexpr int CHUNKS = (KV ? 2 : 1) * CP / 32;
+#pragma unroll 1
+        for (int ch = grp; ch < CHUNKS; ch += G) {
+          const int c = ch * 32 % CP;
+          const bool is_dv = KV && ch * 32 < CP;
+          T *dst;
+          float times = p.scale / sigma;
+          if constexpr (KV) {
+            dst = (is_dv ? (T *)a.dv : (T *)a.dk) + (row * p.groups + group) * p.channels;
+            if (is_dv) times = A::BF16 ? 1.f : 1.f / 4096.f;
           } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            dst = (T *)a.dq + (row * p.heads + head0) * p.channels;
+          }
+          if (!ok) times = nan;
+          float o[32] = {};
+          if (count > 0 && ok) {
+            t5_ld32(t_acc + lane_base + ch * 32, o);
+            t5_wait_ld32(o);
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -365,13 +386,14 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
             uint32_t *po = reinterpret_cast<uint32_t *>(&out);
 #pragma unroll
             for (int k = 0; k < 4; ++k) po[k] = A::pack(o[i + 2 * k] * times, o[i + 2 * k + 1] * times);
-            if (store && cc + i < p.channels) *reinterpret_cast<uint4 *>(dst + cc + i) = out;
+            if (store && c + i < p.channels) *reinterpret_cast<uint4 *>(dst + c + i) = out;
           }
         }
       }
     }
-    it += steps;
-    if (steps > 0) ++passes;
+    step0 += walk.all_steps();
+    stage0 += walk.all_stages();
+    if (count > 0) ++passes;
     t5_fence_before();
     __syncthreads();
     t5_fence_after();
@@ -382,7 +404,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
     }
     if (!tile.next(next_row, pass)) break;
   }
-  if (*failed && element && row < tile.t1 && half == 0) {
+  if (*failed && element && row < tile.t1 && grp == 0) {
     // a wait ran out: nothing of this block is to be trusted
     for (int c = 0; c < p.channels; ++c) {
       const T nan = at_round<T>(__int_as_float(0x7fffffff));
@@ -394,17 +416,17 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
       }
     }
   }
-  if (*failed && warp == F::EL_WARPS) {
+  if (*failed && warp == COPY) {
     at_drain(&r_full, 1, 1);
     at_drain(full, F::STAGES, issued);
   }
-  if (*failed && warp == F::EL_WARPS + 1) {
-    if (lane == 0) t5_commit(&drained);
+  if (*failed && warp == PRODUCT) {
+    if (t5_elect()) t5_commit(&drained);
     __syncwarp();
     at_drain(&drained, 1, 1);
   }
   __syncthreads();
-  if (warp == F::EL_WARPS) t5_dealloc(tmem, F::TMEM);
+  if (warp == COPY) t5_dealloc(tmem, F::TMEM);
 }
 
 }  // namespace b200c

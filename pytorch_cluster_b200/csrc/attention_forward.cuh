@@ -1,9 +1,9 @@
 // Forward attention on the tensor cores: 128 queries of one head per block, see attention_tensor.cuh.
 //
-// Two score accumulators, so that the product of the next step's scores runs while this step's softmax does; the weights
-// go back into the accumulator they came from.  The running maximum is only raised (and the result in tensor memory
-// rescaled) when a row's maximum rises by more than 8 powers of two: until then weights up to 2^8 are exact enough in
-// either type, and the rescaling, a round trip through tensor memory, is rare.
+// Each group of warps has its own running maximum, sum and result of its steps; they are joined at the end.  The maximum
+// is not looked for in every step: weights are formed against the one in use, and only where their sum over the step's 32
+// columns passes 2^10 (or no maximum is known yet) is it raised to the step's and the result in tensor memory, the sum
+// and the step's weights brought to it.  Weights up to 2^10 are as exact in either type as weights up to 1.
 // Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.
 #pragma once
 
@@ -13,14 +13,19 @@ namespace b200c {
 
 template <int CP>
 struct AtForward {
-  static constexpr int STAGES = CP == 64 ? 3 : 2;
-  static constexpr int THREADS = 192;  // 4 softmax warps, 1 copy warp, 1 product warp
+  static constexpr int G = 2;
+  static constexpr int BLOCKS = CP == 64 ? 2 : 1;  // resident blocks per SM: tensor memory
+  static constexpr int STAGES = CP == 64 ? 3 : 4;
+  static constexpr int EL_WARPS = 4 * G, EL_THREADS = 32 * EL_WARPS;
+  static constexpr int THREADS = EL_THREADS + 64;  // the groups, a copy warp, a product warp
   static constexpr int Q_BYTES = AT_ROWS * CP * 2, TILE_BYTES = AT_COLS * CP * 2;
   static constexpr int POS_BYTES = AT_MAX_DIMS * AT_COLS * 4;
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
   static constexpr int SMEM = Q_BYTES + STAGES * (STAGE_BYTES + POS_BYTES) + 1024;
-  static constexpr int TMEM = 256;
-  static constexpr float RAISE = 8.f;
+  static constexpr int GROUP_COLS = AT_SUB + AT_SUB / 2;  // scores, weights
+  static constexpr int TMEM = CP == 64 ? 256 : 512;
+  static_assert(G * (GROUP_COLS + CP) <= TMEM, "tensor memory");
+  static constexpr float MOST = 1024.f;  // sum of a step's weights that needs no new maximum
 };
 
 struct AtForwardMaps {
@@ -28,59 +33,79 @@ struct AtForwardMaps {
 };
 
 template <typename T, int CP, int DIM, bool CAP>
-__global__ void __launch_bounds__(AtForward<CP>::THREADS, 2)
+__global__ void __launch_bounds__(AtForward<CP>::THREADS, AtForward<CP>::BLOCKS)
 attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __grid_constant__ AttnArgs a,
                          T *__restrict__ rest) {
   using F = AtForward<CP>;
   using A = AtType<T>;
-  constexpr int ATOMS = CP / 64;
+  constexpr int ATOMS = CP / 64, G = F::G, COPY = F::EL_WARPS, PRODUCT = F::EL_WARPS + 1;
   extern __shared__ unsigned char at_raw[];
   unsigned char *smem = at_raw + ((1024u - (t5_smem(at_raw) & 1023u)) & 1023u);
   unsigned char *sq = smem;
   unsigned char *stages = smem + F::Q_BYTES;
   float *spos = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[2], p_ready[2], o_done, done, drained;
+  // s_full / s_free: a group's scores are in / have been read; w_ready: its weights are in; a_done: its second product is
+  __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[G], s_free[G], w_ready[G],
+      a_done[G], done, drained;
   __shared__ uint32_t tmem_s;
   __shared__ int failed_s, bad_s;
+  __shared__ AtTileShared shared_tile;
+  __shared__ float s_top[G][AT_ROWS], s_sum[G][AT_ROWS];
   volatile int *failed = &failed_s;
 
   const b200c_attention_t &p = a.p;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = t5_warp(), lane = tid & 31;
   const int head = blockIdx.y, group = head / (p.heads / p.groups);
   AtTile tile;
   tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
 
-  if (tid == 0) {
+  if (tid == 64) {
     t5_mbar_init(&q_full, 1);
     for (int i = 0; i < F::STAGES; ++i) {
       t5_mbar_init(&full[i], 1);
       t5_mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < G; ++i) {
       t5_mbar_init(&s_full[i], 1);
-      t5_mbar_init(&p_ready[i], AT_ROWS);
+      t5_mbar_init(&s_free[i], 4);
+      t5_mbar_init(&w_ready[i], 4);
+      t5_mbar_init(&a_done[i], 1);
     }
-    t5_mbar_init(&o_done, 1);
     t5_mbar_init(&done, 1);
     t5_mbar_init(&drained, 1);
     failed_s = 0;
     bad_s = 0;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 4) t5_alloc(&tmem_s, F::TMEM);
+  if (warp == COPY) t5_alloc(&tmem_s, F::TMEM);
+  tile.search(shared_tile, warp, lane);
   t5_fence_before();
   __syncthreads();
   t5_fence_after();
   const uint32_t tmem = tmem_s;
-  const uint32_t t_o = tmem + 2 * AT_COLS;
+  const uint32_t t_o = tmem + G * F::GROUP_COLS;  // G results
+  // the copy warp: the queries once
+  if (warp == COPY && lane == 0) {
+    t5_mbar_expect(&q_full, F::Q_BYTES);
+    for (int at = 0; at < ATOMS; ++at)
+      t5_tma_3d(sq + at * (AT_ROWS * 128), &maps.q, at * 64, head, (int)tile.t0, &q_full);
+    t5_mbar_arrive(&q_full);
+  }
+  tile.found(shared_tile);
+  if (tile.listed()) {
+    if (tid <= tile.b_last - tile.b_first) shared_tile.ends[tid] = tile.ptr_r[tile.b_first + 1 + tid];
+    __syncthreads();
+  }
 
-  // softmax threads: a row each
-  const int64_t row = tile.t0 + tid;
+  // element threads: a row each
+  const bool element = warp < F::EL_WARPS;
+  const int grp = warp >> 2, lrow = tid & (AT_ROWS - 1);
+  const int64_t row = tile.t0 + lrow;
   int64_t row_lo = 0, row_hi = 0;  // the columns it sees
   int row_segment = -1;
   float pos[DIM == 0 ? 1 : DIM], slope2 = 0.f;
-  if (warp < 4 && row < tile.t1) {
-    row_segment = segment_of(tile.ptr_r, tile.segments, row);
+  if (element && row < tile.t1) {
+    row_segment = tile.segment(shared_tile, row);
     int64_t lo, hi;
     at_segment(tile.ptr_r, p.m, row_segment, lo, hi);
     if (row >= lo && row < hi) at_segment(tile.ptr_c, p.n, row_segment, row_lo, row_hi);
@@ -88,38 +113,35 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   if constexpr (DIM > 0) {
     slope2 = p.slope[head] * AT_LOG2E;
 #pragma unroll
-    for (int d = 0; d < DIM; ++d) pos[d] = warp < 4 && row < tile.t1 && d < p.dims ? p.pos_q[row * p.dims + d] : 0.f;
+    for (int d = 0; d < DIM; ++d) pos[d] = element && row < tile.t1 && d < p.dims ? p.pos_q[row * p.dims + d] : 0.f;
   }
   const float pre = CAP ? 2.f * AT_LOG2E * p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
-
-  // the copy warp: the queries once
-  if (warp == 4 && lane == 0) {
-    t5_mbar_expect(&q_full, F::Q_BYTES);
-    for (int at = 0; at < ATOMS; ++at)
-      t5_tma_3d(sq + at * (AT_ROWS * 128), &maps.q, at * 64, head, (int)tile.t0, &q_full);
-    t5_mbar_arrive(&q_full);
-  }
 
   bool by_example = false;
   int64_t next_row = tile.t0;
   AtPass pass = tile.all();
   const bool mixed = tile.b_first != tile.b_last;
-  uint32_t it = 0;      // steps so far, over all passes
-  uint32_t passes = 0;  // passes with steps
-  uint32_t issued = 0;  // copy warp: steps whose copies were issued
+  uint32_t step0 = 0, stage0 = 0, passes = 0;  // steps, stages and passes with steps so far
+  uint32_t issued = 0;                         // copy warp: stages whose copies were issued
   bool ok = true;
-  if (warp == 5) ok = __all_sync(FULL_MASK, t5_mbar_wait(&q_full, 0, failed));
+  if (warp == PRODUCT) ok = t5_mbar_wait_warp(&q_full, 0, failed);
 
   for (;;) {
     const int64_t count = pass.c_hi - pass.c_lo;
-    const uint32_t steps = (uint32_t)((count + AT_COLS - 1) / AT_COLS);
-    if (warp == 4) {
+    const AtWalk walk(count, 1);
+    if (warp == COPY) {
       // ---- copies
-      for (uint32_t s = 0; s < steps && ok; ++s) {
-        const uint32_t g = it + s, st = g % F::STAGES, round = g / F::STAGES;
-        if (round > 0) ok = __all_sync(FULL_MASK, t5_mbar_wait(&empty[st], (round - 1) & 1, failed));
+      AtRing<F::STAGES> ring(stage0);
+      uint32_t c = 0;
+      for (uint32_t g = stage0; g < stage0 + walk.all_stages() && ok; ++g, ring.next()) {
+        const uint32_t st = ring.st;
+        const int64_t c0 = pass.c_lo + (int64_t)c * AT_COLS;
+        // the columns' coordinates are on their way while the stage is waited for
+        float place[DIM == 0 ? 1 : 2 * DIM];
+        at_fetch_places<DIM>(place, p.pos_k, p.dims, c0, pass.c_hi, lane);
+        // the stage's round before this one is through
+        if (g >= F::STAGES) ok = t5_mbar_wait_warp(&empty[st], ring.parity ^ 1u, failed);
         if (!ok) break;
-        const int64_t c0 = pass.c_lo + (int64_t)s * AT_COLS;
         unsigned char *dst = stages + st * F::STAGE_BYTES;
         if (lane == 0) {
           t5_mbar_expect(&full[st], F::STAGE_BYTES);
@@ -129,169 +151,206 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           }
         }
         if constexpr (DIM > 0) {
-          float *sp = spos + st * (AT_MAX_DIMS * AT_COLS);
-          for (int i = lane; i < AT_COLS * DIM; i += 32) {
-            const int c = i / DIM, d = i - c * DIM;
-            sp[d * AT_COLS + c] = c0 + c < pass.c_hi && d < p.dims ? p.pos_k[(c0 + c) * p.dims + d] : 0.f;
-          }
+          at_put_places<DIM>(spos + st * (AT_MAX_DIMS * AT_COLS), place, lane);
           __syncwarp();
         }
         if (lane == 0) t5_mbar_arrive(&full[st]);
         issued = g + 1;
+        ++c;
       }
-    } else if (warp == 5) {
-      // ---- products
-      const uint32_t id_s = t5_idesc(A::BF16, AT_COLS, false), id_o = t5_idesc(A::BF16, CP, true);
-      for (uint32_t s = 0; s <= steps && steps > 0 && ok; ++s) {
-        if (s < steps) {
-          const uint32_t g = it + s, st = g % F::STAGES;
-          ok = __all_sync(FULL_MASK, t5_mbar_wait(&full[st], (g / F::STAGES) & 1, failed));
-          // the accumulator holds the weights of two steps ago: products of different accumulators are not ordered
-          if (ok && s > 1) ok = __all_sync(FULL_MASK, t5_mbar_wait(&o_done, (g - 2) & 1, failed));
+    } else if (warp == PRODUCT) {
+      // ---- products: the scores of step i + G, then the second product of step i
+      const uint32_t id_s = t5_idesc(A::BF16, AT_SUB, false), id_o = t5_idesc(A::BF16, CP, true);
+      const uint64_t d_q = t5_desc(t5_smem(sq)), d_k = t5_desc(t5_smem(stages)),
+                     d_v = t5_desc(t5_smem(stages + F::TILE_BYTES), AT_COLS * 128);
+      const uint32_t total = walk.all_steps();
+      AtRing<F::STAGES> ring_s(stage0), ring_o(stage0);
+      AtAt at_s, at_o;
+      uint32_t js = 0;  // steps whose scores were issued
+      for (uint32_t jo = 0; jo < total && ok; ++jo) {
+        for (; js < total && js <= jo + G && ok; ++js) {
+          const uint32_t i = step0 + js, gr = i % G, k = i / G;
+          if (at_s.half() == 0) ok = t5_mbar_wait_warp(&full[ring_s.st], ring_s.parity, failed);
+          if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[gr], (k - 1) & 1, failed);
           if (!ok) break;
           t5_fence_after();
-          if (lane == 0) {
-            const uint32_t sk = t5_smem(stages + st * F::STAGE_BYTES);
+          const uint64_t d = d_k + (ring_s.st * F::STAGE_BYTES + at_s.half() * (AT_SUB * 128)) / 16;
+          if (t5_elect()) {
 #pragma unroll
-            for (int ks = 0; ks < CP / 16; ++ks) {
-              const uint64_t da = t5_desc(t5_smem(sq) + (ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32);
-              const uint64_t db = t5_desc(sk + (ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32);
-              t5_mma_ss(tmem + (g & 1) * AT_COLS, da, db, id_s, ks > 0);
-            }
-            t5_commit(&s_full[g & 1]);
+          for (int ks = 0; ks < CP / 16; ++ks)
+            t5_mma_ss(tmem + gr * F::GROUP_COLS, d_q + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
+                      d + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
+          t5_commit(&s_full[gr]);
           }
           __syncwarp();
+          if (at_s.last_of_stage(walk)) ring_s.next();
+          at_s.move(walk, 1);
         }
-        if (s > 0) {
-          const uint32_t g = it + s - 1, st = g % F::STAGES;
-          ok = __all_sync(FULL_MASK, t5_mbar_wait(&p_ready[g & 1], (g >> 1) & 1, failed));
-          if (!ok) break;
-          t5_fence_after();
-          if (lane == 0) {
-            const uint32_t sv = t5_smem(stages + st * F::STAGE_BYTES + F::TILE_BYTES);
+        if (!ok) break;
+        const uint32_t i = step0 + jo, gr = i % G, k = i / G;
+        ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
+        if (!ok) break;
+        t5_fence_after();
+        const uint64_t d = d_v + (ring_o.st * F::STAGE_BYTES + at_o.half() * (AT_SUB * 128)) / 16;
+        const bool last = at_o.last_of_stage(walk);
+        if (t5_elect()) {
 #pragma unroll
-            for (int ks = 0; ks < AT_COLS / 16; ++ks)
-              t5_mma_ts(t_o, tmem + (g & 1) * AT_COLS + ks * 8, t5_desc(sv + ks * 2048, AT_COLS * 128), id_o,
-                        s > 1 || ks > 0);
-            t5_commit(&empty[st]);
-            t5_commit(&o_done);
-            if (s == steps) t5_commit(&done);
-          }
-          __syncwarp();
+        for (int ks = 0; ks < AT_SUB / 16; ++ks)
+          t5_mma_ts(t_o + gr * CP, tmem + gr * F::GROUP_COLS + AT_SUB + ks * 8, d + ks * (2048 / 16), id_o,
+                    jo >= G || ks > 0);
+        t5_commit(&a_done[gr]);
+        if (last) t5_commit(&empty[ring_o.st]);
+        if (jo + 1 == total) t5_commit(&done);
         }
+        __syncwarp();
+        if (last) ring_o.next();
+        at_o.move(walk, 1);
       }
     } else {
       // ---- softmax
-      const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+      const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t t_s = tmem + grp * F::GROUP_COLS + lane_base, t_p = t_s + AT_SUB, t_r = t_o + grp * CP + lane_base;
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
-      // the row's columns relative to the pass's first; 64 columns fit an int many times over
+      // the row's columns relative to the pass's first
       const int64_t lo64 = mine ? row_lo - pass.c_lo : 0, hi64 = mine ? row_hi - pass.c_lo : 0;
       const int lo = (int)(lo64 < 0 ? 0 : lo64 > count ? count : lo64), hi = (int)(hi64 < 0 ? 0 : hi64 > count ? count : hi64);
-      float top = -pos_inf<float>(), sum = 0.f;
+      const bool scan = mixed && !by_example;
+      float top = -pos_inf<float>(), sub = 0.f, sum = 0.f;  // sub: what the scores are taken relative to
       uint32_t bad = 0u;
-      for (uint32_t s = 0; s < steps && ok; ++s) {
-        const uint32_t g = it + s, st = g % F::STAGES;
-        const int base = (int)(s * AT_COLS);
-        const bool last = base + AT_COLS > (int)count;
-        if (DIM > 0 || mixed || last)
-          ok = __all_sync(FULL_MASK, t5_mbar_wait(&full[st], (g / F::STAGES) & 1, failed));
-        if (mixed && !by_example && ok)
-          bad |= at_scan<T, CP>(stages + st * F::STAGE_BYTES + F::TILE_BYTES, tid, AT_ROWS);
-        if (ok) ok = __all_sync(FULL_MASK, t5_mbar_wait(&s_full[g & 1], (g >> 1) & 1, failed));
+      AtAt at;
+      const uint32_t j0 = (grp + G - step0 % G) % G, total = walk.all_steps();  // the group's first step
+      at.move(walk, j0);
+      for (uint32_t j = j0; j < total && ok; j += G, at.move(walk, G)) {
+        const uint32_t g = stage0 + at.stage(walk), st = g % F::STAGES, k = (step0 + j) / G;
+        const int base = at.base();
+        const bool tail = base + AT_SUB > (int)count, first = j < G;
+        unsigned char *values = stages + st * F::STAGE_BYTES + F::TILE_BYTES + at.half() * (AT_SUB * 128);
+        if (DIM > 0 || scan || tail)
+          ok = t5_mbar_wait_warp(&full[st], (g / F::STAGES) & 1, failed);
+        if (scan && ok) bad |= at_scan<T, CP>(values, lrow);
+        if (ok) ok = t5_mbar_wait_warp(&s_full[grp], k & 1, failed);
         if (!ok) break;
         t5_fence_after();
-        const uint32_t t_s = tmem + (g & 1) * AT_COLS + lane_base;
-        uint32_t w[32];
-        const bool any = __any_sync(FULL_MASK, hi > base && lo < base + AT_COLS && lo < hi);
+        uint32_t w[AT_SUB / 2];
+        const bool any = __any_sync(FULL_MASK, hi > base && lo < base + AT_SUB && lo < hi);
         if (any) {
-          float x[AT_COLS];
+          float x[AT_SUB];
           t5_ld32(t_s, x);
-          t5_ld32(t_s + 32, x + 32);
           t5_wait_ld32(x);
-          t5_wait_ld32(x + 32);
-          const float *cp = spos + st * (AT_MAX_DIMS * AT_COLS);
-          at_logits<DIM, CAP, false>(x, nullptr, cp, pos, slope2, pre, post);
-          at_logits<DIM, CAP, false>(x + 32, nullptr, cp + 32, pos, slope2, pre, post);
-          if (!__all_sync(FULL_MASK, lo <= base && hi >= base + AT_COLS)) {
+          t5_fence_before();
+          __syncwarp();
+          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
+          at_logits<DIM, CAP, false, false>(x, nullptr, spos + st * (AT_MAX_DIMS * AT_COLS) + at.half() * AT_SUB, pos, slope2,
+                                            pre, post, sub, nullptr);
+          if (!__all_sync(FULL_MASK, lo <= base && hi >= base + AT_SUB)) {
 #pragma unroll
-            for (int j = 0; j < AT_COLS; ++j)
+            for (int j = 0; j < AT_SUB; ++j)
               if (base + j < lo || base + j >= hi) x[j] = -pos_inf<float>();
           }
-          float m0 = top, m1 = x[0], m2 = x[1], m3 = x[2];
+          float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-          for (int j = 3; j + 3 < AT_COLS; j += 4) {
-            m0 = fmaxf(m0, x[j]);
-            m1 = fmaxf(m1, x[j + 1]);
-            m2 = fmaxf(m2, x[j + 2]);
-            m3 = fmaxf(m3, x[j + 3]);
+          for (int j = 0; j < AT_SUB; j += 2) {
+            const float e0 = t5_ex2(x[j]), e1 = t5_ex2(x[j + 1]);
+            l0 += e0;
+            l1 += e1;
+            w[j >> 1] = A::pack(e0, e1);
           }
-          m0 = fmaxf(fmaxf(m0, m1), fmaxf(fmaxf(m2, m3), x[AT_COLS - 1]));
-          const bool raise = m0 > top + F::RAISE || (top == -pos_inf<float>() && m0 > top);
+          l0 += l1;
+          const bool raise = top == -pos_inf<float>() || !(l0 <= F::MOST);
           if (__any_sync(FULL_MASK, raise)) {
-            const float to = raise ? m0 : top;
-            const float shrink = raise ? t5_ex2(top - to) : 1.f;  // from -inf: 0
+            float m = x[0];
+#pragma unroll
+            for (int j = 1; j < AT_SUB; ++j) m = fmaxf(m, x[j]);
+            m += sub;
+            const float to = raise && m > top ? m : top;
+            const float shrink = to == top ? 1.f : t5_ex2(top - to);  // from -inf: 0
+            const float to_sub = to == -pos_inf<float>() ? 0.f : to;
+            l0 = l1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < AT_SUB; j += 2) {
+              const float e0 = t5_ex2(x[j] + (sub - to_sub)), e1 = t5_ex2(x[j + 1] + (sub - to_sub));
+              l0 += e0;
+              l1 += e1;
+              w[j >> 1] = A::pack(e0, e1);
+            }
+            l0 += l1;
             top = to;
+            sub = to_sub;
             sum *= shrink;
-            if (s > 0) {
-              // the product of the step before has to be in
-              ok = __all_sync(FULL_MASK, t5_mbar_wait(&o_done, (g - 1) & 1, failed));
+            if (!first) {
+              // the product of the group's step before has to be in
+              ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
               if (!ok) break;
               t5_fence_after();
 #pragma unroll
               for (int c = 0; c < CP; c += 32) {
                 float o[32];
-                t5_ld32(t_o + lane_base + c, o);
+                t5_ld32(t_r + c, o);
                 t5_wait_ld32(o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] *= shrink;
-                t5_st32(t_o + lane_base + c, reinterpret_cast<const uint32_t *>(o));
+                t5_st32(t_r + c, o);
               }
             }
           }
-          const float sub = top == -pos_inf<float>() ? 0.f : top;
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int j = 0; j < AT_COLS; j += 2) {
-            const float e0 = t5_ex2(x[j] - sub), e1 = t5_ex2(x[j + 1] - sub);
-            l0 += e0;
-            l1 += e1;
-            w[j >> 1] = A::pack(e0, e1);
-          }
-          sum += l0 + l1;
+          sum += l0;
         } else {
+          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) w[j] = 0u;
+          for (int j = 0; j < AT_SUB / 2; ++j) w[j] = 0u;
         }
-        t5_st32(t_s, w);
+        // the weights of the group's step before have been taken
+        if (!first) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
+        if (!ok) break;
+        t5_fence_after();
+        t5_st16(t_p, w);
         t5_wait_st();
-        if (last) {
-          at_clear<CP>(stages + st * F::STAGE_BYTES + F::TILE_BYTES, (int)count - base, tid, AT_ROWS);
+        if (tail) {
+          at_clear<CP>(values, (int)count - base, lrow);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         t5_fence_before();
-        t5_mbar_arrive(&p_ready[g & 1]);
+        __syncwarp();
+        if (lane == 0) t5_mbar_arrive(&w_ready[grp]);
       }
-      if (ok && steps > 0) {
-        ok = __all_sync(FULL_MASK, t5_mbar_wait(&done, passes & 1, failed));
+      if (ok && count > 0) {
+        ok = t5_mbar_wait_warp(&done, passes & 1, failed);
         t5_fence_after();
       }
       if (bad) bad_s = 1;
-      const bool redo = mixed && !by_example;
-      if (redo) {  // the softmax warps agree on whether this pass counts
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      }
-      if (!(redo && *(volatile int *)&bad_s)) {
-        const bool store = mine && row < tile.t1;
-        const float nan = __int_as_float(0x7fffffff);
-        const float inv = !ok ? nan : sum == 0.f ? 0.f : 1.f / sum;
+      s_top[grp][lrow] = top;
+      s_sum[grp][lrow] = sum;
+      asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
+      if (!(scan && *(volatile int *)&bad_s)) {
+        // join the groups: each takes CP / G channels of the row
+        const uint32_t steps = walk.all_steps();
+        float all_top = -pos_inf<float>(), all_sum = 0.f, part[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) all_top = fmaxf(all_top, s_top[g][lrow]);
+        const float all_sub = all_top == -pos_inf<float>() ? 0.f : all_top;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          part[g] = t5_ex2(s_top[g][lrow] - all_sub);
+          all_sum = fmaf(part[g], s_sum[g][lrow], all_sum);
+        }
+        const bool store = mine && row < tile.t1, none = all_sum == 0.f;
+        const float nan = __int_as_float(0x7fffffff), inv = none ? 0.f : 1.f / all_sum;
         T *dst = (T *)a.out + (row * p.heads + head) * p.channels;
         T *dst2 = rest ? rest + (row * p.heads + head) * p.channels : nullptr;
 #pragma unroll
-        for (int c = 0; c < CP; c += 32) {
-          float o[32];
-          if (steps > 0 && ok) {
-            t5_ld32(t_o + lane_base + c, o);
-            t5_wait_ld32(o);
+        for (int cc = 0; cc < CP / G; cc += 32) {
+          const int c = grp * (CP / G) + cc;
+          float r[32] = {};
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            // a group without a step in this pass has no result
+            if ((g + G - step0 % G) % G < steps && ok) {
+              float o[32];
+              t5_ld32(t_o + g * CP + lane_base + c, o);
+              t5_wait_ld32(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[i] = fmaf(o[i], part[g], r[i]);
+            }
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -299,12 +358,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             uint32_t *po = reinterpret_cast<uint32_t *>(&out), *pl = reinterpret_cast<uint32_t *>(&low);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float x0 = 0.f, x1 = 0.f;
-              if (steps > 0 && (sum != 0.f || !ok)) {
-                x0 = o[i + 2 * e] * inv;
-                x1 = o[i + 2 * e + 1] * inv;
-              }
-              if (!ok) x0 = x1 = nan;
+              const float x0 = !ok ? nan : none ? 0.f : r[i + 2 * e] * inv;
+              const float x1 = !ok ? nan : none ? 0.f : r[i + 2 * e + 1] * inv;
               po[e] = A::pack(x0, x1);
               const T *h = reinterpret_cast<const T *>(&po[e]);
               pl[e] = A::pack(x0 - at_float(h[0]), x1 - at_float(h[1]));
@@ -315,11 +370,13 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             }
           }
         }
-        if (a.lse && store) a.lse[(int64_t)head * p.m + row] = sum == 0.f ? pos_inf<float>() : top + log2f(sum);
+        if (a.lse && store && grp == 0)
+          a.lse[(int64_t)head * p.m + row] = none ? pos_inf<float>() : all_top + log2f(all_sum);
       }
     }
-    it += steps;
-    if (steps > 0) ++passes;
+    step0 += walk.all_steps();
+    stage0 += walk.all_stages();
+    if (count > 0) ++passes;
     t5_fence_before();
     __syncthreads();
     t5_fence_after();
@@ -330,22 +387,22 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
     }
     if (!tile.next(next_row, pass)) break;
   }
-  if (*failed && warp < 4 && row < tile.t1) {
+  if (*failed && element && grp == 0 && row < tile.t1) {
     // a wait ran out: nothing of this block is to be trusted
     T *dst = (T *)a.out + (row * p.heads + head) * p.channels;
     for (int c = 0; c < p.channels; ++c) dst[c] = at_round<T>(__int_as_float(0x7fffffff));
   }
-  if (*failed && warp == 4) {
+  if (*failed && warp == COPY) {
     at_drain(&q_full, 1, 1);
     at_drain(full, F::STAGES, issued);
   }
-  if (*failed && warp == 5) {
-    if (lane == 0) t5_commit(&drained);
+  if (*failed && warp == PRODUCT) {
+    if (t5_elect()) t5_commit(&drained);
     __syncwarp();
     at_drain(&drained, 1, 1);
   }
   __syncthreads();
-  if (warp == 4) t5_dealloc(tmem, F::TMEM);
+  if (warp == COPY) t5_dealloc(tmem, F::TMEM);
 }
 
 }  // namespace b200c

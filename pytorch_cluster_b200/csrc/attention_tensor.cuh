@@ -1,14 +1,19 @@
 // Attention on the 5th-generation tensor cores, 16-bit types (see attention.cuh for the formulas): what the forward
 // and the backward kernel share.
 //
-// A block owns 128 rows of one side and walks the other side's rows of the same examples ("columns") in tiles of 64:
+// A block owns 128 rows of one side and walks the other side's rows of the same examples ("columns"), 64 to a stage of
+// the copies and 32 to a step of the arithmetic:
 //   forward: rows = queries of a head,  columns = keys;     S = Q K^T,  then O += P V
 //   dq:      rows = queries of a head,  columns = keys;     S = Q K^T, dP = dO V^T,  then dQ += dS K
 //   dk, dv:  rows = keys of a group,    columns = queries;  S' = K Q^T, dP' = V dO^T,  then dV += P' dO, dK += dS' Q
 // One warp brings the operands to shared memory (TMA, 128-byte swizzle, a ring of stages, with the columns' coordinates
-// and statistics beside them), one thread issues the products, and the other warps read the scores from tensor
-// memory, a row per thread, and put the 16-bit weights back there, where the second products take them as their
-// first operand.  The first products have both operands K-major; the second take the column tile MN-major, as it stands.
+// and statistics beside them) and one thread issues the products.  The other warps form G groups of four that take the
+// steps in turn: they read the scores from tensor memory, a row per thread, and put the 16-bit weights back there,
+// where the second products take them as their first operand.  The first products have both operands K-major; the second
+// take the column tile MN-major, as it stands.  Exponentials and roots bound these kernels, not the products: everything
+// is arranged so that the groups never wait for a product.  A group hands its scores' place back as soon as it has read them, so
+// that the scores of its next step are formed while it works on this one, and the weights have a place of
+// their own.
 //
 // A tile may hold rows of several (short) examples.  Its columns are then the union of their ranges, one pass over
 // them, every row masked to its own range.  A masked weight is 0, and 0 times a NaN or an infinity of another example would be
@@ -22,16 +27,40 @@
 namespace b200c {
 
 constexpr int AT_ROWS = 128;  // rows of a block = lanes of tensor memory
-constexpr int AT_COLS = 64;   // columns of a step
+constexpr int AT_COLS = 64;   // columns of a stage
+constexpr int AT_SUB = 32;    // columns of a step
 
 // tensor map of [rows, heads, channels] with boxes of 64 channels x box_rows rows of one head
 int attention_tensor_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int heads, int channels,
                          int64_t row_stride, int64_t head_stride, int box_rows);
 
-// Rows [r_lo, r_hi) of the block's tile and the columns they see.
+// segment_of for a whole warp: 32 probes at a time, a third of the dependent loads
+__device__ __forceinline__ int at_segment_of_warp(const int64_t *__restrict__ ptr, int num_segments, int64_t row,
+                                                  int lane) {
+  if (ptr == nullptr) return 0;
+  int lo = 0, hi = num_segments - 1;
+  while (lo < hi) {
+    const int step = (hi - lo + 32) / 32;
+    const int64_t want = (int64_t)lo + (int64_t)(lane + 1) * step - 1;
+    const int pos = want < hi ? (int)want : hi;
+    const unsigned found = __ballot_sync(FULL_MASK, pos == hi || ptr[pos + 1] > row);
+    const int k = __ffs(found) - 1;
+    lo += k * step;
+    hi = __shfl_sync(FULL_MASK, pos, k);
+  }
+  return lo;
+}
+
+// The columns of a pass over the tile.
 struct AtPass {
   int64_t c_lo, c_hi;
   int segment;  // -1: all rows of the tile
+};
+
+// What the threads of a block find out together about its rows.
+struct AtTileShared {
+  int b_first, b_last;
+  int64_t ends[AT_ROWS];  // ptr[b_first + 1 ...], as far as the tile's segments go
 };
 
 struct AtTile {
@@ -49,8 +78,32 @@ struct AtTile {
     ptr_r = pr;
     ptr_c = pc;
     segments = (int)segs;
-    b_first = segment_of(pr, segments, t0);
-    b_last = segment_of(pr, segments, t1 - 1);
+  }
+  // by warps 0 and 1, before a block-wide barrier; the rest after it
+  __device__ __forceinline__ void search(AtTileShared &sh, int warp, int lane) const {
+    if (warp < 2) {
+      const int b = at_segment_of_warp(ptr_r, segments, warp == 0 ? t0 : t1 - 1, lane);
+      if (lane == 0) (warp == 0 ? sh.b_first : sh.b_last) = b;
+    }
+  }
+  __device__ __forceinline__ void found(const AtTileShared &sh) {
+    b_first = sh.b_first;
+    b_last = sh.b_last;
+  }
+  __device__ __forceinline__ bool listed() const { return b_last > b_first && b_last - b_first < AT_ROWS; }
+  // the segment of a row of the tile; `ends` is filled where listed()
+  __device__ __forceinline__ int segment(const AtTileShared &sh, int64_t row) const {
+    if (b_first == b_last) return b_first;
+    if (!listed()) return segment_of(ptr_r, segments, row);
+    int lo = 0, hi = b_last - b_first;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sh.ends[mid] > row)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    return b_first + lo;
   }
   __device__ __forceinline__ AtPass all() const {
     AtPass p;
@@ -107,31 +160,103 @@ __device__ __forceinline__ uint32_t at_not_finite(const uint4 &w) {
           ((w.w & A::EXP) + A::ONE)) & 0x80008000u;
 }
 
-// Looks through a column tile ([CP / 64][64 rows][128 bytes]); returns non-zero if a value is not finite.
+// Looks through 32 rows of a column tile ([CP / 64][64 rows][128 bytes]) with 128 threads; non-zero if a value is not
+// finite.
 template <typename T, int CP>
-__device__ __forceinline__ uint32_t at_scan(const unsigned char *tile, int tid, int threads) {
+__device__ __forceinline__ uint32_t at_scan(const unsigned char *tile, int tid) {
   uint32_t bad = 0u;
-  for (int i = tid; i < CP * 8; i += threads) bad |= at_not_finite<T>(reinterpret_cast<const uint4 *>(tile)[i]);
-  return bad;
-}
-// Clears rows [count, 64) of a column tile.
-template <int CP>
-__device__ __forceinline__ void at_clear(unsigned char *tile, int count, int tid, int threads) {
-  const int each = (AT_COLS - count) * 8;
 #pragma unroll
   for (int a = 0; a < CP / 64; ++a)
-    for (int i = tid; i < each; i += threads)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      bad |= at_not_finite<T>(reinterpret_cast<const uint4 *>(tile + a * (AT_COLS * 128))[i * 128 + tid]);
+  return bad;
+}
+// Clears rows [count, 32) of them.
+template <int CP>
+__device__ __forceinline__ void at_clear(unsigned char *tile, int count, int tid) {
+#pragma unroll
+  for (int a = 0; a < CP / 64; ++a)
+    for (int i = tid; i < (AT_SUB - count) * 8; i += 128)
       reinterpret_cast<uint4 *>(tile + a * (AT_COLS * 128) + count * 128)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// The bias and the cap of 32 scores of a row: s[j] (dot products) become log2 e (t - slope |pos - pos_j|).
-// col_pos: [dims][64] coordinates of the step's columns.  u[j] = tanh of the capped score, where wanted.
-template <int DIM, bool CAP, bool KEEP>
-__device__ __forceinline__ void at_logits(float *s, float *u, const float *col_pos, const float *pos, float slope2,
-                                          float pre, float post) {
+// The stages and steps of a pass: `heads` walks over `count` columns.
+struct AtWalk {
+  uint32_t stages, steps;  // of one head
+  uint32_t heads;
+  __device__ __forceinline__ AtWalk(int64_t count, int heads_)
+      : stages((uint32_t)((count + AT_COLS - 1) / AT_COLS)), steps((uint32_t)((count + AT_SUB - 1) / AT_SUB)),
+        heads(count > 0 ? heads_ : 0) {}
+  __device__ __forceinline__ uint32_t all_stages() const { return stages * heads; }
+  __device__ __forceinline__ uint32_t all_steps() const { return steps * heads; }
+};
+
+// A position in the walk that moves n steps at a time: head e, step c of it.
+struct AtAt {
+  uint32_t e = 0, c = 0;
+  __device__ __forceinline__ void move(const AtWalk &w, uint32_t n) {
+    c += n;
+    while (c >= w.steps && e < w.heads) {
+      c -= w.steps;
+      ++e;
+    }
+  }
+  __device__ __forceinline__ uint32_t stage(const AtWalk &w) const { return e * w.stages + (c >> 1); }
+  __device__ __forceinline__ int base() const { return (int)(c * AT_SUB); }
+  __device__ __forceinline__ uint32_t half() const { return c & 1u; }
+  __device__ __forceinline__ bool last_of_stage(const AtWalk &w) const { return (c & 1u) || c + 1 == w.steps; }
+};
+
+// The place in a ring of stages, with the parity of its current round.
+template <int STAGES>
+struct AtRing {
+  uint32_t st, parity;
+  __device__ __forceinline__ explicit AtRing(uint32_t g) : st(g % STAGES), parity((g / STAGES) & 1u) {}
+  __device__ __forceinline__ void next() {
+    if (++st == STAGES) {
+      st = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// Coordinates of a stage's columns: a lane's share in registers, then [dims][64] in shared memory.
+template <int DIM>
+__device__ __forceinline__ void at_fetch_places(float *v, const float *__restrict__ src, int dims, int64_t c0,
+                                                int64_t c_hi, int lane) {
 #pragma unroll
-  for (int j4 = 0; j4 < 32; j4 += 4) {
-    float d2[4] = {};
+  for (int n = 0; n < 2 * DIM; ++n) {
+    const int i = n * 32 + lane, c = i / DIM, d = i - c * DIM;
+    v[n] = c0 + c < c_hi && d < dims ? src[(c0 + c) * dims + d] : 0.f;
+  }
+}
+template <int DIM>
+__device__ __forceinline__ void at_put_places(float *dst, const float *v, int lane) {
+#pragma unroll
+  for (int n = 0; n < 2 * DIM; ++n) {
+    const int i = n * 32 + lane, c = i / DIM, d = i - c * DIM;
+    dst[d * AT_COLS + c] = v[n];
+  }
+}
+template <>
+__device__ __forceinline__ void at_fetch_places<0>(float *, const float *__restrict__, int, int64_t, int64_t, int) {}
+template <>
+__device__ __forceinline__ void at_put_places<0>(float *, const float *, int) {}
+
+// The bias and the cap of 32 scores of a row: s[j] (dot products) become log2 e (t - slope |pos - pos_j|) - sub, with one
+// `sub` of the row or, with COL, one per column.  col_pos: [dims][64] coordinates of the stage's columns, from the step's
+// first.  u[j] = tanh of the capped score, where wanted.
+template <int DIM, bool CAP, bool KEEP, bool COL>
+__device__ __forceinline__ void at_logits(float *s, float *u, const float *col_pos, const float *pos, float slope2,
+                                          float pre, float post, float sub, const float *col_sub) {
+#pragma unroll
+  for (int j4 = 0; j4 < AT_SUB; j4 += 4) {
+    float d2[4] = {}, off[4] = {sub, sub, sub, sub};
+    if constexpr (COL) {
+      const float4 x = *reinterpret_cast<const float4 *>(col_sub + j4);
+      off[0] = x.x, off[1] = x.y, off[2] = x.z, off[3] = x.w;
+    }
     if constexpr (DIM > 0) {
 #pragma unroll
       for (int d = 0; d < DIM; ++d) {
@@ -140,7 +265,7 @@ __device__ __forceinline__ void at_logits(float *s, float *u, const float *col_p
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float df = pos[d] - xs[j];
-          d2[j] = DIM == 1 ? fabsf(df) : fmaf(df, df, d2[j]);
+          d2[j] = DIM == 1 ? fabsf(df) : d == 0 ? df * df : fmaf(df, df, d2[j]);
         }
       }
     }
@@ -151,9 +276,9 @@ __device__ __forceinline__ void at_logits(float *s, float *u, const float *col_p
         // tanh(y) = 1 - 2 / (e^2y + 1); pre = 2 log2 e scale / cap, post = cap log2 e
         const float w = fmaf(-2.f, t5_rcp(t5_ex2(s[j4 + j] * pre) + 1.f), 1.f);
         if constexpr (KEEP) u[j4 + j] = w;
-        t = w * post;
+        t = fmaf(w, post, -off[j]);
       } else {
-        t = s[j4 + j] * pre;  // pre = scale log2 e
+        t = fmaf(s[j4 + j], pre, -off[j]);  // pre = scale log2 e
       }
       if constexpr (DIM == 1)
         t = fmaf(-slope2, d2[j], t);

@@ -31,7 +31,7 @@ struct AtForwardCall {
 template <typename T, int CP, int DIM, bool CAP, bool KV>
 struct AtBackwardCall {
   static int run(const AttnArgs &a) {
-    using F = AtBackward<CP>;
+    using F = AtBackward<CP, KV>;
     const b200c_attention_t &p = a.p;
     const int64_t row = (int64_t)p.heads * p.channels;
     const int q_box = KV ? AT_COLS : AT_ROWS, k_box = KV ? AT_ROWS : AT_COLS;
