@@ -18,15 +18,16 @@ struct AtBackward {
   static constexpr int BLOCKS = CP == 64 && !KV ? 2 : 1;
   static constexpr int G = CP == 64 && !KV ? 2 : CP == 128 && KV ? 2 : 4;
   static constexpr int EL_WARPS = 4 * G, EL_THREADS = 32 * EL_WARPS;
-  static constexpr int THREADS = EL_THREADS + 64;
+  static constexpr int THREADS = EL_THREADS + 96;
   static constexpr int STAGES = BLOCKS == 2 ? 3 : 4;
   static constexpr int ROW_BYTES = AT_ROWS * CP * 2, TILE_BYTES = AT_COLS * CP * 2;
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
   static constexpr int SIDE_FLOATS = (AT_MAX_DIMS + 2) * AT_COLS;  // coordinates, lse, D of a stage's columns
   static constexpr int SMEM = 2 * ROW_BYTES + STAGES * (STAGE_BYTES + SIDE_FLOATS * 4) + 1024;
-  static constexpr int GROUP_COLS = 2 * AT_SUB + (KV ? 2 : 1) * (AT_SUB / 2);  // S, dP, dS, P
+  static constexpr int W_COLS = (KV ? 2 : 1) * (AT_SUB / 2);  // a group's dS, P
+  static constexpr int PAIRS = G / 2, PAIR_COLS = 2 * AT_COLS + 2 * W_COLS;  // S, dP of a stage, two groups' weights
   static constexpr int TMEM = BLOCKS == 2 ? 256 : 512;
-  static_assert(G * GROUP_COLS + (KV ? 2 : 1) * CP <= TMEM, "tensor memory");
+  static_assert(PAIRS * PAIR_COLS + (KV ? 2 : 1) * CP <= TMEM, "tensor memory");
   static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 
@@ -52,14 +53,14 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
                           const float *__restrict__ norms) {
   using F = AtBackward<CP, KV>;
   using A = AtType<T>;
-  constexpr int ATOMS = CP / 64, G = F::G, COPY = F::EL_WARPS, PRODUCT = F::EL_WARPS + 1;
+  constexpr int ATOMS = CP / 64, G = F::G, COPY = F::EL_WARPS, SCORE = F::EL_WARPS + 1, SUM = F::EL_WARPS + 2;
   extern __shared__ unsigned char at_raw[];
   unsigned char *smem = at_raw + ((1024u - (t5_smem(at_raw) & 1023u)) & 1023u);
   unsigned char *rows0 = smem, *rows1 = smem + F::ROW_BYTES, *stages = smem + 2 * F::ROW_BYTES;
   float *side = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  // s_full / s_free: a group's scores are in / have been read; w_ready: its weights are in; a_done: its second product is
-  __shared__ __align__(8) uint64_t r_full, full[F::STAGES], empty[F::STAGES], s_full[G], s_free[G], w_ready[G],
-      a_done[G], done, drained;
+  // s_full / s_free: a pair's scores are in / have been read; w_ready: a group's weights are in; a_done: their product is
+  __shared__ __align__(8) uint64_t r_full, full[F::STAGES], empty[F::STAGES], s_full[F::PAIRS], s_free[F::PAIRS],
+      w_ready[G], a_done[G], done, drained[2];
   __shared__ uint32_t tmem_s;
   __shared__ int failed_s, bad_s;
   __shared__ AtTileShared shared_tile;
@@ -83,14 +84,17 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
       t5_mbar_init(&full[i], 1);
       t5_mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < G; ++i) {
+    for (int i = 0; i < F::PAIRS; ++i) {
       t5_mbar_init(&s_full[i], 1);
-      t5_mbar_init(&s_free[i], 4);
+      t5_mbar_init(&s_free[i], 8);
+    }
+    for (int i = 0; i < G; ++i) {
       t5_mbar_init(&w_ready[i], 4);
       t5_mbar_init(&a_done[i], 1);
     }
     t5_mbar_init(&done, 1);
-    t5_mbar_init(&drained, 1);
+    t5_mbar_init(&drained[0], 1);
+    t5_mbar_init(&drained[1], 1);
     failed_s = 0;
     bad_s = 0;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -101,7 +105,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   __syncthreads();
   t5_fence_after();
   const uint32_t tmem = tmem_s;
-  const uint32_t t_acc = tmem + G * F::GROUP_COLS;  // dq, or dv and dk side by side
+  const uint32_t t_acc = tmem + F::PAIRS * F::PAIR_COLS;  // dq, or dv and dk side by side
   if (warp == COPY && lane == 0) {
     t5_mbar_expect(&r_full, 2 * F::ROW_BYTES);
     for (int at = 0; at < ATOMS; ++at) {
@@ -146,18 +150,18 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   int64_t next_row = tile.t0;
   AtPass pass = tile.all();
   const bool mixed = tile.b_first != tile.b_last;
-  uint32_t step0 = 0, stage0 = 0, passes = 0, issued = 0;
+  uint32_t stage0 = 0, passes = 0, issued = 0;
   bool ok = true;
-  if (warp == PRODUCT) ok = t5_mbar_wait_warp(&r_full, 0, failed);
+  if (warp == SCORE) ok = t5_mbar_wait_warp(&r_full, 0, failed);
 
   for (;;) {
     const int64_t count = pass.c_hi - pass.c_lo;
-    const AtWalk walk(count, heads);
+    const uint32_t each = at_stages(count), stages_now = each * heads;
     if (warp == COPY) {
       // ---- copies
       AtRing<F::STAGES> ring(stage0);
       uint32_t e = 0, c = 0;
-      for (uint32_t g = stage0; g < stage0 + walk.all_stages() && ok; ++g, ring.next()) {
+      for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
         const uint32_t st = ring.st;
         const int64_t c0 = pass.c_lo + (int64_t)c * AT_COLS;
         const int head = KV ? head0 + (int)e : group;
@@ -196,95 +200,97 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
         __syncwarp();
         if (lane == 0) t5_mbar_arrive(&full[st]);
         issued = g + 1;
-        if (++c == walk.stages) {
+        if (++c == each) {
           c = 0;
           ++e;
         }
       }
-    } else if (warp == PRODUCT) {
-      // ---- products: the scores of step i + G, then the second products of step i
-      const uint32_t id_s = t5_idesc(A::BF16, AT_SUB, false), id_a = t5_idesc(A::BF16, CP, true);
+    } else if (warp == SCORE) {
+      // ---- scores
+      const uint32_t id = t5_idesc(A::BF16, AT_COLS, false);
       const uint64_t d_r0 = t5_desc(t5_smem(rows0)), d_r1 = t5_desc(t5_smem(rows1)), d_c0 = t5_desc(t5_smem(stages)),
-                     d_c1 = t5_desc(t5_smem(stages + F::TILE_BYTES)),
-                     d_m0 = t5_desc(t5_smem(stages), AT_COLS * 128),
-                     d_m1 = t5_desc(t5_smem(stages + F::TILE_BYTES), AT_COLS * 128);
-      const uint32_t total = walk.all_steps();
-      AtRing<F::STAGES> ring_s(stage0), ring_a(stage0);
-      AtAt at_s, at_a;
-      uint32_t js = 0;  // steps whose scores were issued
-      for (uint32_t ja = 0; ja < total && ok; ++ja) {
-        for (; js < total && js <= ja + G && ok; ++js) {
-          const uint32_t i = step0 + js, gr = i % G, k = i / G;
-          if (at_s.half() == 0) ok = t5_mbar_wait_warp(&full[ring_s.st], ring_s.parity, failed);
-          if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[gr], (k - 1) & 1, failed);
-          if (!ok) break;
-          t5_fence_after();
-          const uint32_t off = (ring_s.st * F::STAGE_BYTES + at_s.half() * (AT_SUB * 128)) / 16;
-          const uint32_t t_s = tmem + gr * F::GROUP_COLS;
-          if (t5_elect()) {
+                     d_c1 = t5_desc(t5_smem(stages + F::TILE_BYTES));
+      AtRing<F::STAGES> ring(stage0);
+      for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
+        const uint32_t pair = g % F::PAIRS, k = g / F::PAIRS;
+        ok = t5_mbar_wait_warp(&full[ring.st], ring.parity, failed);
+        if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[pair], (k - 1) & 1, failed);
+        if (!ok) break;
+        t5_fence_after();
+        const uint32_t off = ring.st * (F::STAGE_BYTES / 16), t_s = tmem + pair * F::PAIR_COLS;
+        if (t5_elect()) {
 #pragma unroll
           for (int ks = 0; ks < CP / 16; ++ks)
             t5_mma_ss(t_s, d_r0 + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
-                      d_c0 + off + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
+                      d_c0 + off + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id, ks > 0);
 #pragma unroll
           for (int ks = 0; ks < CP / 16; ++ks)
-            t5_mma_ss(t_s + AT_SUB, d_r1 + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
-                      d_c1 + off + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
-          t5_commit(&s_full[gr]);
-          }
-          __syncwarp();
-          if (at_s.last_of_stage(walk)) ring_s.next();
-          at_s.move(walk, 1);
-        }
-        if (!ok) break;
-        const uint32_t i = step0 + ja, gr = i % G, k = i / G;
-        ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
-        if (!ok) break;
-        t5_fence_after();
-        const uint32_t off = (ring_a.st * F::STAGE_BYTES + at_a.half() * (AT_SUB * 128)) / 16;
-        const uint32_t w = tmem + gr * F::GROUP_COLS + 2 * AT_SUB;
-        const bool last = at_a.last_of_stage(walk);
-        if (t5_elect()) {
-#pragma unroll
-        for (int ks = 0; ks < AT_SUB / 16; ++ks) {
-          if constexpr (KV)
-            t5_mma_ts(t_acc, w + AT_SUB / 2 + ks * 8, d_m1 + off + ks * (2048 / 16), id_a, ja > 0 || ks > 0);
-          t5_mma_ts(t_acc + (KV ? CP : 0), w + ks * 8, d_m0 + off + ks * (2048 / 16), id_a, ja > 0 || ks > 0);
-        }
-        t5_commit(&a_done[gr]);
-        if (last) t5_commit(&empty[ring_a.st]);
-        if (ja + 1 == total) t5_commit(&done);
+            t5_mma_ss(t_s + AT_COLS, d_r1 + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
+                      d_c1 + off + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id, ks > 0);
+          t5_commit(&s_full[pair]);
         }
         __syncwarp();
-        if (last) ring_a.next();
-        at_a.move(walk, 1);
+      }
+    } else if (warp == SUM) {
+      // ---- products with the weights
+      const uint32_t id = t5_idesc(A::BF16, CP, true);
+      const uint64_t d_c0 = t5_desc(t5_smem(stages), AT_COLS * 128),
+                     d_c1 = t5_desc(t5_smem(stages + F::TILE_BYTES), AT_COLS * 128);
+      AtRing<F::STAGES> ring(stage0);
+      for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
+        const uint32_t pair = g % F::PAIRS, k = g / F::PAIRS;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t gr = 2 * pair + h;
+          if (ok) ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
+          if (!ok) break;
+          t5_fence_after();
+          const uint32_t off = ring.st * (F::STAGE_BYTES / 16) + h * (AT_SUB * 128 / 16);
+          const uint32_t w = tmem + pair * F::PAIR_COLS + 2 * AT_COLS + h * F::W_COLS;
+          const bool more = g != stage0 || h > 0;
+          if (t5_elect()) {
+#pragma unroll
+            for (int ks = 0; ks < AT_SUB / 16; ++ks) {
+              if constexpr (KV)
+                t5_mma_ts(t_acc, w + AT_SUB / 2 + ks * 8, d_c1 + off + ks * (2048 / 16), id, more || ks > 0);
+              t5_mma_ts(t_acc + (KV ? CP : 0), w + ks * 8, d_c0 + off + ks * (2048 / 16), id, more || ks > 0);
+            }
+            t5_commit(&a_done[gr]);
+            if (h == 1) t5_commit(&empty[ring.st]);
+            if (h == 1 && g + 1 == stage0 + stages_now) t5_commit(&done);
+          }
+          __syncwarp();
+        }
       }
     } else {
       // ---- elements
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t t_s = tmem + grp * F::GROUP_COLS + lane_base, t_w = t_s + 2 * AT_SUB;
+      const uint32_t pair = grp >> 1, half = grp & 1, t_pair = tmem + pair * F::PAIR_COLS + lane_base;
+      const uint32_t t_s = t_pair + half * AT_SUB, t_w = t_pair + 2 * AT_COLS + half * F::W_COLS;
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
       const int64_t lo64 = mine ? row_lo - pass.c_lo : 0, hi64 = mine ? row_hi - pass.c_lo : 0;
       const int lo = (int)(lo64 < 0 ? 0 : lo64 > count ? count : lo64), hi = (int)(hi64 < 0 ? 0 : hi64 > count ? count : hi64);
       const bool scan = mixed && !by_example;
       uint32_t bad = 0u;
-      AtAt at;
-      const uint32_t j0 = (grp + G - step0 % G) % G, total = walk.all_steps();  // the group's first step
-      at.move(walk, j0);
-      for (uint32_t j = j0; j < total && ok; j += G, at.move(walk, G)) {
-        const uint32_t g = stage0 + at.stage(walk), st = g % F::STAGES, k = (step0 + j) / G;
-        const int base = at.base();
+      uint32_t e = 0, c = (pair + F::PAIRS - stage0 % F::PAIRS) % F::PAIRS;  // the pair's first stage
+      for (uint32_t g = stage0 + c; g < stage0 + stages_now && ok; g += F::PAIRS, c += F::PAIRS) {
+        while (c >= each) {
+          c -= each;
+          ++e;
+        }
+        const uint32_t st = g % F::STAGES, k = g / F::PAIRS;
+        const int base = (int)(c * AT_COLS + half * AT_SUB);
         const bool tail = base + AT_SUB > (int)count;
-        unsigned char *stage = stages + st * F::STAGE_BYTES + at.half() * (AT_SUB * 128);
-        const float *sd = side + st * F::SIDE_FLOATS + at.half() * AT_SUB;
+        unsigned char *stage = stages + st * F::STAGE_BYTES + half * (AT_SUB * 128);
+        const float *sd = side + st * F::SIDE_FLOATS + half * AT_SUB;
         float slope2 = 0.f;
-        if constexpr (DIM > 0) slope2 = __ldg(p.slope + head0 + at.e) * AT_LOG2E;
+        if constexpr (DIM > 0) slope2 = __ldg(p.slope + head0 + e) * AT_LOG2E;
         ok = t5_mbar_wait_warp(&full[st], (g / F::STAGES) & 1, failed);
         if (scan && ok) {
           bad |= at_scan<T, CP>(stage, lrow);
           if constexpr (KV) bad |= at_scan<T, CP>(stage + F::TILE_BYTES, lrow);
         }
-        if (ok) ok = t5_mbar_wait_warp(&s_full[grp], k & 1, failed);
+        if (ok) ok = t5_mbar_wait_warp(&s_full[pair], k & 1, failed);
         if (!ok) break;
         t5_fence_after();
         uint32_t w[AT_SUB / 2], wp[KV ? AT_SUB / 2 : 1];
@@ -292,12 +298,12 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
         if (any) {
           float x[AT_SUB], dp[AT_SUB], u[CAP ? AT_SUB : 1];
           t5_ld32(t_s, x);
-          t5_ld32(t_s + AT_SUB, dp);
+          t5_ld32(t_s + AT_COLS, dp);
           t5_wait_ld32(x);
           t5_wait_ld32(dp);
           t5_fence_before();
           __syncwarp();
-          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
+          if (lane == 0) t5_mbar_arrive(&s_free[pair]);
           at_logits<DIM, CAP, CAP, KV>(x, u, sd, pos, slope2, pre, post, lse, sd + AT_MAX_DIMS * AT_COLS);
           const bool whole = __all_sync(FULL_MASK, lo <= base && hi >= base + AT_SUB);
 #pragma unroll
@@ -328,7 +334,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
             if constexpr (KV) wp[j] = A::pack(x[2 * j], x[2 * j + 1]);
           }
         } else {
-          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
+          if (lane == 0) t5_mbar_arrive(&s_free[pair]);
 #pragma unroll
           for (int j = 0; j < AT_SUB / 2; ++j) {
             w[j] = 0u;
@@ -336,15 +342,15 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           }
         }
         // the weights of the group's step before have been taken
-        if (j >= G) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
+        if (g - stage0 >= F::PAIRS) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
         if (!ok) break;
         t5_fence_after();
         t5_st16(t_w, w);
         if constexpr (KV) t5_st16(t_w + AT_SUB / 2, wp);
         t5_wait_st();
         if (tail) {
-          at_clear<CP>(stage, (int)count - base, lrow);
-          if constexpr (KV) at_clear<CP>(stage + F::TILE_BYTES, (int)count - base, lrow);
+          at_clear<CP>(stage, (int)count > base ? (int)count - base : 0, lrow);
+          if constexpr (KV) at_clear<CP>(stage + F::TILE_BYTES, (int)count > base ? (int)count - base : 0, lrow);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         t5_fence_before();
@@ -391,8 +397,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
         }
       }
     }
-    step0 += walk.all_steps();
-    stage0 += walk.all_stages();
+    stage0 += stages_now;
     if (count > 0) ++passes;
     t5_fence_before();
     __syncthreads();
@@ -420,10 +425,11 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
     at_drain(&r_full, 1, 1);
     at_drain(full, F::STAGES, issued);
   }
-  if (*failed && warp == PRODUCT) {
-    if (t5_elect()) t5_commit(&drained);
+  if (*failed && (warp == SCORE || warp == SUM)) {
+    uint64_t *bar = &drained[warp == SUM];
+    if (t5_elect()) t5_commit(bar);
     __syncwarp();
-    at_drain(&drained, 1, 1);
+    at_drain(bar, 1, 1);
   }
   __syncthreads();
   if (warp == COPY) t5_dealloc(tmem, F::TMEM);

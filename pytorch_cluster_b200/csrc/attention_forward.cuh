@@ -17,14 +17,14 @@ struct AtForward {
   static constexpr int BLOCKS = CP == 64 ? 2 : 1;  // resident blocks per SM: tensor memory
   static constexpr int STAGES = CP == 64 ? 3 : 4;
   static constexpr int EL_WARPS = 4 * G, EL_THREADS = 32 * EL_WARPS;
-  static constexpr int THREADS = EL_THREADS + 64;  // the groups, a copy warp, a product warp
+  static constexpr int THREADS = EL_THREADS + 96;  // the groups, a copy warp, two product warps
   static constexpr int Q_BYTES = AT_ROWS * CP * 2, TILE_BYTES = AT_COLS * CP * 2;
   static constexpr int POS_BYTES = AT_MAX_DIMS * AT_COLS * 4;
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
   static constexpr int SMEM = Q_BYTES + STAGES * (STAGE_BYTES + POS_BYTES) + 1024;
-  static constexpr int GROUP_COLS = AT_SUB + AT_SUB / 2;  // scores, weights
+  static constexpr int PAIRS = G / 2, PAIR_COLS = AT_COLS + AT_SUB;  // scores of a stage, two groups' weights
   static constexpr int TMEM = CP == 64 ? 256 : 512;
-  static_assert(G * (GROUP_COLS + CP) <= TMEM, "tensor memory");
+  static_assert(PAIRS * PAIR_COLS + G * CP <= TMEM, "tensor memory");
   static constexpr float MOST = 1024.f;  // sum of a step's weights that needs no new maximum
 };
 
@@ -38,15 +38,15 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
                          T *__restrict__ rest) {
   using F = AtForward<CP>;
   using A = AtType<T>;
-  constexpr int ATOMS = CP / 64, G = F::G, COPY = F::EL_WARPS, PRODUCT = F::EL_WARPS + 1;
+  constexpr int ATOMS = CP / 64, G = F::G, COPY = F::EL_WARPS, SCORE = F::EL_WARPS + 1, SUM = F::EL_WARPS + 2;
   extern __shared__ unsigned char at_raw[];
   unsigned char *smem = at_raw + ((1024u - (t5_smem(at_raw) & 1023u)) & 1023u);
   unsigned char *sq = smem;
   unsigned char *stages = smem + F::Q_BYTES;
   float *spos = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  // s_full / s_free: a group's scores are in / have been read; w_ready: its weights are in; a_done: its second product is
-  __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[G], s_free[G], w_ready[G],
-      a_done[G], done, drained;
+  // s_full / s_free: a pair's scores are in / have been read; w_ready: a group's weights are in; a_done: their product is
+  __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[F::PAIRS], s_free[F::PAIRS],
+      w_ready[G], a_done[G], done, drained[2];
   __shared__ uint32_t tmem_s;
   __shared__ int failed_s, bad_s;
   __shared__ AtTileShared shared_tile;
@@ -65,14 +65,17 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       t5_mbar_init(&full[i], 1);
       t5_mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < G; ++i) {
+    for (int i = 0; i < F::PAIRS; ++i) {
       t5_mbar_init(&s_full[i], 1);
-      t5_mbar_init(&s_free[i], 4);
+      t5_mbar_init(&s_free[i], 8);
+    }
+    for (int i = 0; i < G; ++i) {
       t5_mbar_init(&w_ready[i], 4);
       t5_mbar_init(&a_done[i], 1);
     }
     t5_mbar_init(&done, 1);
-    t5_mbar_init(&drained, 1);
+    t5_mbar_init(&drained[0], 1);
+    t5_mbar_init(&drained[1], 1);
     failed_s = 0;
     bad_s = 0;
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -83,7 +86,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   __syncthreads();
   t5_fence_after();
   const uint32_t tmem = tmem_s;
-  const uint32_t t_o = tmem + G * F::GROUP_COLS;  // G results
+  const uint32_t t_o = tmem + F::PAIRS * F::PAIR_COLS;  // G results
   // the copy warp: the queries once
   if (warp == COPY && lane == 0) {
     t5_mbar_expect(&q_full, F::Q_BYTES);
@@ -121,19 +124,19 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   int64_t next_row = tile.t0;
   AtPass pass = tile.all();
   const bool mixed = tile.b_first != tile.b_last;
-  uint32_t step0 = 0, stage0 = 0, passes = 0;  // steps, stages and passes with steps so far
-  uint32_t issued = 0;                         // copy warp: stages whose copies were issued
+  uint32_t stage0 = 0, passes = 0;  // stages, and passes with any, so far
+  uint32_t issued = 0;              // copy warp: stages whose copies were issued
   bool ok = true;
-  if (warp == PRODUCT) ok = t5_mbar_wait_warp(&q_full, 0, failed);
+  if (warp == SCORE) ok = t5_mbar_wait_warp(&q_full, 0, failed);
 
   for (;;) {
     const int64_t count = pass.c_hi - pass.c_lo;
-    const AtWalk walk(count, 1);
+    const uint32_t each = at_stages(count), stages_now = each;
     if (warp == COPY) {
       // ---- copies
       AtRing<F::STAGES> ring(stage0);
       uint32_t c = 0;
-      for (uint32_t g = stage0; g < stage0 + walk.all_stages() && ok; ++g, ring.next()) {
+      for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
         const uint32_t st = ring.st;
         const int64_t c0 = pass.c_lo + (int64_t)c * AT_COLS;
         // the columns' coordinates are on their way while the stage is waited for
@@ -158,58 +161,59 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         issued = g + 1;
         ++c;
       }
-    } else if (warp == PRODUCT) {
-      // ---- products: the scores of step i + G, then the second product of step i
-      const uint32_t id_s = t5_idesc(A::BF16, AT_SUB, false), id_o = t5_idesc(A::BF16, CP, true);
-      const uint64_t d_q = t5_desc(t5_smem(sq)), d_k = t5_desc(t5_smem(stages)),
-                     d_v = t5_desc(t5_smem(stages + F::TILE_BYTES), AT_COLS * 128);
-      const uint32_t total = walk.all_steps();
-      AtRing<F::STAGES> ring_s(stage0), ring_o(stage0);
-      AtAt at_s, at_o;
-      uint32_t js = 0;  // steps whose scores were issued
-      for (uint32_t jo = 0; jo < total && ok; ++jo) {
-        for (; js < total && js <= jo + G && ok; ++js) {
-          const uint32_t i = step0 + js, gr = i % G, k = i / G;
-          if (at_s.half() == 0) ok = t5_mbar_wait_warp(&full[ring_s.st], ring_s.parity, failed);
-          if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[gr], (k - 1) & 1, failed);
-          if (!ok) break;
-          t5_fence_after();
-          const uint64_t d = d_k + (ring_s.st * F::STAGE_BYTES + at_s.half() * (AT_SUB * 128)) / 16;
-          if (t5_elect()) {
-#pragma unroll
-          for (int ks = 0; ks < CP / 16; ++ks)
-            t5_mma_ss(tmem + gr * F::GROUP_COLS, d_q + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
-                      d + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
-          t5_commit(&s_full[gr]);
-          }
-          __syncwarp();
-          if (at_s.last_of_stage(walk)) ring_s.next();
-          at_s.move(walk, 1);
-        }
-        if (!ok) break;
-        const uint32_t i = step0 + jo, gr = i % G, k = i / G;
-        ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
+    } else if (warp == SCORE) {
+      // ---- scores
+      const uint32_t id = t5_idesc(A::BF16, AT_COLS, false);
+      const uint64_t d_q = t5_desc(t5_smem(sq)), d_k = t5_desc(t5_smem(stages));
+      AtRing<F::STAGES> ring(stage0);
+      for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
+        const uint32_t pair = g % F::PAIRS, k = g / F::PAIRS;
+        ok = t5_mbar_wait_warp(&full[ring.st], ring.parity, failed);
+        if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[pair], (k - 1) & 1, failed);
         if (!ok) break;
         t5_fence_after();
-        const uint64_t d = d_v + (ring_o.st * F::STAGE_BYTES + at_o.half() * (AT_SUB * 128)) / 16;
-        const bool last = at_o.last_of_stage(walk);
+        const uint64_t d = d_k + ring.st * (F::STAGE_BYTES / 16);
         if (t5_elect()) {
 #pragma unroll
-        for (int ks = 0; ks < AT_SUB / 16; ++ks)
-          t5_mma_ts(t_o + gr * CP, tmem + gr * F::GROUP_COLS + AT_SUB + ks * 8, d + ks * (2048 / 16), id_o,
-                    jo >= G || ks > 0);
-        t5_commit(&a_done[gr]);
-        if (last) t5_commit(&empty[ring_o.st]);
-        if (jo + 1 == total) t5_commit(&done);
+          for (int ks = 0; ks < CP / 16; ++ks)
+            t5_mma_ss(tmem + pair * F::PAIR_COLS, d_q + ((ks >> 2) * (AT_ROWS * 128) + (ks & 3) * 32) / 16,
+                      d + ((ks >> 2) * (AT_COLS * 128) + (ks & 3) * 32) / 16, id, ks > 0);
+          t5_commit(&s_full[pair]);
         }
         __syncwarp();
-        if (last) ring_o.next();
-        at_o.move(walk, 1);
+      }
+    } else if (warp == SUM) {
+      // ---- products with the weights
+      const uint32_t id = t5_idesc(A::BF16, CP, true);
+      const uint64_t d_v = t5_desc(t5_smem(stages + F::TILE_BYTES), AT_COLS * 128);
+      AtRing<F::STAGES> ring(stage0);
+      for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
+        const uint32_t pair = g % F::PAIRS, k = g / F::PAIRS;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t gr = 2 * pair + h;
+          if (ok) ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
+          if (!ok) break;
+          t5_fence_after();
+          const uint64_t d = d_v + ring.st * (F::STAGE_BYTES / 16) + h * (AT_SUB * 128 / 16);
+          const uint32_t w = tmem + pair * F::PAIR_COLS + AT_COLS + h * (AT_SUB / 2);
+          if (t5_elect()) {
+#pragma unroll
+            for (int ks = 0; ks < AT_SUB / 16; ++ks)
+              t5_mma_ts(t_o + gr * CP, w + ks * 8, d + ks * (2048 / 16), id, g - stage0 >= F::PAIRS || ks > 0);
+            t5_commit(&a_done[gr]);
+            if (h == 1) t5_commit(&empty[ring.st]);
+            if (h == 1 && g + 1 == stage0 + stages_now) t5_commit(&done);
+          }
+          __syncwarp();
+        }
       }
     } else {
       // ---- softmax
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t t_s = tmem + grp * F::GROUP_COLS + lane_base, t_p = t_s + AT_SUB, t_r = t_o + grp * CP + lane_base;
+      const uint32_t pair = grp >> 1, half = grp & 1, t_pair = tmem + pair * F::PAIR_COLS + lane_base;
+      const uint32_t t_s = t_pair + half * AT_SUB, t_p = t_pair + AT_COLS + half * (AT_SUB / 2),
+                     t_r = t_o + grp * CP + lane_base;
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
       // the row's columns relative to the pass's first
       const int64_t lo64 = mine ? row_lo - pass.c_lo : 0, hi64 = mine ? row_hi - pass.c_lo : 0;
@@ -217,18 +221,16 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       const bool scan = mixed && !by_example;
       float top = -pos_inf<float>(), sub = 0.f, sum = 0.f;  // sub: what the scores are taken relative to
       uint32_t bad = 0u;
-      AtAt at;
-      const uint32_t j0 = (grp + G - step0 % G) % G, total = walk.all_steps();  // the group's first step
-      at.move(walk, j0);
-      for (uint32_t j = j0; j < total && ok; j += G, at.move(walk, G)) {
-        const uint32_t g = stage0 + at.stage(walk), st = g % F::STAGES, k = (step0 + j) / G;
-        const int base = at.base();
-        const bool tail = base + AT_SUB > (int)count, first = j < G;
-        unsigned char *values = stages + st * F::STAGE_BYTES + F::TILE_BYTES + at.half() * (AT_SUB * 128);
+      const uint32_t c0 = (pair + F::PAIRS - stage0 % F::PAIRS) % F::PAIRS;  // the pair's first stage
+      for (uint32_t c = c0; c < each && ok; c += F::PAIRS) {
+        const uint32_t g = stage0 + c, st = g % F::STAGES, k = g / F::PAIRS;
+        const int base = (int)(c * AT_COLS + half * AT_SUB);
+        const bool tail = base + AT_SUB > (int)count, first = g - stage0 < F::PAIRS;
+        unsigned char *values = stages + st * F::STAGE_BYTES + F::TILE_BYTES + half * (AT_SUB * 128);
         if (DIM > 0 || scan || tail)
           ok = t5_mbar_wait_warp(&full[st], (g / F::STAGES) & 1, failed);
         if (scan && ok) bad |= at_scan<T, CP>(values, lrow);
-        if (ok) ok = t5_mbar_wait_warp(&s_full[grp], k & 1, failed);
+        if (ok) ok = t5_mbar_wait_warp(&s_full[pair], k & 1, failed);
         if (!ok) break;
         t5_fence_after();
         uint32_t w[AT_SUB / 2];
@@ -239,8 +241,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           t5_wait_ld32(x);
           t5_fence_before();
           __syncwarp();
-          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
-          at_logits<DIM, CAP, false, false>(x, nullptr, spos + st * (AT_MAX_DIMS * AT_COLS) + at.half() * AT_SUB, pos, slope2,
+          if (lane == 0) t5_mbar_arrive(&s_free[pair]);
+          at_logits<DIM, CAP, false, false>(x, nullptr, spos + st * (AT_MAX_DIMS * AT_COLS) + half * AT_SUB, pos, slope2,
                                             pre, post, sub, nullptr);
           if (!__all_sync(FULL_MASK, lo <= base && hi >= base + AT_SUB)) {
 #pragma unroll
@@ -295,7 +297,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           }
           sum += l0;
         } else {
-          if (lane == 0) t5_mbar_arrive(&s_free[grp]);
+          if (lane == 0) t5_mbar_arrive(&s_free[pair]);
 #pragma unroll
           for (int j = 0; j < AT_SUB / 2; ++j) w[j] = 0u;
         }
@@ -306,7 +308,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         t5_st16(t_p, w);
         t5_wait_st();
         if (tail) {
-          at_clear<CP>(values, (int)count - base, lrow);
+          at_clear<CP>(values, (int)count > base ? (int)count - base : 0, lrow);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         t5_fence_before();
@@ -323,7 +325,6 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
       if (!(scan && *(volatile int *)&bad_s)) {
         // join the groups: each takes CP / G channels of the row
-        const uint32_t steps = walk.all_steps();
         float all_top = -pos_inf<float>(), all_sum = 0.f, part[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) all_top = fmaxf(all_top, s_top[g][lrow]);
@@ -343,8 +344,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           float r[32] = {};
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            // a group without a step in this pass has no result
-            if ((g + G - step0 % G) % G < steps && ok) {
+            // a group without a stage in this pass has no result
+            if ((g / 2 + F::PAIRS - (stage0 % F::PAIRS)) % F::PAIRS < each && ok) {
               float o[32];
               t5_ld32(t_o + g * CP + lane_base + c, o);
               t5_wait_ld32(o);
@@ -374,8 +375,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           a.lse[(int64_t)head * p.m + row] = none ? pos_inf<float>() : all_top + log2f(all_sum);
       }
     }
-    step0 += walk.all_steps();
-    stage0 += walk.all_stages();
+    stage0 += stages_now;
     if (count > 0) ++passes;
     t5_fence_before();
     __syncthreads();
@@ -396,10 +396,11 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
     at_drain(&q_full, 1, 1);
     at_drain(full, F::STAGES, issued);
   }
-  if (*failed && warp == PRODUCT) {
-    if (t5_elect()) t5_commit(&drained);
+  if (*failed && (warp == SCORE || warp == SUM)) {
+    uint64_t *bar = &drained[warp == SUM];
+    if (t5_elect()) t5_commit(bar);
     __syncwarp();
-    at_drain(&drained, 1, 1);
+    at_drain(bar, 1, 1);
   }
   __syncthreads();
   if (warp == COPY) t5_dealloc(tmem, F::TMEM);

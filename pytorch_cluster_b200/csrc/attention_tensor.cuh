@@ -1,19 +1,18 @@
 // Attention on the 5th-generation tensor cores, 16-bit types (see attention.cuh for the formulas): what the forward
 // and the backward kernel share.
 //
-// A block owns 128 rows of one side and walks the other side's rows of the same examples ("columns"), 64 to a stage of
-// the copies and 32 to a step of the arithmetic:
+// A block owns 128 rows of one side and walks the other side's rows of the same examples ("columns"), 64 to a stage:
 //   forward: rows = queries of a head,  columns = keys;     S = Q K^T,  then O += P V
 //   dq:      rows = queries of a head,  columns = keys;     S = Q K^T, dP = dO V^T,  then dQ += dS K
 //   dk, dv:  rows = keys of a group,    columns = queries;  S' = K Q^T, dP' = V dO^T,  then dV += P' dO, dK += dS' Q
 // One warp brings the operands to shared memory (TMA, 128-byte swizzle, a ring of stages, with the columns' coordinates
-// and statistics beside them) and one thread issues the products.  The other warps form G groups of four that take the
-// steps in turn: they read the scores from tensor memory, a row per thread, and put the 16-bit weights back there,
-// where the second products take them as their first operand.  The first products have both operands K-major; the second
-// take the column tile MN-major, as it stands.  Exponentials and roots bound these kernels, not the products: everything
-// is arranged so that the groups never wait for a product.  A group hands its scores' place back as soon as it has read them, so
-// that the scores of its next step are formed while it works on this one, and the weights have a place of
-// their own.
+// and statistics beside them), one issues the products of the scores, one the products with the weights.  The other warps form G
+// groups of four; a pair of groups takes a stage, 32 columns each: they read the scores from tensor memory, a row per
+// thread, and put the 16-bit weights back there, where the second products take them as their first operand.  The
+// first products have both operands K-major; the second take the column tile MN-major, as it stands.  Exponentials and
+// roots bound these kernels, not the products: everything is arranged so that the groups never wait for a product.
+// They hand the scores' place back as soon as they have read them, so that the next scores are formed while they work on
+// these, and the weights have a place of their own.
 //
 // A tile may hold rows of several (short) examples.  Its columns are then the union of their ranges, one pass over
 // them, every row masked to its own range.  A masked weight is 0, and 0 times a NaN or an infinity of another example would be
@@ -28,7 +27,7 @@ namespace b200c {
 
 constexpr int AT_ROWS = 128;  // rows of a block = lanes of tensor memory
 constexpr int AT_COLS = 64;   // columns of a stage
-constexpr int AT_SUB = 32;    // columns of a step
+constexpr int AT_SUB = 32;    // columns of a group's share of it
 
 // tensor map of [rows, heads, channels] with boxes of 64 channels x box_rows rows of one head
 int attention_tensor_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int heads, int channels,
@@ -181,32 +180,8 @@ __device__ __forceinline__ void at_clear(unsigned char *tile, int count, int tid
       reinterpret_cast<uint4 *>(tile + a * (AT_COLS * 128) + count * 128)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// The stages and steps of a pass: `heads` walks over `count` columns.
-struct AtWalk {
-  uint32_t stages, steps;  // of one head
-  uint32_t heads;
-  __device__ __forceinline__ AtWalk(int64_t count, int heads_)
-      : stages((uint32_t)((count + AT_COLS - 1) / AT_COLS)), steps((uint32_t)((count + AT_SUB - 1) / AT_SUB)),
-        heads(count > 0 ? heads_ : 0) {}
-  __device__ __forceinline__ uint32_t all_stages() const { return stages * heads; }
-  __device__ __forceinline__ uint32_t all_steps() const { return steps * heads; }
-};
-
-// A position in the walk that moves n steps at a time: head e, step c of it.
-struct AtAt {
-  uint32_t e = 0, c = 0;
-  __device__ __forceinline__ void move(const AtWalk &w, uint32_t n) {
-    c += n;
-    while (c >= w.steps && e < w.heads) {
-      c -= w.steps;
-      ++e;
-    }
-  }
-  __device__ __forceinline__ uint32_t stage(const AtWalk &w) const { return e * w.stages + (c >> 1); }
-  __device__ __forceinline__ int base() const { return (int)(c * AT_SUB); }
-  __device__ __forceinline__ uint32_t half() const { return c & 1u; }
-  __device__ __forceinline__ bool last_of_stage(const AtWalk &w) const { return (c & 1u) || c + 1 == w.steps; }
-};
+// Stages of a pass: `heads` walks over `count` columns.
+__device__ __forceinline__ uint32_t at_stages(int64_t count) { return (uint32_t)((count + AT_COLS - 1) / AT_COLS); }
 
 // The place in a ring of stages, with the parity of its current round.
 template <int STAGES>
