@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "attention.cuh"
+#include "tcgen05.cuh"
 
 namespace b200c {
 
@@ -215,14 +216,314 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_kernel(AttnArgs a, i
   }
 }
 
-// joins the splits of a (row, head), one warp each
+// ---- 16-bit types ------------------------------------------------------------------------------------------------
+// The same split over examples, key heads and keys, with the two products on the tensor cores.  Up to 16 rows are too few for
+// a tcgen05 tile of 128; warp-wide products of 16 x 8 x 16 take them as they are, so a warp spends a few hundred
+// instructions on 16 KB of keys and values and memory is the only bound.  Each of the block's warps has a ring of its own in shared
+// memory, 32 keys and values to a stage, filled by asynchronous 16-byte copies two stages ahead: no barrier
+// between warps until the end.  A row of 2 * CP bytes keeps its 16-byte chunk c at c ^ (row & 7), so that neither the copies nor
+// the matrix loads meet bank conflicts.  Weights are rounded to the 16-bit type; maxima, sums and results are fp32.
+// Shared memory of keys past the split's end is cleared: their weights are 0, and 0 times whatever stood there must be 0.
+constexpr int AF_KEYS = 32;    // keys of a stage
+constexpr int AF_STAGES = 3;
+constexpr int AF_ROWS = 16;    // rows (query, head of the group) of a pass
+
 template <typename T>
-__global__ void __launch_bounds__(256) attention_few_join_kernel(AttnArgs a, int splits,
-                                                                 const float *__restrict__ parts) {
+__device__ __forceinline__ void af_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void af_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void af_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t af_pack(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+}
+
+template <int CP>
+struct AfTensor {
+  static constexpr int CHUNKS = CP / 8;  // 16-byte chunks of a row
+  static constexpr int TILE = AF_KEYS * CP * 2, STAGE = 2 * TILE + AF_KEYS * AT_MAX_DIMS * 4;
+  static constexpr int SMEM = AF_WARPS * AF_STAGES * STAGE;
+  static constexpr int PART = AF_ROWS * (CP + 2);  // floats of a warp's part, over its ring at the end
+  static_assert(PART * 4 <= AF_STAGES * STAGE, "a warp's part fits its ring");
+};
+
+template <typename T, int CP, int DIM, bool CAP>
+__global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnArgs a, int splits,
+                                                                          float *__restrict__ parts) {
+  using F = AfTensor<CP>;
+  constexpr int KT = CP / 16, NT = AF_KEYS / 8, CT = CP / 8;
+  extern __shared__ __align__(128) unsigned char af_smem[];
   const b200c_attention_t &p = a.p;
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (i >= p.m * p.heads) return;
+  const int per_group = p.heads / p.groups;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = blockIdx.x % splits;
+  const int group = (blockIdx.x / splits) % p.groups;
+  const int64_t b = blockIdx.x / (splits * p.groups);
+  int64_t q_lo, q_hi, k_lo, k_hi;
+  at_segment(p.ptr_q, p.m, b, q_lo, q_hi);
+  at_segment(p.ptr_k, p.n, b, k_lo, k_hi);
+  const int64_t rows = (q_hi - q_lo) * per_group;
+  const int64_t each = ((k_hi - k_lo + splits - 1) / splits + AF_KEYS - 1) / AF_KEYS * AF_KEYS;
+  const int64_t lo = k_lo + split * each, hi = lo + each < k_hi ? lo + each : k_hi;
+  const T *k = (const T *)p.k + group * p.k_head;
+  const T *v = (const T *)p.v + group * p.v_head;
+  unsigned char *ring = af_smem + warp * (AF_STAGES * F::STAGE);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  // tanh(y) = 1 - 2 / (e^2y + 1)
+  const float pre = CAP ? 2.f * AT_LOG2E * p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
+  const int chunks = p.channels / 8;
+  // this warp's steps of 32 keys: lo + 32 (warp + 4 i)
+  const int64_t all_steps = hi > lo ? (hi - lo + AF_KEYS - 1) / AF_KEYS : 0;
+  const int64_t steps = all_steps > warp ? (all_steps - warp + AF_WARPS - 1) / AF_WARPS : 0;
+
+  // a lane copies chunk my_c of rows my_r, my_r + 32 / CHUNKS, ...
+  constexpr int PER = 32 / F::CHUNKS, COPIES = AF_KEYS / PER;
+  const int my_r = lane / F::CHUNKS, my_c = lane % F::CHUNKS;
+  const int64_t first = lo + warp * AF_KEYS + my_r;
+  const T *k_at = k + first * p.k_row + my_c * 8, *v_at = v + first * p.v_row + my_c * 8;  // of the next step fetched
+  int fetch_slot = 0;
+  int64_t fetch_j = lo + warp * AF_KEYS;
+  auto rewind = [&]() {
+    k_at = k + first * p.k_row + my_c * 8;
+    v_at = v + first * p.v_row + my_c * 8;
+    fetch_slot = 0;
+    fetch_j = lo + warp * AF_KEYS;
+  };
+  auto fetch = [&]() {
+    if (fetch_j < hi) {
+      const uint32_t st = ring_at + fetch_slot * F::STAGE;
+      const bool whole = fetch_j + AF_KEYS <= hi;
+#pragma unroll
+      for (int n = 0; n < COPIES; ++n) {
+        const int r = n * PER + my_r;
+        const uint32_t dk = st + r * (CP * 2) + ((my_c ^ (r & 7)) << 4);
+        if (my_c < chunks && (whole || fetch_j + r < hi)) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dk), "l"(k_at + n * PER * p.k_row) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dk + F::TILE), "l"(v_at + n * PER * p.v_row)
+                       : "memory");
+        } else {
+          unsigned char *z = ring + (dk - ring_at);
+          *reinterpret_cast<uint4 *>(z) = *reinterpret_cast<uint4 *>(z + F::TILE) = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      if constexpr (DIM > 0) {
+        float *sp = reinterpret_cast<float *>(ring + fetch_slot * F::STAGE + 2 * F::TILE);
+        const float *src = p.pos_k + fetch_j * p.dims;
+#pragma unroll
+        for (int n = 0; n < DIM; ++n) {  // [dims][32 keys]
+          const int i = n * 32 + lane, j = i / DIM, d = i - j * DIM;
+          if (d < p.dims && (whole || fetch_j + j < hi))
+            cp_async_4(sp + d * AF_KEYS + j, src + j * p.dims + d);
+          else
+            sp[d * AF_KEYS + j] = 0.f;
+        }
+      }
+    }
+    cp_async_commit();
+    fetch_slot = fetch_slot + 1 == AF_STAGES ? 0 : fetch_slot + 1;
+    fetch_j += AF_WARPS * AF_KEYS;
+    k_at += AF_WARPS * AF_KEYS * p.k_row;
+    v_at += AF_WARPS * AF_KEYS * p.v_row;
+  };
+
+  for (int64_t r0 = 0; r0 < rows; r0 += AF_ROWS) {
+    // the rows' queries as the first operand: lane holds rows lane / 4 and lane / 4 + 8, channels 2 (lane % 4) + {0, 1, 8, 9}
+    const int gr = lane >> 2, gc = (lane & 3) * 2;
+    uint32_t qf[KT][4];
+    float pos[2][DIM == 0 ? 1 : DIM], slope[2] = {}, top[2], sum[2] = {}, o[CT][4] = {};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t r = r0 + gr + 8 * e;
+      const bool there = r < rows;
+      const int64_t row = q_lo + (there ? r : 0) / per_group;
+      const int head = group * per_group + (int)((there ? r : 0) % per_group);
+      const T *src = (const T *)p.q + row * p.q_row + head * p.q_head;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = t * 16 + h * 8 + gc;
+          qf[t][e + 2 * h] = there && c < p.channels ? *reinterpret_cast<const uint32_t *>(src + c) : 0u;
+        }
+      top[e] = -pos_inf<float>();
+      if constexpr (DIM > 0) {
+        slope[e] = p.slope[head] * AT_LOG2E;
+#pragma unroll
+        for (int d = 0; d < DIM; ++d) pos[e][d] = there && d < p.dims ? p.pos_q[row * p.dims + d] : 0.f;
+      }
+    }
+    const bool both = rows - r0 > 8;  // whether rows 8 .. 15 are taken at all
+    rewind();
+#pragma unroll
+    for (int i = 0; i < AF_STAGES - 1; ++i) fetch();
+    int slot = 0;
+    for (int64_t i = 0; i < steps; ++i, slot = slot + 1 == AF_STAGES ? 0 : slot + 1) {
+      cp_async_wait<AF_STAGES - 2>();
+      __syncwarp();
+      const int64_t j0 = lo + (warp + i * AF_WARPS) * AF_KEYS;
+      const uint32_t st = ring_at + slot * F::STAGE;
+      const float *sp = reinterpret_cast<const float *>(ring + slot * F::STAGE + 2 * F::TILE) + gc;
+      float s[NT][4] = {};
+      // scores: 8 keys a tile; one matrix load brings 16 keys of 16 channels
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          const int r = n * 8 + (lane & 7) + ((lane & 16) >> 1), c = 2 * t + ((lane >> 3) & 1);
+          uint32_t kf[4];
+          af_ldmatrix(kf, st + r * (CP * 2) + ((c ^ (r & 7)) << 4));
+          af_mma<T>(s[n], qf[t], kf[0], kf[1]);
+          af_mma<T>(s[n + 1], qf[t], kf[2], kf[3]);
+        }
+      const bool whole = j0 + AF_KEYS <= hi;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (e == 1 && !both) break;
+        float m = top[e];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int j = n * 8 + gc + u;
+            float t;
+            if constexpr (CAP)
+              t = post * fmaf(-2.f, t5_rcp(t5_ex2(s[n][2 * e + u] * pre) + 1.f), 1.f);
+            else
+              t = s[n][2 * e + u] * pre;
+            if constexpr (DIM > 0) {
+              float d2 = 0.f;
+#pragma unroll
+              for (int d = 0; d < DIM; ++d) {
+                const float df = pos[e][d] - sp[d * AF_KEYS + n * 8 + u];
+                d2 = DIM == 1 ? fabsf(df) : fmaf(df, df, d2);
+              }
+              t = fmaf(-slope[e], DIM == 1 ? d2 : t5_sqrt(d2), t);
+            }
+            if (!whole && j0 + j >= hi) t = -pos_inf<float>();
+            s[n][2 * e + u] = t;
+            m = fmaxf(m, t);
+          }
+        m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 2));
+        const float base = m == -pos_inf<float>() ? 0.f : m;
+        const float shrink = t5_ex2(top[e] - base);
+        top[e] = m;
+        float part = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float w = t5_ex2(s[n][2 * e + u] - base);
+            s[n][2 * e + u] = w;
+            part += w;
+          }
+        sum[e] = fmaf(sum[e], shrink, part);
+#pragma unroll
+        for (int n = 0; n < CT; ++n) {
+          o[n][2 * e] *= shrink;
+          o[n][2 * e + 1] *= shrink;
+        }
+      }
+      if (!both) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][2] = s[n][3] = 0.f;
+      }
+#pragma unroll
+      for (int t = 0; t < NT / 2; ++t) {  // 16 keys of the weights against 16 channels a matrix load
+        const uint32_t wf[4] = {af_pack<T>(s[2 * t][0], s[2 * t][1]), af_pack<T>(s[2 * t][2], s[2 * t][3]),
+                                af_pack<T>(s[2 * t + 1][0], s[2 * t + 1][1]), af_pack<T>(s[2 * t + 1][2], s[2 * t + 1][3])};
+#pragma unroll
+        for (int n = 0; n < CT; n += 2) {
+          const int r = t * 16 + (lane & 15), c = n + (lane >> 4);
+          uint32_t vf[4];
+          af_ldmatrix_t(vf, st + F::TILE + r * (CP * 2) + ((c ^ (r & 7)) << 4));
+          af_mma<T>(o[n], wf, vf[0], vf[1]);
+          af_mma<T>(o[n + 1], wf, vf[2], vf[3]);
+        }
+      }
+      __syncwarp();  // the stage is read: it takes the step two ahead
+      fetch();
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    // a warp's part over its ring: rows of CP results, the maximum and the sum
+    float *mine = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      sum[e] += __shfl_xor_sync(FULL_MASK, sum[e], 1);
+      sum[e] += __shfl_xor_sync(FULL_MASK, sum[e], 2);
+      float *dst = mine + (gr + 8 * e) * (CP + 2);
+#pragma unroll
+      for (int n = 0; n < CT; ++n) {
+        dst[n * 8 + gc] = o[n][2 * e];
+        dst[n * 8 + gc + 1] = o[n][2 * e + 1];
+      }
+      if ((lane & 3) == 0) {
+        dst[CP] = top[e];
+        dst[CP + 1] = sum[e];
+      }
+    }
+    __syncthreads();
+    for (int t = tid; t < AF_ROWS * CP; t += AF_THREADS) {
+      const int i = t / CP, c = t % CP;
+      if (r0 + i >= rows) break;
+      float m = -pos_inf<float>(), acc = 0.f, l = 0.f;
+      const float *src[AF_WARPS];
+#pragma unroll
+      for (int w = 0; w < AF_WARPS; ++w) {
+        src[w] = reinterpret_cast<const float *>(af_smem + w * (AF_STAGES * F::STAGE)) + i * (CP + 2);
+        m = fmaxf(m, src[w][CP]);
+      }
+      const float base = m == -pos_inf<float>() ? 0.f : m;
+#pragma unroll
+      for (int w = 0; w < AF_WARPS; ++w) {
+        const float f = exp2f(src[w][CP] - base);
+        acc = fmaf(src[w][c], f, acc);
+        l = fmaf(src[w][CP + 1], f, l);
+      }
+      const int64_t r = r0 + i;
+      const int64_t at = ((q_lo + r / per_group) * p.heads + group * per_group + r % per_group) * splits + split;
+      float *dst = parts + at * (p.channels + 2);
+      if (c < p.channels) dst[2 + c] = acc;
+      if (c == 0) {
+        dst[0] = m;
+        dst[1] = l;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// joins the splits of a (row, head), in ascending order: a block of four warps each, a channel per thread
+template <typename T>
+__global__ void __launch_bounds__(128) attention_few_join_kernel(AttnArgs a, int splits, const float *__restrict__ parts) {
+  __shared__ float factor[128];
+  __shared__ float s_top[4], s_sum[4];
+  const b200c_attention_t &p = a.p;
+  const int64_t i = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = i / p.heads;
   const int head = (int)(i % p.heads);
   int64_t lo, hi;
@@ -230,26 +531,33 @@ __global__ void __launch_bounds__(256) attention_few_join_kernel(AttnArgs a, int
   const bool inside = row >= lo && row < hi;
   const int width = p.channels + 2;
   const float *src = parts + i * splits * width;
-  float m = -pos_inf<float>(), l = 0.f;
-  if (inside) {
-    for (int s = lane; s < splits; s += 32) m = fmaxf(m, src[(int64_t)s * width]);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
-  }
-  const float base = m == -pos_inf<float>() ? 0.f : m;
-  if (inside)
-    for (int s = 0; s < splits; ++s) l = fmaf(src[(int64_t)s * width + 1], exp2f(src[(int64_t)s * width] - base), l);
+  // at most 128 splits: one per thread (attention_few_splits)
+  const bool mine = inside && tid < splits;
+  const float top = mine ? src[(int64_t)tid * width] : -pos_inf<float>(), sum = mine ? src[(int64_t)tid * width + 1] : 0.f;
+  float m = top;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
+  if (lane == 0) s_top[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  const float f = exp2f(top - (m == -pos_inf<float>() ? 0.f : m));
+  factor[tid] = f;
+  float l = sum * f;
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(FULL_MASK, l, o);
+  if (lane == 0) s_sum[warp] = l;
+  __syncthreads();
+  l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *out = (T *)a.out + i * p.channels;
-  for (int c = lane; c < p.channels; c += 32) {
+  if (tid < p.channels) {
     float acc = 0.f;
-    if (inside)
-      for (int s = 0; s < splits; ++s)
-        acc = fmaf(src[(int64_t)s * width + 2 + c], exp2f(src[(int64_t)s * width] - base), acc);
+    if (inside) {
+#pragma unroll 8
+      for (int s = 0; s < splits; ++s) acc = fmaf(src[(int64_t)s * width + 2 + tid], factor[s], acc);
+    }
     const T r = at_round<T>(acc * inv);
-    out[c] = r;
-    if (a.rest) ((T *)a.rest)[i * p.channels + c] = at_round<T>(acc * inv - at_float(r));
+    ((T *)a.out)[i * p.channels + tid] = r;
+    if (a.rest) ((T *)a.rest)[i * p.channels + tid] = at_round<T>(acc * inv - at_float(r));
   }
-  if (a.lse && lane == 0) a.lse[(int64_t)head * p.m + row] = l == 0.f ? pos_inf<float>() : m + log2f(l);
+  if (a.lse && tid == 0) a.lse[(int64_t)head * p.m + row] = l == 0.f ? pos_inf<float>() : m + log2f(l);
 }
 
 // Queries of a group per example, on average, up to which this kernel is taken.  It reads the keys once for every
@@ -263,10 +571,11 @@ int attention_few_splits(const b200c_attention_t &p) {
   if (p.m * per_group > AF_MAX_ROWS * segs || p.n < 64 * segs) return 0;
   const int64_t blocks = segs * p.groups;
   if (blocks > (1ll << 24)) return 0;
-  // about eight blocks per SM, so that ragged examples even out
-  int64_t splits = (148 * 8 + blocks - 1) / blocks;
+  // about four blocks per SM, so that ragged examples even out; 128 at most (the join)
+  int64_t splits = (148 * 4 + blocks - 1) / blocks;
   const int64_t most = p.n / segs / AF_MIN_KEYS;
   if (splits > most) splits = most;
+  if (splits > 128) splits = 128;
   return (int)(splits < 1 ? 1 : splits);
 }
 
@@ -274,15 +583,44 @@ size_t attention_few_workspace_bytes(const b200c_attention_t &p) {
   return (size_t)p.m * p.heads * attention_few_splits(p) * (p.channels + 2) * 4;
 }
 
+template <typename T>
+static int af_join(const AttnArgs &a, int splits, float *parts) {
+  const int64_t rows = a.p.m * a.p.heads;
+  attention_few_join_kernel<T><<<(unsigned)rows, 128, 0, a.stream>>>(a, splits, parts);
+  B200C_LAUNCH_CHECK("attention_few_join_kernel");
+  return B200C_OK;
+}
+
 template <typename T, int LPK, int QB>
 static int af_launch(const AttnArgs &a, int splits, int vec, float *parts) {
   const unsigned blocks = (unsigned)(a.p.num_segments * a.p.groups * splits);
   attention_few_kernel<T, LPK, QB><<<blocks, AF_THREADS, 0, a.stream>>>(a, splits, vec, parts);
   B200C_LAUNCH_CHECK("attention_few_kernel");
-  const int64_t rows = a.p.m * a.p.heads;
-  attention_few_join_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, a.stream>>>(a, splits, parts);
-  B200C_LAUNCH_CHECK("attention_few_join_kernel");
-  return B200C_OK;
+  return af_join<T>(a, splits, parts);
+}
+
+template <typename T, int CP, int DIM, bool CAP>
+static int af_launch_tensor(const AttnArgs &a, int splits, float *parts) {
+  using F = AfTensor<CP>;
+  static unsigned long long configured = 0ull;
+  B200C_CUDA(opt_in_shared_memory(attention_few_tensor_kernel<T, CP, DIM, CAP>, F::SMEM, configured));
+  const unsigned blocks = (unsigned)(a.p.num_segments * a.p.groups * splits);
+  attention_few_tensor_kernel<T, CP, DIM, CAP><<<blocks, AF_THREADS, F::SMEM, a.stream>>>(a, splits, parts);
+  B200C_LAUNCH_CHECK("attention_few_tensor_kernel");
+  return af_join<T>(a, splits, parts);
+}
+template <typename T, int CP, bool CAP>
+static int af_tensor_dims(const AttnArgs &a, int splits, float *parts) {
+  if (a.p.dims == 0) return af_launch_tensor<T, CP, 0, CAP>(a, splits, parts);
+  if (a.p.dims == 1) return af_launch_tensor<T, CP, 1, CAP>(a, splits, parts);
+  if (a.p.dims <= 3) return af_launch_tensor<T, CP, 3, CAP>(a, splits, parts);
+  return af_launch_tensor<T, CP, 8, CAP>(a, splits, parts);
+}
+template <typename T>
+static int af_tensor(const AttnArgs &a, int splits, float *parts) {
+  if (a.p.channels <= 64)
+    return a.p.cap > 0.f ? af_tensor_dims<T, 64, true>(a, splits, parts) : af_tensor_dims<T, 64, false>(a, splits, parts);
+  return a.p.cap > 0.f ? af_tensor_dims<T, 128, true>(a, splits, parts) : af_tensor_dims<T, 128, false>(a, splits, parts);
 }
 
 template <typename T, int LPK>
@@ -299,6 +637,11 @@ static int af_channels(const AttnArgs &a, int splits, float *parts) {
   const b200c_attention_t &p = a.p;
   const int vec = ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0 && p.channels % VL == 0 &&
                   p.k_row % VL == 0 && p.v_row % VL == 0 && p.k_head % VL == 0 && p.v_head % VL == 0;
+  if constexpr (sizeof(T) == 2) {
+    // queries are read as pairs of channels
+    const bool pairs = ((uintptr_t)p.q & 3) == 0 && p.q_row % 2 == 0 && p.q_head % 2 == 0;
+    if (vec && pairs) return af_tensor<T>(a, splits, parts);
+  }
   if (p.channels <= 32) return af_rows<T, 32 / VL>(a, splits, vec, parts);
   if (p.channels <= 64) return af_rows<T, 64 / VL>(a, splits, vec, parts);
   return af_rows<T, 128 / VL>(a, splits, vec, parts);

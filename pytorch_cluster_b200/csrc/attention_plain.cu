@@ -395,49 +395,69 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
   }
 }
 
-// D_i = do_i . o_i, one warp per (row, head); norms[0] rises to the largest |do_i|^2
-template <typename T>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const T *__restrict__ dout, const T *__restrict__ out,
-                                                              const T *__restrict__ rest, int64_t m, int heads,
-                                                              int channels, float *__restrict__ delta,
-                                                              float *__restrict__ norms) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (i >= m * heads) return;
-  float s = 0.f, sq = 0.f;
-  for (int c = lane; c < channels; c += 32) {
-    const float g = at_float(dout[i * channels + c]);
-    float o = at_float(out[i * channels + c]);
-    if (rest) o += at_float(rest[i * channels + c]);
-    s = fmaf(g, o, s);
-    sq = fmaf(g, g, sq);
+// What the backward pass needs beforehand: D_i = do_i . o_i per (row, head), and for fp16 the largest |do_i|^2 and |v_j|^2
+// of any row (norms[0], norms[1]; non-negative floats order like their bits, and a maximum does not depend on
+// the order).  LP lanes share a row, VL channels at a time; the blocks past the first `do_blocks` take the rows of v.
+template <typename T, int VL>
+struct alignas(sizeof(T) * VL) ApVec {
+  T v[VL];
+};
+template <typename T, int VL, int LP>
+__global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, float *__restrict__ delta,
+                                                                float *__restrict__ norms, int64_t do_rows,
+                                                                unsigned do_blocks) {
+  using V = ApVec<T, VL>;
+  __shared__ float s_most[8];
+  const b200c_attention_t &p = a.p;
+  const int part = threadIdx.x % LP, units = p.channels / VL;
+  const bool values = blockIdx.x >= do_blocks;
+  const unsigned block = values ? blockIdx.x - do_blocks : blockIdx.x, blocks = values ? gridDim.x - do_blocks : do_blocks;
+  const int64_t rows = values ? p.n * p.groups : do_rows;
+  const V *dout = (const V *)a.dout, *out = (const V *)a.out, *rest = (const V *)a.rest;
+  float most = 0.f;
+  // whole warps take the same number of steps (the sums are shuffles)
+  for (int64_t i0 = (int64_t)block * (256 / LP); i0 < rows; i0 += (int64_t)blocks * (256 / LP)) {
+    const int64_t i = i0 + threadIdx.x / LP;
+    float s = 0.f, sq = 0.f;
+    if (i < rows) {
+      const V *v = values ? reinterpret_cast<const V *>((const T *)p.v + (i / p.groups) * p.v_row + (i % p.groups) * p.v_head)
+                          : dout + i * units;
+      for (int u = part; u < units; u += LP) {
+        const V g = v[u];
+        if (values) {
+#pragma unroll
+          for (int c = 0; c < VL; ++c) sq = fmaf(at_float(g.v[c]), at_float(g.v[c]), sq);
+        } else {
+          const V o = out[i * units + u];
+          V r{};
+          if (rest) r = rest[i * units + u];
+#pragma unroll
+          for (int c = 0; c < VL; ++c) {
+            const float x = at_float(g.v[c]);
+            s = fmaf(x, at_float(o.v[c]), s);
+            if (rest) s = fmaf(x, at_float(r.v[c]), s);
+            sq = fmaf(x, x, sq);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int o = LP / 2; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(FULL_MASK, s, o);
+      sq += __shfl_xor_sync(FULL_MASK, sq, o);
+    }
+    if (!values && part == 0 && i < rows) delta[(i % p.heads) * p.m + i / p.heads] = s;
+    most = fmaxf(most, sq);
   }
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(FULL_MASK, s, o);
-    sq += __shfl_xor_sync(FULL_MASK, sq, o);
+  if (norms == nullptr) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL_MASK, most, o));
+  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) most = fmaxf(most, s_most[w]);
+    atomicMax((unsigned *)norms + (values ? 1 : 0), __float_as_uint(most));
   }
-  if (lane == 0) {
-    delta[(i % heads) * m + i / heads] = s;
-    // non-negative floats order like their bits; a maximum does not depend on the order
-    if (norms && __float_as_uint(sq) > __float_as_uint(*(volatile float *)norms))
-      atomicMax((unsigned *)norms, __float_as_uint(sq));
-  }
-}
-
-// norms[1] rises to the largest |v_j|^2
-template <typename T>
-__global__ void __launch_bounds__(256) attention_value_norm_kernel(const T *__restrict__ v, int64_t n, int groups,
-                                                                   int channels, int64_t row_stride,
-                                                                   int64_t head_stride, float *__restrict__ norms) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (i >= n * groups) return;
-  const T *row = v + (i / groups) * row_stride + (i % groups) * head_stride;
-  float sq = 0.f;
-  for (int c = lane; c < channels; c += 32) sq = fmaf(at_float(row[c]), at_float(row[c]), sq);
-  for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(FULL_MASK, sq, o);
-  if (lane == 0 && __float_as_uint(sq) > __float_as_uint(*(volatile float *)(norms + 1)))
-    atomicMax((unsigned *)(norms + 1), __float_as_uint(sq));
 }
 
 template <typename T, int CP>
@@ -487,22 +507,31 @@ static int ap_any(const AttnArgs &a, bool forward) {
 int launch_attention_plain_forward(const AttnArgs &a) { return ap_any(a, true); }
 int launch_attention_plain_backward(const AttnArgs &a) { return ap_any(a, false); }
 
+template <typename T, int VL, int LP>
+static int ap_prepare_launch(const AttnArgs &a, float *delta, float *norms) {
+  const int64_t rows = a.p.m * a.p.heads, values = norms ? a.p.n * a.p.groups : 0;
+  const auto blocks = [](int64_t r) {
+    const int64_t want = (r + 256 / LP - 1) / (256 / LP);
+    return (unsigned)(want < 148 * 8 ? want : 148 * 8);
+  };
+  const unsigned b0 = blocks(rows), b1 = blocks(values);
+  if (norms) B200C_CUDA(cudaMemsetAsync(norms, 0, 8, a.stream));
+  if (b0 + b1 == 0) return B200C_OK;
+  attention_prepare_kernel<T, VL, LP><<<b0 + b1, 256, 0, a.stream>>>(a, delta, norms, rows, b0);
+  B200C_LAUNCH_CHECK("attention_prepare_kernel");
+  return B200C_OK;
+}
+
 template <typename T>
 static int ap_delta(const AttnArgs &a, float *delta, float *norms) {
+  constexpr int VL = 16 / (int)sizeof(T);
   const b200c_attention_t &p = a.p;
-  const int64_t rows = p.m * p.heads, values = p.n * p.groups;
-  if (norms) B200C_CUDA(cudaMemsetAsync(norms, 0, 8, a.stream));
-  if (rows > 0) {
-    attention_delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, a.stream>>>(
-        (const T *)a.dout, (const T *)a.out, (const T *)a.rest, p.m, p.heads, p.channels, delta, norms);
-    B200C_LAUNCH_CHECK("attention_delta_kernel");
-  }
-  if (norms && values > 0) {
-    attention_value_norm_kernel<T><<<(unsigned)((values + 7) / 8), 256, 0, a.stream>>>(
-        (const T *)p.v, p.n, p.groups, p.channels, p.v_row, p.v_head, norms);
-    B200C_LAUNCH_CHECK("attention_value_norm_kernel");
-  }
-  return B200C_OK;
+  const bool vec = p.channels % VL == 0 && p.v_row % VL == 0 && p.v_head % VL == 0 &&
+                   (((uintptr_t)a.dout | (uintptr_t)a.out | (uintptr_t)a.rest | (uintptr_t)p.v) & 15) == 0;
+  if (!vec) return ap_prepare_launch<T, 1, 32>(a, delta, norms);
+  if (p.channels <= 4 * VL) return ap_prepare_launch<T, VL, 4>(a, delta, norms);
+  if (p.channels <= 8 * VL) return ap_prepare_launch<T, VL, 8>(a, delta, norms);
+  return ap_prepare_launch<T, VL, 16>(a, delta, norms);
 }
 
 int launch_attention_delta(const AttnArgs &a, float *delta, float *norms) {

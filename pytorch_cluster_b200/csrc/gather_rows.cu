@@ -2,10 +2,12 @@
 //   out[e] = scale x[index[e]],   dx[n] = scale sum_{e : index[e] = n} dout[e]
 // An index outside [0, rows) is padding (knn's -1): it gives a row of zeros and receives no gradient.
 //
-// Both directions are bound by memory: the forward pass is one copy with 16-byte accesses.  The backward pass has to
+// Both directions are bound by memory: the forward pass is one copy with 16-byte accesses, four edges per thread so that
+// enough loads are on their way behind the indices.  The backward pass has to
 // bring equal indices together.  It sorts (index, e) pairs with a stable radix sort — as few passes of up to 9 bits as the
-// row count needs, each a histogram, a scan and a scatter of 8 bytes per pair — and then adds dout's
-// rows in that order, in fp32, each thread owning 16 bytes of the channels over a fixed number of consecutive pairs.
+// row count needs, each a histogram per block, a scan of the blocks' counts per digit, and a scatter of 8 bytes per pair by
+// way of shared memory, where a block's pairs are put in order first, so that they leave in runs — and then adds dout's
+// rows in that order, in fp32, each thread owning 16 bytes of the channels over 64 consecutive pairs.
 // Sums that cross such a piece's border go to the workspace and are joined in order.  No atomics touch a sum, so
 // the result is the same from run to run, and an index that occurs a million times costs no more than a million
 // different ones.
@@ -19,6 +21,8 @@ constexpr int GR_WARPS = GR_THREADS / 32;
 constexpr int GR_ITEMS = 16;                       // pairs per thread of a sort block
 constexpr int GR_TILE = GR_THREADS * GR_ITEMS;     // pairs per sort block
 constexpr int GR_MAX_BITS = 9;
+constexpr int GR_EDGES = 4;                        // edges per thread of the forward pass
+constexpr int GR_LONG_WARPS = 32;                  // of a block that joins a long run
 constexpr int GR_SHORT = 16;                       // pieces a single thread joins; longer runs get a block
 
 template <typename T, int VL>
@@ -42,95 +46,193 @@ __device__ __forceinline__ __nv_bfloat16 gr_round<__nv_bfloat16>(float v) { retu
 template <typename T, int VL>
 __global__ void __launch_bounds__(GR_THREADS) gather_rows_kernel(const T *__restrict__ x,
                                                                  const int64_t *__restrict__ index, int64_t rows,
-                                                                 int64_t edges, int units, float scale,
+                                                                 int64_t total, int units, float scale,
                                                                  T *__restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * GR_THREADS + threadIdx.x;
-  if (i >= edges * units) return;
-  const int64_t e = i / units, u = i - e * units;
-  const int64_t row = index[e];
-  GrVec<T, VL> r;
-  if (row >= 0 && row < rows) {
-    r = reinterpret_cast<const GrVec<T, VL> *>(x)[row * units + u];
+  // thread t of a block takes units t, t + 256, t + 512, ... of the block's share
+  const int64_t base = (int64_t)blockIdx.x * (GR_THREADS * GR_EDGES) + threadIdx.x;
+  int64_t from[GR_EDGES];
 #pragma unroll
-    for (int c = 0; c < VL; ++c) r.v[c] = gr_round<T>(gr_float(r.v[c]) * scale);
-  } else {
-#pragma unroll
-    for (int c = 0; c < VL; ++c) r.v[c] = gr_round<T>(0.f);
+  for (int n = 0; n < GR_EDGES; ++n) {
+    const int64_t i = base + n * GR_THREADS;
+    from[n] = -1;
+    if (i < total) {
+      const int64_t e = total <= 0xffffffffLL ? (int64_t)((uint32_t)i / (uint32_t)units) : i / units;
+      const int64_t row = index[e];
+      if (row >= 0 && row < rows) from[n] = row * units + (i - e * units);
+    }
   }
-  reinterpret_cast<GrVec<T, VL> *>(out)[i] = r;
+  GrVec<T, VL> r[GR_EDGES];
+#pragma unroll
+  for (int n = 0; n < GR_EDGES; ++n) {
+    if (from[n] >= 0) {
+      r[n] = reinterpret_cast<const GrVec<T, VL> *>(x)[from[n]];
+    } else {
+#pragma unroll
+      for (int c = 0; c < VL; ++c) r[n].v[c] = gr_round<T>(0.f);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < GR_EDGES; ++n) {
+    const int64_t i = base + n * GR_THREADS;
+    if (i >= total) break;
+    if (from[n] >= 0) {
+#pragma unroll
+      for (int c = 0; c < VL; ++c) r[n].v[c] = gr_round<T>(gr_float(r[n].v[c]) * scale);
+    }
+    reinterpret_cast<GrVec<T, VL> *>(out)[i] = r[n];
+  }
 }
 
 // ---- stable radix sort of (key, edge) ------------------------------------------------------------------------
-// The first pass reads the indices themselves (keys == nullptr); an index outside [0, rows) becomes the key `rows`.
-__device__ __forceinline__ uint32_t gr_key(const int64_t *index, const uint32_t *keys, int64_t rows, int64_t i) {
-  if (keys) return keys[i];
+// The first pass reads the indices themselves (pairs == nullptr); an index outside [0, rows) becomes the key `rows`.
+__device__ __forceinline__ uint2 gr_pair(const int64_t *index, const uint2 *pairs, int64_t rows, int64_t i) {
+  if (pairs) return pairs[i];
   const int64_t v = index[i];
-  return (uint32_t)(v >= 0 && v < rows ? v : rows);
+  return make_uint2((uint32_t)(v >= 0 && v < rows ? v : rows), (uint32_t)i);
 }
 
+// counts[digit][block]
 __global__ void __launch_bounds__(GR_THREADS) gather_sort_count_kernel(const int64_t *__restrict__ index,
-                                                                       const uint32_t *__restrict__ keys, int64_t rows,
+                                                                       const uint2 *__restrict__ pairs, int64_t rows,
                                                                        int64_t edges, int shift, int bits,
-                                                                       int32_t *__restrict__ counts) {
+                                                                       uint32_t *__restrict__ counts) {
   __shared__ int hist[1 << GR_MAX_BITS];
   const int bins = 1 << bits;
   for (int i = threadIdx.x; i < bins; i += GR_THREADS) hist[i] = 0;
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * GR_TILE;
-#pragma unroll 4
+#pragma unroll 8
   for (int r = 0; r < GR_ITEMS; ++r) {
     const int64_t i = base + r * GR_THREADS + threadIdx.x;
-    if (i < edges) atomicAdd(&hist[(gr_key(index, keys, rows, i) >> shift) & (bins - 1)], 1);
+    if (i < edges) atomicAdd(&hist[(gr_pair(index, pairs, rows, i).x >> shift) & (bins - 1)], 1);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < bins; i += GR_THREADS) counts[(int64_t)i * gridDim.x + blockIdx.x] = hist[i];
 }
 
+// exclusive sum over one warp-sized batch per warp of the block; returns this thread's, and the block's total
+__device__ __forceinline__ uint32_t gr_block_scan(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(FULL_MASK, in, o);
+    if (lane >= o) in += t;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = in;
+  __syncthreads();
+  uint32_t before = 0u;
+  total = 0u;
+#pragma unroll
+  for (int w = 0; w < GR_WARPS; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  return before + in - v;
+}
+
+// a block per digit: its counts become exclusive sums over the blocks, totals[digit] their total
+__global__ void __launch_bounds__(GR_THREADS) gather_sort_scan_kernel(uint32_t *__restrict__ counts, int64_t blocks,
+                                                                      uint32_t *__restrict__ totals) {
+  __shared__ uint32_t warp_sums[GR_WARPS];
+  uint32_t *mine = counts + (int64_t)blockIdx.x * blocks;
+  uint32_t run = 0u;
+  for (int64_t i0 = 0; i0 < blocks; i0 += GR_THREADS * 4) {
+    uint32_t v[4], sum = 0u, total;
+    const int64_t i = i0 + threadIdx.x * 4;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      v[n] = i + n < blocks ? mine[i + n] : 0u;
+      sum += v[n];
+    }
+    uint32_t at = run + gr_block_scan(sum, warp_sums, total);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (i + n < blocks) mine[i + n] = at;
+      at += v[n];
+    }
+    run += total;
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = run;
+}
+
 __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
-    const int64_t *__restrict__ index, const uint32_t *__restrict__ keys, const uint32_t *__restrict__ vals,
-    int64_t rows, int64_t edges, int shift, int bits, const int64_t *__restrict__ offsets,
-    uint32_t *__restrict__ keys_out, uint32_t *__restrict__ vals_out) {
-  // next[w][d]: where warp w puts its next pair of digit d (32 bits: at most 2^31 - 1 pairs)
-  __shared__ uint32_t next[GR_WARPS][1 << GR_MAX_BITS];
+    const int64_t *__restrict__ index, const uint2 *__restrict__ pairs, int64_t rows, int64_t edges, int shift,
+    int bits, const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
+  constexpr int MOST = 1 << GR_MAX_BITS;
+  extern __shared__ __align__(16) unsigned char gr_smem[];
+  uint2 *sorted = reinterpret_cast<uint2 *>(gr_smem);                          // the block's pairs, by digit
+  uint32_t(*next)[MOST] = reinterpret_cast<uint32_t(*)[MOST]>(sorted + GR_TILE);  // where warp w puts its next pair of digit d
+  uint32_t *shift_to = reinterpret_cast<uint32_t *>(next + GR_WARPS);          // out position - position in `sorted`, per digit
+  __shared__ uint32_t warp_sums[GR_WARPS];
   const int bins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < GR_WARPS * bins; i += GR_THREADS) next[i / bins][i % bins] = 0u;
+  for (int i = threadIdx.x; i < GR_WARPS * MOST; i += GR_THREADS) next[0][i] = 0u;
   __syncthreads();
   // a warp owns GR_ITEMS * 32 consecutive pairs, so that warp, round and lane together keep the order
   const int64_t base = (int64_t)blockIdx.x * GR_TILE + warp * (GR_ITEMS * 32) + lane;
-  uint32_t key[GR_ITEMS];
+  uint2 pair[GR_ITEMS];
 #pragma unroll
   for (int r = 0; r < GR_ITEMS; ++r) {
     const int64_t i = base + r * 32;
-    key[r] = i < edges ? gr_key(index, keys, rows, i) : 0u;
-    if (i < edges) atomicAdd(&next[warp][(key[r] >> shift) & (bins - 1)], 1u);
+    pair[r] = i < edges ? gr_pair(index, pairs, rows, i) : make_uint2(0u, 0u);
   }
-  __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += GR_THREADS) {
-    uint32_t at = (uint32_t)offsets[(int64_t)d * gridDim.x + blockIdx.x];
 #pragma unroll
-    for (int w = 0; w < GR_WARPS; ++w) {
-      const uint32_t c = next[w][d];
-      next[w][d] = at;
-      at += c;
+  for (int r = 0; r < GR_ITEMS; ++r)
+    if (base + r * 32 < edges) atomicAdd(&next[warp][(pair[r].x >> shift) & (bins - 1)], 1u);
+  __syncthreads();
+  // two digits per thread: the block's and all blocks' exclusive sums over the digits
+  const int d0 = threadIdx.x * 2;
+  uint32_t here[2] = {}, all[2] = {}, unused;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+    if (d0 + n < bins) {
+      for (int w = 0; w < GR_WARPS; ++w) here[n] += next[w][d0 + n];
+      all[n] = totals[d0 + n];
     }
-  }
+  uint32_t at_here = gr_block_scan(here[0] + here[1], warp_sums, unused);
+  uint32_t at_all = gr_block_scan(all[0] + all[1], warp_sums, unused);
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+    if (d0 + n < bins) {
+      shift_to[d0 + n] = at_all + counts[(int64_t)(d0 + n) * gridDim.x + blockIdx.x] - at_here;
+      uint32_t at = at_here;
+      for (int w = 0; w < GR_WARPS; ++w) {
+        const uint32_t c = next[w][d0 + n];
+        next[w][d0 + n] = at;
+        at += c;
+      }
+      at_here += here[n];
+      at_all += all[n];
+    }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < GR_ITEMS; ++r) {
-    const int64_t i = base + r * 32;
-    const bool have = i < edges;
-    const uint32_t digit = have ? (key[r] >> shift) & (bins - 1) : (uint32_t)bins;
-    const unsigned same = __match_any_sync(FULL_MASK, digit);
+    const bool have = base + r * 32 < edges;
+    const uint32_t digit = have ? (pair[r].x >> shift) & (bins - 1) : (uint32_t)bins;
+    // the lanes with this digit, a ballot per bit (match_any takes three times as long where digits differ)
+    unsigned same = __ballot_sync(FULL_MASK, have);
+    if (!have) same = ~same;
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (digit >> b) & 1u;
+      const unsigned ones = __ballot_sync(FULL_MASK, one);
+      same &= one ? ones : ~ones;
+    }
     const int rank = __popc(same & ((1u << lane) - 1u));
     uint32_t at = 0u;
-    if (have) at = next[warp][digit] + rank;
+    if (have) at = next[warp][digit];
     __syncwarp();
-    if (have && rank == 0) next[warp][digit] += __popc(same);
+    if (have && rank == 0) next[warp][digit] = at + __popc(same);
     __syncwarp();
-    if (have) {
-      keys_out[at] = key[r];
-      vals_out[at] = vals ? vals[i] : (uint32_t)i;
-    }
+    if (have) sorted[at + rank] = pair[r];
+  }
+  __syncthreads();
+  const int64_t left = edges - (int64_t)blockIdx.x * GR_TILE;
+  const int count = left < GR_TILE ? (int)left : GR_TILE;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += GR_THREADS) {
+    const uint2 p = sorted[i];
+    out[(uint32_t)i + shift_to[(p.x >> shift) & (bins - 1)]] = p;
   }
 }
 
@@ -139,8 +241,7 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
 // before or begins there and leaves its end; part[2 g + 1] that of a run that begins inside and leaves the end.
 template <typename T, int VL>
 __global__ void __launch_bounds__(GR_THREADS) gather_sum_kernel(const T *__restrict__ dout,
-                                                                const uint32_t *__restrict__ keys,
-                                                                const uint32_t *__restrict__ vals, int64_t rows,
+                                                                const uint2 *__restrict__ keys, int64_t rows,
                                                                 int64_t edges, int units, int piece, int64_t pieces,
                                                                 float scale, T *__restrict__ dx,
                                                                 float *__restrict__ part) {
@@ -151,8 +252,8 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sum_kernel(const T *__restr
   const int64_t lo = g * piece, hi = lo + piece < edges ? lo + piece : edges;
   const GrVec<T, VL> *src = reinterpret_cast<const GrVec<T, VL> *>(dout);
   float acc[VL] = {};
-  uint32_t run = keys[lo];
-  bool whole = lo == 0 || keys[lo - 1] != run;  // the run began at or after this piece's start
+  uint32_t run = keys[lo].x;
+  bool whole = lo == 0 || keys[lo - 1].x != run;  // the run began at or after this piece's start
   bool first = true;                            // and is the piece's first
   auto flush = [&](bool ends) {
     if (whole && ends) {
@@ -168,15 +269,20 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sum_kernel(const T *__restr
       for (int c = 0; c < VL; ++c) dst[c] = acc[c];
     }
   };
+  // the pairs of the next rows are on their way while these rows are
+  uint2 pair[AHEAD];
+#pragma unroll
+  for (int n = 0; n < AHEAD; ++n) pair[n] = keys[lo + n < hi ? lo + n : hi - 1];
   for (int64_t i0 = lo; i0 < hi; i0 += AHEAD) {
     uint32_t key[AHEAD];
     GrVec<T, VL> row[AHEAD];
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) {
-      const int64_t i = i0 + n < hi ? i0 + n : hi - 1;
-      key[n] = keys[i];
-      row[n] = src[(int64_t)vals[i] * units + u];
+      key[n] = pair[n].x;
+      row[n] = src[(int64_t)pair[n].y * units + u];
     }
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) pair[n] = keys[i0 + AHEAD + n < hi ? i0 + AHEAD + n : hi - 1];
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) {
       if (i0 + n < hi) {
@@ -193,22 +299,22 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sum_kernel(const T *__restr
       }
     }
   }
-  flush(hi == edges || keys[hi] != run);
+  flush(hi == edges || keys[hi].x != run);
 }
 
 // Where the run that leaves piece g began in g: its pieces are g .. last; returns last, or -1 if none does.
-__device__ __forceinline__ int64_t gr_run(const uint32_t *keys, int64_t edges, int piece, int64_t pieces, int64_t g,
+__device__ __forceinline__ int64_t gr_run(const uint2 *keys, int64_t edges, int piece, int64_t pieces, int64_t g,
                                           uint32_t &run, int &slot) {
   const int64_t lo = g * piece, hi = lo + piece;
   if (hi >= edges) return -1;
-  run = keys[hi - 1];
-  if (keys[hi] != run) return -1;
-  slot = keys[lo] == run ? 0 : 1;
-  if (slot == 0 && lo > 0 && keys[lo - 1] == run) return -1;  // began earlier
+  run = keys[hi - 1].x;
+  if (keys[hi].x != run) return -1;
+  slot = keys[lo].x == run ? 0 : 1;
+  if (slot == 0 && lo > 0 && keys[lo - 1].x == run) return -1;  // began earlier
   int64_t a = g + 1, b = pieces - 1;  // the last piece whose first key is the run's
   while (a < b) {
     const int64_t mid = (a + b + 1) >> 1;
-    if (keys[mid * piece] == run)
+    if (keys[mid * piece].x == run)
       a = mid;
     else
       b = mid - 1;
@@ -217,12 +323,12 @@ __device__ __forceinline__ int64_t gr_run(const uint32_t *keys, int64_t edges, i
 }
 
 template <typename T, int VL>
-__global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint32_t *__restrict__ keys, int64_t rows,
+__global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint2 *__restrict__ keys, int64_t rows,
                                                                  int64_t edges, int units, int piece, int64_t pieces,
                                                                  float scale, T *__restrict__ dx,
                                                                  const float *__restrict__ part,
                                                                  int *__restrict__ num_long,
-                                                                 uint32_t *__restrict__ long_runs) {
+                                                                 uint2 *__restrict__ long_runs) {
   const int64_t id = (int64_t)blockIdx.x * GR_THREADS + threadIdx.x;
   const int64_t g = id / units, u = id - g * units;
   if (g >= pieces) return;
@@ -231,7 +337,7 @@ __global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint32_t 
   const int64_t last = gr_run(keys, edges, piece, pieces, g, run, slot);
   if (last < 0 || run >= rows) return;
   if (last - g > GR_SHORT) {
-    if (u == 0) long_runs[atomicAdd(num_long, 1)] = (uint32_t)g;
+    if (u == 0) long_runs[atomicAdd(num_long, 1)] = make_uint2((uint32_t)g, (uint32_t)last);
     return;
   }
   float acc[VL];
@@ -246,37 +352,42 @@ __global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint32_t 
   reinterpret_cast<GrVec<T, VL> *>(dx)[(int64_t)run * units + u] = r;
 }
 
-// A block per (long run, 32 channels): 8 warps add contiguous shares of its pieces, then one adds the shares in order.
+// A block per (long run, 32 channels): its warps add contiguous shares of its pieces, then one adds the shares in order.
 template <typename T>
-__global__ void __launch_bounds__(GR_THREADS) gather_join_long_kernel(const uint32_t *__restrict__ keys, int64_t rows,
+__global__ void __launch_bounds__(32 * GR_LONG_WARPS) gather_join_long_kernel(const uint2 *__restrict__ keys, int64_t rows,
                                                                       int64_t edges, int channels, int piece,
                                                                       int64_t pieces, float scale, T *__restrict__ dx,
                                                                       const float *__restrict__ part,
                                                                       const int *__restrict__ num_long,
-                                                                      const uint32_t *__restrict__ long_runs) {
-  __shared__ float share[GR_WARPS][32];
+                                                                      const uint2 *__restrict__ long_runs) {
+  __shared__ float share[GR_LONG_WARPS][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slabs = (channels + 31) / 32;
   const int64_t tasks = (int64_t)*num_long * slabs;
   for (int64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-    const int64_t g = long_runs[t / slabs];
+    const uint2 pieces_of = long_runs[t / slabs];
+    const int64_t g = pieces_of.x, n = (int64_t)pieces_of.y - g + 1;
+    const uint32_t run = keys[(g + 1) * piece].x;
     const int c = (int)(t % slabs) * 32 + lane;
-    uint32_t run = 0;
-    int slot = 0;
-    const int64_t last = gr_run(keys, edges, piece, pieces, g, run, slot);
-    const int64_t n = last - g + 1, each = (n + GR_WARPS - 1) / GR_WARPS;
-    const int64_t a = warp * each, b = a + each < n ? a + each : n;
+    const int64_t each = (n + GR_LONG_WARPS - 1) / GR_LONG_WARPS;
+    int64_t a = warp * each;
+    const int64_t b = a + each < n ? a + each : n;
     float acc = 0.f;
     if (c < channels) {
+      const float *src = part + 2 * g * channels + c;
+      if (a == 0) {  // the run's first piece, where it need not begin at the start
+        acc = src[keys[g * piece].x == run ? 0 : channels];
+        a = 1;
+      }
 #pragma unroll 8
-      for (int64_t h = a; h < b; ++h) acc += part[(2 * (g + h) + (h == 0 ? slot : 0)) * channels + c];
+      for (int64_t h = a; h < b; ++h) acc += src[2 * h * channels];
     }
     share[warp][lane] = acc;
     __syncthreads();
     if (warp == 0 && c < channels) {
       acc = 0.f;
 #pragma unroll
-      for (int w = 0; w < GR_WARPS; ++w) acc += share[w][lane];
+      for (int w = 0; w < GR_LONG_WARPS; ++w) acc += share[w][lane];
       dx[(int64_t)run * channels + c] = gr_round<T>(acc * scale);
     }
     __syncthreads();
@@ -289,7 +400,7 @@ static size_t gr_align(size_t v) { return (v + 255) / 256 * 256; }
 struct GrPlan {
   int bits, passes, piece;
   int64_t blocks, pieces;
-  size_t keys, counts, offsets, scan, part, runs, total;
+  size_t pairs, counts, totals, part, runs, total;
 };
 
 static GrPlan gr_plan(int64_t rows, int64_t edges, int64_t channels) {
@@ -303,22 +414,22 @@ static GrPlan gr_plan(int64_t rows, int64_t edges, int64_t channels) {
   p.piece = 64;
   p.pieces = (edges + p.piece - 1) / p.piece;
   const int64_t bins = (1ll << p.bits) * p.blocks;
-  p.keys = gr_align((size_t)edges * 4);
+  p.pairs = gr_align((size_t)edges * 8);
   p.counts = gr_align((size_t)bins * 4);
-  p.offsets = gr_align((size_t)(bins + 1) * 8);
-  p.scan = gr_align(b200c_scan_workspace_bytes(bins));
+  p.totals = gr_align((size_t)4 << p.bits);
   p.part = gr_align((size_t)p.pieces * 2 * channels * 4);
-  p.runs = gr_align((size_t)(p.pieces + 1) * 4);
-  p.total = 4 * p.keys + p.counts + p.offsets + p.scan + p.part + p.runs;
+  p.runs = gr_align((size_t)(p.pieces + 1) * 8);
+  p.total = 2 * p.pairs + p.counts + p.totals + p.part + p.runs;
   return p;
 }
 
 template <typename T, int VL>
 static int gr_forward(const void *x, const int64_t *index, int64_t rows, int64_t edges, int64_t channels, float scale,
                       void *out, cudaStream_t stream) {
-  const int64_t threads = edges * (channels / VL);
-  gather_rows_kernel<T, VL><<<(unsigned)((threads + GR_THREADS - 1) / GR_THREADS), GR_THREADS, 0, stream>>>(
-      (const T *)x, index, rows, edges, (int)(channels / VL), scale, (T *)out);
+  const int64_t total = edges * (channels / VL);
+  constexpr int SHARE = GR_THREADS * GR_EDGES;
+  gather_rows_kernel<T, VL><<<(unsigned)((total + SHARE - 1) / SHARE), GR_THREADS, 0, stream>>>(
+      (const T *)x, index, rows, total, (int)(channels / VL), scale, (T *)out);
   B200C_LAUNCH_CHECK("gather_rows_kernel");
   return B200C_OK;
 }
@@ -328,46 +439,43 @@ static int gr_backward(const void *dout, const int64_t *index, int64_t rows, int
                        float scale, void *dx, void *workspace, cudaStream_t stream) {
   const GrPlan p = gr_plan(rows, edges, channels);
   char *ws = (char *)workspace;
-  uint32_t *keys[2], *vals[2];
-  for (int i = 0; i < 2; ++i) {
-    keys[i] = (uint32_t *)ws, ws += p.keys;
-    vals[i] = (uint32_t *)ws, ws += p.keys;
-  }
-  int32_t *counts = (int32_t *)ws;
+  uint2 *pairs[2];
+  for (int i = 0; i < 2; ++i) pairs[i] = (uint2 *)ws, ws += p.pairs;
+  uint32_t *counts = (uint32_t *)ws;
   ws += p.counts;
-  int64_t *offsets = (int64_t *)ws;
-  ws += p.offsets;
-  void *scan = ws;
-  ws += p.scan;
+  uint32_t *totals = (uint32_t *)ws;
+  ws += p.totals;
   float *part = (float *)ws;
   ws += p.part;
   int *num_long = (int *)ws;
-  uint32_t *long_runs = (uint32_t *)ws + 1;
+  uint2 *long_runs = (uint2 *)ws + 1;
 
   B200C_CUDA(cudaMemsetAsync(dx, 0, (size_t)rows * channels * sizeof(T), stream));  // rows that no index names
-  const uint32_t *k = nullptr, *v = nullptr;
+  constexpr size_t scatter_smem = (size_t)GR_TILE * 8 + (size_t)(GR_WARPS + 1) * (4 << GR_MAX_BITS);
+  static unsigned long long configured = 0ull;
+  B200C_CUDA(opt_in_shared_memory(gather_sort_scatter_kernel, scatter_smem, configured));
+  const uint2 *k = nullptr;
   for (int pass = 0; pass < p.passes; ++pass) {
     gather_sort_count_kernel<<<(unsigned)p.blocks, GR_THREADS, 0, stream>>>(index, k, rows, edges, pass * p.bits,
                                                                             p.bits, counts);
     B200C_LAUNCH_CHECK("gather_sort_count_kernel");
-    int st = b200c_exclusive_scan(counts, (1ll << p.bits) * p.blocks, offsets, scan, p.scan, stream);
-    if (st != B200C_OK) return st;
-    gather_sort_scatter_kernel<<<(unsigned)p.blocks, GR_THREADS, 0, stream>>>(
-        index, k, v, rows, edges, pass * p.bits, p.bits, offsets, keys[pass & 1], vals[pass & 1]);
+    gather_sort_scan_kernel<<<1u << p.bits, GR_THREADS, 0, stream>>>(counts, p.blocks, totals);
+    B200C_LAUNCH_CHECK("gather_sort_scan_kernel");
+    gather_sort_scatter_kernel<<<(unsigned)p.blocks, GR_THREADS, scatter_smem, stream>>>(
+        index, k, rows, edges, pass * p.bits, p.bits, counts, totals, pairs[pass & 1]);
     B200C_LAUNCH_CHECK("gather_sort_scatter_kernel");
-    k = keys[pass & 1];
-    v = vals[pass & 1];
+    k = pairs[pass & 1];
   }
   B200C_CUDA(cudaMemsetAsync(num_long, 0, 4, stream));
   const int units = (int)(channels / VL);
   const unsigned blocks = (unsigned)((p.pieces * units + GR_THREADS - 1) / GR_THREADS);
-  gather_sum_kernel<T, VL><<<blocks, GR_THREADS, 0, stream>>>((const T *)dout, k, v, rows, edges, units, p.piece,
-                                                              p.pieces, scale, (T *)dx, part);
+  gather_sum_kernel<T, VL><<<blocks, GR_THREADS, 0, stream>>>((const T *)dout, k, rows, edges, units, p.piece, p.pieces,
+                                                              scale, (T *)dx, part);
   B200C_LAUNCH_CHECK("gather_sum_kernel");
   gather_join_kernel<T, VL><<<blocks, GR_THREADS, 0, stream>>>(k, rows, edges, units, p.piece, p.pieces, scale,
                                                                (T *)dx, part, num_long, long_runs);
   B200C_LAUNCH_CHECK("gather_join_kernel");
-  gather_join_long_kernel<T><<<296, GR_THREADS, 0, stream>>>(k, rows, edges, (int)channels, p.piece, p.pieces, scale,
+  gather_join_long_kernel<T><<<296, 32 * GR_LONG_WARPS, 0, stream>>>(k, rows, edges, (int)channels, p.piece, p.pieces, scale,
                                                              (T *)dx, part, num_long, long_runs);
   B200C_LAUNCH_CHECK("gather_join_long_kernel");
   return B200C_OK;
