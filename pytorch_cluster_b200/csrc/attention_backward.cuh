@@ -4,7 +4,9 @@
 // Forming the scores once per direction costs two products more than one kernel for both would, which the tensor
 // cores have to spare here; in return no sum is shared between blocks, so there are no atomics.  The statistics of the
 // softmax are known, so the groups' steps need nothing of one another and share one accumulator.
-// P and dS enter the second products in the 16-bit type.  In fp16, whose range is small, P is kept times 2^12 and dS times a
+// P and dS enter the second products in the 16-bit type.  dq takes dS in two parts, rounded and what rounding left, because the
+// rows of dS sum to zero and a rounded one does not: dq's error was 1.5 times that of its own rounding, now it is
+// that (for dk and dv, 1.4 times, tensor memory has no room left).  In fp16, whose range is small, P is kept times 2^12 and dS times a
 // power of two that brings the largest value that |do| and |v| allow to 2^14; both are taken out of the fp32 sums.
 #pragma once
 
@@ -24,7 +26,7 @@ struct AtBackward {
   static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
   static constexpr int SIDE_FLOATS = (AT_MAX_DIMS + 2) * AT_COLS;  // coordinates, lse, D of a stage's columns
   static constexpr int SMEM = 2 * ROW_BYTES + STAGES * (STAGE_BYTES + SIDE_FLOATS * 4) + 1024;
-  static constexpr int W_COLS = (KV ? 2 : 1) * (AT_SUB / 2);  // a group's dS, P
+  static constexpr int W_COLS = AT_SUB;  // a group's dS and P, or dS in two parts
   static constexpr int PAIRS = G / 2, PAIR_COLS = 2 * AT_COLS + 2 * W_COLS;  // S, dP of a stage, two groups' weights
   static constexpr int TMEM = BLOCKS == 2 ? 256 : 512;
   static_assert(PAIRS * PAIR_COLS + (KV ? 2 : 1) * CP <= TMEM, "tensor memory");
@@ -251,9 +253,11 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           if (t5_elect()) {
 #pragma unroll
             for (int ks = 0; ks < AT_SUB / 16; ++ks) {
+              t5_mma_ts(t_acc + (KV ? CP : 0), w + ks * 8, d_c0 + off + ks * (2048 / 16), id, more || ks > 0);
               if constexpr (KV)
                 t5_mma_ts(t_acc, w + AT_SUB / 2 + ks * 8, d_c1 + off + ks * (2048 / 16), id, more || ks > 0);
-              t5_mma_ts(t_acc + (KV ? CP : 0), w + ks * 8, d_c0 + off + ks * (2048 / 16), id, more || ks > 0);
+              else
+                t5_mma_ts(t_acc, w + AT_SUB / 2 + ks * 8, d_c0 + off + ks * (2048 / 16), id, true);
             }
             t5_commit(&a_done[gr]);
             if (h == 1) t5_commit(&empty[ring.st]);
@@ -268,8 +272,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
       const uint32_t pair = grp >> 1, half = grp & 1, t_pair = tmem + pair * F::PAIR_COLS + lane_base;
       const uint32_t t_s = t_pair + half * AT_SUB, t_w = t_pair + 2 * AT_COLS + half * F::W_COLS;
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
-      const int64_t lo64 = mine ? row_lo - pass.c_lo : 0, hi64 = mine ? row_hi - pass.c_lo : 0;
-      const int lo = (int)(lo64 < 0 ? 0 : lo64 > count ? count : lo64), hi = (int)(hi64 < 0 ? 0 : hi64 > count ? count : hi64);
+      const AtSeen seen(row_lo, row_hi, pass, mine);
       const bool scan = mixed && !by_example;
       uint32_t bad = 0u;
       uint32_t e = 0, c = (pair + F::PAIRS - stage0 % F::PAIRS) % F::PAIRS;  // the pair's first stage
@@ -285,17 +288,18 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
         const float *sd = side + st * F::SIDE_FLOATS + half * AT_SUB;
         float slope2 = 0.f;
         if constexpr (DIM > 0) slope2 = __ldg(p.slope + head0 + e) * AT_LOG2E;
-        ok = t5_mbar_wait_warp(&full[st], (g / F::STAGES) & 1, failed);
-        if (scan && ok) {
+        // the scores in, and what came with the columns
+        ok = t5_mbar_wait_both(&s_full[pair], k & 1, &full[st], (g / F::STAGES) & 1, true, failed);
+        if (!ok) break;
+        if (scan) {
           bad |= at_scan<T, CP>(stage, lrow);
           if constexpr (KV) bad |= at_scan<T, CP>(stage + F::TILE_BYTES, lrow);
         }
-        if (ok) ok = t5_mbar_wait_warp(&s_full[pair], k & 1, failed);
-        if (!ok) break;
         t5_fence_after();
-        uint32_t w[AT_SUB / 2], wp[KV ? AT_SUB / 2 : 1];
-        const bool any = __any_sync(FULL_MASK, hi > base && lo < base + AT_SUB && lo < hi);
-        if (any) {
+        uint32_t w[AT_SUB / 2], w2[AT_SUB / 2];  // dS; P, or the rest of dS
+        // asked here, answered when the weights are there to be stored
+        bool taken = g - stage0 < F::PAIRS || t5_mbar_try(&a_done[grp], (k - 1) & 1);
+        if (seen.any(base)) {
           float x[AT_SUB], dp[AT_SUB], u[CAP ? AT_SUB : 1];
           t5_ld32(t_s, x);
           t5_ld32(t_s + AT_COLS, dp);
@@ -305,7 +309,6 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           __syncwarp();
           if (lane == 0) t5_mbar_arrive(&s_free[pair]);
           at_logits<DIM, CAP, CAP, KV>(x, u, sd, pos, slope2, pre, post, lse, sd + AT_MAX_DIMS * AT_COLS);
-          const bool whole = __all_sync(FULL_MASK, lo <= base && hi >= base + AT_SUB);
 #pragma unroll
           for (int j4 = 0; j4 < AT_SUB; j4 += 4) {
             float de[4] = {delta, delta, delta, delta};
@@ -323,30 +326,30 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
               dp[j4 + j] = ds;
             }
           }
-          if (!whole) {
+          if (!seen.all(base)) {
 #pragma unroll
             for (int j = 0; j < AT_SUB; ++j)
-              if (base + j < lo || base + j >= hi) x[j] = dp[j] = 0.f;
+              if (base + j < seen.lo || base + j >= seen.hi) x[j] = dp[j] = 0.f;
           }
 #pragma unroll
           for (int j = 0; j < AT_SUB / 2; ++j) {
             w[j] = A::pack(dp[2 * j], dp[2 * j + 1]);
-            if constexpr (KV) wp[j] = A::pack(x[2 * j], x[2 * j + 1]);
+            if constexpr (KV)
+              w2[j] = A::pack(x[2 * j], x[2 * j + 1]);
+            else
+              w2[j] = A::pack(dp[2 * j] - A::low(w[j]), dp[2 * j + 1] - A::high(w[j]));
           }
         } else {
           if (lane == 0) t5_mbar_arrive(&s_free[pair]);
 #pragma unroll
-          for (int j = 0; j < AT_SUB / 2; ++j) {
-            w[j] = 0u;
-            if constexpr (KV) wp[j] = 0u;
-          }
+          for (int j = 0; j < AT_SUB / 2; ++j) w[j] = w2[j] = 0u;
         }
         // the weights of the group's step before have been taken
-        if (g - stage0 >= F::PAIRS) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
+        if (!__all_sync(FULL_MASK, taken)) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
         if (!ok) break;
         t5_fence_after();
         t5_st16(t_w, w);
-        if constexpr (KV) t5_st16(t_w + AT_SUB / 2, wp);
+        t5_st16(t_w + AT_SUB / 2, w2);
         t5_wait_st();
         if (tail) {
           at_clear<CP>(stage, (int)count > base ? (int)count - base : 0, lrow);

@@ -4,7 +4,9 @@
 // is not looked for in every step: weights are formed against the one in use, and only where their sum over the step's 32
 // columns passes 2^10 (or no maximum is known yet) is it raised to the step's and the result in tensor memory, the sum
 // and the step's weights brought to it.  Weights up to 2^10 are as exact in either type as weights up to 1.
-// Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.
+// Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.  The result
+// is divided by the sum of the rounded weights, not of the exact ones (which the statistics keep): where few
+// keys share the weight their roundings then cancel, and D = do . o, which the gradients need, is as much better.
 #pragma once
 
 #include "attention_tensor.cuh"
@@ -50,7 +52,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   __shared__ uint32_t tmem_s;
   __shared__ int failed_s, bad_s;
   __shared__ AtTileShared shared_tile;
-  __shared__ float s_top[G][AT_ROWS], s_sum[G][AT_ROWS];
+  __shared__ float s_top[G][AT_ROWS], s_sum[G][AT_ROWS], s_sum16[G][AT_ROWS];
   volatile int *failed = &failed_s;
 
   const b200c_attention_t &p = a.p;
@@ -215,11 +217,10 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       const uint32_t t_s = t_pair + half * AT_SUB, t_p = t_pair + AT_COLS + half * (AT_SUB / 2),
                      t_r = t_o + grp * CP + lane_base;
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
-      // the row's columns relative to the pass's first
-      const int64_t lo64 = mine ? row_lo - pass.c_lo : 0, hi64 = mine ? row_hi - pass.c_lo : 0;
-      const int lo = (int)(lo64 < 0 ? 0 : lo64 > count ? count : lo64), hi = (int)(hi64 < 0 ? 0 : hi64 > count ? count : hi64);
+      const AtSeen seen(row_lo, row_hi, pass, mine);
       const bool scan = mixed && !by_example;
-      float top = -pos_inf<float>(), sub = 0.f, sum = 0.f;  // sub: what the scores are taken relative to
+      // sub: what the scores are taken relative to; sums of the weights, exact and rounded
+      float top = -pos_inf<float>(), sub = 0.f, sum = 0.f, sum16 = 0.f;
       uint32_t bad = 0u;
       const uint32_t c0 = (pair + F::PAIRS - stage0 % F::PAIRS) % F::PAIRS;  // the pair's first stage
       for (uint32_t c = c0; c < each && ok; c += F::PAIRS) {
@@ -227,15 +228,15 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         const int base = (int)(c * AT_COLS + half * AT_SUB);
         const bool tail = base + AT_SUB > (int)count, first = g - stage0 < F::PAIRS;
         unsigned char *values = stages + st * F::STAGE_BYTES + F::TILE_BYTES + half * (AT_SUB * 128);
-        if (DIM > 0 || scan || tail)
-          ok = t5_mbar_wait_warp(&full[st], (g / F::STAGES) & 1, failed);
-        if (scan && ok) bad |= at_scan<T, CP>(values, lrow);
-        if (ok) ok = t5_mbar_wait_warp(&s_full[pair], k & 1, failed);
+        // the scores in, and what came with the columns, where it is read here
+        ok = t5_mbar_wait_both(&s_full[pair], k & 1, &full[st], (g / F::STAGES) & 1, DIM > 0 || scan || tail, failed);
         if (!ok) break;
+        if (scan) bad |= at_scan<T, CP>(values, lrow);
         t5_fence_after();
         uint32_t w[AT_SUB / 2];
-        const bool any = __any_sync(FULL_MASK, hi > base && lo < base + AT_SUB && lo < hi);
-        if (any) {
+        // asked here, answered when the weights are there to be stored
+        bool taken = first || t5_mbar_try(&a_done[grp], (k - 1) & 1);
+        if (seen.any(base)) {
           float x[AT_SUB];
           t5_ld32(t_s, x);
           t5_wait_ld32(x);
@@ -244,18 +245,20 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           if (lane == 0) t5_mbar_arrive(&s_free[pair]);
           at_logits<DIM, CAP, false, false>(x, nullptr, spos + st * (AT_MAX_DIMS * AT_COLS) + half * AT_SUB, pos, slope2,
                                             pre, post, sub, nullptr);
-          if (!__all_sync(FULL_MASK, lo <= base && hi >= base + AT_SUB)) {
+          if (!seen.all(base)) {
 #pragma unroll
             for (int j = 0; j < AT_SUB; ++j)
-              if (base + j < lo || base + j >= hi) x[j] = -pos_inf<float>();
+              if (base + j < seen.lo || base + j >= seen.hi) x[j] = -pos_inf<float>();
           }
-          float l0 = 0.f, l1 = 0.f;
+          float l0 = 0.f, l1 = 0.f, r0 = 0.f, r1 = 0.f;
 #pragma unroll
           for (int j = 0; j < AT_SUB; j += 2) {
             const float e0 = t5_ex2(x[j]), e1 = t5_ex2(x[j + 1]);
             l0 += e0;
             l1 += e1;
             w[j >> 1] = A::pack(e0, e1);
+            r0 += A::low(w[j >> 1]);
+            r1 += A::high(w[j >> 1]);
           }
           l0 += l1;
           const bool raise = top == -pos_inf<float>() || !(l0 <= F::MOST);
@@ -267,18 +270,21 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             const float to = raise && m > top ? m : top;
             const float shrink = to == top ? 1.f : t5_ex2(top - to);  // from -inf: 0
             const float to_sub = to == -pos_inf<float>() ? 0.f : to;
-            l0 = l1 = 0.f;
+            l0 = l1 = r0 = r1 = 0.f;
 #pragma unroll
             for (int j = 0; j < AT_SUB; j += 2) {
               const float e0 = t5_ex2(x[j] + (sub - to_sub)), e1 = t5_ex2(x[j + 1] + (sub - to_sub));
               l0 += e0;
               l1 += e1;
               w[j >> 1] = A::pack(e0, e1);
+              r0 += A::low(w[j >> 1]);
+              r1 += A::high(w[j >> 1]);
             }
             l0 += l1;
             top = to;
             sub = to_sub;
             sum *= shrink;
+            sum16 *= shrink;
             if (!first) {
               // the product of the group's step before has to be in
               ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
@@ -296,13 +302,14 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             }
           }
           sum += l0;
+          sum16 += r0 + r1;
         } else {
           if (lane == 0) t5_mbar_arrive(&s_free[pair]);
 #pragma unroll
           for (int j = 0; j < AT_SUB / 2; ++j) w[j] = 0u;
         }
         // the weights of the group's step before have been taken
-        if (!first) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
+        if (!__all_sync(FULL_MASK, taken)) ok = t5_mbar_wait_warp(&a_done[grp], (k - 1) & 1, failed);
         if (!ok) break;
         t5_fence_after();
         t5_st16(t_p, w);
@@ -322,10 +329,11 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       if (bad) bad_s = 1;
       s_top[grp][lrow] = top;
       s_sum[grp][lrow] = sum;
+      s_sum16[grp][lrow] = sum16;
       asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
       if (!(scan && *(volatile int *)&bad_s)) {
         // join the groups: each takes CP / G channels of the row
-        float all_top = -pos_inf<float>(), all_sum = 0.f, part[G];
+        float all_top = -pos_inf<float>(), all_sum = 0.f, all_sum16 = 0.f, part[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) all_top = fmaxf(all_top, s_top[g][lrow]);
         const float all_sub = all_top == -pos_inf<float>() ? 0.f : all_top;
@@ -333,9 +341,10 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         for (int g = 0; g < G; ++g) {
           part[g] = t5_ex2(s_top[g][lrow] - all_sub);
           all_sum = fmaf(part[g], s_sum[g][lrow], all_sum);
+          all_sum16 = fmaf(part[g], s_sum16[g][lrow], all_sum16);
         }
         const bool store = mine && row < tile.t1, none = all_sum == 0.f;
-        const float nan = __int_as_float(0x7fffffff), inv = none ? 0.f : 1.f / all_sum;
+        const float nan = __int_as_float(0x7fffffff), inv = none ? 0.f : 1.f / all_sum16;
         T *dst = (T *)a.out + (row * p.heads + head) * p.channels;
         T *dst2 = rest ? rest + (row * p.heads + head) * p.channels : nullptr;
 #pragma unroll

@@ -138,6 +138,8 @@ struct AtType<__nv_bfloat16> {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
   }
+  __device__ __forceinline__ static float low(uint32_t v) { return __uint_as_float(v << 16); }
+  __device__ __forceinline__ static float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 };
 template <>
 struct AtType<__half> {
@@ -150,6 +152,8 @@ struct AtType<__half> {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
   }
+  __device__ __forceinline__ static float low(uint32_t v) { return __low2float(*reinterpret_cast<const __half2 *>(&v)); }
+  __device__ __forceinline__ static float high(uint32_t v) { return __high2float(*reinterpret_cast<const __half2 *>(&v)); }
 };
 
 template <typename T>
@@ -194,6 +198,24 @@ struct AtRing {
       parity ^= 1u;
     }
   }
+};
+
+// The columns [lo, hi) that the rows of a warp see, relative to the pass's first: a step can be skipped where no row sees
+// any of its columns, and needs no mask where every row sees all of them.
+struct AtSeen {
+  int lo, hi, any_lo, any_hi, all_lo, all_hi;
+  __device__ __forceinline__ AtSeen(int64_t row_lo, int64_t row_hi, const AtPass &pass, bool mine) {
+    const int64_t count = pass.c_hi - pass.c_lo, l = mine ? row_lo - pass.c_lo : 0, h = mine ? row_hi - pass.c_lo : 0;
+    lo = (int)(l < 0 ? 0 : l > count ? count : l);
+    hi = (int)(h < 0 ? 0 : h > count ? count : h);
+    const bool none = lo >= hi;
+    any_lo = __reduce_min_sync(FULL_MASK, none ? 0x7fffffff : lo);
+    any_hi = __reduce_max_sync(FULL_MASK, none ? 0 : hi);
+    all_lo = __reduce_max_sync(FULL_MASK, none ? 0x7fffffff : lo);
+    all_hi = __reduce_min_sync(FULL_MASK, none ? 0 : hi);
+  }
+  __device__ __forceinline__ bool any(int base) const { return base < any_hi && base + AT_SUB > any_lo; }
+  __device__ __forceinline__ bool all(int base) const { return base >= all_lo && base + AT_SUB <= all_hi; }
 };
 
 // Coordinates of a stage's columns: a lane's share in registers, then [dims][64] in shared memory.

@@ -58,6 +58,14 @@ __device__ __forceinline__ bool t5_mbar_wait_warp(uint64_t *bar, uint32_t parity
   return __all_sync(FULL_MASK, t5_mbar_wait(bar, parity, failed));
 }
 
+// two barriers at once (the second only if `second`): where both are over already, one round trip instead of two
+__device__ __forceinline__ bool t5_mbar_wait_both(uint64_t *a, uint32_t pa, uint64_t *b, uint32_t pb, bool second,
+                                                  volatile int *failed) {
+  const bool ta = t5_mbar_try(a, pa), tb = !second || t5_mbar_try(b, pb);
+  if (__all_sync(FULL_MASK, ta && tb)) return true;
+  return t5_mbar_wait_warp(a, pa, failed) && (!second || t5_mbar_wait_warp(b, pb, failed));
+}
+
 // a box of a 3-d tensor to shared memory, without multicast
 __device__ __forceinline__ void t5_tma_3d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, uint64_t *bar) {
   asm volatile(
