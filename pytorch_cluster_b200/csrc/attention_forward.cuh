@@ -145,7 +145,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         float place[DIM == 0 ? 1 : 2 * DIM];
         at_fetch_places<DIM>(place, p.pos_k, p.dims, c0, pass.c_hi, lane);
         // the stage's round before this one is through
-        if (g >= F::STAGES) ok = t5_mbar_wait_warp(&empty[st], ring.parity ^ 1u, failed);
+        if (g >= F::STAGES) ok = t5_mbar_wait_idle(&empty[st], ring.parity ^ 1u, failed);
         if (!ok) break;
         unsigned char *dst = stages + st * F::STAGE_BYTES;
         if (lane == 0) {
@@ -170,8 +170,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       AtRing<F::STAGES> ring(stage0);
       for (uint32_t g = stage0; g < stage0 + stages_now && ok; ++g, ring.next()) {
         const uint32_t pair = g % F::PAIRS, k = g / F::PAIRS;
-        ok = t5_mbar_wait_warp(&full[ring.st], ring.parity, failed);
-        if (ok && k > 0) ok = t5_mbar_wait_warp(&s_free[pair], (k - 1) & 1, failed);
+        ok = t5_mbar_wait_idle(&full[ring.st], ring.parity, failed);
+        if (ok && k > 0) ok = t5_mbar_wait_idle(&s_free[pair], (k - 1) & 1, failed);
         if (!ok) break;
         t5_fence_after();
         const uint64_t d = d_k + ring.st * (F::STAGE_BYTES / 16);
@@ -194,7 +194,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t gr = 2 * pair + h;
-          if (ok) ok = t5_mbar_wait_warp(&w_ready[gr], k & 1, failed);
+          if (ok) ok = t5_mbar_wait_idle(&w_ready[gr], k & 1, failed);
           if (!ok) break;
           t5_fence_after();
           const uint64_t d = d_v + ring.st * (F::STAGE_BYTES / 16) + h * (AT_SUB * 128 / 16);

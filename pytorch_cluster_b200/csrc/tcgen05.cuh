@@ -53,6 +53,19 @@ __device__ __forceinline__ bool t5_mbar_wait(uint64_t *bar, uint32_t parity, vol
   return false;
 }
 
+// The same for a warp that has nothing else to do and whose answer is not waited for at once: it sleeps between
+// its looks, which otherwise take issue slots from the warps that work (forward 692 -> 688 us, dq 754 -> 740).
+constexpr unsigned T5_SLEEP_NS = 60;
+__device__ __forceinline__ bool t5_mbar_wait_idle(uint64_t *bar, uint32_t parity, volatile int *failed) {
+  bool over = __all_sync(FULL_MASK, t5_mbar_try(bar, parity));
+  for (int i = 0; i < T5_SPIN_LIMIT / 8 && !over; ++i) {
+    __nanosleep(T5_SLEEP_NS);
+    over = __all_sync(FULL_MASK, t5_mbar_try(bar, parity));
+    if (!over && __any_sync(FULL_MASK, *failed)) return false;
+  }
+  if (!over) *failed = 1;
+  return over;
+}
 // the same by a whole warp, with one answer
 __device__ __forceinline__ bool t5_mbar_wait_warp(uint64_t *bar, uint32_t parity, volatile int *failed) {
   return __all_sync(FULL_MASK, t5_mbar_wait(bar, parity, failed));
