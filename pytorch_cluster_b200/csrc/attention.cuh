@@ -50,16 +50,16 @@ __device__ __forceinline__ __nv_bfloat16 at_round<__nv_bfloat16>(float v) { retu
 
 // Rows [lo, hi) of one side that belong to segment b, clipped to the rows there are: an unsorted batch vector gives
 // wrong segments, never an access out of range.
+__device__ __forceinline__ void at_clip(int64_t from, int64_t to, int64_t rows, int64_t &lo, int64_t &hi) {
+  lo = from < 0 ? 0 : from;
+  hi = to > rows ? rows : to;
+  if (hi < lo) hi = lo;
+}
 __device__ __forceinline__ void at_segment(const int64_t *__restrict__ ptr, int64_t rows, int64_t b, int64_t &lo,
                                            int64_t &hi) {
   lo = 0;
   hi = rows;
-  if (ptr == nullptr) return;
-  lo = ptr[b];
-  hi = ptr[b + 1];
-  if (lo < 0) lo = 0;
-  if (hi > rows) hi = rows;
-  if (hi < lo) hi = lo;
+  if (ptr != nullptr) at_clip(ptr[b], ptr[b + 1], rows, lo, hi);
 }
 
 int launch_attention_plain_forward(const AttnArgs &a);

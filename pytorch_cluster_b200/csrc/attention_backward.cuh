@@ -29,6 +29,7 @@ struct AtBackward {
   static constexpr int W_COLS = AT_SUB;  // a group's dS and P, or dS in two parts
   static constexpr int PAIRS = G / 2, PAIR_COLS = 2 * AT_COLS + 2 * W_COLS;  // S, dP of a stage, two groups' weights
   static constexpr int TMEM = BLOCKS == 2 ? 256 : 512;
+  static_assert(STAGES * STAGE_BYTES >= 2 * ROW_BYTES, "the ring takes the block's rows");
   static_assert(PAIRS * PAIR_COLS + (KV ? 2 : 1) * CP <= TMEM, "tensor memory");
   static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
@@ -80,6 +81,21 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   else
     tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
 
+  // element threads: a row each
+  const bool element = warp < F::EL_WARPS;
+  const int grp = warp >> 2, lrow = tid & (AT_ROWS - 1);
+  const int64_t row = tile.t0 + lrow;
+  float pos[DIM == 0 ? 1 : DIM], lse = 0.f, delta = 0.f;
+  if constexpr (DIM > 0) {
+    const float *src = KV ? p.pos_k : p.pos_q;
+#pragma unroll
+    for (int d = 0; d < DIM; ++d) pos[d] = element && row < tile.t1 && d < p.dims ? src[row * p.dims + d] : 0.f;
+  }
+  if (!KV && element && row < tile.t1) {
+    lse = a.lse[(int64_t)head0 * p.m + row] - A::SHIFT;
+    delta = a.delta[(int64_t)head0 * p.m + row];
+  }
+
   if (tid == 64) {
     t5_mbar_init(&r_full, 1);
     for (int i = 0; i < F::STAGES; ++i) {
@@ -118,31 +134,19 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   }
   tile.found(shared_tile);
   if (tile.listed()) {
-    if (tid <= tile.b_last - tile.b_first) shared_tile.ends[tid] = tile.ptr_r[tile.b_first + 1 + tid];
+    tile.list(shared_tile, tid);
     __syncthreads();
   }
 
-  // element threads: a row each
-  const bool element = warp < F::EL_WARPS;
-  const int grp = warp >> 2, lrow = tid & (AT_ROWS - 1);
-  const int64_t row = tile.t0 + lrow;
+  // element threads: the columns that the row sees
   int64_t row_lo = 0, row_hi = 0;
   int row_segment = -1;
-  float pos[DIM == 0 ? 1 : DIM], lse = 0.f, delta = 0.f;
   if (element && row < tile.t1) {
     row_segment = tile.segment(shared_tile, row);
     int64_t lo, hi;
-    at_segment(tile.ptr_r, tile.rows, row_segment, lo, hi);
-    if (row >= lo && row < hi) at_segment(tile.ptr_c, tile.cols, row_segment, row_lo, row_hi);
-    if (!KV) {
-      lse = a.lse[(int64_t)head0 * p.m + row] - A::SHIFT;
-      delta = a.delta[(int64_t)head0 * p.m + row];
-    }
-  }
-  if constexpr (DIM > 0) {
-    const float *src = KV ? p.pos_k : p.pos_q;
-#pragma unroll
-    for (int d = 0; d < DIM; ++d) pos[d] = element && row < tile.t1 && d < p.dims ? src[row * p.dims + d] : 0.f;
+    tile.rows_of(shared_tile, row_segment, lo, hi);
+    if (row >= lo && row < hi) tile.cols_of(shared_tile, row_segment, row_lo, row_hi);
+    if (grp == 0) shared_tile.segment[lrow] = row_segment;
   }
   const float pre = CAP ? 2.f * AT_LOG2E * p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
   const float sigma = at_sigma<T>(norms);
@@ -150,7 +154,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
 
   bool by_example = false;
   int64_t next_row = tile.t0;
-  AtPass pass = tile.all();
+  AtPass pass = tile.all(shared_tile);
   const bool mixed = tile.b_first != tile.b_last;
   uint32_t stage0 = 0, passes = 0, issued = 0;
   bool ok = true;
@@ -367,7 +371,6 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
       if (bad) bad_s = 1;
       if (scan) asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
       if (!(scan && *(volatile int *)&bad_s)) {
-        const bool store = mine && row < tile.t1;
         const float nan = __int_as_float(0x7fffffff);
         // the results' channels in chunks of 32, dealt out to the groups
         constexpr int CHUNKS = (KV ? 2 : 1) * CP / 32;
@@ -375,15 +378,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
         for (int ch = grp; ch < CHUNKS; ch += G) {
           const int c = ch * 32 % CP;
           const bool is_dv = KV && ch * 32 < CP;
-          T *dst;
-          float times = p.scale / sigma;
-          if constexpr (KV) {
-            dst = (is_dv ? (T *)a.dv : (T *)a.dk) + (row * p.groups + group) * p.channels;
-            if (is_dv) times = A::BF16 ? 1.f : 1.f / 4096.f;
-          } else {
-            dst = (T *)a.dq + (row * p.heads + head0) * p.channels;
-          }
-          if (!ok) times = nan;
+          const float times = !ok ? nan : is_dv ? (A::BF16 ? 1.f : 1.f / 4096.f) : p.scale / sigma;
           float o[32] = {};
           if (count > 0 && ok) {
             t5_ld32(t_acc + lane_base + ch * 32, o);
@@ -395,9 +390,21 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
             uint32_t *po = reinterpret_cast<uint32_t *>(&out);
 #pragma unroll
             for (int k = 0; k < 4; ++k) po[k] = A::pack(o[i + 2 * k] * times, o[i + 2 * k + 1] * times);
-            if (store && c + i < p.channels) *reinterpret_cast<uint4 *>(dst + c + i) = out;
+            at_put<CP>(is_dv || !KV ? stages : stages + F::ROW_BYTES, lrow, (c + i) / 8, out);
           }
         }
+        asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
+        if constexpr (KV) {
+          const int64_t stride = (int64_t)p.groups * p.channels;
+          at_write_rows<T, CP>(stages, shared_tile, tile, pass, (T *)a.dv + (int64_t)group * p.channels, stride, p.channels,
+                               tid, F::EL_THREADS);
+          at_write_rows<T, CP>(stages + F::ROW_BYTES, shared_tile, tile, pass, (T *)a.dk + (int64_t)group * p.channels,
+                               stride, p.channels, tid, F::EL_THREADS);
+        } else {
+          at_write_rows<T, CP>(stages, shared_tile, tile, pass, (T *)a.dq + (int64_t)head0 * p.channels,
+                               (int64_t)p.heads * p.channels, p.channels, tid, F::EL_THREADS);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring takes copies again
       }
     }
     stage0 += stages_now;

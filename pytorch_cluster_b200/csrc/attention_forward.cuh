@@ -26,6 +26,7 @@ struct AtForward {
   static constexpr int SMEM = Q_BYTES + STAGES * (STAGE_BYTES + POS_BYTES) + 1024;
   static constexpr int PAIRS = G / 2, PAIR_COLS = AT_COLS + AT_SUB;  // scores of a stage, two groups' weights
   static constexpr int TMEM = CP == 64 ? 256 : 512;
+  static_assert(STAGES * STAGE_BYTES >= 2 * Q_BYTES, "the ring takes the block's rows");
   static_assert(PAIRS * PAIR_COLS + G * CP <= TMEM, "tensor memory");
   static constexpr float MOST = 1024.f;  // sum of a step's weights that needs no new maximum
 };
@@ -60,6 +61,17 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   const int head = blockIdx.y, group = head / (p.heads / p.groups);
   AtTile tile;
   tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
+
+  // element threads: a row each
+  const bool element = warp < F::EL_WARPS;
+  const int grp = warp >> 2, lrow = tid & (AT_ROWS - 1);
+  const int64_t row = tile.t0 + lrow;
+  float pos[DIM == 0 ? 1 : DIM], slope2 = 0.f;
+  if constexpr (DIM > 0) {
+    slope2 = p.slope[head] * AT_LOG2E;
+#pragma unroll
+    for (int d = 0; d < DIM; ++d) pos[d] = element && row < tile.t1 && d < p.dims ? p.pos_q[row * p.dims + d] : 0.f;
+  }
 
   if (tid == 64) {
     t5_mbar_init(&q_full, 1);
@@ -98,33 +110,25 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   }
   tile.found(shared_tile);
   if (tile.listed()) {
-    if (tid <= tile.b_last - tile.b_first) shared_tile.ends[tid] = tile.ptr_r[tile.b_first + 1 + tid];
+    tile.list(shared_tile, tid);
     __syncthreads();
   }
 
-  // element threads: a row each
-  const bool element = warp < F::EL_WARPS;
-  const int grp = warp >> 2, lrow = tid & (AT_ROWS - 1);
-  const int64_t row = tile.t0 + lrow;
-  int64_t row_lo = 0, row_hi = 0;  // the columns it sees
+  // element threads: the columns that the row sees
+  int64_t row_lo = 0, row_hi = 0;
   int row_segment = -1;
-  float pos[DIM == 0 ? 1 : DIM], slope2 = 0.f;
   if (element && row < tile.t1) {
     row_segment = tile.segment(shared_tile, row);
     int64_t lo, hi;
-    at_segment(tile.ptr_r, p.m, row_segment, lo, hi);
-    if (row >= lo && row < hi) at_segment(tile.ptr_c, p.n, row_segment, row_lo, row_hi);
-  }
-  if constexpr (DIM > 0) {
-    slope2 = p.slope[head] * AT_LOG2E;
-#pragma unroll
-    for (int d = 0; d < DIM; ++d) pos[d] = element && row < tile.t1 && d < p.dims ? p.pos_q[row * p.dims + d] : 0.f;
+    tile.rows_of(shared_tile, row_segment, lo, hi);
+    if (row >= lo && row < hi) tile.cols_of(shared_tile, row_segment, row_lo, row_hi);
+    if (grp == 0) shared_tile.segment[lrow] = row_segment;
   }
   const float pre = CAP ? 2.f * AT_LOG2E * p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
 
   bool by_example = false;
   int64_t next_row = tile.t0;
-  AtPass pass = tile.all();
+  AtPass pass = tile.all(shared_tile);
   const bool mixed = tile.b_first != tile.b_last;
   uint32_t stage0 = 0, passes = 0;  // stages, and passes with any, so far
   uint32_t issued = 0;              // copy warp: stages whose copies were issued
@@ -250,6 +254,18 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             for (int j = 0; j < AT_SUB; ++j)
               if (base + j < seen.lo || base + j >= seen.hi) x[j] = -pos_inf<float>();
           }
+          // rows that see their first columns here (sub is 0): the maximum is looked for
+          const bool fresh = top == -pos_inf<float>() && seen.lo < base + AT_SUB && seen.hi > base && seen.lo < seen.hi;
+          if (__any_sync(FULL_MASK, fresh)) {
+            float m = x[0];
+#pragma unroll
+            for (int j = 1; j < AT_SUB; ++j) m = fmaxf(m, x[j]);
+            if (fresh && m > -pos_inf<float>()) {
+              top = sub = m;
+#pragma unroll
+              for (int j = 0; j < AT_SUB; ++j) x[j] -= m;
+            }
+          }
           float l0 = 0.f, l1 = 0.f, r0 = 0.f, r1 = 0.f;
 #pragma unroll
           for (int j = 0; j < AT_SUB; j += 2) {
@@ -261,7 +277,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             r1 += A::high(w[j >> 1]);
           }
           l0 += l1;
-          const bool raise = top == -pos_inf<float>() || !(l0 <= F::MOST);
+          const bool raise = !(l0 <= F::MOST);
           if (__any_sync(FULL_MASK, raise)) {
             float m = x[0];
 #pragma unroll
@@ -343,10 +359,9 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           all_sum = fmaf(part[g], s_sum[g][lrow], all_sum);
           all_sum16 = fmaf(part[g], s_sum16[g][lrow], all_sum16);
         }
-        const bool store = mine && row < tile.t1, none = all_sum == 0.f;
+        const bool none = all_sum == 0.f;
         const float nan = __int_as_float(0x7fffffff), inv = none ? 0.f : 1.f / all_sum16;
-        T *dst = (T *)a.out + (row * p.heads + head) * p.channels;
-        T *dst2 = rest ? rest + (row * p.heads + head) * p.channels : nullptr;
+        unsigned char *tile_out = stages, *tile_rest = stages + AT_ROWS * CP * 2;
 #pragma unroll
         for (int cc = 0; cc < CP / G; cc += 32) {
           const int c = grp * (CP / G) + cc;
@@ -374,14 +389,20 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
               const T *h = reinterpret_cast<const T *>(&po[e]);
               pl[e] = A::pack(x0 - at_float(h[0]), x1 - at_float(h[1]));
             }
-            if (store && c + i < p.channels) {
-              *reinterpret_cast<uint4 *>(dst + c + i) = out;
-              if (dst2) *reinterpret_cast<uint4 *>(dst2 + c + i) = low;
-            }
+            at_put<CP>(tile_out, lrow, (c + i) / 8, out);
+            if (rest) at_put<CP>(tile_rest, lrow, (c + i) / 8, low);
           }
         }
-        if (a.lse && store && grp == 0)
+        if (a.lse && mine && row < tile.t1 && grp == 0)
           a.lse[(int64_t)head * p.m + row] = none ? pos_inf<float>() : all_top + log2f(all_sum);
+        asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
+        const int64_t stride = (int64_t)p.heads * p.channels;
+        at_write_rows<T, CP>(tile_out, shared_tile, tile, pass, (T *)a.out + (int64_t)head * p.channels, stride,
+                             p.channels, tid, F::EL_THREADS);
+        if (rest)
+          at_write_rows<T, CP>(tile_rest, shared_tile, tile, pass, rest + (int64_t)head * p.channels, stride, p.channels,
+                               tid, F::EL_THREADS);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring takes copies again
       }
     }
     stage0 += stages_now;

@@ -59,7 +59,8 @@ struct AtPass {
 // What the threads of a block find out together about its rows.
 struct AtTileShared {
   int b_first, b_last;
-  int64_t ends[AT_ROWS];  // ptr[b_first + 1 ...], as far as the tile's segments go
+  int64_t r[AT_ROWS + 1], c[AT_ROWS + 1];  // both sides' pointers from b_first on, as far as the tile's segments go
+  int segment[AT_ROWS];                    // of each row
 };
 
 struct AtTile {
@@ -89,26 +90,45 @@ struct AtTile {
     b_first = sh.b_first;
     b_last = sh.b_last;
   }
-  __device__ __forceinline__ bool listed() const { return b_last > b_first && b_last - b_first < AT_ROWS; }
-  // the segment of a row of the tile; `ends` is filled where listed()
+  // whether the tile's segments are few enough to be listed; then all threads do so, and a barrier follows
+  __device__ __forceinline__ bool listed() const { return ptr_r != nullptr && b_last - b_first < AT_ROWS - 1; }
+  __device__ __forceinline__ void list(AtTileShared &sh, int tid) const {
+    if (tid <= b_last - b_first + 1) {
+      sh.r[tid] = ptr_r[b_first + tid];
+      sh.c[tid] = ptr_c[b_first + tid];
+    }
+  }
   __device__ __forceinline__ int segment(const AtTileShared &sh, int64_t row) const {
     if (b_first == b_last) return b_first;
     if (!listed()) return segment_of(ptr_r, segments, row);
     int lo = 0, hi = b_last - b_first;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (sh.ends[mid] > row)
+      if (sh.r[mid + 1] > row)
         hi = mid;
       else
         lo = mid + 1;
     }
     return b_first + lo;
   }
-  __device__ __forceinline__ AtPass all() const {
+  // rows and columns of a segment of the tile, clipped as at_segment does
+  __device__ __forceinline__ void rows_of(const AtTileShared &sh, int b, int64_t &lo, int64_t &hi) const {
+    if (listed())
+      at_clip(sh.r[b - b_first], sh.r[b - b_first + 1], rows, lo, hi);
+    else
+      at_segment(ptr_r, rows, b, lo, hi);
+  }
+  __device__ __forceinline__ void cols_of(const AtTileShared &sh, int b, int64_t &lo, int64_t &hi) const {
+    if (listed())
+      at_clip(sh.c[b - b_first], sh.c[b - b_first + 1], cols, lo, hi);
+    else
+      at_segment(ptr_c, cols, b, lo, hi);
+  }
+  __device__ __forceinline__ AtPass all(const AtTileShared &sh) const {
     AtPass p;
     int64_t unused;
-    at_segment(ptr_c, cols, b_first, p.c_lo, unused);
-    at_segment(ptr_c, cols, b_last, unused, p.c_hi);
+    cols_of(sh, b_first, p.c_lo, unused);
+    cols_of(sh, b_last, unused, p.c_hi);
     if (p.c_hi < p.c_lo) p.c_hi = p.c_lo;
     p.segment = -1;
     return p;
@@ -283,6 +303,27 @@ __device__ __forceinline__ void at_logits(float *s, float *u, const float *col_p
         t = fmaf(-slope2, t5_sqrt(d2[j]), t);
       s[j4 + j] = t;
     }
+  }
+}
+
+// A block's rows leave by way of shared memory (the ring, idle at the end of a pass): a thread has 16 bytes of its row in
+// hand at a time, and 32 rows' worth of them would be 32 places for the memory to go to.  16-byte chunk c of row r is kept
+// at c ^ (r & 7).
+template <int CP>
+__device__ __forceinline__ void at_put(unsigned char *tile, int r, int chunk, const uint4 &v) {
+  *reinterpret_cast<uint4 *>(tile + r * (CP * 2) + ((chunk ^ (r & 7)) << 4)) = v;
+}
+// rows of the pass to dst + row * stride (elements)
+template <typename T, int CP>
+__device__ __forceinline__ void at_write_rows(const unsigned char *tile, const AtTileShared &sh, const AtTile &t,
+                                              const AtPass &pass, T *dst, int64_t stride, int channels, int tid,
+                                              int threads) {
+  constexpr int CHUNKS = CP / 8;
+  for (int i = tid; i < AT_ROWS * CHUNKS; i += threads) {
+    const int r = i / CHUNKS, c = i % CHUNKS;
+    if (t.t0 + r < t.t1 && (pass.segment < 0 || pass.segment == sh.segment[r]) && c * 8 < channels)
+      *reinterpret_cast<uint4 *>(dst + (t.t0 + r) * stride + c * 8) =
+          *reinterpret_cast<const uint4 *>(tile + r * (CP * 2) + ((c ^ (r & 7)) << 4));
   }
 }
 
