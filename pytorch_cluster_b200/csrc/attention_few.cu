@@ -7,10 +7,7 @@
 // split's keys in turn, U keys ahead of their use, each with a running maximum, sum and result of its own, which are
 // joined by shuffles and through shared memory at the end.  The splits' parts go to the workspace in fp32 and a second kernel joins
 // them, in ascending order of the splits.
-#include <type_traits>
-
-#include "attention.cuh"
-#include "tcgen05.cuh"
+#include "attention_warp.cuh"
 
 namespace b200c {
 
@@ -228,38 +225,6 @@ constexpr int AF_KEYS = 32;    // keys of a stage
 constexpr int AF_STAGES = 3;
 constexpr int AF_ROWS = 16;    // rows (query, head of the group) of a pass
 
-template <typename T>
-__device__ __forceinline__ void af_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void af_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void af_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t af_pack(float lo, float hi) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-  }
-}
-
 template <int CP>
 struct AfTensor {
   static constexpr int CHUNKS = CP / 8;  // 16-byte chunks of a row
@@ -393,9 +358,9 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnAr
         for (int n = 0; n < NT; n += 2) {
           const int r = n * 8 + (lane & 7) + ((lane & 16) >> 1), c = 2 * t + ((lane >> 3) & 1);
           uint32_t kf[4];
-          af_ldmatrix(kf, st + r * (CP * 2) + ((c ^ (r & 7)) << 4));
-          af_mma<T>(s[n], qf[t], kf[0], kf[1]);
-          af_mma<T>(s[n + 1], qf[t], kf[2], kf[3]);
+          aw_ldmatrix(kf, st + r * (CP * 2) + ((c ^ (r & 7)) << 4));
+          aw_mma<T>(s[n], qf[t], kf[0], kf[1]);
+          aw_mma<T>(s[n + 1], qf[t], kf[2], kf[3]);
         }
       const bool whole = j0 + AF_KEYS <= hi;
 #pragma unroll
@@ -452,15 +417,15 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnAr
       }
 #pragma unroll
       for (int t = 0; t < NT / 2; ++t) {  // 16 keys of the weights against 16 channels a matrix load
-        const uint32_t wf[4] = {af_pack<T>(s[2 * t][0], s[2 * t][1]), af_pack<T>(s[2 * t][2], s[2 * t][3]),
-                                af_pack<T>(s[2 * t + 1][0], s[2 * t + 1][1]), af_pack<T>(s[2 * t + 1][2], s[2 * t + 1][3])};
+        const uint32_t wf[4] = {aw_pack<T>(s[2 * t][0], s[2 * t][1]), aw_pack<T>(s[2 * t][2], s[2 * t][3]),
+                                aw_pack<T>(s[2 * t + 1][0], s[2 * t + 1][1]), aw_pack<T>(s[2 * t + 1][2], s[2 * t + 1][3])};
 #pragma unroll
         for (int n = 0; n < CT; n += 2) {
           const int r = t * 16 + (lane & 15), c = n + (lane >> 4);
           uint32_t vf[4];
-          af_ldmatrix_t(vf, st + F::TILE + r * (CP * 2) + ((c ^ (r & 7)) << 4));
-          af_mma<T>(o[n], wf, vf[0], vf[1]);
-          af_mma<T>(o[n + 1], wf, vf[2], vf[3]);
+          aw_ldmatrix_t(vf, st + F::TILE + r * (CP * 2) + ((c ^ (r & 7)) << 4));
+          aw_mma<T>(o[n], wf, vf[0], vf[1]);
+          aw_mma<T>(o[n + 1], wf, vf[2], vf[3]);
         }
       }
       __syncwarp();  // the stage is read: it takes the step two ahead

@@ -55,18 +55,28 @@ bool attention_tensor_applicable(const b200c_attention_t &p) {
          at_side(p.v, p.n, p.groups, p.v_row, p.v_head);
 }
 
+// Mean rows per example, on either side, up to which the kernels of attention_short.cuh are taken (SHORT_RULE).
+constexpr int64_t AT_SHORT_ROWS = 64;
+static bool is_short(const b200c_attention_t &p) {
+  return p.channels <= 64 && p.m <= AT_SHORT_ROWS * p.num_segments && p.n <= AT_SHORT_ROWS * p.num_segments;
+}
+
 int launch_attention_tensor_forward(const AttnArgs &a) {
-  return a.p.dtype == B200C_BF16 ? attention_tensor_forward_bf16(a) : attention_tensor_forward_f16(a);
+  const bool bf16 = a.p.dtype == B200C_BF16;
+  if (is_short(a.p)) return bf16 ? attention_short_forward_bf16(a) : attention_short_forward_f16(a);
+  return bf16 ? attention_tensor_forward_bf16(a) : attention_tensor_forward_f16(a);
 }
 
 int launch_attention_tensor_backward(const AttnArgs &a) {
-  const bool bf16 = a.p.dtype == B200C_BF16;
+  const bool bf16 = a.p.dtype == B200C_BF16, brief = is_short(a.p);
   if (a.dq) {
-    const int st = bf16 ? attention_tensor_dq_bf16(a) : attention_tensor_dq_f16(a);
+    const int st = brief ? bf16 ? attention_short_dq_bf16(a) : attention_short_dq_f16(a)
+                         : bf16 ? attention_tensor_dq_bf16(a) : attention_tensor_dq_f16(a);
     if (st != B200C_OK) return st;
   }
-  if (a.dk) return bf16 ? attention_tensor_dkv_bf16(a) : attention_tensor_dkv_f16(a);
-  return B200C_OK;
+  if (!a.dk) return B200C_OK;
+  if (brief) return bf16 ? attention_short_dkv_bf16(a) : attention_short_dkv_f16(a);
+  return bf16 ? attention_tensor_dkv_bf16(a) : attention_tensor_dkv_f16(a);
 }
 
 }  // namespace b200c

@@ -152,6 +152,11 @@ SHAPES = [
     ([50], [50], 2, 2, 5, 2, None),      # channels that no 16-byte access fits
     ([40, 90], [90, 40], 1, 1, 1, 0, None),
     ([700, 500], [700, 500], 2, 2, 64, 3, None),
+    ([33, 1, 47, 16, 15, 0, 70], [33, 1, 47, 16, 15, 0, 70], 5, 5, 64, 3, 8.0),
+    ([12] * 30, [12] * 30, 8, 2, 16, 1, None),
+    ([2] * 100, [150] + [1] * 99, 4, 1, 48, 0, None),
+    ([40] * 7, [3] * 7, 6, 6, 32, 8, None),
+    ([30, 0, 17, 60, 5], [12, 40, 0, 60, 1], 3, 1, 80, 3, None),  # short examples with more channels
 ]
 
 
@@ -197,13 +202,14 @@ def test_attention_large_scores(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attention_keeps_nan_and_infinities_in_their_example(dtype):
+@pytest.mark.parametrize("channels", [64, 128])  # rows of short examples, 16 at a time and 128 at a time
+def test_attention_keeps_nan_and_infinities_in_their_example(dtype, channels):
     import pytorch_cluster_b200 as pc
 
     lens = [20, 45, 3, 90, 130, 7]
     g = gen(3)
     n, b = sum(lens), ids(lens)
-    q, k, v, do = (rand(g, n, 2, 64, dtype=dtype) for _ in range(4))
+    q, k, v, do = (rand(g, n, 2, channels, dtype=dtype) for _ in range(4))
     pos = rand(g, n, 3, dtype=torch.float32)
     slope = torch.tensor([0.5, 1.0], device="cuda")
 
