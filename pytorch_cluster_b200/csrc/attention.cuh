@@ -32,6 +32,8 @@ struct AttnArgs {
   const float *delta = nullptr;  // [heads, m]: D_i
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // [m, heads, channels], [n, groups, channels] x 2
   const float *norms = nullptr;  // fp16: the largest |do|^2 and |v|^2 of a row
+  float *parts = nullptr;        // forward, split over the columns: [m, heads, splits, channels + 2] (maximum, sum, result)
+  int splits = 1;
   cudaStream_t stream = nullptr;
 };
 
@@ -71,5 +73,7 @@ int launch_attention_tensor_backward(const AttnArgs &a);
 int attention_few_splits(const b200c_attention_t &p);  // 0: not for this call
 size_t attention_few_workspace_bytes(const b200c_attention_t &p);
 int launch_attention_few(const AttnArgs &a, int splits, void *workspace);
+int launch_attention_join(const AttnArgs &a);          // a.parts of a.splits splits to out, rest and lse
+int attention_tensor_splits(const b200c_attention_t &p);  // of a forward pass without statistics
 
 }  // namespace b200c

@@ -7,6 +7,7 @@
 // split's keys in turn, U keys ahead of their use, each with a running maximum, sum and result of its own, which are
 // joined by shuffles and through shared memory at the end.  The splits' parts go to the workspace in fp32 and a second kernel joins
 // them, in ascending order of the splits.
+#include "attention_tensor.cuh"
 #include "attention_warp.cuh"
 
 namespace b200c {
@@ -481,48 +482,74 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnAr
   }
 }
 
-// joins the splits of a (row, head), in ascending order: a block of four warps each, a channel per thread
+// joins the splits of a (row, head), in ascending order, a warp each
 template <typename T>
-__global__ void __launch_bounds__(128) attention_few_join_kernel(AttnArgs a, int splits, const float *__restrict__ parts) {
-  __shared__ float factor[128];
-  __shared__ float s_top[4], s_sum[4];
+__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnArgs a) {
   const b200c_attention_t &p = a.p;
-  const int64_t i = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31, splits = a.splits;
+  if (i >= p.m * p.heads) return;
   const int64_t row = i / p.heads;
-  const int head = (int)(i % p.heads);
-  int64_t lo, hi;
-  at_segment(p.ptr_q, p.m, segment_of(p.ptr_q, p.num_segments, row), lo, hi);
-  const bool inside = row >= lo && row < hi;
-  const int width = p.channels + 2;
-  const float *src = parts + i * splits * width;
-  // at most 128 splits: one per thread (attention_few_splits)
-  const bool mine = inside && tid < splits;
-  const float top = mine ? src[(int64_t)tid * width] : -pos_inf<float>(), sum = mine ? src[(int64_t)tid * width + 1] : 0.f;
-  float m = top;
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
-  if (lane == 0) s_top[warp] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const float f = exp2f(top - (m == -pos_inf<float>() ? 0.f : m));
-  factor[tid] = f;
-  float l = sum * f;
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(FULL_MASK, l, o);
-  if (lane == 0) s_sum[warp] = l;
-  __syncthreads();
-  l = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (tid < p.channels) {
-    float acc = 0.f;
-    if (inside) {
-#pragma unroll 8
-      for (int s = 0; s < splits; ++s) acc = fmaf(src[(int64_t)s * width + 2 + tid], factor[s], acc);
-    }
-    const T r = at_round<T>(acc * inv);
-    ((T *)a.out)[i * p.channels + tid] = r;
-    if (a.rest) ((T *)a.rest)[i * p.channels + tid] = at_round<T>(acc * inv - at_float(r));
+  const int head = (int)(i % p.heads), width = p.channels + 2;
+  const float *src = a.parts + i * splits * width;
+  float top[4], sum[4], m = -pos_inf<float>();  // at most 128 splits: four per lane (attention_few_splits)
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int s = n * 32 + lane;
+    top[n] = s < splits ? src[(int64_t)s * width] : -pos_inf<float>();
+    sum[n] = s < splits ? src[(int64_t)s * width + 1] : 0.f;
   }
-  if (a.lse && tid == 0) a.lse[(int64_t)head * p.m + row] = l == 0.f ? pos_inf<float>() : m + log2f(l);
+  int64_t lo, hi;
+  at_segment(p.ptr_q, p.m, at_segment_of_warp(p.ptr_q, (int)p.num_segments, row, lane), lo, hi);
+  const bool inside = row >= lo && row < hi;  // else nothing was written there
+#pragma unroll
+  for (int n = 0; n < 4; ++n) m = fmaxf(m, top[n]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
+  const float sub = m == -pos_inf<float>() ? 0.f : m;
+  float l = 0.f;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    top[n] = t5_ex2(top[n] - sub);  // now the split's factor
+    l = fmaf(sum[n], top[n], l);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(FULL_MASK, l, o);
+  if (!inside) l = 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float acc[AT_MAX_CHANNELS / 32] = {};
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int most = splits - n * 32 < 32 ? splits - n * 32 : 32;
+#pragma unroll 4
+    for (int s = 0; s < most; ++s) {
+      const float f = __shfl_sync(FULL_MASK, top[n], s);
+#pragma unroll
+      for (int c = 0; c < AT_MAX_CHANNELS / 32; ++c)
+        if (c * 32 + lane < p.channels) acc[c] = fmaf(src[(int64_t)(n * 32 + s) * width + 2 + c * 32 + lane], f, acc[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < AT_MAX_CHANNELS / 32; ++c)
+    if (c * 32 + lane < p.channels) {
+      const float x = l == 0.f ? 0.f : acc[c] * inv;
+      const T r = at_round<T>(x);
+      ((T *)a.out)[i * p.channels + c * 32 + lane] = r;
+      if (a.rest) ((T *)a.rest)[i * p.channels + c * 32 + lane] = at_round<T>(x - at_float(r));
+    }
+  if (a.lse && lane == 0) a.lse[(int64_t)head * p.m + row] = l == 0.f ? pos_inf<float>() : m + log2f(l);
+}
+
+int launch_attention_join(const AttnArgs &a) {
+  const int64_t rows = a.p.m * a.p.heads;
+  if (a.p.dtype == B200C_F32)
+    attention_join_kernel<float><<<(unsigned)((rows + 7) / 8), 256, 0, a.stream>>>(a);
+  else if (a.p.dtype == B200C_F16)
+    attention_join_kernel<__half><<<(unsigned)((rows + 7) / 8), 256, 0, a.stream>>>(a);
+  else
+    attention_join_kernel<__nv_bfloat16><<<(unsigned)((rows + 7) / 8), 256, 0, a.stream>>>(a);
+  B200C_LAUNCH_CHECK("attention_join_kernel");
+  return B200C_OK;
 }
 
 // Queries of a group per example, on average, up to which this kernel is taken.  It reads the keys once for every
@@ -548,12 +575,11 @@ size_t attention_few_workspace_bytes(const b200c_attention_t &p) {
   return (size_t)p.m * p.heads * attention_few_splits(p) * (p.channels + 2) * 4;
 }
 
-template <typename T>
 static int af_join(const AttnArgs &a, int splits, float *parts) {
-  const int64_t rows = a.p.m * a.p.heads;
-  attention_few_join_kernel<T><<<(unsigned)rows, 128, 0, a.stream>>>(a, splits, parts);
-  B200C_LAUNCH_CHECK("attention_few_join_kernel");
-  return B200C_OK;
+  AttnArgs j = a;
+  j.splits = splits;
+  j.parts = parts;
+  return launch_attention_join(j);
 }
 
 template <typename T, int LPK, int QB>
@@ -561,7 +587,7 @@ static int af_launch(const AttnArgs &a, int splits, int vec, float *parts) {
   const unsigned blocks = (unsigned)(a.p.num_segments * a.p.groups * splits);
   attention_few_kernel<T, LPK, QB><<<blocks, AF_THREADS, 0, a.stream>>>(a, splits, vec, parts);
   B200C_LAUNCH_CHECK("attention_few_kernel");
-  return af_join<T>(a, splits, parts);
+  return af_join(a, splits, parts);
 }
 
 template <typename T, int CP, int DIM, bool CAP>
@@ -572,7 +598,7 @@ static int af_launch_tensor(const AttnArgs &a, int splits, float *parts) {
   const unsigned blocks = (unsigned)(a.p.num_segments * a.p.groups * splits);
   attention_few_tensor_kernel<T, CP, DIM, CAP><<<blocks, AF_THREADS, F::SMEM, a.stream>>>(a, splits, parts);
   B200C_LAUNCH_CHECK("attention_few_tensor_kernel");
-  return af_join<T>(a, splits, parts);
+  return af_join(a, splits, parts);
 }
 template <typename T, int CP, bool CAP>
 static int af_tensor_dims(const AttnArgs &a, int splits, float *parts) {

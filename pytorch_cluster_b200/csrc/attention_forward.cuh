@@ -129,6 +129,15 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   bool by_example = false;
   int64_t next_row = tile.t0;
   AtPass pass = tile.all(shared_tile);
+  // this block's share of a pass's columns, in whole stages
+  auto share = [&]() {
+    if (a.splits <= 1) return;
+    const int64_t each = (pass.c_hi - pass.c_lo + (int64_t)a.splits * AT_COLS - 1) / ((int64_t)a.splits * AT_COLS) * AT_COLS;
+    pass.c_lo += each * blockIdx.z;
+    if (pass.c_lo > pass.c_hi) pass.c_lo = pass.c_hi;
+    if (pass.c_lo + each < pass.c_hi) pass.c_hi = pass.c_lo + each;
+  };
+  share();
   const bool mixed = tile.b_first != tile.b_last;
   uint32_t stage0 = 0, passes = 0;  // stages, and passes with any, so far
   uint32_t issued = 0;              // copy warp: stages whose copies were issued
@@ -377,6 +386,19 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
               for (int i = 0; i < 32; ++i) r[i] = fmaf(o[i], part[g], r[i]);
             }
           }
+          if (a.splits > 1) {
+            if (mine && row < tile.t1) {
+              float *dst = a.parts + ((row * p.heads + head) * a.splits + blockIdx.z) * (p.channels + 2);
+              if (c == 0) {
+                dst[0] = ok ? all_top : nan;
+                dst[1] = all_sum16;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c + i < p.channels) dst[2 + c + i] = ok ? r[i] : nan;
+            }
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint4 out, low;
@@ -397,7 +419,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           a.lse[(int64_t)head * p.m + row] = none ? pos_inf<float>() : all_top + log2f(all_sum);
         asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
         const int64_t stride = (int64_t)p.heads * p.channels;
-        at_write_rows<T, CP>(tile_out, shared_tile, tile, pass, (T *)a.out + (int64_t)head * p.channels, stride,
+        if (a.splits == 1) at_write_rows<T, CP>(tile_out, shared_tile, tile, pass, (T *)a.out + (int64_t)head * p.channels, stride,
                              p.channels, tid, F::EL_THREADS);
         if (rest)
           at_write_rows<T, CP>(tile_rest, shared_tile, tile, pass, rest + (int64_t)head * p.channels, stride, p.channels,
@@ -416,8 +438,11 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       by_example = true;
     }
     if (!tile.next(next_row, pass)) break;
+    share();
   }
-  if (*failed && element && grp == 0 && row < tile.t1) {
+  if (*failed && element && grp == 0 && row < tile.t1 && a.splits > 1) {
+    a.parts[((row * p.heads + head) * a.splits + blockIdx.z) * (p.channels + 2) + 1] = __int_as_float(0x7fffffff);
+  } else if (*failed && element && grp == 0 && row < tile.t1) {
     // a wait ran out: nothing of this block is to be trusted
     T *dst = (T *)a.out + (row * p.heads + head) * p.channels;
     for (int c = 0; c < p.channels; ++c) dst[c] = at_round<T>(__int_as_float(0x7fffffff));

@@ -61,8 +61,23 @@ static bool is_short(const b200c_attention_t &p) {
   return p.channels <= 64 && p.m <= AT_SHORT_ROWS * p.num_segments && p.n <= AT_SHORT_ROWS * p.num_segments;
 }
 
+// A small call leaves most SMs without a block of 128 rows: the columns are dealt out to several, 128 and more to each, as long
+// as that fills the SMs, and a second kernel joins them (one cloud of 1024 points, 4 heads: 33 -> SPLIT_US us).
+int attention_tensor_splits(const b200c_attention_t &p) {
+  if (!attention_tensor_applicable(p) || is_short(p)) return 1;
+  const int64_t blocks = (p.m + AT_ROWS - 1) / AT_ROWS * p.heads;
+  int64_t splits = 148 / blocks;
+  const int64_t most = p.n / p.num_segments / 128;
+  if (splits > most) splits = most;
+  return (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
+}
+
 int launch_attention_tensor_forward(const AttnArgs &a) {
   const bool bf16 = a.p.dtype == B200C_BF16;
+  if (a.splits > 1) {
+    const int st = bf16 ? attention_tensor_forward_bf16(a) : attention_tensor_forward_f16(a);
+    return st != B200C_OK ? st : launch_attention_join(a);
+  }
   if (is_short(a.p)) return bf16 ? attention_short_forward_bf16(a) : attention_short_forward_f16(a);
   return bf16 ? attention_tensor_forward_bf16(a) : attention_tensor_forward_f16(a);
 }

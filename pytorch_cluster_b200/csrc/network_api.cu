@@ -147,7 +147,10 @@ static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 extern "C" size_t b200c_attention_workspace_bytes(const b200c_attention_t *a) {
   if (check_attention(a) != B200C_OK) return 0;
-  return attention_few_workspace_bytes(*a);
+  const size_t few = attention_few_workspace_bytes(*a);
+  if (few > 0) return few;
+  const int splits = attention_tensor_splits(*a);
+  return splits > 1 ? (size_t)a->m * a->heads * splits * (a->channels + 2) * 4 : 0;
 }
 
 extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, void *rest, float *lse, void *workspace,
@@ -169,8 +172,12 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
   a.stream = (cudaStream_t)stream;
   const int splits = attention_few_splits(*p);
   if (splits > 0) return launch_attention_few(a, splits, workspace);
-  if (attention_tensor_applicable(*p) && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0)
+  if (attention_tensor_applicable(*p) && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0) {
+    // the statistics of a training step need the exact sums, which the joined parts do not carry
+    if (lse == nullptr && rest == nullptr) a.splits = attention_tensor_splits(*p);
+    a.parts = (float *)workspace;
     return launch_attention_tensor_forward(a);
+  }
   return launch_attention_plain_forward(a);
 }
 
