@@ -3,13 +3,16 @@
 // A block of 256 threads owns 64 rows of one head and walks the other side's rows of the same example in tiles of
 // 64: one pass over the keys with the running maximum and sum of the softmax.  Operands are widened to fp32 and kept
 // transposed in shared memory ([channel][row], rows padded to 68 so that the 16-byte reads of both products are
-// free of bank conflicts); a thread holds a 4 x 4 tile of the scores and 4 x channels/16 of the result.
+// free of bank conflicts); a thread holds a 4 x 4 tile of the scores and 4 x channels/16 of the result.  Where shared memory
+// has room for two blocks per SM all the same, the next tile is on its way (asynchronous copies for fp32) while this
+// one is worked on.  tanh is CUDA's: an error of the hardware's form would be multiplied by the cap.
 // Tiles hold rows of several examples where examples are short; those are processed one example after the other, so
 // that a NaN in one example never meets another one's zeros.
 // The backward pass is two kernels of the same shape: one owns 64 queries and sums dq over the keys, one owns 64 keys and
 // sums dk and dv over the queries of all heads of its group.  Scores are formed twice, but nothing is
 // added atomically: the result does not depend on the order of the blocks.
 #include "attention.cuh"
+#include "tcgen05.cuh"
 
 namespace b200c {
 
@@ -17,14 +20,26 @@ constexpr int AP_T = 64;        // rows and columns of a tile
 constexpr int AP_LD = AP_T + 4;
 constexpr int AP_THREADS = 256;
 
-// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]
-template <typename T>
+__device__ __forceinline__ void ap_copy(float *dst, const float *src, bool there) {
+  const unsigned bytes = there ? 4u : 0u;  // nothing is read where there is nothing: zeros are written
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+
+// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]; fp32 asynchronously
+template <typename T, int CP>
 __device__ __forceinline__ void ap_load(float *dst, const T *__restrict__ src, int64_t row_stride, int64_t row0,
-                                        int64_t lo, int64_t hi, int channels, int padded, int tid) {
-  for (int i = tid; i < AP_T * padded; i += AP_THREADS) {
-    const int r = i / padded, c = i - r * padded;
+                                        int64_t lo, int64_t hi, int channels, int tid) {
+#pragma unroll 4
+  for (int i = tid; i < AP_T * CP; i += AP_THREADS) {
+    const int r = i / CP, c = i - r * CP;
     const int64_t row = row0 + r;
-    dst[c * AP_LD + r] = (row >= lo && row < hi && c < channels) ? at_float(src[row * row_stride + c]) : 0.f;
+    const bool there = row >= lo && row < hi && c < channels;
+    if constexpr (sizeof(T) == 4)
+      ap_copy(dst + c * AP_LD + r, there ? src + row * row_stride + c : src, there);
+    else
+      dst[c * AP_LD + r] = there ? at_float(src[row * row_stride + c]) : 0.f;
   }
 }
 
@@ -33,7 +48,8 @@ __device__ __forceinline__ void ap_load_pos(float *dst, const float *__restrict_
   for (int i = tid; i < AP_T * dims; i += AP_THREADS) {
     const int r = i / dims, d = i - r * dims;
     const int64_t row = row0 + r;
-    dst[d * AP_LD + r] = (row >= lo && row < hi) ? src[row * dims + d] : 0.f;
+    const bool there = row >= lo && row < hi;
+    ap_copy(dst + d * AP_LD + r, there ? src + row * dims + d : src, there);
   }
 }
 
@@ -73,6 +89,7 @@ __device__ __forceinline__ void ap_accumulate(const float *w, const float *b, in
 template <bool BEND>
 __device__ __forceinline__ void ap_logits(float (&s)[4][4], float (&bend)[4][4], const float *pa, const float *pb,
                                           int dims, int ty, int tx, float scale, float cap, float slope) {
+  const float inv_cap = cap > 0.f ? 1.f / cap : 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -80,7 +97,7 @@ __device__ __forceinline__ void ap_logits(float (&s)[4][4], float (&bend)[4][4],
       float t = s[i][j] * scale;
       if (BEND) bend[i][j] = 1.f;
       if (cap > 0.f) {
-        const float u = tanhf(t / cap);
+        const float u = tanhf(t * inv_cap);
         t = cap * u;
         if (BEND) bend[i][j] = 1.f - u * u;
       }
@@ -90,7 +107,7 @@ __device__ __forceinline__ void ap_logits(float (&s)[4][4], float (&bend)[4][4],
           const float df = pa[d * AP_LD + 4 * ty + i] - pb[d * AP_LD + 4 * tx + j];
           d2 = fmaf(df, df, d2);
         }
-        t = fmaf(-slope, sqrtf(d2), t);
+        t = fmaf(-slope, t5_sqrt(d2), t);
       }
       s[i][j] = t * AT_LOG2E;
     }
@@ -105,18 +122,22 @@ __device__ __forceinline__ float ap_sum16(float v) {
   return v;
 }
 
-template <int CP>
+// floats of shared memory: `own` tiles of the block's rows, two of the columns in BUFS sets (with coordinates and statistics), the
+// weights.  Two sets where two blocks then still fit an SM.
+template <int CP, int OWN>
 struct ApSmem {
-  static constexpr int TILE = CP * AP_LD, W = AP_T * AP_LD, POS = AT_MAX_DIMS * AP_LD;
+  static constexpr int TILE = CP * AP_LD, W = AP_T * AP_LD, POS = AT_MAX_DIMS * AP_LD, STAT = 2 * AP_T;
+  static constexpr int SET = 2 * TILE + POS + STAT;
+  static constexpr int BUFS = (OWN * TILE + POS + W + 2 * SET) * 4 <= 113 * 1024 ? 2 : 1;
+  static constexpr int FLOATS = OWN * TILE + POS + W + BUFS * SET;
 };
 
 template <typename T, int CP>
 __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(AttnArgs a) {
   constexpr int NC = CP / 16;
-  using S = ApSmem<CP>;
+  using S = ApSmem<CP, 1>;
   extern __shared__ __align__(16) float ap_smem[];
-  float *sq = ap_smem, *sk = sq + S::TILE, *sv = sk + S::TILE, *sw = sv + S::TILE, *spq = sw + S::W,
-        *spk = spq + S::POS;
+  float *sq = ap_smem, *sw = sq + S::TILE, *spq = sw + S::W, *sets = spq + S::POS;
   const b200c_attention_t &p = a.p;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int head = blockIdx.y, group = head / (p.heads / p.groups);
@@ -127,7 +148,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
   const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
   T *out = (T *)a.out, *rest = (T *)a.rest;
 
-  ap_load(sq, q, p.q_row, t0, t0, t1, p.channels, CP, tid);
+  ap_load<T, CP>(sq, q, p.q_row, t0, t0, t1, p.channels, tid);
   if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, t0, t0, t1, tid);
   // rows of no example stay at zero
   for (int64_t row = t0; row < t1; ++row) {
@@ -155,12 +176,29 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
     float o[4][NC] = {}, top[4], sum[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) top[i] = -pos_inf<float>();
-    for (int64_t c0 = k_lo; c0 < k_hi; c0 += AP_T) {
-      __syncthreads();
-      ap_load(sk, k, p.k_row, c0, k_lo, k_hi, p.channels, CP, tid);
-      ap_load(sv, v, p.v_row, c0, k_lo, k_hi, p.channels, CP, tid);
+    auto fetch = [&](int64_t c0, int set) {
+      float *sk = sets + set * S::SET, *sv = sk + S::TILE, *spk = sv + S::TILE;
+      ap_load<T, CP>(sk, k, p.k_row, c0, k_lo, k_hi, p.channels, tid);
+      ap_load<T, CP>(sv, v, p.v_row, c0, k_lo, k_hi, p.channels, tid);
       if (p.dims > 0) ap_load_pos(spk, p.pos_k, p.dims, c0, k_lo, k_hi, tid);
+    };
+    int set = 0;
+    __syncthreads();
+    if (S::BUFS == 2 && k_lo < k_hi) fetch(k_lo, 0);
+    for (int64_t c0 = k_lo; c0 < k_hi; c0 += AP_T) {
+      // this tile is in; nobody reads the other set any more
+      if (S::BUFS == 1) {
+        __syncthreads();
+        fetch(c0, 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
       __syncthreads();
+      const float *sk = sets + set * S::SET, *sv = sk + S::TILE, *spk = sv + S::TILE;
+      if (S::BUFS == 2) {
+        set ^= 1;
+        if (c0 + AP_T < k_hi) fetch(c0 + AP_T, set);
+      }
       float s[4][4] = {}, unused[4][4];
       ap_scores(sq, sk, p.channels, ty, tx, s);
       ap_logits<false>(s, unused, spq, spk, p.dims, ty, tx, p.scale, p.cap, slope);
@@ -174,12 +212,12 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
         }
         m = ap_max16(m);
         const float base = m == -pos_inf<float>() ? 0.f : m;
-        const float shrink = exp2f(top[i] - base);
+        const float shrink = t5_ex2(top[i] - base);
         top[i] = m;
         float part = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][j] = exp2f(s[i][j] - base);
+          s[i][j] = t5_ex2(s[i][j] - base);
           part += s[i][j];
         }
         sum[i] = fmaf(sum[i], shrink, ap_sum16(part));
@@ -208,16 +246,16 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
         a.lse[(int64_t)head * p.m + row] = sum[i] == 0.f ? pos_inf<float>() : top[i] + log2f(sum[i]);
     }
   }
+  cp_async_wait<0>();  // a block without a tile still has its own rows' copies under way
 }
 
 // dq of 64 queries of one head
 template <typename T, int CP>
 __global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs a) {
   constexpr int NC = CP / 16;
-  using S = ApSmem<CP>;
+  using S = ApSmem<CP, 2>;
   extern __shared__ __align__(16) float ap_smem[];
-  float *sq = ap_smem, *sdo = sq + S::TILE, *sk = sdo + S::TILE, *sv = sk + S::TILE, *sw = sv + S::TILE,
-        *spq = sw + S::W, *spk = spq + S::POS;
+  float *sq = ap_smem, *sdo = sq + S::TILE, *sw = sdo + S::TILE, *spq = sw + S::W, *sets = spq + S::POS;
   const b200c_attention_t &p = a.p;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int head = blockIdx.y, group = head / (p.heads / p.groups);
@@ -230,8 +268,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs
   const float slope = p.dims > 0 ? p.slope[head] : 0.f;
   const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
 
-  ap_load(sq, q, p.q_row, t0, t0, t1, p.channels, CP, tid);
-  ap_load(sdo, dout, qrow, t0, t0, t1, p.channels, CP, tid);
+  ap_load<T, CP>(sq, q, p.q_row, t0, t0, t1, p.channels, tid);
+  ap_load<T, CP>(sdo, dout, qrow, t0, t0, t1, p.channels, tid);
   if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, t0, t0, t1, tid);
   for (int64_t row = t0; row < t1; ++row) {
     const int b = segment_of(p.ptr_q, p.num_segments, row);
@@ -259,12 +297,29 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs
     if (q_hi > t1) q_hi = t1;
     if (q_lo >= q_hi) continue;
     float acc[4][NC] = {};
-    for (int64_t c0 = k_lo; c0 < k_hi; c0 += AP_T) {
-      __syncthreads();
-      ap_load(sk, k, p.k_row, c0, k_lo, k_hi, p.channels, CP, tid);
-      ap_load(sv, v, p.v_row, c0, k_lo, k_hi, p.channels, CP, tid);
+    auto fetch = [&](int64_t c0, int set) {
+      float *sk = sets + set * S::SET, *sv = sk + S::TILE, *spk = sv + S::TILE;
+      ap_load<T, CP>(sk, k, p.k_row, c0, k_lo, k_hi, p.channels, tid);
+      ap_load<T, CP>(sv, v, p.v_row, c0, k_lo, k_hi, p.channels, tid);
       if (p.dims > 0) ap_load_pos(spk, p.pos_k, p.dims, c0, k_lo, k_hi, tid);
+    };
+    int set = 0;
+    __syncthreads();
+    if (S::BUFS == 2 && k_lo < k_hi) fetch(k_lo, 0);
+    for (int64_t c0 = k_lo; c0 < k_hi; c0 += AP_T) {
+      // this tile is in; nobody reads the other set any more
+      if (S::BUFS == 1) {
+        __syncthreads();
+        fetch(c0, 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
       __syncthreads();
+      const float *sk = sets + set * S::SET, *sv = sk + S::TILE, *spk = sv + S::TILE;
+      if (S::BUFS == 2) {
+        set ^= 1;
+        if (c0 + AP_T < k_hi) fetch(c0 + AP_T, set);
+      }
       float s[4][4] = {}, dp[4][4] = {}, bend[4][4];
       ap_scores(sq, sk, p.channels, ty, tx, s);
       ap_scores(sdo, sv, p.channels, ty, tx, dp);
@@ -274,7 +329,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const bool there = c0 + 4 * tx + j < k_hi && lse[i] < pos_inf<float>();
-          const float w = exp2f(s[i][j] - lse[i]) * (dp[i][j] - delta[i]) * bend[i][j];
+          const float w = t5_ex2(s[i][j] - lse[i]) * (dp[i][j] - delta[i]) * bend[i][j];
           s[i][j] = there || lse[i] != lse[i] ? w : 0.f;
           if (c0 + 4 * tx + j >= k_hi) s[i][j] = 0.f;
         }
@@ -295,16 +350,16 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs
       }
     }
   }
+  cp_async_wait<0>();  // a block without a tile still has its own rows' copies under way
 }
 
 // dk and dv of 64 keys of one group
 template <typename T, int CP>
 __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArgs a) {
   constexpr int NC = CP / 16;
-  using S = ApSmem<CP>;
+  using S = ApSmem<CP, 2>;
   extern __shared__ __align__(16) float ap_smem[];
-  float *sk = ap_smem, *sv = sk + S::TILE, *sq = sv + S::TILE, *sdo = sq + S::TILE, *sw = sdo + S::TILE,
-        *spq = sw + S::W, *spk = spq + S::POS, *slse = spk + S::POS, *sdelta = slse + AP_T;
+  float *sk = ap_smem, *sv = sk + S::TILE, *sw = sv + S::TILE, *spk = sw + S::W, *sets = spk + S::POS;
   const b200c_attention_t &p = a.p;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int group = blockIdx.y, per_group = p.heads / p.groups;
@@ -314,8 +369,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
   T *dk = (T *)a.dk + (int64_t)group * p.channels, *dv = (T *)a.dv + (int64_t)group * p.channels;
   const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.n ? t0 + AP_T : p.n;
 
-  ap_load(sk, k, p.k_row, t0, t0, t1, p.channels, CP, tid);
-  ap_load(sv, v, p.v_row, t0, t0, t1, p.channels, CP, tid);
+  ap_load<T, CP>(sk, k, p.k_row, t0, t0, t1, p.channels, tid);
+  ap_load<T, CP>(sv, v, p.v_row, t0, t0, t1, p.channels, tid);
   if (p.dims > 0) ap_load_pos(spk, p.pos_k, p.dims, t0, t0, t1, tid);
   for (int64_t row = t0; row < t1; ++row) {
     const int b = segment_of(p.ptr_k, p.num_segments, row);
@@ -339,17 +394,35 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
     for (int e = 0; e < per_group; ++e) {
       const int head = group * per_group + e;
       const float slope = p.dims > 0 ? p.slope[head] : 0.f;
-      for (int64_t c0 = q_lo; c0 < q_hi; c0 += AP_T) {
-        __syncthreads();
-        ap_load(sq, (const T *)p.q + (int64_t)head * p.q_head, p.q_row, c0, q_lo, q_hi, p.channels, CP, tid);
-        ap_load(sdo, (const T *)a.dout + (int64_t)head * p.channels, qrow, c0, q_lo, q_hi, p.channels, CP, tid);
+      const T *q = (const T *)p.q + (int64_t)head * p.q_head, *dout = (const T *)a.dout + (int64_t)head * p.channels;
+      auto fetch = [&](int64_t c0, int set) {
+        float *sq = sets + set * S::SET, *sdo = sq + S::TILE, *spq = sdo + S::TILE, *stat = spq + S::POS;
+        ap_load<T, CP>(sq, q, p.q_row, c0, q_lo, q_hi, p.channels, tid);
+        ap_load<T, CP>(sdo, dout, qrow, c0, q_lo, q_hi, p.channels, tid);
         if (p.dims > 0) ap_load_pos(spq, p.pos_q, p.dims, c0, q_lo, q_hi, tid);
         if (tid < AP_T) {
           const bool there = c0 + tid < q_hi;
-          slse[tid] = there ? a.lse[(int64_t)head * p.m + c0 + tid] : pos_inf<float>();
-          sdelta[tid] = there ? a.delta[(int64_t)head * p.m + c0 + tid] : 0.f;
+          stat[tid] = there ? a.lse[(int64_t)head * p.m + c0 + tid] : pos_inf<float>();
+          stat[AP_T + tid] = there ? a.delta[(int64_t)head * p.m + c0 + tid] : 0.f;
         }
+      };
+      int set = 0;
+      __syncthreads();
+      if (S::BUFS == 2 && q_lo < q_hi) fetch(q_lo, 0);
+      for (int64_t c0 = q_lo; c0 < q_hi; c0 += AP_T) {
+        if (S::BUFS == 1) {
+          __syncthreads();
+          fetch(c0, 0);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
         __syncthreads();
+        const float *sq = sets + set * S::SET, *sdo = sq + S::TILE, *spq = sdo + S::TILE, *slse = spq + S::POS,
+                    *sdelta = slse + AP_T;
+        if (S::BUFS == 2) {
+          set ^= 1;
+          if (c0 + AP_T < q_hi) fetch(c0 + AP_T, set);
+        }
         float s[4][4] = {}, dp[4][4] = {}, bend[4][4];
         ap_scores(sk, sq, p.channels, ty, tx, s);
         ap_scores(sv, sdo, p.channels, ty, tx, dp);
@@ -360,7 +433,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
           const bool none = lse == pos_inf<float>();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[i][j] = none ? 0.f : exp2f(s[i][j] - lse);
+            s[i][j] = none ? 0.f : t5_ex2(s[i][j] - lse);
             dp[i][j] = none ? 0.f : s[i][j] * (dp[i][j] - delta) * bend[i][j];
           }
         }
@@ -393,6 +466,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
       }
     }
   }
+  cp_async_wait<0>();  // a block without a tile still has its own rows' copies under way
 }
 
 // What the backward pass needs beforehand: D_i = do_i . o_i per (row, head), and for fp16 the largest |do_i|^2 and |v_j|^2
@@ -462,7 +536,8 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, floa
 
 template <typename T, int CP>
 static int ap_forward(const AttnArgs &a) {
-  constexpr size_t smem = (3 * ApSmem<CP>::TILE + ApSmem<CP>::W + 2 * ApSmem<CP>::POS) * 4;
+  constexpr size_t smem = ApSmem<CP, 1>::FLOATS * 4;
+  static_assert(smem <= 227 * 1024, "shared memory of a block");
   static unsigned long long configured = 0ull;
   B200C_CUDA(opt_in_shared_memory(attention_plain_forward_kernel<T, CP>, smem, configured));
   const dim3 grid((unsigned)((a.p.m + AP_T - 1) / AP_T), (unsigned)a.p.heads);
@@ -473,7 +548,7 @@ static int ap_forward(const AttnArgs &a) {
 
 template <typename T, int CP>
 static int ap_backward(const AttnArgs &a) {
-  constexpr size_t smem = (4 * ApSmem<CP>::TILE + ApSmem<CP>::W + 2 * ApSmem<CP>::POS + 2 * AP_T) * 4;
+  constexpr size_t smem = ApSmem<CP, 2>::FLOATS * 4;
   static_assert(smem <= 227 * 1024, "shared memory of a block");
   static unsigned long long configured_q = 0ull, configured_kv = 0ull;
   if (a.dq && a.p.m > 0) {
@@ -494,6 +569,7 @@ static int ap_backward(const AttnArgs &a) {
 template <typename T>
 static int ap_dispatch(const AttnArgs &a, bool forward) {
   if (a.p.channels <= 32) return forward ? ap_forward<T, 32>(a) : ap_backward<T, 32>(a);
+  if (a.p.channels <= 48) return forward ? ap_forward<T, 48>(a) : ap_backward<T, 48>(a);
   if (a.p.channels <= 64) return forward ? ap_forward<T, 64>(a) : ap_backward<T, 64>(a);
   return forward ? ap_forward<T, 128>(a) : ap_backward<T, 128>(a);
 }

@@ -40,7 +40,7 @@ struct AsOperand {
 };
 
 template <typename T, int CP, int DIM, bool CAP, AsRole ROLE>
-__global__ void __launch_bounds__(32 * AS_WARPS) attention_short_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(32 * AS_WARPS, CP == 32 ? 3 : 2) attention_short_kernel(const __grid_constant__ AttnArgs a) {
   using S = AsTiles<CP>;
   using A = AtType<T>;
   constexpr bool KV = ROLE == AS_DKV, FORWARD = ROLE == AS_FORWARD;
@@ -100,48 +100,44 @@ __global__ void __launch_bounds__(32 * AS_WARPS) attention_short_kernel(const __
     const int64_t count = c_hi - c_lo;
     const int blocks = (int)((count + AS_COLS - 1) / AS_COLS);  // per head
 
-    // copies of step (u, e, j): the unit's rows with its first step, the columns' tiles and what belongs to them
+    // copies of step (u, e, j): the unit's rows with its first step, the columns' tiles and what belongs to them.  A lane
+    // copies chunk my_c of rows my_r, my_r + PER, ...
+    constexpr int PER = 32 / CHUNKS;
+    const int my_r = lane / CHUNKS, my_c = lane % CHUNKS;
+    const T *r0_at = (const T *)rows0.base + (t0 + my_r) * rows0.row + my_c * 8;
+    const T *r1_at = (const T *)rows1.base + (t0 + my_r) * rows1.row + my_c * 8;
+    const T *c0_at = (const T *)cols0.base + (c_lo + my_r) * cols0.row + my_c * 8;
+    const T *c1_at = (const T *)cols1.base + (c_lo + my_r) * cols1.row + my_c * 8;
+    const int my_rows = my_c < chunks ? (int)(tile.t1 - t0) - my_r : 0;  // this lane's rows lie below that
+    auto copy = [&](uint32_t dst, const T *src, bool there) {  // nothing is read where there is nothing: zeros are written
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(there ? src : (const T *)cols0.base),
+                   "r"(there ? 16u : 0u)
+                   : "memory");
+    };
     auto fetch = [&](int u, int e, int64_t j, int stage) {
       if (u < u_hi) {
         const int head = KV ? u * per_group + e : u, col_head = KV ? head : u / per_group;
         if (e == 0 && j == 0) {
           const uint32_t dst = at_mine + (u & 1) * (2 * S::ROWS);
-          for (int i = lane; i < AS_ROWS * CHUNKS; i += 32) {
-            const int r = i / CHUNKS, c = i % CHUNKS;
-            const uint32_t off = aw_at<CP>(r, c);
-            const bool there = t0 + r < tile.t1 && c < chunks;
-            if (there) {
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst + off),
-                           "l"((const T *)rows0.base + (t0 + r) * rows0.row + u * rows0.head + c * 8)
-                           : "memory");
-              if (!FORWARD)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst + S::ROWS + off),
-                             "l"((const T *)rows1.base + (t0 + r) * rows1.row + u * rows1.head + c * 8)
-                             : "memory");
-            } else {
-              unsigned char *z = mine + (u & 1) * (2 * S::ROWS) + off;
-              *reinterpret_cast<uint4 *>(z) = make_uint4(0u, 0u, 0u, 0u);
-              if (!FORWARD) *reinterpret_cast<uint4 *>(z + S::ROWS) = make_uint4(0u, 0u, 0u, 0u);
-            }
+          const T *s0 = r0_at + u * rows0.head, *s1 = r1_at + u * rows1.head;
+#pragma unroll
+          for (int n = 0; n < AS_ROWS / PER; ++n) {
+            const uint32_t off = aw_at<CP>(n * PER + my_r, my_c);
+            copy(dst + off, s0 + n * PER * rows0.row, n * PER < my_rows);
+            if (!FORWARD) copy(dst + S::ROWS + off, s1 + n * PER * rows1.row, n * PER < my_rows);
           }
         }
         const int64_t j0 = c_lo + j * AS_COLS;
+        const int my_cols = my_c < chunks ? (int)(c_hi - j0 < AS_COLS ? c_hi - j0 : AS_COLS) - my_r : 0;
         unsigned char *st = mine + 4 * S::ROWS + stage * S::STAGE;
         const uint32_t at_st = at_mine + 4 * S::ROWS + stage * S::STAGE;
-        for (int i = lane; i < AS_COLS * CHUNKS; i += 32) {
-          const int r = i / CHUNKS, c = i % CHUNKS;
-          const uint32_t off = aw_at<CP>(r, c);
-          if (j0 + r < c_hi && c < chunks) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(at_st + off),
-                         "l"((const T *)cols0.base + (j0 + r) * cols0.row + col_head * cols0.head + c * 8)
-                         : "memory");
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(at_st + S::COLS + off),
-                         "l"((const T *)cols1.base + (j0 + r) * cols1.row + col_head * cols1.head + c * 8)
-                         : "memory");
-          } else {
-            *reinterpret_cast<uint4 *>(st + off) = *reinterpret_cast<uint4 *>(st + S::COLS + off) =
-                make_uint4(0u, 0u, 0u, 0u);
-          }
+        const T *s0 = c0_at + j * AS_COLS * cols0.row + col_head * cols0.head;
+        const T *s1 = c1_at + j * AS_COLS * cols1.row + col_head * cols1.head;
+#pragma unroll
+        for (int n = 0; n < AS_COLS / PER; ++n) {
+          const uint32_t off = aw_at<CP>(n * PER + my_r, my_c);
+          copy(at_st + off, s0 + n * PER * cols0.row, n * PER < my_cols);
+          copy(at_st + S::COLS + off, s1 + n * PER * cols1.row, n * PER < my_cols);
         }
         float *side = reinterpret_cast<float *>(st + 2 * S::COLS);
         if constexpr (DIM > 0) {
