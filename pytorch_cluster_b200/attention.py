@@ -77,7 +77,7 @@ def attention(
         pos_q, pos_k, slope: coordinates ``[M, D]`` and ``[N, D]`` (D at most 8, taken as fp32) and ``[H]``
             slopes of the bias by distance; all three or none.  They are constants: no gradient reaches them.
         scale: of the dot products, ``C ** -0.5`` by default.
-        cap: a positive number, or None.
+        cap: a positive finite number, or None.
         batch_size: the number of examples; skips its inference and the host reads that takes (needed under stream
             capture).  Rows with ids at or above it belong to no example.
 
@@ -91,8 +91,8 @@ def attention(
             raise RuntimeError("Input mismatch")
     if scale is None:
         scale = float(q.size(-1)) ** -0.5 if q.size(-1) > 0 else 1.0
-    if cap is not None and not cap > 0:
-        raise ValueError("`cap` needs to be positive")
+    if cap is not None and not 0 < cap < float("inf"):
+        raise ValueError("`cap` needs to be positive and finite")
     if (pos_q is None) != (pos_k is None) or (pos_q is None) != (slope is None):
         raise ValueError("`pos_q`, `pos_k` and `slope` come together")
     if pos_q is not None and pos_k is not None and slope is not None:

@@ -22,6 +22,9 @@ namespace b200c {
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr int AT_MAX_CHANNELS = 128;
 constexpr int AT_MAX_DIMS = 8;
+// The kernels for 16-bit types form tanh(y) as 1 - 2 / (e^2y + 1), right to 4e-7 absolutely, which the cap multiplies; above
+// this cap (1e-4 of a score) CUDA's tanh is called, in the plain kernels.
+constexpr float AT_MAX_FAST_CAP = 256.f;
 
 struct AttnArgs {
   b200c_attention_t p;

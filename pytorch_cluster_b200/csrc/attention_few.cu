@@ -631,7 +631,7 @@ static int af_channels(const AttnArgs &a, int splits, float *parts) {
   if constexpr (sizeof(T) == 2) {
     // queries are read as pairs of channels
     const bool pairs = ((uintptr_t)p.q & 3) == 0 && p.q_row % 2 == 0 && p.q_head % 2 == 0;
-    if (vec && pairs) return af_tensor<T>(a, splits, parts);
+    if (vec && pairs && !(p.cap > AT_MAX_FAST_CAP)) return af_tensor<T>(a, splits, parts);
   }
   if (p.channels <= 32) return af_rows<T, 32 / VL>(a, splits, vec, parts);
   if (p.channels <= 64) return af_rows<T, 64 / VL>(a, splits, vec, parts);

@@ -1,4 +1,4 @@
-// Attention and its gradients where examples are a few dozen rows (molecules): 16-bit types, up to 64 channels.
+// Attention and its gradients where examples are a few dozen rows (molecules): 16-bit types, up to 32 channels.
 //
 // The tcgen05 kernels work on 128 rows against 64 columns; with examples of 30 rows three quarters of that is masked.
 // Here a warp owns 16 rows and walks the columns of their example 32 at a time with warp-wide products of 16 x 8 x 16,
@@ -40,7 +40,7 @@ struct AsOperand {
 };
 
 template <typename T, int CP, int DIM, bool CAP, AsRole ROLE>
-__global__ void __launch_bounds__(32 * AS_WARPS, CP == 32 ? 3 : 2) attention_short_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const __grid_constant__ AttnArgs a) {
   using S = AsTiles<CP>;
   using A = AtType<T>;
   constexpr bool KV = ROLE == AS_DKV, FORWARD = ROLE == AS_FORWARD;
@@ -389,8 +389,7 @@ static int as_dims(const AttnArgs &a) {
 }
 template <typename T, AsRole ROLE>
 static int as_dispatch(const AttnArgs &a) {
-  if (a.p.channels <= 32) return a.p.cap > 0.f ? as_dims<T, 32, true, ROLE>(a) : as_dims<T, 32, false, ROLE>(a);
-  return a.p.cap > 0.f ? as_dims<T, 64, true, ROLE>(a) : as_dims<T, 64, false, ROLE>(a);
+  return a.p.cap > 0.f ? as_dims<T, 32, true, ROLE>(a) : as_dims<T, 32, false, ROLE>(a);
 }
 
 }  // namespace b200c

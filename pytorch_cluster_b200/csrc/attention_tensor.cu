@@ -50,19 +50,25 @@ static bool at_side(const void *base, int64_t rows, int heads, int64_t row_strid
 
 bool attention_tensor_applicable(const b200c_attention_t &p) {
   constexpr int64_t most = 0x7fffffffLL - 1024;  // column numbers of a step past the last stay in 32 bits
-  return p.dtype != B200C_F32 && p.channels % 8 == 0 && p.m > 0 && p.n > 0 && p.m < most && p.n < most &&
+  return p.dtype != B200C_F32 && p.channels % 8 == 0 && !(p.cap > AT_MAX_FAST_CAP) && p.m > 0 && p.n > 0 && p.m < most && p.n < most &&
          at_side(p.q, p.m, p.heads, p.q_row, p.q_head) && at_side(p.k, p.n, p.groups, p.k_row, p.k_head) &&
          at_side(p.v, p.n, p.groups, p.v_row, p.v_head);
 }
 
-// Mean rows per example, on either side, up to which the kernels of attention_short.cuh are taken (SHORT_RULE).
-constexpr int64_t AT_SHORT_ROWS = 64;
+// Up to 32 channels and 128 rows per example on average (either side) the kernels of attention_short.cuh are taken.  Measured
+// on 60000 rows, 8 heads, three coordinates, bfloat16, forward / gradient in us, 128-row tiles against 16-row ones:
+//   32 channels: 16 rows 185 / 437, 125 / 254;  64 rows 220 / 488, 151 / 331;  128 rows 251 / 567, 208 / 463;
+//                192 rows 277 / 633, 266 / 594
+//   64 channels: 16 rows 188 / 465, 198 / 471;  64 rows 220 / 510, 250 / 602
+constexpr int64_t AT_SHORT_ROWS = 128;
+constexpr int AT_SHORT_CHANNELS = 32;
 static bool is_short(const b200c_attention_t &p) {
-  return p.channels <= 64 && p.m <= AT_SHORT_ROWS * p.num_segments && p.n <= AT_SHORT_ROWS * p.num_segments;
+  return p.channels <= AT_SHORT_CHANNELS && p.m <= AT_SHORT_ROWS * p.num_segments &&
+         p.n <= AT_SHORT_ROWS * p.num_segments;
 }
 
 // A small call leaves most SMs without a block of 128 rows: the columns are dealt out to several, 128 and more to each, as long
-// as that fills the SMs, and a second kernel joins them (one cloud of 1024 points, 4 heads: 33 -> SPLIT_US us).
+// as that fills the SMs, and a second kernel joins them (one cloud of 1024 points, 4 heads: 33 -> 25 us).
 int attention_tensor_splits(const b200c_attention_t &p) {
   if (!attention_tensor_applicable(p) || is_short(p)) return 1;
   const int64_t blocks = (p.m + AT_ROWS - 1) / AT_ROWS * p.heads;
