@@ -364,6 +364,8 @@ static int nr_launch(const NormRotateArgs &a, bool forward, float *parts) {
   int rpb = nr_rows_per_block(a, LP);
   const int64_t most = a.side[0].rows > a.side[1].rows ? a.side[0].rows : a.side[1].rows;
   while (rpb > 1 && (most + rpb - 1) / rpb < 296) rpb /= 2;  // small calls: more blocks rather than fuller ones
+  // with the 8 KB of the weights' sums, below the 48 KB that a block has without asking
+  while (rpb > 1 && (size_t)(rpb + a.dims + 2) * a.half * 8 > 40 * 1024) --rpb;
   const size_t smem = (size_t)(rpb + a.dims + 2) * a.half * 8;  // sines and cosines, frequencies, weights
   const int64_t chunks = (most + rpb - 1) / rpb;
   const unsigned sides = a.joint ? 1u : 2u;

@@ -199,10 +199,15 @@ def test_attention_large_scores(dtype):
     check_attention(dtype, [400], [400], 2, 2, 32, 1, seed=9, qscale=12.0)
     check_attention(dtype, [400], [400], 2, 2, 32, 3, seed=10, slope_scale=40.0)
     check_attention(dtype, [130], [130], 2, 2, 32, 0, seed=11, scale=-0.5)
+    check_attention(dtype, [300], [300], 2, 2, 64, 2, seed=12, qscale=12.0)
+    # a cap that bends nothing, and one that bends all
+    check_attention(dtype, [140, 30], [140, 30], 2, 2, 64, 0, cap=5000.0, seed=13)
+    check_attention(dtype, [1], [900], 2, 2, 64, 0, cap=5000.0, seed=14)
+    check_attention(dtype, [140, 30], [140, 30], 2, 2, 64, 0, cap=0.01, seed=15)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("channels", [64, 128])  # rows of short examples, 16 at a time and 128 at a time
+@pytest.mark.parametrize("channels", [32, 64, 128])  # 16 rows at a time, 128, and 128 of twice the width
 def test_attention_keeps_nan_and_infinities_in_their_example(dtype, channels):
     import pytorch_cluster_b200 as pc
 
@@ -366,7 +371,8 @@ def test_attention_captured_and_replayed():
     one = rand(g, 2, 4, 64, dtype=torch.bfloat16)
 
     def run():
-        return pc.attention(*ts, b, b, batch_size=2), pc.attention(one, *ts[1:], bq, b, batch_size=2)
+        return (pc.attention(*ts, b, b, batch_size=2), pc.attention(one, *ts[1:], bq, b, batch_size=2),
+                pc.attention(ts[0][..., :24], ts[1][..., :24], ts[2][..., :24], b, b, batch_size=2))
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -385,6 +391,43 @@ def test_attention_captured_and_replayed():
         for graph, outs in graphs:
             graph.replay()
             assert all(torch.equal(x, y) for x, y in zip(outs, run()))
+
+
+def test_attention_training_step_captured():
+    import pytorch_cluster_b200 as pc
+
+    g = gen(13)
+    lens = [130, 300]
+    b, n = ids(lens), sum(lens)
+    ts = [rand(g, n, 2, 64, dtype=torch.float16) for _ in range(3)]
+    pos, slope = rand(g, n, 3, dtype=torch.float32), torch.tensor([1.0, 0.5], device="cuda")
+    do = rand(g, n, 2, 64, dtype=torch.float16)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in ts]
+        out = pc.attention(*leaves, b, b, pos, pos, slope, batch_size=2)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in [*ts, do]:
+        t.copy_(rand(g, *t.shape, dtype=t.dtype))
+    graph.replay()
+    assert all(torch.equal(x, y) for x, y in zip(got, step()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("channels", [64, 128])
+def test_attention_small_calls_split_over_the_keys(dtype, channels):
+    check_attention(dtype, [1000], [1000], 2, 1, channels, 3, seed=31, train=False)
+    check_attention(dtype, [200, 700, 77], [900, 300, 640], 2, 2, channels, 0, cap=20.0, seed=32, train=False)
+    check_attention(dtype, [128, 128], [4000, 1], 1, 1, channels, 1, seed=33, train=False)
 
 
 # ---- norm_rotate ---------------------------------------------------------------------------------------------
@@ -443,6 +486,8 @@ ROTATE = [
     (64, 0, 2, 2, 48, 1, True, False),
     (129, None, 2, 2, 250, 3, True, False),
     (4099, None, 2, 1, 96, 1, False, True),
+    (700, None, 1, 1, 256, 8, True, False),
+    (600, 601, 1, 2, 256, 7, True, False),
 ]
 
 

@@ -143,6 +143,8 @@ def test_mismatched_cuda_tensors_are_refused():
         pc.attention(q, k, k, ok, ok)
     with pytest.raises(ValueError, match="positive"):
         pc.attention(q, k, k, cap=0.0)
+    with pytest.raises(ValueError, match="finite"):
+        pc.attention(q, k, k, cap=float("inf"))
     with pytest.raises(ValueError, match="together"):
         pc.attention(q, k, k, pos_q=torch.rand(6, 3, **d))
     p = dict(pos_q=torch.rand(6, 3, **d), pos_k=torch.rand(5, 3, **d), slope=torch.rand(4, **d))
