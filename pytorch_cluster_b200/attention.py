@@ -1,28 +1,8 @@
 """``attention``: softmax attention inside the examples of a ragged batch, differentiable, on top of
-``torch.ops.torch_cluster.attention_forward`` / ``attention_backward``."""
+``torch.ops.torch_cluster.attention``."""
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
-
-
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap):
-        out, rest, lse = torch.ops.torch_cluster.attention_forward(q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale,
-                                                                   cap, True)
-        ctx.save_for_backward(q, k, v, out, rest, lse, ptr_q, ptr_k, pos_q, pos_k, slope)
-        ctx.scale, ctx.cap = scale, cap
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        tensors = ctx.saved_tensors
-        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq, dk, dv = torch.ops.torch_cluster.attention_backward(dout, *tensors, ctx.scale, ctx.cap, need_q, need_kv)
-        return (dq if need_q else None, dk if ctx.needs_input_grad[1] else None,
-                dv if ctx.needs_input_grad[2] else None, None, None, None, None, None, None, None)
 
 
 def _segments(batch_q: Optional[torch.Tensor], batch_k: Optional[torch.Tensor], rows_q: int, rows_k: int,
@@ -101,7 +81,5 @@ def attention(
         pos_k = pos_q if same else _places("pos_k", pos_k)
         slope = _places("slope", slope)
     ptr_q, ptr_k = _segments(batch_q, batch_k, q.size(0), k.size(0), batch_size)
-    args = (q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, float(scale), 0.0 if cap is None else float(cap))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(*args)
-    return torch.ops.torch_cluster.attention_forward(*args, False)[0]
+    return torch.ops.torch_cluster.attention(q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, float(scale),
+                                             0.0 if cap is None else float(cap))

@@ -1,21 +1,6 @@
 """``gather_rows``: rows of node features along an edge list, differentiable, on top of
 ``torch.ops.torch_cluster.gather_rows``."""
 import torch
-from torch.autograd.function import once_differentiable
-
-
-class _GatherRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, index, scale):
-        ctx.save_for_backward(index)
-        ctx.rows, ctx.scale = x.size(0), scale
-        return torch.ops.torch_cluster.gather_rows(x, index, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        index, = ctx.saved_tensors
-        return torch.ops.torch_cluster.gather_rows_backward(dout, index, ctx.rows, ctx.scale), None, None
 
 
 def gather_rows(
@@ -39,7 +24,4 @@ def gather_rows(
     """
     if not x.is_cuda:
         raise RuntimeError("x must be CUDA tensor")
-    scale = float(scale)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _GatherRows.apply(x, index, scale)
-    return torch.ops.torch_cluster.gather_rows(x, index, scale)
+    return torch.ops.torch_cluster.gather_rows(x, index, float(scale))

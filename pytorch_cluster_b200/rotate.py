@@ -3,24 +3,6 @@ pass, differentiable, on top of ``torch.ops.torch_cluster.norm_rotate``."""
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
-
-
-class _NormRotate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, pos_q, pos_k, freq, weight_q, weight_k, eps):
-        ctx.save_for_backward(q, k, pos_q, pos_k, freq, weight_q, weight_k)
-        ctx.eps = eps
-        return torch.ops.torch_cluster.norm_rotate(q, k, pos_q, pos_k, freq, weight_q, weight_k, eps)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        q, k, pos_q, pos_k, freq, weight_q, weight_k = ctx.saved_tensors
-        gq, gk, gwq, gwk = torch.ops.torch_cluster.norm_rotate_backward(
-            dq, dk, q, k, pos_q, pos_k, freq, weight_q, weight_k, ctx.eps)
-        return (gq, gk, None, None, None, gwq if weight_q is not None else None,
-                gwk if weight_k is not None else None, None)
 
 
 def _constant(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -79,8 +61,4 @@ def norm_rotate(
         weight_q = weight_q.float()
     if weight_k is not None:
         weight_k = weight_k.float()
-    eps = float(eps)
-    args = (q, k, pos[0], pos[1], freq, weight_q, weight_k, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, weight_q, weight_k)):
-        return _NormRotate.apply(*args)
-    return torch.ops.torch_cluster.norm_rotate(*args)
+    return torch.ops.torch_cluster.norm_rotate(q, k, pos[0], pos[1], freq, weight_q, weight_k, float(eps))
