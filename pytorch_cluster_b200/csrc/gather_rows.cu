@@ -24,6 +24,13 @@ constexpr int GR_MAX_BITS = 9;
 constexpr int GR_EDGES = 4;                        // edges per thread of the forward pass
 constexpr int GR_LONG_WARPS = 32;                  // of a block that joins a long run
 constexpr int GR_SHORT = 16;                       // pieces a single thread joins; longer runs get a block
+// Calls of up to GR_ONE pairs sort in one block and leave every join to a thread: 4 launches for 11, 75 -> 66 us of a
+// training step of 1100 edges, which the host's launches bound.  Up to GR_FEW blocks the scatter adds up the counts
+// that it needs itself, in place of a launch per pass.
+constexpr int GR_ONE_THREADS = 1024;
+constexpr int GR_ONE_ITEMS = 16;
+constexpr int GR_ONE = GR_ONE_THREADS * GR_ONE_ITEMS;
+constexpr int GR_FEW = 32;
 
 template <typename T, int VL>
 struct alignas(sizeof(T) * VL) GrVec {
@@ -111,6 +118,7 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_count_kernel(const int
 }
 
 // exclusive sum over one warp-sized batch per warp of the block; returns this thread's, and the block's total
+template <int WARPS = GR_WARPS>
 __device__ __forceinline__ uint32_t gr_block_scan(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t in = v;
@@ -125,7 +133,7 @@ __device__ __forceinline__ uint32_t gr_block_scan(uint32_t v, uint32_t *warp_sum
   uint32_t before = 0u;
   total = 0u;
 #pragma unroll
-  for (int w = 0; w < GR_WARPS; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) before += warp_sums[w];
     total += warp_sums[w];
   }
@@ -157,6 +165,26 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scan_kernel(uint32_t *
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
+// The place of this lane's pair: those of a digit follow one another in the order of the lanes.  next[digit] is the warp's
+// next place and moves on.  The lanes with one digit are found by a ballot per bit (match_any takes three times as
+// long where digits differ).
+__device__ __forceinline__ uint32_t gr_place(bool have, uint32_t digit, int bits, uint32_t *next) {
+  unsigned same = __ballot_sync(FULL_MASK, have);
+  if (!have) same = ~same;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1u;
+    const unsigned ones = __ballot_sync(FULL_MASK, one);
+    same &= one ? ones : ~ones;
+  }
+  const int rank = __popc(same & ((1u << (threadIdx.x & 31)) - 1u));
+  uint32_t at = 0u;
+  if (have) at = next[digit];
+  __syncwarp();
+  if (have && rank == 0) next[digit] = at + __popc(same);
+  __syncwarp();
+  return at + rank;
+}
+
 __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
     const int64_t *__restrict__ index, const uint2 *__restrict__ pairs, int64_t rows, int64_t edges, int shift,
     int bits, const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
@@ -183,19 +211,30 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
   __syncthreads();
   // two digits per thread: the block's and all blocks' exclusive sums over the digits
   const int d0 = threadIdx.x * 2;
-  uint32_t here[2] = {}, all[2] = {}, unused;
+  uint32_t here[2] = {}, all[2] = {}, earlier[2] = {}, unused;
 #pragma unroll
   for (int n = 0; n < 2; ++n)
     if (d0 + n < bins) {
       for (int w = 0; w < GR_WARPS; ++w) here[n] += next[w][d0 + n];
-      all[n] = totals[d0 + n];
+      const uint32_t *mine = counts + (int64_t)(d0 + n) * gridDim.x;
+      if (totals) {
+        all[n] = totals[d0 + n];
+        earlier[n] = mine[blockIdx.x];
+      } else {
+#pragma unroll 8
+        for (unsigned b = 0; b < gridDim.x; ++b) {
+          const uint32_t c = mine[b];
+          all[n] += c;
+          if (b < blockIdx.x) earlier[n] += c;
+        }
+      }
     }
   uint32_t at_here = gr_block_scan(here[0] + here[1], warp_sums, unused);
   uint32_t at_all = gr_block_scan(all[0] + all[1], warp_sums, unused);
 #pragma unroll
   for (int n = 0; n < 2; ++n)
     if (d0 + n < bins) {
-      shift_to[d0 + n] = at_all + counts[(int64_t)(d0 + n) * gridDim.x + blockIdx.x] - at_here;
+      shift_to[d0 + n] = at_all + earlier[n] - at_here;
       uint32_t at = at_here;
       for (int w = 0; w < GR_WARPS; ++w) {
         const uint32_t c = next[w][d0 + n];
@@ -210,21 +249,8 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
   for (int r = 0; r < GR_ITEMS; ++r) {
     const bool have = base + r * 32 < edges;
     const uint32_t digit = have ? (pair[r].x >> shift) & (bins - 1) : (uint32_t)bins;
-    // the lanes with this digit, a ballot per bit (match_any takes three times as long where digits differ)
-    unsigned same = __ballot_sync(FULL_MASK, have);
-    if (!have) same = ~same;
-    for (int b = 0; b < bits; ++b) {
-      const bool one = (digit >> b) & 1u;
-      const unsigned ones = __ballot_sync(FULL_MASK, one);
-      same &= one ? ones : ~ones;
-    }
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    uint32_t at = 0u;
-    if (have) at = next[warp][digit];
-    __syncwarp();
-    if (have && rank == 0) next[warp][digit] = at + __popc(same);
-    __syncwarp();
-    if (have) sorted[at + rank] = pair[r];
+    const uint32_t at = gr_place(have, digit, bits, next[warp]);
+    if (have) sorted[at] = pair[r];
   }
   __syncthreads();
   const int64_t left = edges - (int64_t)blockIdx.x * GR_TILE;
@@ -234,6 +260,56 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
     const uint2 p = sorted[i];
     out[(uint32_t)i + shift_to[(p.x >> shift) & (bins - 1)]] = p;
   }
+}
+
+// All passes in one block; the pairs stay in shared memory between them.
+__global__ void __launch_bounds__(GR_ONE_THREADS) gather_sort_one_kernel(const int64_t *__restrict__ index, int64_t rows,
+                                                                        int edges, int passes, int bits,
+                                                                        uint2 *__restrict__ out) {
+  constexpr int MOST = 1 << GR_MAX_BITS, WARPS = GR_ONE_THREADS / 32;
+  extern __shared__ __align__(16) unsigned char gr_smem[];
+  uint2 *sorted = reinterpret_cast<uint2 *>(gr_smem);
+  uint32_t(*next)[MOST] = reinterpret_cast<uint32_t(*)[MOST]>(sorted + GR_ONE);
+  __shared__ uint32_t warp_sums[WARPS];
+  const int bins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int items = (edges + GR_ONE_THREADS - 1) / GR_ONE_THREADS;  // a warp owns items * 32 consecutive pairs
+  const int base = warp * items * 32 + lane;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    for (int i = threadIdx.x; i < WARPS * MOST; i += GR_ONE_THREADS) next[0][i] = 0u;
+    __syncthreads();
+    uint2 pair[GR_ONE_ITEMS];
+#pragma unroll
+    for (int r = 0; r < GR_ONE_ITEMS; ++r) {
+      const int i = base + r * 32;
+      const bool have = r < items && i < edges;
+      pair[r] = !have ? make_uint2(0u, 0u) : pass == 0 ? gr_pair(index, nullptr, rows, i) : sorted[i];
+      if (have) atomicAdd(&next[warp][(pair[r].x >> shift) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    const int d = threadIdx.x;  // a digit per thread
+    uint32_t here = 0u, unused;
+    if (d < bins)
+      for (int w = 0; w < WARPS; ++w) here += next[w][d];
+    uint32_t at = gr_block_scan<WARPS>(here, warp_sums, unused);
+    if (d < bins)
+      for (int w = 0; w < WARPS; ++w) {
+        const uint32_t c = next[w][d];
+        next[w][d] = at;
+        at += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < GR_ONE_ITEMS; ++r) {
+      if (r >= items) break;
+      const bool have = base + r * 32 < edges;
+      const uint32_t digit = have ? (pair[r].x >> shift) & (bins - 1) : (uint32_t)bins;
+      const uint32_t to = gr_place(have, digit, bits, next[warp]);
+      if (have) sorted[to] = pair[r];
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < edges; i += GR_ONE_THREADS) out[i] = sorted[i];
 }
 
 // ---- sums over runs of equal keys ----------------------------------------------------------------------------
@@ -326,7 +402,7 @@ template <typename T, int VL>
 __global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint2 *__restrict__ keys, int64_t rows,
                                                                  int64_t edges, int units, int piece, int64_t pieces,
                                                                  float scale, T *__restrict__ dx,
-                                                                 const float *__restrict__ part,
+                                                                 const float *__restrict__ part, int most,
                                                                  int *__restrict__ num_long,
                                                                  uint2 *__restrict__ long_runs) {
   const int64_t id = (int64_t)blockIdx.x * GR_THREADS + threadIdx.x;
@@ -336,13 +412,14 @@ __global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint2 *__
   int slot;
   const int64_t last = gr_run(keys, edges, piece, pieces, g, run, slot);
   if (last < 0 || run >= rows) return;
-  if (last - g > GR_SHORT) {
+  if (last - g > most) {
     if (u == 0) long_runs[atomicAdd(num_long, 1)] = make_uint2((uint32_t)g, (uint32_t)last);
     return;
   }
   float acc[VL];
 #pragma unroll
   for (int c = 0; c < VL; ++c) acc[c] = part[((2 * g + slot) * units + u) * VL + c];
+#pragma unroll 8
   for (int64_t h = g + 1; h <= last; ++h)
 #pragma unroll
     for (int c = 0; c < VL; ++c) acc[c] += part[(2 * h * units + u) * VL + c];
@@ -451,30 +528,45 @@ static int gr_backward(const void *dout, const int64_t *index, int64_t rows, int
   uint2 *long_runs = (uint2 *)ws + 1;
 
   B200C_CUDA(cudaMemsetAsync(dx, 0, (size_t)rows * channels * sizeof(T), stream));  // rows that no index names
-  constexpr size_t scatter_smem = (size_t)GR_TILE * 8 + (size_t)(GR_WARPS + 1) * (4 << GR_MAX_BITS);
-  static unsigned long long configured = 0ull;
-  B200C_CUDA(opt_in_shared_memory(gather_sort_scatter_kernel, scatter_smem, configured));
+  const bool one = edges <= GR_ONE;
   const uint2 *k = nullptr;
-  for (int pass = 0; pass < p.passes; ++pass) {
-    gather_sort_count_kernel<<<(unsigned)p.blocks, GR_THREADS, 0, stream>>>(index, k, rows, edges, pass * p.bits,
-                                                                            p.bits, counts);
-    B200C_LAUNCH_CHECK("gather_sort_count_kernel");
-    gather_sort_scan_kernel<<<1u << p.bits, GR_THREADS, 0, stream>>>(counts, p.blocks, totals);
-    B200C_LAUNCH_CHECK("gather_sort_scan_kernel");
-    gather_sort_scatter_kernel<<<(unsigned)p.blocks, GR_THREADS, scatter_smem, stream>>>(
-        index, k, rows, edges, pass * p.bits, p.bits, counts, totals, pairs[pass & 1]);
-    B200C_LAUNCH_CHECK("gather_sort_scatter_kernel");
-    k = pairs[pass & 1];
+  if (one) {
+    constexpr size_t smem = (size_t)GR_ONE * 8 + (size_t)(GR_ONE_THREADS / 32) * (4 << GR_MAX_BITS);
+    static unsigned long long configured = 0ull;
+    B200C_CUDA(opt_in_shared_memory(gather_sort_one_kernel, smem, configured));
+    gather_sort_one_kernel<<<1, GR_ONE_THREADS, smem, stream>>>(index, rows, (int)edges, p.passes, p.bits, pairs[0]);
+    B200C_LAUNCH_CHECK("gather_sort_one_kernel");
+    k = pairs[0];
+  } else {
+    constexpr size_t smem = (size_t)GR_TILE * 8 + (size_t)(GR_WARPS + 1) * (4 << GR_MAX_BITS);
+    static unsigned long long configured = 0ull;
+    B200C_CUDA(opt_in_shared_memory(gather_sort_scatter_kernel, smem, configured));
+    const bool few = p.blocks <= GR_FEW;
+    for (int pass = 0; pass < p.passes; ++pass) {
+      gather_sort_count_kernel<<<(unsigned)p.blocks, GR_THREADS, 0, stream>>>(index, k, rows, edges, pass * p.bits,
+                                                                              p.bits, counts);
+      B200C_LAUNCH_CHECK("gather_sort_count_kernel");
+      if (!few) {
+        gather_sort_scan_kernel<<<1u << p.bits, GR_THREADS, 0, stream>>>(counts, p.blocks, totals);
+        B200C_LAUNCH_CHECK("gather_sort_scan_kernel");
+      }
+      gather_sort_scatter_kernel<<<(unsigned)p.blocks, GR_THREADS, smem, stream>>>(
+          index, k, rows, edges, pass * p.bits, p.bits, counts, few ? nullptr : totals, pairs[pass & 1]);
+      B200C_LAUNCH_CHECK("gather_sort_scatter_kernel");
+      k = pairs[pass & 1];
+    }
+    B200C_CUDA(cudaMemsetAsync(num_long, 0, 4, stream));
   }
-  B200C_CUDA(cudaMemsetAsync(num_long, 0, 4, stream));
   const int units = (int)(channels / VL);
   const unsigned blocks = (unsigned)((p.pieces * units + GR_THREADS - 1) / GR_THREADS);
   gather_sum_kernel<T, VL><<<blocks, GR_THREADS, 0, stream>>>((const T *)dout, k, rows, edges, units, p.piece, p.pieces,
                                                               scale, (T *)dx, part);
   B200C_LAUNCH_CHECK("gather_sum_kernel");
   gather_join_kernel<T, VL><<<blocks, GR_THREADS, 0, stream>>>(k, rows, edges, units, p.piece, p.pieces, scale,
-                                                               (T *)dx, part, num_long, long_runs);
+                                                               (T *)dx, part, one ? GR_ONE : GR_SHORT, num_long,
+                                                               long_runs);
   B200C_LAUNCH_CHECK("gather_join_kernel");
+  if (one) return B200C_OK;
   gather_join_long_kernel<T><<<296, 32 * GR_LONG_WARPS, 0, stream>>>(k, rows, edges, (int)channels, p.piece, p.pieces, scale,
                                                              (T *)dx, part, num_long, long_runs);
   B200C_LAUNCH_CHECK("gather_join_long_kernel");

@@ -566,6 +566,9 @@ GATHER = [
     (100, 70001, 128, "skewed"), (70000, 5000, 7, "any"), (513, 4097, 130, "padded"), (40, 333, 3, "padded"),
     (300000, 20000, 4, "any"), (17, 0, 16, "any"), (0, 12, 16, "padded"), (4096, 4096, 64, "sorted"),
     (9, 64, 16, "all"), (1000000, 100, 16, "any"),
+    # around the sizes at which the sort changes: one block, few blocks, many
+    (700, 16383, 8, "all"), (700, 16385, 8, "padded"), (2000, 131073, 8, "any"), (2000, 131072, 8, "skewed"),
+    (300000, 16384, 4, "any"), (300000, 140001, 4, "padded"), (40, 16385, 8, "all"),
 ]
 
 
