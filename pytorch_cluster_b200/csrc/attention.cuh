@@ -37,6 +37,7 @@ struct AttnArgs {
   const float *norms = nullptr;  // fp16: the largest |do|^2 and |v|^2 of a row
   float *parts = nullptr;        // forward, split over the columns: [m, heads, splits, channels + 2] (maximum, sum, result)
   int splits = 1;
+  int *order = nullptr;          // place for the tiles' order (attention_tensor_ordered), queries' and keys' in turn
   cudaStream_t stream = nullptr;
 };
 
@@ -78,5 +79,6 @@ size_t attention_few_workspace_bytes(const b200c_attention_t &p);
 int launch_attention_few(const AttnArgs &a, int splits, void *workspace);
 int launch_attention_join(const AttnArgs &a);          // a.parts of a.splits splits to out, rest and lse
 int attention_tensor_splits(const b200c_attention_t &p);  // of a forward pass without statistics
+size_t attention_tensor_order_bytes(const b200c_attention_t &p);  // of `order`, 0: tiles are taken as they come
 
 }  // namespace b200c

@@ -72,14 +72,15 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   const b200c_attention_t &p = a.p;
   const int tid = threadIdx.x, warp = t5_warp(), lane = tid & 31;
   const int per_group = p.heads / p.groups;
-  const int head0 = KV ? (int)blockIdx.y * per_group : (int)blockIdx.y;
-  const int group = KV ? (int)blockIdx.y : head0 / per_group;
+  const int per_tile = KV ? p.groups : p.heads, which = (int)(blockIdx.x % (unsigned)per_tile);
+  const int head0 = KV ? which * per_group : which;
+  const int group = KV ? which : head0 / per_group;
   const int heads = KV ? per_group : 1;  // heads whose columns are walked
   AtTile tile;
   if (KV)
-    tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_k, p.ptr_q, p.n, p.m, p.num_segments);
+    tile.init(at_tile_of(a.order, per_tile) * AT_ROWS, p.ptr_k, p.ptr_q, p.n, p.m, p.num_segments);
   else
-    tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
+    tile.init(at_tile_of(a.order, per_tile) * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
 
   // element threads: a row each
   const bool element = warp < F::EL_WARPS;

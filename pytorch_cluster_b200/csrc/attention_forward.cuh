@@ -58,9 +58,9 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
 
   const b200c_attention_t &p = a.p;
   const int tid = threadIdx.x, warp = t5_warp(), lane = tid & 31;
-  const int head = blockIdx.y, group = head / (p.heads / p.groups);
+  const int head = (int)(blockIdx.x % (unsigned)p.heads), group = head / (p.heads / p.groups);
   AtTile tile;
-  tile.init((int64_t)blockIdx.x * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
+  tile.init(at_tile_of(a.order, p.heads) * AT_ROWS, p.ptr_q, p.ptr_k, p.m, p.n, p.num_segments);
 
   // element threads: a row each
   const bool element = warp < F::EL_WARPS;

@@ -78,25 +78,113 @@ int attention_tensor_splits(const b200c_attention_t &p) {
   return (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
 }
 
-int launch_attention_tensor_forward(const AttnArgs &a) {
+// Tiles of long examples come to the SMs most columns first.  An order costs a launch of some 5 us and is made where blocks
+// outnumber what the GPU holds at once, take long (1024 columns and more) and are not so many that the last ones hardly count.
+constexpr int AT_ORDER_TILES = 4096, AT_ORDER_BINS = 256;
+static bool at_ordered(const b200c_attention_t &p, int64_t rows, int64_t cols, int per_tile) {
+  const int64_t tiles = (rows + AT_ROWS - 1) / AT_ROWS;
+  return p.num_segments > 1 && tiles <= AT_ORDER_TILES && tiles * per_tile > 2 * 148 && cols >= 1024 * p.num_segments;
+}
+size_t attention_tensor_order_bytes(const b200c_attention_t &p) {
+  if (!attention_tensor_applicable(p) || is_short(p)) return 0;
+  const bool any = at_ordered(p, p.m, p.n, p.heads) || at_ordered(p, p.n, p.m, p.groups);
+  return any ? (size_t)AT_ORDER_TILES * 4 : 0;
+}
+
+__global__ void __launch_bounds__(1024) attention_order_kernel(const int64_t *__restrict__ ptr_r,
+                                                              const int64_t *__restrict__ ptr_c, int64_t rows,
+                                                              int64_t cols, int segments, int tiles,
+                                                              int *__restrict__ order) {
+  __shared__ int most, at[AT_ORDER_BINS + 1];
+  const int tid = threadIdx.x;
+  if (tid == 0) most = 1;
+  if (tid <= AT_ORDER_BINS) at[tid] = 0;
+  __syncthreads();
+  int cost[AT_ORDER_TILES / 1024];
+#pragma unroll
+  for (int i = 0; i < AT_ORDER_TILES / 1024; ++i) {
+    const int64_t t0 = ((int64_t)i * 1024 + tid) * AT_ROWS;
+    cost[i] = -1;
+    if (i * 1024 + tid >= tiles) continue;
+    int64_t lo, hi, unused;
+    at_segment(ptr_c, cols, segment_of(ptr_r, segments, t0), lo, unused);
+    at_segment(ptr_c, cols, segment_of(ptr_r, segments, t0 + AT_ROWS < rows ? t0 + AT_ROWS - 1 : rows - 1), unused, hi);
+    cost[i] = hi > lo ? (int)(hi - lo) : 0;
+    atomicMax(&most, cost[i]);
+  }
+  __syncthreads();
+  // a counting sort, dearest bin first; the order within a bin is whatever it is: it moves blocks, not results
+  const float to_bin = (float)(AT_ORDER_BINS - 1) / (float)most;
+#pragma unroll
+  for (int i = 0; i < AT_ORDER_TILES / 1024; ++i)
+    if (cost[i] >= 0) {
+      const int bin = (int)((float)cost[i] * to_bin);
+      cost[i] = AT_ORDER_BINS - 1 - (bin < AT_ORDER_BINS ? bin : AT_ORDER_BINS - 1);
+      atomicAdd(&at[cost[i] + 1], 1);
+    }
+  __syncthreads();
+  if (tid < 32) {
+    int before = 0;
+    for (int b0 = 0; b0 < AT_ORDER_BINS; b0 += 32) {
+      int v = at[b0 + tid + 1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(FULL_MASK, v, o);
+        if (tid >= o) v += u;
+      }
+      at[b0 + tid + 1] = before + v;
+      before += __shfl_sync(FULL_MASK, v, 31);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < AT_ORDER_TILES / 1024; ++i)
+    if (cost[i] >= 0) order[atomicAdd(&at[cost[i]], 1)] = i * 1024 + tid;
+}
+
+// a with its tiles' order, or without
+static int at_order(AttnArgs &a, bool keys) {
+  const b200c_attention_t &p = a.p;
+  const int64_t rows = keys ? p.n : p.m, cols = keys ? p.m : p.n;
+  if (a.order == nullptr || !at_ordered(p, rows, cols, keys ? p.groups : p.heads)) {
+    a.order = nullptr;
+    return B200C_OK;
+  }
+  attention_order_kernel<<<1, 1024, 0, a.stream>>>(keys ? p.ptr_k : p.ptr_q, keys ? p.ptr_q : p.ptr_k, rows, cols,
+                                                   (int)p.num_segments, (int)((rows + AT_ROWS - 1) / AT_ROWS), a.order);
+  B200C_LAUNCH_CHECK("attention_order_kernel");
+  return B200C_OK;
+}
+
+int launch_attention_tensor_forward(const AttnArgs &args) {
+  AttnArgs a = args;
   const bool bf16 = a.p.dtype == B200C_BF16;
   if (a.splits > 1) {
     const int st = bf16 ? attention_tensor_forward_bf16(a) : attention_tensor_forward_f16(a);
     return st != B200C_OK ? st : launch_attention_join(a);
   }
   if (is_short(a.p)) return bf16 ? attention_short_forward_bf16(a) : attention_short_forward_f16(a);
+  const int st = at_order(a, false);
+  if (st != B200C_OK) return st;
   return bf16 ? attention_tensor_forward_bf16(a) : attention_tensor_forward_f16(a);
 }
 
-int launch_attention_tensor_backward(const AttnArgs &a) {
-  const bool bf16 = a.p.dtype == B200C_BF16, brief = is_short(a.p);
+int launch_attention_tensor_backward(const AttnArgs &args) {
+  AttnArgs a = args;
+  const bool bf16 = a.p.dtype == B200C_BF16;
+  int st = B200C_OK;
+  if (is_short(a.p)) {
+    if (a.dq) st = bf16 ? attention_short_dq_bf16(a) : attention_short_dq_f16(a);
+    if (st != B200C_OK || !a.dk) return st;
+    return bf16 ? attention_short_dkv_bf16(a) : attention_short_dkv_f16(a);
+  }
   if (a.dq) {
-    const int st = brief ? bf16 ? attention_short_dq_bf16(a) : attention_short_dq_f16(a)
-                         : bf16 ? attention_tensor_dq_bf16(a) : attention_tensor_dq_f16(a);
+    if ((st = at_order(a, false)) == B200C_OK) st = bf16 ? attention_tensor_dq_bf16(a) : attention_tensor_dq_f16(a);
     if (st != B200C_OK) return st;
   }
   if (!a.dk) return B200C_OK;
-  if (brief) return bf16 ? attention_short_dkv_bf16(a) : attention_short_dkv_f16(a);
+  a.order = args.order;
+  if ((st = at_order(a, true)) != B200C_OK) return st;
   return bf16 ? attention_tensor_dkv_bf16(a) : attention_tensor_dkv_f16(a);
 }
 

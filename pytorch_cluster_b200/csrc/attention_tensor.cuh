@@ -50,6 +50,13 @@ __device__ __forceinline__ int at_segment_of_warp(const int64_t *__restrict__ pt
   return lo;
 }
 
+// The tile of this block: the heads of a tile run side by side, tiles in the order given, so that what runs last is cheap
+// (16 clouds of 1594 to 2555 points: forward 642 -> 613 us, dq 705 -> 637; 8 of 4000 points with 128 channels 1344 -> 1223).
+__device__ __forceinline__ int64_t at_tile_of(const int *order, int per_tile) {
+  const unsigned i = blockIdx.x / (unsigned)per_tile;
+  return order ? order[i] : (int64_t)i;
+}
+
 // The columns of a pass over the tile.
 struct AtPass {
   int64_t c_lo, c_hi;

@@ -19,7 +19,7 @@ struct AtForwardCall {
     if (st == B200C_OK)
       st = attention_tensor_map(&maps.v, p.v, p.dtype, p.n, p.groups, p.channels, p.v_row, p.v_head, AT_COLS);
     if (st != B200C_OK) return st;
-    const dim3 grid((unsigned)((p.m + AT_ROWS - 1) / AT_ROWS), (unsigned)p.heads, (unsigned)a.splits);
+    const dim3 grid((unsigned)((p.m + AT_ROWS - 1) / AT_ROWS * p.heads), 1, (unsigned)a.splits);
     static unsigned long long configured = 0ull;
     B200C_CUDA(opt_in_shared_memory(attention_forward_kernel<T, CP, DIM, CAP>, F::SMEM, configured));
     attention_forward_kernel<T, CP, DIM, CAP><<<grid, F::THREADS, F::SMEM, a.stream>>>(maps, a, (T *)a.rest);
@@ -46,7 +46,7 @@ struct AtBackwardCall {
     if (st == B200C_OK)
       st = attention_tensor_map(v, p.v, p.dtype, p.n, p.groups, p.channels, p.v_row, p.v_head, k_box);
     if (st != B200C_OK) return st;
-    const dim3 grid((unsigned)(((KV ? p.n : p.m) + AT_ROWS - 1) / AT_ROWS), (unsigned)(KV ? p.groups : p.heads));
+    const dim3 grid((unsigned)(((KV ? p.n : p.m) + AT_ROWS - 1) / AT_ROWS * (KV ? p.groups : p.heads)));
     static unsigned long long configured = 0ull;
     B200C_CUDA(opt_in_shared_memory(attention_backward_kernel<T, CP, DIM, CAP, KV>, F::SMEM, configured));
     attention_backward_kernel<T, CP, DIM, CAP, KV><<<grid, F::THREADS, F::SMEM, a.stream>>>(maps, a, a.norms);

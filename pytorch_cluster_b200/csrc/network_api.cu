@@ -150,7 +150,8 @@ extern "C" size_t b200c_attention_workspace_bytes(const b200c_attention_t *a) {
   const size_t few = attention_few_workspace_bytes(*a);
   if (few > 0) return few;
   const int splits = attention_tensor_splits(*a);
-  return splits > 1 ? (size_t)a->m * a->heads * splits * (a->channels + 2) * 4 : 0;
+  if (splits > 1) return (size_t)a->m * a->heads * splits * (a->channels + 2) * 4;
+  return attention_tensor_order_bytes(*a);
 }
 
 extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, void *rest, float *lse, void *workspace,
@@ -175,7 +176,10 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
   if (attention_tensor_applicable(*p) && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0) {
     // the statistics of a training step need the exact sums, which the joined parts do not carry
     if (lse == nullptr && rest == nullptr) a.splits = attention_tensor_splits(*p);
-    a.parts = (float *)workspace;
+    if (a.splits > 1)
+      a.parts = (float *)workspace;
+    else if (attention_tensor_splits(*p) == 1 && need > 0)
+      a.order = (int *)workspace;
     return launch_attention_tensor_forward(a);
   }
   return launch_attention_plain_forward(a);
@@ -183,7 +187,7 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
 
 extern "C" size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a) {
   if (check_attention(a) != B200C_OK) return 0;
-  return align256((size_t)a->m * a->heads * 4) + 256;  // D, and the largest norms
+  return align256((size_t)a->m * a->heads * 4) + 256 + attention_tensor_order_bytes(*a);  // D, the largest norms, order
 }
 
 extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const void *rest, const float *lse,
@@ -212,6 +216,7 @@ extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *
   a.stream = (cudaStream_t)stream;
   float *norms = (float *)((char *)workspace + align256((size_t)p->m * p->heads * 4));
   a.norms = norms;
+  if (attention_tensor_order_bytes(*p) > 0) a.order = (int *)((char *)norms + 256);
   if ((st = launch_attention_delta(a, (float *)workspace, norms)) != B200C_OK) return st;
   if (attention_tensor_applicable(*p) &&
       (((uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0)

@@ -430,6 +430,12 @@ def test_attention_small_calls_split_over_the_keys(dtype, channels):
     check_attention(dtype, [128, 128], [4000, 1], 1, 1, channels, 1, seed=33, train=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens, groups, channels", [([1600, 0, 1900], 16, 16), ([300, 3000, 900], 4, 72)])
+def test_attention_many_tiles_of_uneven_examples(dtype, lens, groups, channels):
+    check_attention(dtype, lens, lens, 16, groups, channels, 3 if groups == 4 else 0, seed=41)
+
+
 # ---- norm_rotate ---------------------------------------------------------------------------------------------
 
 def rotate_plain(x, pos, freq, weight, eps, dy=None):
