@@ -6,8 +6,10 @@
 // free of bank conflicts); a thread holds a 4 x 4 tile of the scores and 4 x channels/16 of the result.  Where shared memory
 // has room for two blocks per SM all the same, the next tile is on its way (asynchronous copies for fp32) while this
 // one is worked on.  tanh is CUDA's: an error of the hardware's form would be multiplied by the cap.
-// Tiles hold rows of several examples where examples are short; those are processed one example after the other, so
-// that a NaN in one example never meets another one's zeros.
+// Tiles begin with an example, so that a block walks one example's columns (fp32, 8 clouds of 256 to 676 points: forward
+// 223 -> 136 us, dq 264 -> 165, dk and dv 317 -> 196 against 64 rows wherever they fall).  Where examples are shorter
+// than 16 rows, tiles hold rows of several; those are processed one example after the other, so that a NaN in one
+// example never meets another one's zeros.
 // The backward pass is two kernels of the same shape: one owns 64 queries and sums dq over the keys, one owns 64 keys and
 // sums dk and dv over the queries of all heads of its group.  Scores are formed twice, but nothing is
 // added atomically: the result does not depend on the order of the blocks.
@@ -132,6 +134,39 @@ struct ApSmem {
   static constexpr int FLOATS = OWN * TILE + POS + W + BUFS * SET;
 };
 
+// Whether tiles begin with an example; the blocks of a launch then.
+__host__ __device__ __forceinline__ bool ap_aligned(const int64_t *ptr, int64_t rows, int64_t segments) {
+  return ptr != nullptr && segments <= rows / 16;
+}
+static unsigned ap_blocks(const int64_t *ptr, int64_t rows, int64_t segments) {
+  return (unsigned)(ap_aligned(ptr, rows, segments) ? rows / AP_T + segments : (rows + AP_T - 1) / AP_T);
+}
+// The rows [t0, t1) of tile i, or false where there are none.  The tiles of segment b are numbered from (first row of b) / 64 + b,
+// which leaves room for all of them; rows outside every segment go with the first or the last.
+__device__ __forceinline__ bool ap_tile(const int64_t *__restrict__ ptr, int64_t rows, int segments, int64_t i,
+                                        int64_t &t0, int64_t &t1) {
+  t0 = i * AP_T;
+  int64_t end = rows;
+  if (ap_aligned(ptr, rows, segments)) {
+    const auto first = [&](int b) {
+      const int64_t at = b == 0 ? 0 : ptr[b];
+      return at < 0 ? 0 : at > rows ? rows : at;
+    };
+    int lo = 0, hi = segments - 1;  // the last segment whose number is not above i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first(mid) / AP_T + mid <= i)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    t0 = first(lo) + (i - first(lo) / AP_T - lo) * AP_T;
+    if (lo + 1 < segments) end = first(lo + 1);
+  }
+  t1 = t0 + AP_T < end ? t0 + AP_T : end;
+  return t0 < t1;
+}
+
 template <typename T, int CP>
 __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(AttnArgs a) {
   constexpr int NC = CP / 16;
@@ -145,7 +180,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_forward_kernel(Att
   const T *k = (const T *)p.k + (int64_t)group * p.k_head;
   const T *v = (const T *)p.v + (int64_t)group * p.v_head;
   const float slope = p.dims > 0 ? p.slope[head] : 0.f;
-  const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
+  int64_t t0, t1;
+  if (!ap_tile(p.ptr_q, p.m, (int)p.num_segments, blockIdx.x, t0, t1)) return;
   T *out = (T *)a.out, *rest = (T *)a.rest;
 
   ap_load<T, CP>(sq, q, p.q_row, t0, t0, t1, p.channels, tid);
@@ -266,7 +302,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dq_kernel(AttnArgs
   const T *dout = (const T *)a.dout + (int64_t)head * p.channels;
   T *dq = (T *)a.dq + (int64_t)head * p.channels;
   const float slope = p.dims > 0 ? p.slope[head] : 0.f;
-  const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.m ? t0 + AP_T : p.m;
+  int64_t t0, t1;
+  if (!ap_tile(p.ptr_q, p.m, (int)p.num_segments, blockIdx.x, t0, t1)) return;
 
   ap_load<T, CP>(sq, q, p.q_row, t0, t0, t1, p.channels, tid);
   ap_load<T, CP>(sdo, dout, qrow, t0, t0, t1, p.channels, tid);
@@ -367,7 +404,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
   const T *k = (const T *)p.k + (int64_t)group * p.k_head;
   const T *v = (const T *)p.v + (int64_t)group * p.v_head;
   T *dk = (T *)a.dk + (int64_t)group * p.channels, *dv = (T *)a.dv + (int64_t)group * p.channels;
-  const int64_t t0 = (int64_t)blockIdx.x * AP_T, t1 = t0 + AP_T < p.n ? t0 + AP_T : p.n;
+  int64_t t0, t1;
+  if (!ap_tile(p.ptr_k, p.n, (int)p.num_segments, blockIdx.x, t0, t1)) return;
 
   ap_load<T, CP>(sk, k, p.k_row, t0, t0, t1, p.channels, tid);
   ap_load<T, CP>(sv, v, p.v_row, t0, t0, t1, p.channels, tid);
@@ -540,7 +578,7 @@ static int ap_forward(const AttnArgs &a) {
   static_assert(smem <= 227 * 1024, "shared memory of a block");
   static unsigned long long configured = 0ull;
   B200C_CUDA(opt_in_shared_memory(attention_plain_forward_kernel<T, CP>, smem, configured));
-  const dim3 grid((unsigned)((a.p.m + AP_T - 1) / AP_T), (unsigned)a.p.heads);
+  const dim3 grid(ap_blocks(a.p.ptr_q, a.p.m, a.p.num_segments), (unsigned)a.p.heads);
   attention_plain_forward_kernel<T, CP><<<grid, AP_THREADS, smem, a.stream>>>(a);
   B200C_LAUNCH_CHECK("attention_plain_forward_kernel");
   return B200C_OK;
@@ -553,13 +591,13 @@ static int ap_backward(const AttnArgs &a) {
   static unsigned long long configured_q = 0ull, configured_kv = 0ull;
   if (a.dq && a.p.m > 0) {
     B200C_CUDA(opt_in_shared_memory(attention_plain_dq_kernel<T, CP>, smem, configured_q));
-    const dim3 grid((unsigned)((a.p.m + AP_T - 1) / AP_T), (unsigned)a.p.heads);
+    const dim3 grid(ap_blocks(a.p.ptr_q, a.p.m, a.p.num_segments), (unsigned)a.p.heads);
     attention_plain_dq_kernel<T, CP><<<grid, AP_THREADS, smem, a.stream>>>(a);
     B200C_LAUNCH_CHECK("attention_plain_dq_kernel");
   }
   if (a.dk && a.p.n > 0) {
     B200C_CUDA(opt_in_shared_memory(attention_plain_dkv_kernel<T, CP>, smem, configured_kv));
-    const dim3 grid((unsigned)((a.p.n + AP_T - 1) / AP_T), (unsigned)a.p.groups);
+    const dim3 grid(ap_blocks(a.p.ptr_k, a.p.n, a.p.num_segments), (unsigned)a.p.groups);
     attention_plain_dkv_kernel<T, CP><<<grid, AP_THREADS, smem, a.stream>>>(a);
     B200C_LAUNCH_CHECK("attention_plain_dkv_kernel");
   }
