@@ -12,7 +12,8 @@
 // the sums over i running over all heads of the key's group.  p is formed again from the forward pass's
 //   lse_i = log2 sum_j exp(z_ij)      (+inf for rows that give zeros, so that p = 0),
 // stored [heads, m].  D is a small difference of what the rounded outputs give where few keys share the weight, so the
-// forward pass of a training step also keeps what rounding took from out, in out's type.  Scores are kept in units of log 2: exp(z) = 2^(z log2 e).
+// forward pass of a training step also keeps what rounding took from out, in out's type.  Scores are kept in units of
+// log 2: exp(z) = 2^(z log2 e).
 #pragma once
 
 #include "common.cuh"
@@ -22,8 +23,8 @@ namespace b200c {
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr int AT_MAX_CHANNELS = 128;
 constexpr int AT_MAX_DIMS = 8;
-// The kernels for 16-bit types form tanh(y) as 1 - 2 / (e^2y + 1), right to 4e-7 absolutely, which the cap multiplies; above
-// this cap (1e-4 of a score) CUDA's tanh is called, in the plain kernels.
+// The kernels for 16-bit types form tanh(y) as 1 - 2 / (e^2y + 1), right to 4e-7 absolutely, which the cap multiplies;
+// above this cap (1e-4 of a score) CUDA's tanh is called, in the plain kernels.
 constexpr float AT_MAX_FAST_CAP = 256.f;
 
 struct AttnArgs {
@@ -35,7 +36,8 @@ struct AttnArgs {
   const float *delta = nullptr;  // [heads, m]: D_i
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // [m, heads, channels], [n, groups, channels] x 2
   const float *norms = nullptr;  // fp16: the largest |do|^2 and |v|^2 of a row
-  float *parts = nullptr;        // forward, split over the columns: [m, heads, splits, channels + 2] (maximum, sum, result)
+  // forward, split over the columns: [m, heads, splits, channels + 2] (maximum, sum, result)
+  float *parts = nullptr;
   int splits = 1;
   int *order = nullptr;          // place for the tiles' order (attention_tensor_ordered), queries' and keys' in turn
   cudaStream_t stream = nullptr;

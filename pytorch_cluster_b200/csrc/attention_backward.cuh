@@ -4,10 +4,11 @@
 // Forming the scores once per direction costs two products more than one kernel for both would, which the tensor
 // cores have to spare here; in return no sum is shared between blocks, so there are no atomics.  The statistics of the
 // softmax are known, so the groups' steps need nothing of one another and share one accumulator.
-// P and dS enter the second products in the 16-bit type.  dq takes dS in two parts, rounded and what rounding left, because the
-// rows of dS sum to zero and a rounded one does not: dq's error was 1.5 times that of its own rounding, now it is
-// that (for dk and dv, 1.4 times, tensor memory has no room left).  In fp16, whose range is small, P is kept times 2^12 and dS times a
-// power of two that brings the largest value that |do| and |v| allow to 2^14; both are taken out of the fp32 sums.
+// P and dS enter the second products in the 16-bit type.  dq takes dS in two parts, rounded and what rounding left,
+// because the rows of dS sum to zero and a rounded one does not: dq's error was 1.5 times that of its own rounding, now
+// it is that (for dk and dv, 1.4 times, tensor memory has no room left).  In fp16, whose range is small, P is kept
+// times 2^12 and dS times a power of two that brings the largest value that |do| and |v| allow to 2^14; both are taken
+// out of the fp32 sums.
 #pragma once
 
 #include "attention_tensor.cuh"
@@ -16,7 +17,8 @@ namespace b200c {
 
 template <int CP, bool KV>
 struct AtBackward {
-  // groups and resident blocks per SM, as tensor memory allows: 16 warps per SM, 8 where two results of 128 channels fill it
+  // groups and resident blocks per SM, as tensor memory allows: 16 warps per SM, 8 where two results of 128 channels
+  // fill it
   static constexpr int BLOCKS = CP == 64 && !KV ? 2 : 1;
   static constexpr int G = CP == 64 && !KV ? 2 : CP == 128 && KV ? 2 : 4;
   static constexpr int EL_WARPS = 4 * G, EL_THREADS = 32 * EL_WARPS;
@@ -61,7 +63,8 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
   unsigned char *smem = at_raw + ((1024u - (t5_smem(at_raw) & 1023u)) & 1023u);
   unsigned char *rows0 = smem, *rows1 = smem + F::ROW_BYTES, *stages = smem + 2 * F::ROW_BYTES;
   float *side = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  // s_full / s_free: a pair's scores are in / have been read; w_ready: a group's weights are in; a_done: their product is
+  // s_full / s_free: a pair's scores are in / have been read; w_ready: a group's weights are in; a_done: their product
+  // is
   __shared__ __align__(8) uint64_t r_full, full[F::STAGES], empty[F::STAGES], s_full[F::PAIRS], s_free[F::PAIRS],
       w_ready[G], a_done[G], done, drained[2];
   __shared__ uint32_t tmem_s;

@@ -5,8 +5,8 @@
 // A block owns one (example, key/value head, split of the example's keys) and takes up to QB rows (query, head of the
 // group) at a time.  LPK lanes share a key, 16 bytes of its channels each; the lane groups of the block walk the
 // split's keys in turn, U keys ahead of their use, each with a running maximum, sum and result of its own, which are
-// joined by shuffles and through shared memory at the end.  The splits' parts go to the workspace in fp32 and a second kernel joins
-// them, in ascending order of the splits.
+// joined by shuffles and through shared memory at the end.  The splits' parts go to the workspace in fp32 and a second
+// kernel joins them, in ascending order of the splits.
 #include "attention_tensor.cuh"
 #include "attention_warp.cuh"
 
@@ -215,13 +215,14 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_kernel(AttnArgs a, i
 }
 
 // ---- 16-bit types ------------------------------------------------------------------------------------------------
-// The same split over examples, key heads and keys, with the two products on the tensor cores.  Up to 16 rows are too few for
-// a tcgen05 tile of 128; warp-wide products of 16 x 8 x 16 take them as they are, so a warp spends a few hundred
-// instructions on 16 KB of keys and values and memory is the only bound.  Each of the block's warps has a ring of its own in shared
-// memory, 32 keys and values to a stage, filled by asynchronous 16-byte copies two stages ahead: no barrier
-// between warps until the end.  A row of 2 * CP bytes keeps its 16-byte chunk c at c ^ (row & 7), so that neither the copies nor
-// the matrix loads meet bank conflicts.  Weights are rounded to the 16-bit type; maxima, sums and results are fp32.
-// Shared memory of keys past the split's end is cleared: their weights are 0, and 0 times whatever stood there must be 0.
+// The same split over examples, key heads and keys, with the two products on the tensor cores.  Up to 16 rows are too
+// few for a tcgen05 tile of 128; warp-wide products of 16 x 8 x 16 take them as they are, so a warp spends a few
+// hundred instructions on 16 KB of keys and values and memory is the only bound.  Each of the block's warps has a ring
+// of its own in shared memory, 32 keys and values to a stage, filled by asynchronous 16-byte copies two stages ahead:
+// no barrier between warps until the end.  A row of 2 * CP bytes keeps its 16-byte chunk c at c ^ (row & 7), so that
+// neither the copies nor the matrix loads meet bank conflicts.  Weights are rounded to the 16-bit type; maxima, sums
+// and results are fp32. Shared memory of keys past the split's end is cleared: their weights are 0, and 0 times
+// whatever stood there must be 0.
 constexpr int AF_KEYS = 32;    // keys of a stage
 constexpr int AF_STAGES = 3;
 constexpr int AF_ROWS = 16;    // rows (query, head of the group) of a pass
@@ -315,7 +316,8 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnAr
   };
 
   for (int64_t r0 = 0; r0 < rows; r0 += AF_ROWS) {
-    // the rows' queries as the first operand: lane holds rows lane / 4 and lane / 4 + 8, channels 2 (lane % 4) + {0, 1, 8, 9}
+    // the rows' queries as the first operand: lane holds rows lane / 4 and lane / 4 + 8, channels 2 (lane % 4) + {0, 1,
+    // 8, 9}
     const int gr = lane >> 2, gc = (lane & 3) * 2;
     uint32_t qf[KT][4];
     float pos[2][DIM == 0 ? 1 : DIM], slope[2] = {}, top[2], sum[2] = {}, o[CT][4] = {};

@@ -1,11 +1,11 @@
 // Forward attention on the tensor cores: 128 queries of one head per block, see attention_tensor.cuh.
 //
-// Each group of warps has its own running maximum, sum and result of its steps; they are joined at the end.  The maximum
-// is not looked for in every step: weights are formed against the one in use, and only where their sum over the step's 32
-// columns passes 2^10 (or no maximum is known yet) is it raised to the step's and the result in tensor memory, the sum
-// and the step's weights brought to it.  Weights up to 2^10 are as exact in either type as weights up to 1.
-// Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.  The result
-// is divided by the sum of the rounded weights, not of the exact ones (which the statistics keep): where few
+// Each group of warps has its own running maximum, sum and result of its steps; they are joined at the end.  The
+// maximum is not looked for in every step: weights are formed against the one in use, and only where their sum over the
+// step's 32 columns passes 2^10 (or no maximum is known yet) is it raised to the step's and the result in tensor
+// memory, the sum and the step's weights brought to it.  Weights up to 2^10 are as exact in either type as weights up
+// to 1. Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.
+// The result is divided by the sum of the rounded weights, not of the exact ones (which the statistics keep): where few
 // keys share the weight their roundings then cancel, and D = do . o, which the gradients need, is as much better.
 #pragma once
 
@@ -47,7 +47,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   unsigned char *sq = smem;
   unsigned char *stages = smem + F::Q_BYTES;
   float *spos = reinterpret_cast<float *>(stages + F::STAGES * F::STAGE_BYTES);
-  // s_full / s_free: a pair's scores are in / have been read; w_ready: a group's weights are in; a_done: their product is
+  // s_full / s_free: a pair's scores are in / have been read; w_ready: a group's weights are in; a_done: their product
+  // is
   __shared__ __align__(8) uint64_t q_full, full[F::STAGES], empty[F::STAGES], s_full[F::PAIRS], s_free[F::PAIRS],
       w_ready[G], a_done[G], done, drained[2];
   __shared__ uint32_t tmem_s;
@@ -132,7 +133,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   // this block's share of a pass's columns, in whole stages
   auto share = [&]() {
     if (a.splits <= 1) return;
-    const int64_t each = (pass.c_hi - pass.c_lo + (int64_t)a.splits * AT_COLS - 1) / ((int64_t)a.splits * AT_COLS) * AT_COLS;
+    const int64_t unit = (int64_t)a.splits * AT_COLS;
+    const int64_t each = (pass.c_hi - pass.c_lo + unit - 1) / unit * AT_COLS;
     pass.c_lo += each * blockIdx.z;
     if (pass.c_lo > pass.c_hi) pass.c_lo = pass.c_hi;
     if (pass.c_lo + each < pass.c_hi) pass.c_hi = pass.c_lo + each;
@@ -419,8 +421,9 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
           a.lse[(int64_t)head * p.m + row] = none ? pos_inf<float>() : all_top + log2f(all_sum);
         asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");
         const int64_t stride = (int64_t)p.heads * p.channels;
-        if (a.splits == 1) at_write_rows<T, CP>(tile_out, shared_tile, tile, pass, (T *)a.out + (int64_t)head * p.channels, stride,
-                             p.channels, tid, F::EL_THREADS);
+        if (a.splits == 1)
+          at_write_rows<T, CP>(tile_out, shared_tile, tile, pass, (T *)a.out + (int64_t)head * p.channels, stride,
+                               p.channels, tid, F::EL_THREADS);
         if (rest)
           at_write_rows<T, CP>(tile_rest, shared_tile, tile, pass, rest + (int64_t)head * p.channels, stride, p.channels,
                                tid, F::EL_THREADS);

@@ -3,16 +3,15 @@
 // A block of 256 threads owns 64 rows of one head and walks the other side's rows of the same example in tiles of
 // 64: one pass over the keys with the running maximum and sum of the softmax.  Operands are widened to fp32 and kept
 // transposed in shared memory ([channel][row], rows padded to 68 so that the 16-byte reads of both products are
-// free of bank conflicts); a thread holds a 4 x 4 tile of the scores and 4 x channels/16 of the result.  Where shared memory
-// has room for two blocks per SM all the same, the next tile is on its way (asynchronous copies for fp32) while this
-// one is worked on.  tanh is CUDA's: an error of the hardware's form would be multiplied by the cap.
-// Tiles begin with an example, so that a block walks one example's columns (fp32, 8 clouds of 256 to 676 points: forward
-// 223 -> 136 us, dq 264 -> 165, dk and dv 317 -> 196 against 64 rows wherever they fall).  Where examples are shorter
-// than 16 rows, tiles hold rows of several; those are processed one example after the other, so that a NaN in one
-// example never meets another one's zeros.
-// The backward pass is two kernels of the same shape: one owns 64 queries and sums dq over the keys, one owns 64 keys and
-// sums dk and dv over the queries of all heads of its group.  Scores are formed twice, but nothing is
-// added atomically: the result does not depend on the order of the blocks.
+// free of bank conflicts); a thread holds a 4 x 4 tile of the scores and 4 x channels/16 of the result.  Where shared
+// memory has room for two blocks per SM all the same, the next tile is on its way (asynchronous copies for fp32) while
+// this one is worked on.  tanh is CUDA's: an error of the hardware's form would be multiplied by the cap. Tiles begin
+// with an example, so that a block walks one example's columns (fp32, 8 clouds of 256 to 676 points: forward 223 -> 136
+// us, dq 264 -> 165, dk and dv 317 -> 196 against 64 rows wherever they fall).  Where examples are shorter than 16
+// rows, tiles hold rows of several; those are processed one example after the other, so that a NaN in one example never
+// meets another one's zeros. The backward pass is two kernels of the same shape: one owns 64 queries and sums dq over
+// the keys, one owns 64 keys and sums dk and dv over the queries of all heads of its group.  Scores are formed twice,
+// but nothing is added atomically: the result does not depend on the order of the blocks.
 #include "attention.cuh"
 #include "tcgen05.cuh"
 
@@ -124,8 +123,8 @@ __device__ __forceinline__ float ap_sum16(float v) {
   return v;
 }
 
-// floats of shared memory: `own` tiles of the block's rows, two of the columns in BUFS sets (with coordinates and statistics), the
-// weights.  Two sets where two blocks then still fit an SM.
+// floats of shared memory: `own` tiles of the block's rows, two of the columns in BUFS sets (with coordinates and
+// statistics), the weights.  Two sets where two blocks then still fit an SM.
 template <int CP, int OWN>
 struct ApSmem {
   static constexpr int TILE = CP * AP_LD, W = AP_T * AP_LD, POS = AT_MAX_DIMS * AP_LD, STAT = 2 * AP_T;
@@ -141,8 +140,8 @@ __host__ __device__ __forceinline__ bool ap_aligned(const int64_t *ptr, int64_t 
 static unsigned ap_blocks(const int64_t *ptr, int64_t rows, int64_t segments) {
   return (unsigned)(ap_aligned(ptr, rows, segments) ? rows / AP_T + segments : (rows + AP_T - 1) / AP_T);
 }
-// The rows [t0, t1) of tile i, or false where there are none.  The tiles of segment b are numbered from (first row of b) / 64 + b,
-// which leaves room for all of them; rows outside every segment go with the first or the last.
+// The rows [t0, t1) of tile i, or false where there are none.  The tiles of segment b are numbered from (first row of
+// b) / 64 + b, which leaves room for all of them; rows outside every segment go with the first or the last.
 __device__ __forceinline__ bool ap_tile(const int64_t *__restrict__ ptr, int64_t rows, int segments, int64_t i,
                                         int64_t &t0, int64_t &t1) {
   t0 = i * AP_T;
@@ -507,8 +506,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
   cp_async_wait<0>();  // a block without a tile still has its own rows' copies under way
 }
 
-// What the backward pass needs beforehand: D_i = do_i . o_i per (row, head), and for fp16 the largest |do_i|^2 and |v_j|^2
-// of any row (norms[0], norms[1]; non-negative floats order like their bits, and a maximum does not depend on
+// What the backward pass needs beforehand: D_i = do_i . o_i per (row, head), and for fp16 the largest |do_i|^2 and
+// |v_j|^2 of any row (norms[0], norms[1]; non-negative floats order like their bits, and a maximum does not depend on
 // the order).  LP lanes share a row, VL channels at a time; the blocks past the first `do_blocks` take the rows of v.
 template <typename T, int VL>
 struct alignas(sizeof(T) * VL) ApVec {
@@ -523,7 +522,8 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, floa
   const b200c_attention_t &p = a.p;
   const int part = threadIdx.x % LP, units = p.channels / VL;
   const bool values = blockIdx.x >= do_blocks;
-  const unsigned block = values ? blockIdx.x - do_blocks : blockIdx.x, blocks = values ? gridDim.x - do_blocks : do_blocks;
+  const unsigned block = values ? blockIdx.x - do_blocks : blockIdx.x;
+  const unsigned blocks = values ? gridDim.x - do_blocks : do_blocks;
   const int64_t rows = values ? p.n * p.groups : do_rows;
   const V *dout = (const V *)a.dout, *out = (const V *)a.out, *rest = (const V *)a.rest;
   float most = 0.f;
@@ -532,8 +532,8 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, floa
     const int64_t i = i0 + threadIdx.x / LP;
     float s = 0.f, sq = 0.f;
     if (i < rows) {
-      const V *v = values ? reinterpret_cast<const V *>((const T *)p.v + (i / p.groups) * p.v_row + (i % p.groups) * p.v_head)
-                          : dout + i * units;
+      const V *v = dout + i * units;
+      if (values) v = reinterpret_cast<const V *>((const T *)p.v + (i / p.groups) * p.v_row + (i % p.groups) * p.v_head);
       for (int u = part; u < units; u += LP) {
         const V g = v[u];
         if (values) {

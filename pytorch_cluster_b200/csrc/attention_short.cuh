@@ -11,7 +11,8 @@
 // worked on; there is no barrier between warps.  16 rows that lie in several examples are taken example by example, and
 // only the example's rows are stored, so that a NaN of one never meets another one's zeros; columns past
 // the example's end are cleared in shared memory for the same reason.
-// Weights are rounded to the type as operands (dS of dq in two parts, see attention_backward.cuh); statistics and sums are fp32.
+// Weights are rounded to the type as operands (dS of dq in two parts, see attention_backward.cuh); statistics and sums
+// are fp32.
 #pragma once
 
 #include "attention_tensor.cuh"
@@ -100,8 +101,8 @@ __global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const
     const int64_t count = c_hi - c_lo;
     const int blocks = (int)((count + AS_COLS - 1) / AS_COLS);  // per head
 
-    // copies of step (u, e, j): the unit's rows with its first step, the columns' tiles and what belongs to them.  A lane
-    // copies chunk my_c of rows my_r, my_r + PER, ...
+    // copies of step (u, e, j): the unit's rows with its first step, the columns' tiles and what belongs to them.  A
+    // lane copies chunk my_c of rows my_r, my_r + PER, ...
     constexpr int PER = 32 / CHUNKS;
     const int my_r = lane / CHUNKS, my_c = lane % CHUNKS;
     const T *r0_at = (const T *)rows0.base + (t0 + my_r) * rows0.row + my_c * 8;
@@ -247,7 +248,8 @@ __global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const
                 if constexpr (FORWARD) {
                   s[n][2 * h + c] = there ? t : -pos_inf<float>();
                 } else {
-                  const float l = KV ? stat[n * 8 + c] - A::SHIFT : lse[h], de = KV ? stat[AS_COLS + n * 8 + c] : delta[h];
+                  const float l = KV ? stat[n * 8 + c] - A::SHIFT : lse[h];
+                  const float de = KV ? stat[AS_COLS + n * 8 + c] : delta[h];
                   const float pr = t5_ex2(t - l);
                   float ds = pr * (dp[n][2 * h + c] - de);
                   if constexpr (CAP) ds *= fmaf(-w, w, 1.f);

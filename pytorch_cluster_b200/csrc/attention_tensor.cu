@@ -29,7 +29,8 @@ int attention_tensor_map(CUtensorMap *map, const void *base, int dtype, int64_t 
   }
   const cuuint64_t dims[3] = {(cuuint64_t)channels, (cuuint64_t)heads, (cuuint64_t)rows};
   // a stride that no coordinate uses still has to be a valid one
-  const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? head_stride : 128) * 2, (cuuint64_t)(rows > 1 ? row_stride : 128) * 2};
+  const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? head_stride : 128) * 2,
+                                 (cuuint64_t)(rows > 1 ? row_stride : 128) * 2};
   const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
   const CUresult r = encode(map, dtype == B200C_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                             3, (void *)base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -50,13 +51,15 @@ static bool at_side(const void *base, int64_t rows, int heads, int64_t row_strid
 
 bool attention_tensor_applicable(const b200c_attention_t &p) {
   constexpr int64_t most = 0x7fffffffLL - 1024;  // column numbers of a step past the last stay in 32 bits
-  return p.dtype != B200C_F32 && p.channels % 8 == 0 && !(p.cap > AT_MAX_FAST_CAP) && p.m > 0 && p.n > 0 && p.m < most && p.n < most &&
+  return p.dtype != B200C_F32 && p.channels % 8 == 0 && !(p.cap > AT_MAX_FAST_CAP) &&
+         p.m > 0 && p.n > 0 && p.m < most && p.n < most &&
          at_side(p.q, p.m, p.heads, p.q_row, p.q_head) && at_side(p.k, p.n, p.groups, p.k_row, p.k_head) &&
          at_side(p.v, p.n, p.groups, p.v_row, p.v_head);
 }
 
-// Up to 32 channels and 128 rows per example on average (either side) the kernels of attention_short.cuh are taken.  Measured
-// on 60000 rows, 8 heads, three coordinates, bfloat16, forward / gradient in us, 128-row tiles against 16-row ones:
+// Up to 32 channels and 128 rows per example on average (either side) the kernels of attention_short.cuh are taken.
+// Measured on 60000 rows, 8 heads, three coordinates, bfloat16, forward / gradient in us, 128-row tiles against 16-row
+// ones:
 //   32 channels: 16 rows 185 / 437, 125 / 254;  64 rows 220 / 488, 151 / 331;  128 rows 251 / 567, 208 / 463;
 //                192 rows 277 / 633, 266 / 594
 //   64 channels: 16 rows 188 / 465, 198 / 471;  64 rows 220 / 510, 250 / 602
@@ -67,8 +70,8 @@ static bool is_short(const b200c_attention_t &p) {
          p.n <= AT_SHORT_ROWS * p.num_segments;
 }
 
-// A small call leaves most SMs without a block of 128 rows: the columns are dealt out to several, 128 and more to each, as long
-// as that fills the SMs, and a second kernel joins them (one cloud of 1024 points, 4 heads: 33 -> 25 us).
+// A small call leaves most SMs without a block of 128 rows: the columns are dealt out to several, 128 and more to each,
+// as long as that fills the SMs, and a second kernel joins them (one cloud of 1024 points, 4 heads: 33 -> 25 us).
 int attention_tensor_splits(const b200c_attention_t &p) {
   if (!attention_tensor_applicable(p) || is_short(p)) return 1;
   const int64_t blocks = (p.m + AT_ROWS - 1) / AT_ROWS * p.heads;
@@ -78,8 +81,9 @@ int attention_tensor_splits(const b200c_attention_t &p) {
   return (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
 }
 
-// Tiles of long examples come to the SMs most columns first.  An order costs a launch of some 5 us and is made where blocks
-// outnumber what the GPU holds at once, take long (1024 columns and more) and are not so many that the last ones hardly count.
+// Tiles of long examples come to the SMs most columns first.  An order costs a launch of some 5 us and is made where
+// blocks outnumber what the GPU holds at once, take long (1024 columns and more) and are not so many that the last ones
+// hardly count.
 constexpr int AT_ORDER_TILES = 4096, AT_ORDER_BINS = 256;
 static bool at_ordered(const b200c_attention_t &p, int64_t rows, int64_t cols, int per_tile) {
   const int64_t tiles = (rows + AT_ROWS - 1) / AT_ROWS;

@@ -6,18 +6,19 @@
 //   dq:      rows = queries of a head,  columns = keys;     S = Q K^T, dP = dO V^T,  then dQ += dS K
 //   dk, dv:  rows = keys of a group,    columns = queries;  S' = K Q^T, dP' = V dO^T,  then dV += P' dO, dK += dS' Q
 // One warp brings the operands to shared memory (TMA, 128-byte swizzle, a ring of stages, with the columns' coordinates
-// and statistics beside them), one issues the products of the scores, one the products with the weights.  The other warps form G
-// groups of four; a pair of groups takes a stage, 32 columns each: they read the scores from tensor memory, a row per
-// thread, and put the 16-bit weights back there, where the second products take them as their first operand.  The
-// first products have both operands K-major; the second take the column tile MN-major, as it stands.  Exponentials and
-// roots bound these kernels, not the products: everything is arranged so that the groups never wait for a product.
-// They hand the scores' place back as soon as they have read them, so that the next scores are formed while they work on
-// these, and the weights have a place of their own.
+// and statistics beside them), one issues the products of the scores, one the products with the weights.  The other
+// warps form G groups of four; a pair of groups takes a stage, 32 columns each: they read the scores from tensor
+// memory, a row per thread, and put the 16-bit weights back there, where the second products take them as their first
+// operand.  The first products have both operands K-major; the second take the column tile MN-major, as it stands.
+// Exponentials and roots bound these kernels, not the products: everything is arranged so that the groups never wait
+// for a product. They hand the scores' place back as soon as they have read them, so that the next scores are formed
+// while they work on these, and the weights have a place of their own.
 //
 // A tile may hold rows of several (short) examples.  Its columns are then the union of their ranges, one pass over
-// them, every row masked to its own range.  A masked weight is 0, and 0 times a NaN or an infinity of another example would be
-// NaN: in such tiles the operand of the second product is looked through for them, and if there is one the pass is
-// repeated example by example.  Column rows past the range's end are cleared in shared memory for the same reason.
+// them, every row masked to its own range.  A masked weight is 0, and 0 times a NaN or an infinity of another example
+// would be NaN: in such tiles the operand of the second product is looked through for them, and if there is one the
+// pass is repeated example by example.  Column rows past the range's end are cleared in shared memory for the same
+// reason.
 #pragma once
 
 #include "attention.cuh"
@@ -50,8 +51,9 @@ __device__ __forceinline__ int at_segment_of_warp(const int64_t *__restrict__ pt
   return lo;
 }
 
-// The tile of this block: the heads of a tile run side by side, tiles in the order given, so that what runs last is cheap
-// (16 clouds of 1594 to 2555 points: forward 642 -> 613 us, dq 705 -> 637; 8 of 4000 points with 128 channels 1344 -> 1223).
+// The tile of this block: the heads of a tile run side by side, tiles in the order given, so that what runs last is
+// cheap (16 clouds of 1594 to 2555 points: forward 642 -> 613 us, dq 705 -> 637; 8 of 4000 points with 128 channels
+// 1344 -> 1223).
 __device__ __forceinline__ int64_t at_tile_of(const int *order, int per_tile) {
   const unsigned i = blockIdx.x / (unsigned)per_tile;
   return order ? order[i] : (int64_t)i;
@@ -227,8 +229,8 @@ struct AtRing {
   }
 };
 
-// The columns [lo, hi) that the rows of a warp see, relative to the pass's first: a step can be skipped where no row sees
-// any of its columns, and needs no mask where every row sees all of them.
+// The columns [lo, hi) that the rows of a warp see, relative to the pass's first: a step can be skipped where no row
+// sees any of its columns, and needs no mask where every row sees all of them.
 struct AtSeen {
   int lo, hi, any_lo, any_hi, all_lo, all_hi;
   __device__ __forceinline__ AtSeen(int64_t row_lo, int64_t row_hi, const AtPass &pass, bool mine) {
@@ -268,9 +270,9 @@ __device__ __forceinline__ void at_fetch_places<0>(float *, const float *__restr
 template <>
 __device__ __forceinline__ void at_put_places<0>(float *, const float *, int) {}
 
-// The bias and the cap of 32 scores of a row: s[j] (dot products) become log2 e (t - slope |pos - pos_j|) - sub, with one
-// `sub` of the row or, with COL, one per column.  col_pos: [dims][64] coordinates of the stage's columns, from the step's
-// first.  u[j] = tanh of the capped score, where wanted.
+// The bias and the cap of 32 scores of a row: s[j] (dot products) become log2 e (t - slope |pos - pos_j|) - sub, with
+// one `sub` of the row or, with COL, one per column.  col_pos: [dims][64] coordinates of the stage's columns, from the
+// step's first.  u[j] = tanh of the capped score, where wanted.
 template <int DIM, bool CAP, bool KEEP, bool COL>
 __device__ __forceinline__ void at_logits(float *s, float *u, const float *col_pos, const float *pos, float slope2,
                                           float pre, float post, float sub, const float *col_sub) {
@@ -313,9 +315,9 @@ __device__ __forceinline__ void at_logits(float *s, float *u, const float *col_p
   }
 }
 
-// A block's rows leave by way of shared memory (the ring, idle at the end of a pass): a thread has 16 bytes of its row in
-// hand at a time, and 32 rows' worth of them would be 32 places for the memory to go to.  16-byte chunk c of row r is kept
-// at c ^ (r & 7).
+// A block's rows leave by way of shared memory (the ring, idle at the end of a pass): a thread has 16 bytes of its row
+// in hand at a time, and 32 rows' worth of them would be 32 places for the memory to go to.  16-byte chunk c of row r
+// is kept at c ^ (r & 7).
 template <int CP>
 __device__ __forceinline__ void at_put(unsigned char *tile, int r, int chunk, const uint4 &v) {
   *reinterpret_cast<uint4 *>(tile + r * (CP * 2) + ((chunk ^ (r & 7)) << 4)) = v;

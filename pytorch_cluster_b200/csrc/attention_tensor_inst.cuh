@@ -1,5 +1,5 @@
-// Dispatch of the tensor-core attention over channels, coordinates and cap.  Channel counts are padded to 64 or 128 with
-// zeros by the copies; coordinates to 1, 3 or 8.
+// Dispatch of the tensor-core attention over channels, coordinates and cap.  Channel counts are padded to 64 or 128
+// with zeros by the copies; coordinates to 1, 3 or 8.
 #pragma once
 
 #include "attention_backward.cuh"

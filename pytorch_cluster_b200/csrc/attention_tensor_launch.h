@@ -1,4 +1,5 @@
-// Launches of the attention kernels for 16-bit types, one translation unit per type and direction (they compile in parallel).
+// Launches of the attention kernels for 16-bit types, one translation unit per type and direction (they compile in
+// parallel).
 #pragma once
 
 #include "attention.cuh"

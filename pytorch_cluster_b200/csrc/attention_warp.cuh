@@ -50,8 +50,8 @@ __device__ __forceinline__ float2 aw_unpack(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
-// Byte offset of 16-byte chunk c of row r in a tile of rows of CP 16-bit values: eight rows of one chunk, which a matrix
-// load takes, and eight chunks of one row, which a copy writes, lie in different banks.
+// Byte offset of 16-byte chunk c of row r in a tile of rows of CP 16-bit values: eight rows of one chunk, which a
+// matrix load takes, and eight chunks of one row, which a copy writes, lie in different banks.
 template <int CP>
 __device__ __forceinline__ uint32_t aw_at(int r, int c) {
   return (uint32_t)(r * (CP * 2) + ((CP == 32 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 4));

@@ -2,15 +2,14 @@
 //   out[e] = scale x[index[e]],   dx[n] = scale sum_{e : index[e] = n} dout[e]
 // An index outside [0, rows) is padding (knn's -1): it gives a row of zeros and receives no gradient.
 //
-// Both directions are bound by memory: the forward pass is one copy with 16-byte accesses, four edges per thread so that
-// enough loads are on their way behind the indices.  The backward pass has to
-// bring equal indices together.  It sorts (index, e) pairs with a stable radix sort — as few passes of up to 9 bits as the
-// row count needs, each a histogram per block, a scan of the blocks' counts per digit, and a scatter of 8 bytes per pair by
-// way of shared memory, where a block's pairs are put in order first, so that they leave in runs — and then adds dout's
-// rows in that order, in fp32, each thread owning 16 bytes of the channels over 64 or more consecutive pairs.
-// Sums that cross such a piece's border go to the workspace and are joined in order.  No atomics touch a sum, so
-// the result is the same from run to run, and an index that occurs a million times costs no more than a million
-// different ones.
+// Both directions are bound by memory: the forward pass is one copy with 16-byte accesses, four edges per thread so
+// that enough loads are on their way behind the indices.  The backward pass has to bring equal indices together.  It
+// sorts (index, e) pairs with a stable radix sort — as few passes of up to 9 bits as the row count needs, each a
+// histogram per block, a scan of the blocks' counts per digit, and a scatter of 8 bytes per pair by way of shared
+// memory, where a block's pairs are put in order first, so that they leave in runs — and then adds dout's rows in that
+// order, in fp32, each thread owning 16 bytes of the channels over 64 or more consecutive pairs. Sums that cross such a
+// piece's border go to the workspace and are joined in order.  No atomics touch a sum, so the result is the same from
+// run to run, and an index that occurs a million times costs no more than a million different ones.
 #include "common.cuh"
 #include "launchers.h"
 
@@ -18,7 +17,8 @@ namespace b200c {
 
 constexpr int GR_THREADS = 256;
 constexpr int GR_WARPS = GR_THREADS / 32;
-constexpr int GR_ITEMS = 10;                       // pairs per thread of a sort block: 16 leave 2.6e6 edges in two waves (85 us of sort, 77 so)
+// pairs per thread of a sort block: 16 leave 2.6e6 edges in two waves of blocks (85 us of sort, 77 so)
+constexpr int GR_ITEMS = 10;
 constexpr int GR_TILE = GR_THREADS * GR_ITEMS;     // pairs per sort block
 constexpr int GR_MAX_BITS = 9;
 constexpr int GR_EDGES = 4;                        // edges per thread of the forward pass
@@ -165,9 +165,9 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scan_kernel(uint32_t *
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-// The place of this lane's pair: those of a digit follow one another in the order of the lanes.  next[digit] is the warp's
-// next place and moves on.  The lanes with one digit are found by a ballot per bit (match_any takes three times as
-// long where digits differ).
+// The place of this lane's pair: those of a digit follow one another in the order of the lanes.  next[digit] is the
+// warp's next place and moves on.  The lanes with one digit are found by a ballot per bit (match_any takes three times
+// as long where digits differ).
 __device__ __forceinline__ uint32_t gr_place(bool have, uint32_t digit, int bits, uint32_t *next) {
   unsigned same = __ballot_sync(FULL_MASK, have);
   if (!have) same = ~same;
@@ -191,8 +191,9 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
   constexpr int MOST = 1 << GR_MAX_BITS;
   extern __shared__ __align__(16) unsigned char gr_smem[];
   uint2 *sorted = reinterpret_cast<uint2 *>(gr_smem);                          // the block's pairs, by digit
-  uint32_t(*next)[MOST] = reinterpret_cast<uint32_t(*)[MOST]>(sorted + GR_TILE);  // where warp w puts its next pair of digit d
-  uint32_t *shift_to = reinterpret_cast<uint32_t *>(next + GR_WARPS);          // out position - position in `sorted`, per digit
+  // where warp w puts its next pair of digit d; out position - position in `sorted`, per digit
+  uint32_t(*next)[MOST] = reinterpret_cast<uint32_t(*)[MOST]>(sorted + GR_TILE);
+  uint32_t *shift_to = reinterpret_cast<uint32_t *>(next + GR_WARPS);
   __shared__ uint32_t warp_sums[GR_WARPS];
   const int bins = 1 << bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < GR_WARPS * MOST; i += GR_THREADS) next[0][i] = 0u;
@@ -387,7 +388,8 @@ __device__ __forceinline__ int64_t gr_run(const uint2 *keys, int64_t edges, int 
   if (keys[hi].x != run) return -1;
   slot = keys[lo].x == run ? 0 : 1;
   if (slot == 0 && lo > 0 && keys[lo - 1].x == run) return -1;  // began earlier
-  // the last piece whose first key is the run's: in steps of twice the size as far as it goes, then of half (most end at once)
+  // the last piece whose first key is the run's: in steps of twice the size as far as it goes, then of half (most end
+  // at once)
   int64_t a = g + 1, step = 1;
   while (a + step < pieces && keys[(a + step) * piece].x == run) a += step, step *= 2;
   for (step /= 2; step > 0; step /= 2)
@@ -426,7 +428,8 @@ __global__ void __launch_bounds__(GR_THREADS) gather_join_kernel(const uint2 *__
   reinterpret_cast<GrVec<T, VL> *>(dx)[(int64_t)run * units + u] = r;
 }
 
-// A block per (long run, 32 channels): its warps add contiguous shares of its pieces, then one adds the shares in order.
+// A block per (long run, 32 channels): its warps add contiguous shares of its pieces, then one adds the shares in
+// order.
 template <typename T>
 __global__ void __launch_bounds__(32 * GR_LONG_WARPS) gather_join_long_kernel(const uint2 *__restrict__ keys, int64_t rows,
                                                                       int64_t edges, int channels, int piece,
@@ -494,9 +497,11 @@ static GrPlan gr_plan(int64_t rows, int64_t edges, int64_t channels) {
   p.blocks = (edges + GR_TILE - 1) / GR_TILE;
   // 64 pairs a piece: the borders' sums then cost an eighth of dout's bytes (16-bit types) at most
   p.piece = 64;
-  // Where rows are named thousands of times (node types), longer pieces leave less to join, as long as there are enough of
-  // them: 1000003 edges of 128 channels on 100 rows, a third of them on one, 139 us of sums and joins -> 127.
-  while (p.piece < 256 && rows > 0 && edges / rows >= 8 * p.piece && edges / (2 * p.piece) * channels >= 148 * 2048) p.piece *= 2;
+  // Where rows are named thousands of times (node types), longer pieces leave less to join, as long as there are enough
+  // of them: 1000003 edges of 128 channels on 100 rows, a third of them on one, 139 us of sums and joins -> 127.
+  while (p.piece < 256 && rows > 0 && edges / rows >= 8 * p.piece &&
+         edges / (2 * p.piece) * channels >= 148 * 2048)
+    p.piece *= 2;
   p.pieces = (edges + p.piece - 1) / p.piece;
   const int64_t bins = (1ll << p.bits) * p.blocks;
   p.pairs = gr_align((size_t)edges * 8);

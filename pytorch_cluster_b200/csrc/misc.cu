@@ -10,7 +10,7 @@ namespace b200c {
 
 // ---- segment pointers ----------------------------------------------------------------------------
 // ptr[i] = lower_bound(batch, i) (torch.bucketize(arange(B + 1), batch), torch_cluster/knn.py:77-79): a warp per
-// boundary looks at 32 places at a time, so that a million rows take four dependent loads instead of twenty (21 -> 7 us
+// boundary looks at 32 places at a time, so that a million rows take four dependent loads instead of twenty (21 -> 12 us
 // for two vectors of 32 clouds, the larger of 1 M rows).
 __global__ void segment_ptr_kernel(const int64_t *__restrict__ batch, int64_t n, int64_t num_segments,
                                    int64_t *__restrict__ ptr) {

@@ -11,6 +11,9 @@ static bool is_network_type(int dtype) { return dtype == B200C_F32 || dtype == B
 static size_t elem_bytes(int dtype) { return dtype == B200C_F32 ? 4 : 2; }
 constexpr int64_t MOST_ROWS = 0x7fffffffLL;
 
+// what every workspace is carved from
+static bool aligned_workspace(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
 static int check_gather(const void *in, const int64_t *index, int64_t rows, int64_t edges, int64_t channels, int dtype,
                         const void *out) {
   B200C_CHECK_ARG(is_network_type(dtype), "unsupported dtype");
@@ -20,7 +23,8 @@ static int check_gather(const void *in, const int64_t *index, int64_t rows, int6
   B200C_CHECK_ARG((edges == 0 || index != nullptr) && (rows == 0 || edges == 0 || (in != nullptr && out != nullptr)),
                   "null pointer");
   const uintptr_t mask = elem_bytes(dtype) - 1;
-  B200C_CHECK_ARG(((uintptr_t)in & mask) == 0 && ((uintptr_t)out & mask) == 0, "misaligned pointer");
+  B200C_CHECK_ARG(((uintptr_t)in & mask) == 0 && ((uintptr_t)out & mask) == 0 && ((uintptr_t)index & 7) == 0,
+                  "misaligned pointer");
   return check_device();
 }
 
@@ -100,6 +104,7 @@ extern "C" int b200c_gather_rows_backward(const void *dout, const int64_t *index
   const int st = check_gather(dout, index, rows, edges, channels, dtype, dx);
   if (st != B200C_OK || rows == 0) return st;
   B200C_CHECK_ARG(dx != nullptr, "null pointer");
+  B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
   if (edges == 0) {
     B200C_CUDA(cudaMemsetAsync(dx, 0, (size_t)rows * channels * elem_bytes(dtype), (cudaStream_t)stream));
     return B200C_OK;
@@ -130,6 +135,7 @@ extern "C" int b200c_norm_rotate_backward(const b200c_norm_rotate_side_t *q, con
   NormRotateArgs a{};
   const int st = check_rotate(q, k, freq, dims, channels, pos_f64, freq_f64, eps, dtype, false, (cudaStream_t)stream, a);
   if (st != B200C_OK) return st;
+  B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
   const size_t need = norm_rotate_workspace_bytes(channels);
   if ((a.dweight[0] || a.dweight[1]) && (workspace == nullptr || workspace_bytes < need)) {
     set_error("norm_rotate workspace too small: %zu < %zu", workspace_bytes, need);
@@ -158,6 +164,7 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
                                        size_t workspace_bytes, b200c_stream_t stream) {
   int st = check_attention(p);
   if (st != B200C_OK) return st;
+  B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
   if ((st = check_device()) != B200C_OK || p->m == 0) return st;
   B200C_CHECK_ARG(out != nullptr, "null output pointer");
   const size_t need = b200c_attention_workspace_bytes(p);
@@ -191,10 +198,11 @@ extern "C" size_t b200c_attention_backward_workspace_bytes(const b200c_attention
 }
 
 extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const void *rest, const float *lse,
-                                        const void *dout, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
-                                        b200c_stream_t stream) {
+                                        const void *dout, void *dq, void *dk, void *dv, void *workspace,
+                                        size_t workspace_bytes, b200c_stream_t stream) {
   int st = check_attention(p);
   if (st != B200C_OK) return st;
+  B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
   if ((st = check_device()) != B200C_OK) return st;
   B200C_CHECK_ARG(p->m == 0 || (out && lse && dout), "null pointer");
   B200C_CHECK_ARG((dk == nullptr) == (dv == nullptr), "dk and dv come together");

@@ -4,13 +4,14 @@
 // Backward: g = the rotation of dy by -a, dw = sum g x r over rows and heads, t = g w,
 //   dx = r t - x r^3 mean_c(t x).
 //
-// Memory bounds both directions (2 and 3 bytes-per-value passes); the rotation's angles are shared by all heads of a row, so a
-// block forms the sines and cosines of its rows once, in shared memory, and uses them for every head of q and, where
-// both have the same positions, of k.  Positions may be far from zero (whole numbers up to millions, in
-// either type): the angle is a sum of products in 64 bits, reduced to [-pi, pi] there, and only then rounded to 32.
-// LP lanes hold a head's row, 16 bytes of either half each; sums over a row are shuffles.  Next to memory it is instructions
-// that cost: offsets are added up from step to step, the root is the hardware's reciprocal root.  The gradient of the weights is
-// summed in registers over a block's rows, then over the blocks in a fixed order: no atomics.
+// Memory bounds both directions (2 and 3 bytes-per-value passes); the rotation's angles are shared by all heads of a
+// row, so a block forms the sines and cosines of its rows once, in shared memory, and uses them for every head of q
+// and, where both have the same positions, of k.  Positions may be far from zero (whole numbers up to millions, in
+// either type): the angle is a sum of products in 64 bits, reduced to [-pi, pi] there, and only then rounded to 32. LP
+// lanes hold a head's row, 16 bytes of either half each; sums over a row are shuffles.  Next to memory it is
+// instructions that cost: offsets are added up from step to step, the root is the hardware's reciprocal root.  The
+// gradient of the weights is summed in registers over a block's rows, then over the blocks in a fixed order: no
+// atomics.
 #include "common.cuh"
 #include "launchers.h"
 
@@ -87,9 +88,9 @@ __device__ __forceinline__ void nr_frequencies(const NormRotateArgs &a, double *
   for (int i = threadIdx.x; i < a.dims * a.half; i += NR_THREADS)
     fr[i] = a.freq_f64 ? ((const double *)a.freq)[i] : (double)((const float *)a.freq)[i];
 }
-// Sines and cosines of rows [row0, row0 + count).  The reduced angle is at most pi, where the hardware's sine and cosine
-// are off by 2^-21 at most: a thousandth of the 16-bit types' steps, but several of fp32's, which calls the exact ones
-// and brings in what rounding took from the angle (error of a rotation of 1024 rows 1.7e-7 -> 0.9e-7).
+// Sines and cosines of rows [row0, row0 + count).  The reduced angle is at most pi, where the hardware's sine and
+// cosine are off by 2^-21 at most: a thousandth of the 16-bit types' steps, but several of fp32's, which calls the
+// exact ones and brings in what rounding took from the angle (error of a rotation of 1024 rows 1.7e-7 -> 0.7e-7).
 template <typename T>
 __device__ __forceinline__ void nr_angles(const b200c_norm_rotate_side_t &s, const NormRotateArgs &a, int64_t row0,
                                           int count, const double *fr, float *cs, float *sn) {
@@ -362,8 +363,8 @@ __global__ void __launch_bounds__(NR_JOIN_THREADS) norm_rotate_weights_kernel(co
 
 // ---- host ----------------------------------------------------------------------------------------------------
 static int nr_rows_per_block(const NormRotateArgs &a, int lanes) {
-  // enough rows that every lane group has eight heads to work on, so that the angles, which all wait for, are a small part of
-  // the time; at most 32 (shared memory)
+  // enough rows that every lane group has eight heads to work on, so that the angles, which all wait for, are a small
+  // part of the time; at most 32 (shared memory)
   const int slots = NR_THREADS / lanes, heads = a.joint ? a.side[0].heads + a.side[1].heads : a.side[0].heads;
   const int rows = (8 * slots + heads - 1) / heads;
   return rows < 1 ? 1 : rows > 32 ? 32 : rows;

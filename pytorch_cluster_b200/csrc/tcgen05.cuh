@@ -10,9 +10,9 @@ namespace b200c {
 
 __device__ __forceinline__ uint32_t t5_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// One lane of the warp, the same every time.  The descriptors of a product live in uniform registers: issued by an elected
-// lane in code that the whole warp runs, they stay there; behind a test of the lane number each would be moved over first
-// (measured: 85 cycles per product against about 20).
+// One lane of the warp, the same every time.  The descriptors of a product live in uniform registers: issued by an
+// elected lane in code that the whole warp runs, they stay there; behind a test of the lane number each would be moved
+// over first (measured: 85 cycles per product against about 20).
 __device__ __forceinline__ bool t5_elect() {
   uint32_t one;
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
@@ -39,10 +39,11 @@ __device__ __forceinline__ bool t5_mbar_try(uint64_t *bar, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-constexpr int T5_SPIN_LIMIT = 1 << 22;  // polls of a wait of some ten nanoseconds each; a step takes a microsecond or two
-// Waits for the phase of the given parity.  A parity tells two neighbouring phases apart, no more: a caller must know that
-// the phase before is over and that the one after cannot end before it has gone on.  Gives up after T5_SPIN_LIMIT polls,
-// or when another thread of the block did (*failed), and says so.
+// polls of a wait, of some ten nanoseconds each; a step takes a microsecond or two
+constexpr int T5_SPIN_LIMIT = 1 << 22;
+// Waits for the phase of the given parity.  A parity tells two neighbouring phases apart, no more: a caller must know
+// that the phase before is over and that the one after cannot end before it has gone on.  Gives up after T5_SPIN_LIMIT
+// polls, or when another thread of the block did (*failed), and says so.
 __device__ __forceinline__ bool t5_mbar_wait(uint64_t *bar, uint32_t parity, volatile int *failed) {
   if (t5_mbar_try(bar, parity)) return true;
   for (int i = 0; i < T5_SPIN_LIMIT; ++i) {
@@ -54,7 +55,8 @@ __device__ __forceinline__ bool t5_mbar_wait(uint64_t *bar, uint32_t parity, vol
 }
 
 // The same for a warp that has nothing else to do and whose answer is not waited for at once: a loop of few
-// instructions, asleep between its looks, which otherwise take issue slots from the warps that work (forward 692 -> 641 us).
+// instructions, asleep between its looks, which otherwise take issue slots from the warps that work (forward 692 -> 641
+// us).
 __device__ __forceinline__ bool t5_mbar_wait_idle(uint64_t *bar, uint32_t parity, volatile int *failed) {
   const uint32_t at = t5_smem(bar);
   uint32_t over = 0;
@@ -136,8 +138,8 @@ __device__ __forceinline__ void t5_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       : "memory");
 }
 
-// Waits for the thread's loads from tensor memory.  The values pass through the instruction, so that no use of them can be
-// moved ahead of it.
+// Waits for the thread's loads from tensor memory.  The values pass through the instruction, so that no use of them can
+// be moved ahead of it.
 __device__ __forceinline__ void t5_wait_ld32(float *v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+f"(v[0]),"+f"(v[1]),"+f"(v[2]),"+f"(v[3]),"+f"(v[4]),"+f"(v[5]),"+f"(v[6]),"+f"(v[7]),

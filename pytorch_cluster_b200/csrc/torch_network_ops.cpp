@@ -36,25 +36,35 @@ bool wants_gradient(std::initializer_list<const torch::Tensor *> tensors) {
   return false;
 }
 
-// The gradients carry no graph of their own.  Where one is asked for, they come out with this node, whose own backward
-// pass refuses, instead of as constants.
+// The gradients carry no graph of their own.  Where one is asked for, they come out of this node, which hangs on what
+// they were formed from and whose own backward pass refuses, instead of as constants.
 struct OnceDifferentiable : torch::autograd::Function<OnceDifferentiable> {
-  static variable_list forward(AutogradContext *, variable_list grads) { return grads; }
+  static variable_list forward(AutogradContext *, at::TensorList tensors, int64_t count) {
+    return {tensors.begin(), tensors.begin() + count};
+  }
   static variable_list backward(AutogradContext *, variable_list) {
     TORCH_CHECK(false, "trying to differentiate twice a function that is differentiable once");
     return {};
   }
 };
 
-variable_list once(variable_list grads) {
+variable_list once(variable_list grads, const variable_list &sources) {
   if (!at::GradMode::is_enabled()) return grads;
-  variable_list have;
+  variable_list tensors;
   for (const auto &g : grads)
-    if (g.defined()) have.push_back(g.requires_grad() ? g : g.detach().requires_grad_());
-  have = OnceDifferentiable::apply(have);
+    if (g.defined()) tensors.push_back(g);
+  const int64_t count = (int64_t)tensors.size();
+  bool any = false;
+  for (const auto &t : sources)
+    if (t.defined()) {
+      tensors.push_back(t);
+      any = any || t.requires_grad();
+    }
+  if (!any) return grads;
+  variable_list out = OnceDifferentiable::apply(at::TensorList(tensors), count);
   size_t at = 0;
   for (auto &g : grads)
-    if (g.defined()) g = have[at++];
+    if (g.defined()) g = out[at++];
   return grads;
 }
 
@@ -133,7 +143,7 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     auto dx = gather_rows_backward(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
                                    ctx->saved_data["scale"].toDouble());
-    return once({dx, {}, {}});
+    return once({dx, {}, {}}, {grads[0]});  // x itself is not in it
   }
 };
 
@@ -269,7 +279,8 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
     auto [dq, dk, dwq, dwk] = norm_rotate_backward(grads[0], grads[1], t[0], t[1], t[2], t[3], t[4], wq, wk,
                                                    ctx->saved_data["eps"].toDouble());
     return once(
-        {dq, dk, {}, {}, {}, wq.has_value() ? dwq : torch::Tensor(), wk.has_value() ? dwk : torch::Tensor(), {}});
+        {dq, dk, {}, {}, {}, wq.has_value() ? dwq : torch::Tensor(), wk.has_value() ? dwk : torch::Tensor(), {}},
+        {grads[0], grads[1], t[0], t[1], t[5], t[6]});
   }
 };
 
@@ -373,8 +384,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_forward(
 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
     torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor rest,
-    torch::Tensor lse, OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q, OptTensor pos_k, OptTensor slope, double scale, double cap,
-    bool need_q, bool need_kv) {
+    torch::Tensor lse, OptTensor ptr_q, OptTensor ptr_k, OptTensor pos_q, OptTensor pos_k, OptTensor slope, double scale,
+    double cap, bool need_q, bool need_kv) {
   OpRange range("torch_cluster::attention_backward");
   at::NoGradGuard no_grad;
   CHECK_CUDA(q);
@@ -389,7 +400,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
   out = out.contiguous();
   lse = lse.contiguous();
   const bool kept = rest.numel() > 0;
-  CHECK_INPUT(!kept || (rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() && rest.device() == q.device()));
+  CHECK_INPUT(!kept ||
+              (rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() && rest.device() == q.device()));
   rest = rest.contiguous();
   auto none = torch::empty({0}, q.options());
   auto dq = need_q ? torch::empty(q.sizes(), q.options()) : none;
@@ -397,8 +409,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
   auto dv = need_kv ? torch::empty(v.sizes(), v.options()) : none;
   const size_t bytes = b200c_attention_backward_workspace_bytes(&t.a);
   auto ws = workspace(bytes, q);
-  check_status(b200c_attention_backward(&t.a, out.data_ptr(), kept ? rest.data_ptr() : nullptr, lse.data_ptr<float>(), dout.data_ptr(),
-                                        need_q ? dq.data_ptr() : nullptr, need_kv ? dk.data_ptr() : nullptr,
+  check_status(b200c_attention_backward(&t.a, out.data_ptr(), kept ? rest.data_ptr() : nullptr, lse.data_ptr<float>(),
+                                        dout.data_ptr(), need_q ? dq.data_ptr() : nullptr, need_kv ? dk.data_ptr() : nullptr,
                                         need_kv ? dv.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
                                         at::cuda::getCurrentCUDAStream().stream()));
   return {dq, dk, dv};
@@ -426,7 +438,7 @@ struct SoftmaxAttention : torch::autograd::Function<SoftmaxAttention> {
     if (need_q) result[0] = dq;
     if (need_k) result[1] = dk;
     if (need_v) result[2] = dv;
-    return once(result);
+    return once(result, {grads[0], t[0], t[1], t[2]});
   }
 };
 

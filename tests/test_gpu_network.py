@@ -393,6 +393,27 @@ def test_attention_captured_and_replayed():
             assert all(torch.equal(x, y) for x, y in zip(outs, run()))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens, channels", [([70, 200], 64), ([9, 30, 4], 32)])
+def test_attention_gradients_of_some_inputs(dtype, lens, channels):
+    import pytorch_cluster_b200 as pc
+
+    g = gen(19)
+    b, n = ids(lens), sum(lens)
+    ts = [rand(g, n, 2, channels, dtype=dtype) for _ in range(3)]
+    do = rand(g, n, 2, channels, dtype=dtype)
+
+    def grads(wanted):
+        leaves = [t.detach().requires_grad_(i in wanted) for i, t in enumerate(ts)]
+        out = pc.attention(*leaves, b, b, batch_size=len(lens))
+        return dict(zip(wanted, torch.autograd.grad(out, [leaves[i] for i in wanted], do)))
+
+    every = grads((0, 1, 2))
+    for wanted in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        for i, got in grads(wanted).items():
+            assert torch.equal(got, every[i]), (wanted, i)
+
+
 def test_attention_training_step_captured():
     import pytorch_cluster_b200 as pc
 

@@ -19,7 +19,7 @@ def test_cpu_tensors_are_refused():
         pc.norm_rotate(h, h, torch.rand(4, 1), torch.rand(4, 1), torch.rand(1, 4))
     with pytest.raises(RuntimeError, match="q must be CUDA tensor"):
         pc.attention(h, h, h)
-    for op in ("gather_rows", "norm_rotate", "attention_forward", "attention_backward"):
+    for op in ("gather_rows", "norm_rotate", "attention"):
         assert hasattr(torch.ops.torch_cluster, op)
 
 
@@ -74,6 +74,18 @@ def test_attention_argument_checks(changes, message):
         assert call() == 1 and message in lib.b200c_last_error()
     assert lib.b200c_attention_workspace_bytes(ctypes.byref(a)) == 0
     assert lib.b200c_attention_forward(None, 1 << 20, None, None, None, 0, None) == 1
+
+
+def test_misaligned_workspaces_are_refused():
+    from pytorch_cluster_b200 import _native
+
+    lib = _native.cabi()
+    p, odd, a = 1 << 20, (1 << 20) + 8, attention_args()
+    assert lib.b200c_attention_forward(ctypes.byref(a), p, None, None, odd, 1 << 30, None) == 1
+    assert b"misaligned workspace" in lib.b200c_last_error()
+    assert lib.b200c_attention_backward(ctypes.byref(a), p, None, p, p, p, p, p, odd, 1 << 30, None) == 1
+    assert b"misaligned workspace" in lib.b200c_last_error()
+    assert lib.b200c_gather_rows(p, p + 4, 4, 4, 8, 1.0, 0, p, None) == 1 and b"misaligned" in lib.b200c_last_error()
 
 
 class Side(ctypes.Structure):
@@ -157,8 +169,13 @@ def test_mismatched_cuda_tensors_are_refused():
             pc.attention(q, k, k, **{**p, name: p[name].clone().requires_grad_()})
     with pytest.raises(RuntimeError, match="coordinates"):
         pc.attention(q, k, k, pos_q=torch.rand(6, 9, **d), pos_k=torch.rand(5, 9, **d), slope=p["slope"])
+    x, e = torch.rand(6, 8, **d).requires_grad_(), torch.zeros(4, dtype=torch.long, **d)
+    # linear: where the outer gradient is a constant, so is the inner one; where it is not, there is no second one
+    assert not torch.autograd.grad(pc.gather_rows(x, e).sum(), x, create_graph=True)[0].requires_grad
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(torch.autograd.grad(pc.gather_rows(x, e).square().sum(), x, create_graph=True)[0].sum(), x)
     out = pc.attention(q.requires_grad_(), k, k)
-    with pytest.raises(RuntimeError):  # once differentiable
+    with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(torch.autograd.grad(out.square().sum(), q, create_graph=True)[0].sum(), q)
 
     f = torch.rand(1, 16, **d)
