@@ -28,19 +28,28 @@ __device__ __forceinline__ void ap_copy(float *dst, const float *src, bool there
                : "memory");
 }
 
-// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]; fp32 asynchronously
+// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]; fp32 asynchronously.  A thread keeps
+// its channel and adds up its address: worked out for every element, addresses were a third of all instructions
+// (forward of 8 clouds of 500 points, 44 channels: 136 -> 119 us).
 template <typename T, int CP>
 __device__ __forceinline__ void ap_load(float *dst, const T *__restrict__ src, int64_t row_stride, int64_t row0,
                                         int64_t lo, int64_t hi, int channels, int tid) {
-#pragma unroll 4
-  for (int i = tid; i < AP_T * CP; i += AP_THREADS) {
-    const int r = i / CP, c = i - r * CP;
-    const int64_t row = row0 + r;
-    const bool there = row >= lo && row < hi && c < channels;
+  constexpr int WIDTH = CP <= 32 ? 32 : CP <= 64 ? 64 : 128, STEP = AP_THREADS / WIDTH;
+  const int c = tid % WIDTH, r0 = tid / WIDTH;
+  if (c >= CP) return;
+  const int64_t from = lo - row0, to = hi - row0;
+  const int r_lo = from < 0 ? 0 : from > AP_T ? AP_T : (int)from;
+  const int r_hi = c >= channels || to < 0 ? 0 : to > AP_T ? AP_T : (int)to;
+  const T *at = src + (row0 + r0) * row_stride + c;
+  const int64_t step = STEP * row_stride;
+  float *to_at = dst + c * AP_LD + r0;
+#pragma unroll 8
+  for (int r = r0; r < AP_T; r += STEP, at += step, to_at += STEP) {
+    const bool there = r >= r_lo && r < r_hi;
     if constexpr (sizeof(T) == 4)
-      ap_copy(dst + c * AP_LD + r, there ? src + row * row_stride + c : src, there);
+      ap_copy(to_at, there ? at : src, there);
     else
-      dst[c * AP_LD + r] = there ? at_float(src[row * row_stride + c]) : 0.f;
+      *to_at = there ? at_float(*at) : 0.f;
   }
 }
 
@@ -86,11 +95,25 @@ __device__ __forceinline__ void ap_accumulate(const float *w, const float *b, in
   }
 }
 
-// log2 e (t - slope |pos_a - pos_b|) of the 4 x 4 tile; bend[i][j] = 1 - (t / cap)^2
+// log2 e (t - slope |pos_a - pos_b|) of the 4 x 4 tile; bend[i][j] = 1 - (t / cap)^2.  Coordinates are read four
+// rows and four columns at a time (forward 119 -> 102 us).
 template <bool BEND>
 __device__ __forceinline__ void ap_logits(float (&s)[4][4], float (&bend)[4][4], const float *pa, const float *pb,
                                           int dims, int ty, int tx, float scale, float cap, float slope) {
   const float inv_cap = cap > 0.f ? 1.f / cap : 0.f;
+  float d2[4][4] = {};
+  for (int d = 0; d < dims; ++d) {
+    const float4 x = *reinterpret_cast<const float4 *>(pa + d * AP_LD + 4 * ty);
+    const float4 y = *reinterpret_cast<const float4 *>(pb + d * AP_LD + 4 * tx);
+    const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float df = xs[i] - ys[j];
+        d2[i][j] = fmaf(df, df, d2[i][j]);
+      }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -102,14 +125,7 @@ __device__ __forceinline__ void ap_logits(float (&s)[4][4], float (&bend)[4][4],
         t = cap * u;
         if (BEND) bend[i][j] = 1.f - u * u;
       }
-      if (dims > 0) {
-        float d2 = 0.f;
-        for (int d = 0; d < dims; ++d) {
-          const float df = pa[d * AP_LD + 4 * ty + i] - pb[d * AP_LD + 4 * tx + j];
-          d2 = fmaf(df, df, d2);
-        }
-        t = fmaf(-slope, t5_sqrt(d2), t);
-      }
+      if (dims > 0) t = fmaf(-slope, t5_sqrt(d2[i][j]), t);
       s[i][j] = t * AT_LOG2E;
     }
 }
