@@ -28,8 +28,8 @@ __device__ __forceinline__ void ap_copy(float *dst, const float *src, bool there
                : "memory");
 }
 
-// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]; fp32 asynchronously.  A thread keeps
-// its channel and adds up its address: worked out for every element, addresses were a third of all instructions
+// rows [row0, row0 + 64) of src (rows outside [lo, hi) are zero) to dst[channel][row]; fp32 asynchronously.  A thread
+// keeps its channel and adds up its address: worked out for every element, addresses were a third of all instructions
 // (forward of 8 clouds of 500 points, 44 channels: 136 -> 119 us).
 template <typename T, int CP>
 __device__ __forceinline__ void ap_load(float *dst, const T *__restrict__ src, int64_t row_stride, int64_t row0,

@@ -31,6 +31,10 @@ constexpr int GR_ONE_THREADS = 1024;
 constexpr int GR_ONE_ITEMS = 16;
 constexpr int GR_ONE = GR_ONE_THREADS * GR_ONE_ITEMS;
 constexpr int GR_FEW = 32;
+// Up to GR_ROWS rows and edges the sort leaves every row's place too, and one kernel writes all rows, zeros included: 2
+// launches for 4 (1100 edges 66 -> 63 us).
+constexpr int GR_ROWS = 4096;
+constexpr int GR_SLOTS = 8;  // warps that share the edges of a row
 
 template <typename T, int VL>
 struct alignas(sizeof(T) * VL) GrVec {
@@ -102,7 +106,9 @@ __device__ __forceinline__ uint2 gr_pair(const int64_t *index, const uint2 *pair
 __global__ void __launch_bounds__(GR_THREADS) gather_sort_count_kernel(const int64_t *__restrict__ index,
                                                                        const uint2 *__restrict__ pairs, int64_t rows,
                                                                        int64_t edges, int shift, int bits,
-                                                                       uint32_t *__restrict__ counts) {
+                                                                       uint32_t *__restrict__ counts,
+                                                                       int *__restrict__ num_long) {
+  if (pairs == nullptr && blockIdx.x == 0 && threadIdx.x == 0) *num_long = 0;  // for the joins
   __shared__ int hist[1 << GR_MAX_BITS];
   const int bins = 1 << bits;
   for (int i = threadIdx.x; i < bins; i += GR_THREADS) hist[i] = 0;
@@ -266,7 +272,8 @@ __global__ void __launch_bounds__(GR_THREADS) gather_sort_scatter_kernel(
 // All passes in one block; the pairs stay in shared memory between them.
 __global__ void __launch_bounds__(GR_ONE_THREADS) gather_sort_one_kernel(const int64_t *__restrict__ index, int64_t rows,
                                                                         int edges, int passes, int bits,
-                                                                        uint2 *__restrict__ out) {
+                                                                        uint2 *__restrict__ out,
+                                                                        int *__restrict__ starts) {
   constexpr int MOST = 1 << GR_MAX_BITS, WARPS = GR_ONE_THREADS / 32;
   extern __shared__ __align__(16) unsigned char gr_smem[];
   uint2 *sorted = reinterpret_cast<uint2 *>(gr_smem);
@@ -311,6 +318,63 @@ __global__ void __launch_bounds__(GR_ONE_THREADS) gather_sort_one_kernel(const i
     __syncthreads();
   }
   for (int i = threadIdx.x; i < edges; i += GR_ONE_THREADS) out[i] = sorted[i];
+  if (starts)
+    for (int64_t row = threadIdx.x; row <= rows; row += GR_ONE_THREADS) {
+      int lo = 0, hi = edges;  // the first pair of this row or a later one
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sorted[mid].x < row)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      starts[row] = lo;
+    }
+}
+
+// A lane per (row, 16 bytes of channels); GR_SLOTS warps take contiguous shares of the row's pairs, which are added in
+// order.
+template <typename T, int VL>
+__global__ void __launch_bounds__(32 * GR_SLOTS) gather_sum_rows_kernel(const T *__restrict__ dout,
+                                                                        const uint2 *__restrict__ keys,
+                                                                        const int *__restrict__ starts, int64_t total,
+                                                                        int units, float scale, T *__restrict__ dx) {
+  constexpr int AHEAD = 4;
+  __shared__ float share[GR_SLOTS][VL][32];
+  const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  const bool have = i < total;
+  const int64_t row = i / units, u = i - row * units;
+  int lo = 0, hi = 0;
+  if (have) {
+    const int first = starts[row], count = starts[row + 1] - first;
+    lo = first + (int)((int64_t)count * slot / GR_SLOTS);
+    hi = first + (int)((int64_t)count * (slot + 1) / GR_SLOTS);
+  }
+  const GrVec<T, VL> *src = reinterpret_cast<const GrVec<T, VL> *>(dout);
+  float acc[VL] = {};
+  for (int j = lo; j < hi; j += AHEAD) {
+    GrVec<T, VL> v[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) v[n] = src[(int64_t)keys[j + n < hi ? j + n : hi - 1].y * units + u];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n)
+      if (j + n < hi) {
+#pragma unroll
+        for (int c = 0; c < VL; ++c) acc[c] += gr_float(v[n].v[c]);
+      }
+  }
+#pragma unroll
+  for (int c = 0; c < VL; ++c) share[slot][c][lane] = acc[c];
+  __syncthreads();
+  if (slot != 0 || !have) return;
+  GrVec<T, VL> r;
+#pragma unroll
+  for (int c = 0; c < VL; ++c) {
+    for (int s = 1; s < GR_SLOTS; ++s) acc[c] += share[s][c][lane];
+    r.v[c] = gr_round<T>(acc[c] * scale);
+  }
+  reinterpret_cast<GrVec<T, VL> *>(dx)[i] = r;
 }
 
 // ---- sums over runs of equal keys ----------------------------------------------------------------------------
@@ -505,6 +569,7 @@ static GrPlan gr_plan(int64_t rows, int64_t edges, int64_t channels) {
   p.pieces = (edges + p.piece - 1) / p.piece;
   const int64_t bins = (1ll << p.bits) * p.blocks;
   p.pairs = gr_align((size_t)edges * 8);
+  if (edges <= GR_ROWS && rows <= GR_ROWS) p.pairs += gr_align((size_t)(rows + 1) * 4);  // the rows' places
   p.counts = gr_align((size_t)bins * 4);
   p.totals = gr_align((size_t)4 << p.bits);
   p.part = gr_align((size_t)p.pieces * 2 * channels * 4);
@@ -540,16 +605,24 @@ static int gr_backward(const void *dout, const int64_t *index, int64_t rows, int
   int *num_long = (int *)ws;
   uint2 *long_runs = (uint2 *)ws + 1;
 
-  B200C_CUDA(cudaMemsetAsync(dx, 0, (size_t)rows * channels * sizeof(T), stream));  // rows that no index names
-  const bool one = edges <= GR_ONE;
+  const bool one = edges <= GR_ONE, whole = edges <= GR_ROWS && rows <= GR_ROWS;
+  if (!whole) B200C_CUDA(cudaMemsetAsync(dx, 0, (size_t)rows * channels * sizeof(T), stream));  // rows of no index
   const uint2 *k = nullptr;
   if (one) {
     constexpr size_t smem = (size_t)GR_ONE * 8 + (size_t)(GR_ONE_THREADS / 32) * (4 << GR_MAX_BITS);
     static unsigned long long configured = 0ull;
     B200C_CUDA(opt_in_shared_memory(gather_sort_one_kernel, smem, configured));
-    gather_sort_one_kernel<<<1, GR_ONE_THREADS, smem, stream>>>(index, rows, (int)edges, p.passes, p.bits, pairs[0]);
+    gather_sort_one_kernel<<<1, GR_ONE_THREADS, smem, stream>>>(index, rows, (int)edges, p.passes, p.bits, pairs[0],
+                                                                 whole ? (int *)pairs[1] : nullptr);
     B200C_LAUNCH_CHECK("gather_sort_one_kernel");
     k = pairs[0];
+    if (whole) {
+      const int64_t total = rows * (channels / VL);
+      gather_sum_rows_kernel<T, VL><<<(unsigned)((total + 31) / 32), 32 * GR_SLOTS, 0, stream>>>(
+          (const T *)dout, k, (const int *)pairs[1], total, (int)(channels / VL), scale, (T *)dx);
+      B200C_LAUNCH_CHECK("gather_sum_rows_kernel");
+      return B200C_OK;
+    }
   } else {
     constexpr size_t smem = (size_t)GR_TILE * 8 + (size_t)(GR_WARPS + 1) * (4 << GR_MAX_BITS);
     static unsigned long long configured = 0ull;
@@ -557,7 +630,7 @@ static int gr_backward(const void *dout, const int64_t *index, int64_t rows, int
     const bool few = p.blocks <= GR_FEW;
     for (int pass = 0; pass < p.passes; ++pass) {
       gather_sort_count_kernel<<<(unsigned)p.blocks, GR_THREADS, 0, stream>>>(index, k, rows, edges, pass * p.bits,
-                                                                              p.bits, counts);
+                                                                              p.bits, counts, num_long);
       B200C_LAUNCH_CHECK("gather_sort_count_kernel");
       if (!few) {
         gather_sort_scan_kernel<<<1u << p.bits, GR_THREADS, 0, stream>>>(counts, p.blocks, totals);
@@ -568,7 +641,6 @@ static int gr_backward(const void *dout, const int64_t *index, int64_t rows, int
       B200C_LAUNCH_CHECK("gather_sort_scatter_kernel");
       k = pairs[pass & 1];
     }
-    B200C_CUDA(cudaMemsetAsync(num_long, 0, 4, stream));
   }
   const int units = (int)(channels / VL);
   const unsigned blocks = (unsigned)((p.pieces * units + GR_THREADS - 1) / GR_THREADS);

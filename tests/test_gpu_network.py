@@ -596,6 +596,8 @@ GATHER = [
     # around the sizes at which the sort changes: one block, few blocks, many
     (700, 16383, 8, "all"), (700, 16385, 8, "padded"), (2000, 131073, 8, "any"), (2000, 131072, 8, "skewed"),
     (300000, 16384, 4, "any"), (300000, 140001, 4, "padded"), (40, 16385, 8, "all"),
+    (4096, 4096, 8, "skewed"), (4097, 4096, 8, "padded"), (4096, 4097, 8, "any"), (3, 4096, 72, "all"),
+    (4095, 7, 9, "padded"), (1, 1, 300, "all"),
 ]
 
 
