@@ -25,14 +25,22 @@ constexpr int AS_HEADS = 4;  // heads (or groups) that a warp takes one after th
 
 enum AsRole { AS_FORWARD, AS_DQ, AS_DKV };
 
-template <int CP>
+template <int CP, int DIM, AsRole ROLE>
 struct AsTiles {
   static constexpr int ROWS = AS_ROWS * CP * 2, COLS = AS_COLS * CP * 2;
-  static constexpr int SIDE = (AT_MAX_DIMS + 2) * AS_COLS * 4;  // coordinates, lse, D of the columns
+  // coordinates of the columns and, where rows are keys, lse and D
+  static constexpr int SIDE = (DIM + (ROLE == AS_DKV ? 2 : 0)) * AS_COLS * 4;
   static constexpr int STAGE = 2 * COLS + SIDE;
   static constexpr int WARP = 2 * 2 * ROWS + 2 * STAGE;  // two sets of both rows' tiles, two stages
   static constexpr int SMEM = AS_WARPS * WARP;
 };
+
+// Blocks per SM: shared memory has room for four, which leave 128 registers; dk and dv do not fit in them (2048
+// molecules, three blocks -> four: forward 126 -> 117 us, dq 128 -> 122, dk and dv 138 -> 164).
+template <int DIM, AsRole ROLE>
+constexpr int as_blocks() {
+  return ROLE != AS_DKV && DIM <= 3 ? 4 : 3;
+}
 
 // [rows, heads, channels] of one operand
 struct AsOperand {
@@ -41,8 +49,8 @@ struct AsOperand {
 };
 
 template <typename T, int CP, int DIM, bool CAP, AsRole ROLE>
-__global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const __grid_constant__ AttnArgs a) {
-  using S = AsTiles<CP>;
+__global__ void __launch_bounds__(32 * AS_WARPS, (as_blocks<DIM, ROLE>())) attention_short_kernel(const __grid_constant__ AttnArgs a) {
+  using S = AsTiles<CP, DIM, ROLE>;
   using A = AtType<T>;
   constexpr bool KV = ROLE == AS_DKV, FORWARD = ROLE == AS_FORWARD;
   constexpr int KT = CP / 16, CT = CP / 8, NT = AS_COLS / 8, CHUNKS = CP / 8;
@@ -153,7 +161,7 @@ __global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const
           }
         }
         if constexpr (KV) {
-          float *stat = side + AT_MAX_DIMS * AS_COLS;
+          float *stat = side + DIM * AS_COLS;
           const int64_t col = (int64_t)head * p.m + j0 + lane;
           if (j0 + lane < c_hi) {
             cp_async_4(stat + lane, a.lse + col);
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const
           }
           const uint32_t st = at_mine + 4 * S::ROWS + stage * S::STAGE;
           const float *side = reinterpret_cast<const float *>(mine + 4 * S::ROWS + stage * S::STAGE + 2 * S::COLS) + gc;
-          const float *stat = side + AT_MAX_DIMS * AS_COLS;
+          const float *stat = side + DIM * AS_COLS;
           const int left = (int)(count - (int64_t)j * AS_COLS < AS_COLS ? count - (int64_t)j * AS_COLS : AS_COLS);
           float s[NT][4] = {}, dp[FORWARD ? 1 : NT][4] = {};
 #pragma unroll
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(32 * AS_WARPS, 3) attention_short_kernel(const
 
 template <typename T, int CP, int DIM, bool CAP, AsRole ROLE>
 static int as_launch(const AttnArgs &a) {
-  using S = AsTiles<CP>;
+  using S = AsTiles<CP, DIM, ROLE>;
   static unsigned long long configured = 0ull;
   B200C_CUDA(opt_in_shared_memory(attention_short_kernel<T, CP, DIM, CAP, ROLE>, S::SMEM, configured));
   const int64_t rows = ROLE == AS_DKV ? a.p.n : a.p.m;
