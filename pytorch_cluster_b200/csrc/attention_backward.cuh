@@ -387,6 +387,12 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
           if (count > 0 && ok) {
             t5_ld32(t_acc + lane_base + ch * 32, o);
             t5_wait_ld32(o);
+            // a row that sees no column (of no example, or of one without) shares the pass of its neighbours, where 0
+            // times a NaN or an infinity of the columns would stay
+            if (row_lo >= row_hi) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
