@@ -35,7 +35,7 @@ struct AttnArgs {
   const void *dout = nullptr;    // [m, heads, channels]
   const float *delta = nullptr;  // [heads, m]: D_i
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;  // [m, heads, channels], [n, groups, channels] x 2
-  const float *norms = nullptr;  // fp16: the largest |do|^2 and |v|^2 of a row
+  const float *norms = nullptr;  // fp16: [segments, groups, 2], the largest |do|^2 and |v|^2 of a row (at_sigma)
   // forward, split over the columns: [m, heads, splits, channels + 2] (maximum, sum, result)
   float *parts = nullptr;
   int splits = 1;
@@ -72,6 +72,7 @@ __device__ __forceinline__ void at_segment(const int64_t *__restrict__ ptr, int6
 
 int launch_attention_plain_forward(const AttnArgs &a);
 int launch_attention_plain_backward(const AttnArgs &a);
+size_t attention_norms_bytes(const b200c_attention_t &p);  // of `norms`: fp16 only
 int launch_attention_delta(const AttnArgs &a, float *delta, float *norms);
 bool attention_tensor_applicable(const b200c_attention_t &p);
 int launch_attention_tensor_forward(const AttnArgs &a);

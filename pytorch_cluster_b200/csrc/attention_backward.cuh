@@ -7,8 +7,7 @@
 // P and dS enter the second products in the 16-bit type.  dq takes dS in two parts, rounded and what rounding left,
 // because the rows of dS sum to zero and a rounded one does not: dq's error was 1.5 times that of its own rounding, now
 // it is that (for dk and dv, 1.4 times, tensor memory has no room left).  In fp16, whose range is small, P is kept
-// times 2^12 and dS times a power of two that brings the largest value that |do| and |v| allow to 2^14; both are taken
-// out of the fp32 sums.
+// times 2^12 and dS times a power of two of its example (at_sigma); both are taken out of the fp32 sums.
 #pragma once
 
 #include "attention_tensor.cuh"
@@ -39,18 +38,6 @@ struct AtBackward {
 struct AtBackwardMaps {
   CUtensorMap row0, row1, col0, col1;  // q, do, k, v or k, v, q, do
 };
-
-// the power of two that dS is kept times (see above); norms: the largest |do|^2 and |v|^2 of a row
-template <typename T>
-__device__ __forceinline__ float at_sigma(const float *norms) {
-  if constexpr (AtType<T>::BF16) {
-    return 1.f;
-  } else {
-    const float most = 2.f * sqrtf(norms[0]) * sqrtf(norms[1]);
-    if (!(most > 1e-30f && most < 1e30f)) return 1.f;
-    return exp2f(14.f - ceilf(log2f(most)));
-  }
-}
 
 template <typename T, int CP, int DIM, bool CAP, bool KV>
 __global__ void __launch_bounds__(AtBackward<CP, KV>::THREADS, AtBackward<CP, KV>::BLOCKS)
@@ -153,7 +140,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
     if (grp == 0) shared_tile.segment[lrow] = row_segment;
   }
   const float pre = CAP ? 2.f * AT_LOG2E * p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
-  const float sigma = at_sigma<T>(norms);
+  const float sigma = at_sigma<T>(norms, p.groups, row_segment, group);  // of the row
   const float sig = A::BF16 ? 1.f : sigma * (1.f / 4096.f);  // P carries 2^SHIFT already
 
   bool by_example = false;

@@ -12,8 +12,9 @@
 // meets another one's zeros. The backward pass is two kernels of the same shape: one owns 64 queries and sums dq over
 // the keys, one owns 64 keys and sums dk and dv over the queries of all heads of its group.  Scores are formed twice,
 // but nothing is added atomically: the result does not depend on the order of the blocks.
-#include "attention.cuh"
-#include "tcgen05.cuh"
+#include <type_traits>
+
+#include "attention_tensor.cuh"
 
 namespace b200c {
 
@@ -523,31 +524,51 @@ __global__ void __launch_bounds__(AP_THREADS) attention_plain_dkv_kernel(AttnArg
 }
 
 // What the backward pass needs beforehand: D_i = do_i . o_i per (row, head), and for fp16 the largest |do_i|^2 and
-// |v_j|^2 of any row (norms[0], norms[1]; non-negative floats order like their bits, and a maximum does not depend on
-// the order).  LP lanes share a row, VL channels at a time; the blocks past the first `do_blocks` take the rows of v.
+// |v_j|^2 of any finite row of an example and key head (norms[b][group][0], [1]; non-negative floats order like their
+// bits, and a maximum does not depend on the order).  LP lanes share a row, VL channels at a time; the blocks past the
+// first `do_blocks` take the rows of v.  A block has consecutive rows, mostly of a few examples, and collects their
+// maxima in shared memory: one at a time they were as many atomics as rows.
+constexpr int AP_NORMS = 1024;  // (example, key head) pairs of a block that are collected
 template <typename T, int VL>
 struct alignas(sizeof(T) * VL) ApVec {
   T v[VL];
 };
-template <typename T, int VL, int LP>
-__global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, float *__restrict__ delta,
-                                                                float *__restrict__ norms, int64_t do_rows,
+template <typename T, int VL, int LP, bool NORMS>
+__global__ void __launch_bounds__(256, NORMS ? 6 : 1) attention_prepare_kernel(AttnArgs a, float *__restrict__ delta,
+                                                                unsigned *__restrict__ norms, int64_t do_rows,
                                                                 unsigned do_blocks) {
   using V = ApVec<T, VL>;
-  __shared__ float s_most[8];
+  constexpr int SLOTS = 256 / LP;
+  __shared__ unsigned s_most[NORMS ? AP_NORMS : 1];
   const b200c_attention_t &p = a.p;
   const int part = threadIdx.x % LP, units = p.channels / VL;
-  const bool values = blockIdx.x >= do_blocks;
+  const bool values = NORMS && blockIdx.x >= do_blocks;
   const unsigned block = values ? blockIdx.x - do_blocks : blockIdx.x;
   const unsigned blocks = values ? gridDim.x - do_blocks : do_blocks;
   const int64_t rows = values ? p.n * p.groups : do_rows;
+  const int heads = values ? p.groups : p.heads;
   const V *dout = (const V *)a.dout, *out = (const V *)a.out, *rest = (const V *)a.rest;
-  float most = 0.f;
+  int64_t from = (int64_t)block * SLOTS, to = rows, step = (int64_t)blocks * SLOTS;
+  // NORMS: the place of example b, relative to row0
+  const int64_t *ptr = values ? p.ptr_k : p.ptr_q;
+  const int64_t side = values ? p.n : p.m;
+  int64_t row0 = 0;
+  int b_first = 0, b = 0, lo = 0, hi = 0;
+  if (NORMS) {
+    step = SLOTS;
+    const int64_t each = ((rows + blocks - 1) / blocks + SLOTS - 1) / SLOTS * SLOTS;
+    from = (int64_t)block * each;
+    if (from + each < to) to = from + each;
+    for (int i = threadIdx.x; i < AP_NORMS; i += 256) s_most[i] = 0u;
+    row0 = from / heads;
+    if (from < to) b = b_first = at_segment_of_warp(ptr, (int)p.num_segments, row0, threadIdx.x & 31);
+    __syncthreads();
+  }
   // whole warps take the same number of steps (the sums are shuffles)
-  for (int64_t i0 = (int64_t)block * (256 / LP); i0 < rows; i0 += (int64_t)blocks * (256 / LP)) {
+  for (int64_t i0 = from; i0 < to; i0 += step) {
     const int64_t i = i0 + threadIdx.x / LP;
     float s = 0.f, sq = 0.f;
-    if (i < rows) {
+    if (i < to) {
       const V *v = dout + i * units;
       if (values) v = reinterpret_cast<const V *>((const T *)p.v + (i / p.groups) * p.v_row + (i % p.groups) * p.v_head);
       for (int u = part; u < units; u += LP) {
@@ -564,7 +585,7 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, floa
             const float x = at_float(g.v[c]);
             s = fmaf(x, at_float(o.v[c]), s);
             if (rest) s = fmaf(x, at_float(r.v[c]), s);
-            sq = fmaf(x, x, sq);
+            if (NORMS) sq = fmaf(x, x, sq);
           }
         }
       }
@@ -572,19 +593,40 @@ __global__ void __launch_bounds__(256) attention_prepare_kernel(AttnArgs a, floa
 #pragma unroll
     for (int o = LP / 2; o > 0; o >>= 1) {
       s += __shfl_xor_sync(FULL_MASK, s, o);
-      sq += __shfl_xor_sync(FULL_MASK, sq, o);
+      if (NORMS) sq += __shfl_xor_sync(FULL_MASK, sq, o);
     }
-    if (!values && part == 0 && i < rows) delta[(i % p.heads) * p.m + i / p.heads] = s;
-    most = fmaxf(most, sq);
+    if (part == 0 && i < to) {
+      const int64_t row = i / heads;
+      const int head = (int)(i - row * heads);
+      if (!values) delta[(int64_t)head * p.m + row] = s;
+      if (NORMS && sq < pos_inf<float>()) {  // not of NaN either
+        const int at = (int)(row - row0), group = values ? head : head / (p.heads / p.groups);
+        if (at < lo || at >= hi) {
+          // most often the next example's
+          int64_t l, h;
+          if (hi > 0 && b + 1 < p.num_segments) ++b;
+          at_segment(ptr, side, b, l, h);
+          if (row < l || row >= h) {
+            b = segment_of(ptr, (int)p.num_segments, row);
+            at_segment(ptr, side, b, l, h);
+          }
+          lo = l > row0 ? (int)(l - row0) : 0;
+          hi = h > row0 ? (int)(h - row0) : 0;
+        }
+        if (at >= lo && at < hi) {  // else of no example
+          const int64_t place = (int64_t)(b - b_first) * p.groups + group;
+          if (place >= 0 && place < AP_NORMS)
+            atomicMax(&s_most[place], __float_as_uint(sq));
+          else
+            atomicMax(norms + 2 * ((int64_t)b * p.groups + group) + (values ? 1 : 0), __float_as_uint(sq));
+        }
+      }
+    }
   }
-  if (norms == nullptr) return;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FULL_MASK, most, o));
-  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) most = fmaxf(most, s_most[w]);
-    atomicMax((unsigned *)norms + (values ? 1 : 0), __float_as_uint(most));
+  if (NORMS) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < AP_NORMS; i += 256)
+      if (s_most[i] != 0u) atomicMax(norms + 2 * ((int64_t)b_first * p.groups + i) + (values ? 1 : 0), s_most[i]);
   }
 }
 
@@ -640,14 +682,16 @@ int launch_attention_plain_backward(const AttnArgs &a) { return ap_any(a, false)
 template <typename T, int VL, int LP>
 static int ap_prepare_launch(const AttnArgs &a, float *delta, float *norms) {
   const int64_t rows = a.p.m * a.p.heads, values = norms ? a.p.n * a.p.groups : 0;
-  const auto blocks = [](int64_t r) {
-    const int64_t want = (r + 256 / LP - 1) / (256 / LP);
-    return (unsigned)(want < 148 * 8 ? want : 148 * 8);
+  constexpr bool NORMS = std::is_same<T, __half>::value;
+  const auto blocks = [](int64_t r, int per_sm) {
+    const int64_t want = (r + 256 / LP - 1) / (256 / LP), most = 148 * per_sm;
+    return (unsigned)(want < most ? want : most);
   };
-  const unsigned b0 = blocks(rows), b1 = blocks(values);
-  if (norms) B200C_CUDA(cudaMemsetAsync(norms, 0, 8, a.stream));
+  // with norms six blocks fit an SM (2048 molecules: D and norms 57 us in blocks of fewer rows, 46 so)
+  const unsigned b0 = blocks(rows, NORMS ? 3 : 8), b1 = blocks(values, 3);
+  if (norms) B200C_CUDA(cudaMemsetAsync(norms, 0, attention_norms_bytes(a.p), a.stream));
   if (b0 + b1 == 0) return B200C_OK;
-  attention_prepare_kernel<T, VL, LP><<<b0 + b1, 256, 0, a.stream>>>(a, delta, norms, rows, b0);
+  attention_prepare_kernel<T, VL, LP, NORMS><<<b0 + b1, 256, 0, a.stream>>>(a, delta, (unsigned *)norms, rows, b0);
   B200C_LAUNCH_CHECK("attention_prepare_kernel");
   return B200C_OK;
 }
@@ -662,6 +706,10 @@ static int ap_delta(const AttnArgs &a, float *delta, float *norms) {
   if (p.channels <= 4 * VL) return ap_prepare_launch<T, VL, 4>(a, delta, norms);
   if (p.channels <= 8 * VL) return ap_prepare_launch<T, VL, 8>(a, delta, norms);
   return ap_prepare_launch<T, VL, 16>(a, delta, norms);
+}
+
+size_t attention_norms_bytes(const b200c_attention_t &p) {
+  return p.dtype == B200C_F16 ? (size_t)p.num_segments * p.groups * 8 : 0;
 }
 
 int launch_attention_delta(const AttnArgs &a, float *delta, float *norms) {

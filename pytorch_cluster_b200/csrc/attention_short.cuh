@@ -77,12 +77,6 @@ __global__ void __launch_bounds__(32 * AS_WARPS, (as_blocks<DIM, ROLE>())) atten
   const int u_lo = blockIdx.y * AS_HEADS, u_hi = u_lo + AS_HEADS < units ? u_lo + AS_HEADS : units;
   const int inner = KV ? per_group : 1;  // heads whose columns are walked per unit
   const float pre = CAP ? 2.f * AT_LOG2E * p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
-  float sigma = 1.f;
-  if constexpr (!FORWARD && !A::BF16) {
-    const float most = 2.f * sqrtf(a.norms[0]) * sqrtf(a.norms[1]);
-    if (most > 1e-30f && most < 1e30f) sigma = exp2f(14.f - ceilf(log2f(most)));
-  }
-  const float sig = A::BF16 ? 1.f : sigma * (1.f / 4096.f);  // P carries 2^SHIFT already
 
   float pos[2][DIM == 0 ? 1 : DIM];
   if constexpr (DIM > 0) {
@@ -177,8 +171,14 @@ __global__ void __launch_bounds__(32 * AS_WARPS, (as_blocks<DIM, ROLE>())) atten
 
     int stage = 0;
     if (blocks > 0) fetch(u_lo, 0, 0, 0);
+    // a lane finds one unit's power of two while that is on its way
+    float sigmas = 1.f;
+    if (!FORWARD && u_lo + (lane & (AS_HEADS - 1)) < u_hi)
+      sigmas = at_sigma<T>(a.norms, p.groups, b, (u_lo + (lane & (AS_HEADS - 1))) / (KV ? 1 : per_group));
     for (int u = u_lo; u < u_hi; ++u) {
       const int head0 = KV ? u * per_group : u;
+      const float sigma = FORWARD || A::BF16 ? 1.f : __shfl_sync(FULL_MASK, sigmas, u - u_lo);
+      const float sig = A::BF16 ? 1.f : sigma * (1.f / 4096.f);  // P carries 2^SHIFT already
       float top[2] = {-pos_inf<float>(), -pos_inf<float>()}, sum[2] = {}, lse[2] = {}, delta[2] = {};
       float acc[CT][4] = {}, acc2[KV ? CT : 1][4] = {};
       if constexpr (ROLE == AS_DQ) {

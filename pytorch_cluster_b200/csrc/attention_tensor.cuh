@@ -185,6 +185,22 @@ struct AtType<__half> {
   __device__ __forceinline__ static float high(uint32_t v) { return __high2float(*reinterpret_cast<const __half2 *>(&v)); }
 };
 
+// The power of two that fp16's dS is kept times: it brings the largest value that |do| and |v| of the row's example and
+// key head allow to 2^14.  With one power for the whole call the examples would not be apart: one with output gradients
+// of 6e4 took all bits from another's of 1e-4.  norms: the largest |do|^2 and |v|^2 of the finite rows, [segments, groups,
+// 2]; b < 0: a row that is not there.
+template <typename T>
+__device__ __forceinline__ float at_sigma(const float *norms, int groups, int b, int group) {
+  if constexpr (AtType<T>::BF16) {
+    return 1.f;
+  } else {
+    if (b < 0) return 1.f;
+    const float2 n = reinterpret_cast<const float2 *>(norms)[(int64_t)b * groups + group];
+    const float most = 2.f * sqrtf(n.x) * sqrtf(n.y);
+    return most > 1e-30f ? exp2f(14.f - ceilf(log2f(most))) : 1.f;
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t at_not_finite(const uint4 &w) {
   using A = AtType<T>;

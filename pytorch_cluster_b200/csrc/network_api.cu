@@ -194,7 +194,8 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
 
 extern "C" size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a) {
   if (check_attention(a) != B200C_OK) return 0;
-  return align256((size_t)a->m * a->heads * 4) + 256 + attention_tensor_order_bytes(*a);  // D, the largest norms, order
+  // D, the largest norms, order; never 0
+  return align256((size_t)a->m * a->heads * 4) + align256(attention_norms_bytes(*a) + 1) + attention_tensor_order_bytes(*a);
 }
 
 extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const void *rest, const float *lse,
@@ -224,7 +225,7 @@ extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *
   a.stream = (cudaStream_t)stream;
   float *norms = (float *)((char *)workspace + align256((size_t)p->m * p->heads * 4));
   a.norms = norms;
-  if (attention_tensor_order_bytes(*p) > 0) a.order = (int *)((char *)norms + 256);
+  if (attention_tensor_order_bytes(*p) > 0) a.order = (int *)((char *)norms + align256(attention_norms_bytes(*p) + 1));
   if ((st = launch_attention_delta(a, (float *)workspace, norms)) != B200C_OK) return st;
   if (attention_tensor_applicable(*p) &&
       (((uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0)

@@ -38,3 +38,48 @@ def test_gradients_of_rows_of_no_example_are_zero(dtype, lens, channels):
             for name, t in zip(("out", "dq", "dk", "dv"), got):
                 assert (t[outside] == 0).all(), (name, which, value)
                 assert_close(t[healthy], *want[name], (name, which, value))
+
+
+# ---- fp16 gradients of unlike magnitudes ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("lens, channels", [([3000, 40], 64), ([100] * 24 + [40], 32), ([700, 40], 128)])
+# which: v, the gradient of the output; a row of the example itself is part of the others' dk and dv, not of their dq
+@pytest.mark.parametrize("which, value, place", [(w, x, p) for w in (2, 3) for x in (math.inf, math.nan, 6e4)
+                                                 for p in ("example", "outside")] +
+                         [(3, math.inf, "row"), (3, math.nan, "row")])
+def test_fp16_gradients_do_not_depend_on_other_examples_magnitudes(lens, channels, which, value, place):
+    g = gen(52)
+    n, b = sum(lens), ids(lens)
+    ts = [rand(g, n, 2, channels, dtype=torch.float16) for _ in range(3)]
+    ts.append(rand(g, n, 2, channels, dtype=torch.float16, scale=1e-4))
+    first = n - lens[-1]
+    want = attention_plain(*(t[:first] for t in ts[:3]), lens[:-1], lens[:-1], dout=ts[3][:first])
+    if place == "row":
+        ts[3][5] = value
+        got = gradients(ts[:3], ts[3], b, b, batch_size=len(lens))
+        keep = torch.arange(first, device="cuda") != 5
+        assert_close(got[1][:first][keep], want["dq"][0][keep], want["dq"][1][keep], "dq")
+        return
+    ts[which][first + 7] = value
+    got = gradients(ts[:3], ts[3], b, b, batch_size=len(lens) - (place == "outside"))
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        assert_close(t[:first], *want[name], name)
+
+
+@pytest.mark.parametrize("rows, groups, channels, gaps", [(2, 16, 32, 1), (3, 8, 16, 4), (40, 4, 24, 1), (300, 2, 64, 2)])
+def test_fp16_gradients_of_many_examples_of_their_own_magnitudes(rows, groups, channels, gaps):
+    """Output gradients from 1e-4 to 1e4, another size for every example and key head; empty examples between them."""
+    g = gen(59)
+    examples = 70000 // rows
+    n = examples * rows
+    b = torch.arange(examples, device="cuda").repeat_interleave(rows) * gaps
+    ts = [rand(g, n, h, channels, dtype=torch.float16) for h in (16, groups, groups)]
+    size = 10 ** (8 * torch.rand(examples, groups, generator=g, device="cuda") - 4)
+    do = torch.randn(n, 16, channels, generator=g, device="cuda")
+    do = (do * size.repeat_interleave(rows, 0).repeat_interleave(16 // groups, 1)[..., None]).half().clamp(-6e4, 6e4)
+    got = gradients(ts, do, b, b, batch_size=examples * gaps)
+    some = torch.randperm(examples, generator=g, device="cuda")[:30].sort().values
+    at = (some[:, None] * rows + torch.arange(rows, device="cuda")).flatten()
+    want = attention_plain(*(t[at] for t in ts), [rows] * 30, [rows] * 30, dout=do[at])
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        assert_close(t[at], *want[name], name)
