@@ -29,6 +29,13 @@ struct OpRange {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// Derivatives are taken backward only.  A tangent would be dropped without a word, which makes the derivative zero.
+void refuse_tangents(const char *op, std::initializer_list<const torch::Tensor *> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const torch::Tensor *t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+}
+
 bool wants_gradient(std::initializer_list<const torch::Tensor *> tensors) {
   if (!at::GradMode::is_enabled()) return false;
   for (const torch::Tensor *t : tensors)
@@ -148,6 +155,7 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
 };
 
 torch::Tensor gather_rows(torch::Tensor x, torch::Tensor index, double scale) {
+  refuse_tangents("gather_rows", {&x});
   CHECK_INPUT(x.dim() == 2);
   if (wants_gradient({&x})) return GatherRows::apply(x, index, scale);
   return gather_rows_forward(x, index, scale);
@@ -288,6 +296,7 @@ std::tuple<torch::Tensor, torch::Tensor> norm_rotate(torch::Tensor q, torch::Ten
                                                      torch::Tensor pos_k, torch::Tensor freq, OptTensor weight_q,
                                                      OptTensor weight_k, double eps) {
   const torch::Tensor wq = or_undefined(weight_q), wk = or_undefined(weight_k);
+  refuse_tangents("norm_rotate", {&q, &k, &pos_q, &pos_k, &freq, &wq, &wk});
   if (!wants_gradient({&q, &k, &wq, &wk}))
     return norm_rotate_forward(q, k, pos_q, pos_k, freq, weight_q, weight_k, eps);
   auto y = NormRotate::apply(q, k, pos_q, pos_k, freq, weight_q, weight_k, eps);
@@ -444,6 +453,8 @@ struct SoftmaxAttention : torch::autograd::Function<SoftmaxAttention> {
 
 torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, OptTensor ptr_q, OptTensor ptr_k,
                         OptTensor pos_q, OptTensor pos_k, OptTensor slope, double scale, double cap) {
+  const torch::Tensor pq = or_undefined(pos_q), pk = or_undefined(pos_k), sl = or_undefined(slope);
+  refuse_tangents("attention", {&q, &k, &v, &pq, &pk, &sl});
   if (wants_gradient({&q, &k, &v}))
     return SoftmaxAttention::apply(q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap);
   return std::get<0>(attention_forward(q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap, false));

@@ -83,3 +83,33 @@ def test_fp16_gradients_of_many_examples_of_their_own_magnitudes(rows, groups, c
     want = attention_plain(*(t[at] for t in ts), [rows] * 30, [rows] * 30, dout=do[at])
     for name, t in zip(("out", "dq", "dk", "dv"), got):
         assert_close(t[at], *want[name], name)
+
+
+# ---- derivatives that do not exist are refused ---------------------------------------------------------------
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwAD
+
+    import pytorch_cluster_b200 as pc
+
+    g = gen(55)
+    h = rand(g, 10, 2, 16, dtype=torch.float32)
+    pos, freq, w = rand(g, 10, 2, dtype=torch.float32), rand(g, 2, 8, dtype=torch.float32), torch.ones(16, device="cuda")
+    slope = torch.ones(2, device="cuda")
+    edges = torch.tensor([1, 2, 3], device="cuda")
+    calls = [(lambda x: pc.gather_rows(x, edges), [h[:, 0]]),
+             (lambda q, k, p, f, wq: pc.norm_rotate(q, k, p, p, f, wq), [h, h, pos, freq, w]),
+             (lambda q, k, v, p, s: pc.attention(q, k, v, pos_q=p, pos_k=pos, slope=s), [h, h, h, pos, slope])]
+    for call, args in calls:
+        for i in range(len(args)):
+            for wants in (False, True):
+                with fwAD.dual_level():
+                    mine = list(args)
+                    primal = mine[i].clone().requires_grad_(wants)
+                    mine[i] = fwAD.make_dual(primal, torch.ones_like(primal))
+                    with pytest.raises(RuntimeError, match="forward-mode|receives no gradient"):
+                        call(*mine)
+                    with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*mine)
+        with fwAD.dual_level():
+            call(*args)  # without tangents nothing is refused

@@ -1,0 +1,27 @@
+"""Calls of gather_rows, norm_rotate and attention that are settled before any CUDA call."""
+import pytest
+import torch
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwAD
+
+    import pytorch_cluster_b200  # noqa: F401
+
+    ops = torch.ops.torch_cluster
+    h, pos, freq, w, slope = (torch.rand(*s) for s in ((4, 2, 8), (4, 2), (2, 4), (8,), (2,)))
+    calls = [(lambda x: ops.gather_rows(x, torch.tensor([0]), 1.0), [h[:, 0]]),
+             (lambda q, k, p, pk, f, wq, wk: ops.norm_rotate(q, k, p, pk, f, wq, wk, 1e-6), [h, h, pos, pos, freq, w, w]),
+             (lambda q, k, v, p, pk, s: ops.attention(q, k, v, None, None, p, pk, s, 1.0, 0.0),
+              [h, h, h, pos, pos, slope])]
+    for call, args in calls:
+        for i in range(len(args)):
+            for wants in (False, True):
+                with fwAD.dual_level():
+                    mine = list(args)
+                    primal = mine[i].clone().requires_grad_(wants)
+                    mine[i] = fwAD.make_dual(primal, torch.ones_like(primal))
+                    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                        call(*mine)
+        with pytest.raises(RuntimeError, match="must be CUDA tensor"):
+            call(*args)
