@@ -220,8 +220,8 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_kernel(AttnArgs a, i
 // hundred instructions on 16 KB of keys and values and memory is the only bound.  Each of the block's warps has a ring
 // of its own in shared memory, 32 keys and values to a stage, filled by asynchronous 16-byte copies two stages ahead:
 // no barrier between warps until the end.  A row of 2 * CP bytes keeps its 16-byte chunk c at c ^ (row & 7), so that
-// neither the copies nor the matrix loads meet bank conflicts.  Weights are rounded to the 16-bit type; maxima, sums
-// and results are fp32. Shared memory of keys past the split's end is cleared: their weights are 0, and 0 times
+// neither the copies nor the matrix loads meet bank conflicts.  Weights are rounded to the 16-bit type (fp16: times 2^15);
+// maxima, sums and results are fp32. Shared memory of keys past the split's end is cleared: their weights are 0, and 0 times
 // whatever stood there must be 0.
 constexpr int AF_KEYS = 32;    // keys of a stage
 constexpr int AF_STAGES = 3;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnAr
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (e == 1 && !both) break;
-        float m = top[e];
+        float m = -pos_inf<float>();
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -395,6 +395,7 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_tensor_kernel(AttnAr
           }
         m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 1));
         m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 2));
+        m = fmaxf(top[e], m - AtType<T>::TOP);  // what the weights are relative to
         const float base = m == -pos_inf<float>() ? 0.f : m;
         const float shrink = t5_ex2(top[e] - base);
         top[e] = m;

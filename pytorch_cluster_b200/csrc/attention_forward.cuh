@@ -2,9 +2,10 @@
 //
 // Each group of warps has its own running maximum, sum and result of its steps; they are joined at the end.  The
 // maximum is not looked for in every step: weights are formed against the one in use, and only where their sum over the
-// step's 32 columns passes 2^10 (or no maximum is known yet) is it raised to the step's and the result in tensor
-// memory, the sum and the step's weights brought to it.  Weights up to 2^10 are as exact in either type as weights up
-// to 1. Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.
+// step's 32 columns passes 2^10 in bf16, 2^6 in fp16 (or no maximum is known yet) is it raised to the step's and the
+// result in tensor memory, the sum and the step's weights brought to it.  bf16 holds weights up to 2^10 as exactly as
+// weights up to 1; fp16 keeps them times 2^9, below 2^15, and loses less than 2^-34 of the row's sum with each.
+// Sums and the result are fp32; the weights are rounded to the 16-bit type as operands of the second product.
 // The result is divided by the sum of the rounded weights, not of the exact ones (which the statistics keep): where few
 // keys share the weight their roundings then cancel, and D = do . o, which the gradients need, is as much better.
 #pragma once
@@ -28,7 +29,6 @@ struct AtForward {
   static constexpr int TMEM = CP == 64 ? 256 : 512;
   static_assert(STAGES * STAGE_BYTES >= 2 * Q_BYTES, "the ring takes the block's rows");
   static_assert(PAIRS * PAIR_COLS + G * CP <= TMEM, "tensor memory");
-  static constexpr float MOST = 1024.f;  // sum of a step's weights that needs no new maximum
 };
 
 struct AtForwardMaps {
@@ -234,7 +234,8 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       const bool mine = pass.segment < 0 || pass.segment == row_segment;
       const AtSeen seen(row_lo, row_hi, pass, mine);
       const bool scan = mixed && !by_example;
-      // sub: what the scores are taken relative to; sums of the weights, exact and rounded
+      // sub: what the scores are taken relative to (0 as long as no maximum is known, then RAISED below it); sums of the
+      // weights, exact and rounded
       float top = -pos_inf<float>(), sub = 0.f, sum = 0.f, sum16 = 0.f;
       uint32_t bad = 0u;
       const uint32_t c0 = (pair + F::PAIRS - stage0 % F::PAIRS) % F::PAIRS;  // the pair's first stage
@@ -272,9 +273,10 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
 #pragma unroll
             for (int j = 1; j < AT_SUB; ++j) m = fmaxf(m, x[j]);
             if (fresh && m > -pos_inf<float>()) {
-              top = sub = m;
+              top = m;
+              sub = m - A::RAISED;
 #pragma unroll
-              for (int j = 0; j < AT_SUB; ++j) x[j] -= m;
+              for (int j = 0; j < AT_SUB; ++j) x[j] -= sub;
             }
           }
           float l0 = 0.f, l1 = 0.f, r0 = 0.f, r1 = 0.f;
@@ -288,15 +290,15 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
             r1 += A::high(w[j >> 1]);
           }
           l0 += l1;
-          const bool raise = !(l0 <= F::MOST);
+          const bool raise = !(l0 <= A::MOST);
           if (__any_sync(FULL_MASK, raise)) {
             float m = x[0];
 #pragma unroll
             for (int j = 1; j < AT_SUB; ++j) m = fmaxf(m, x[j]);
             m += sub;
             const float to = raise && m > top ? m : top;
-            const float shrink = to == top ? 1.f : t5_ex2(top - to);  // from -inf: 0
-            const float to_sub = to == -pos_inf<float>() ? 0.f : to;
+            const float to_sub = to == -pos_inf<float>() ? 0.f : to - A::RAISED;
+            const float shrink = top == -pos_inf<float>() ? 0.f : t5_ex2(sub - to_sub);
             l0 = l1 = r0 = r1 = 0.f;
 #pragma unroll
             for (int j = 0; j < AT_SUB; j += 2) {
@@ -354,7 +356,7 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
         t5_fence_after();
       }
       if (bad) bad_s = 1;
-      s_top[grp][lrow] = top;
+      s_top[grp][lrow] = top == -pos_inf<float>() ? top : sub;  // what the sums are relative to
       s_sum[grp][lrow] = sum;
       s_sum16[grp][lrow] = sum16;
       asm volatile("bar.sync 1, %0;" ::"n"(F::EL_THREADS) : "memory");

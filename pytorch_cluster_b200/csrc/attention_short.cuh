@@ -11,8 +11,8 @@
 // worked on; there is no barrier between warps.  16 rows that lie in several examples are taken example by example, and
 // only the example's rows are stored, so that a NaN of one never meets another one's zeros; columns past
 // the example's end are cleared in shared memory for the same reason.
-// Weights are rounded to the type as operands (dS of dq in two parts, see attention_backward.cuh); statistics and sums
-// are fp32.
+// Weights are rounded to the type as operands (fp16: times 2^15, see AtType; dS of dq in two parts, see
+// attention_backward.cuh); statistics and sums are fp32.
 #pragma once
 
 #include "attention_tensor.cuh"
@@ -269,11 +269,12 @@ __global__ void __launch_bounds__(32 * AS_WARPS, (as_blocks<DIM, ROLE>())) atten
           if constexpr (FORWARD) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float m = top[h];
+              float m = -pos_inf<float>();
 #pragma unroll
               for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
               m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 1));
               m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, 2));
+              m = fmaxf(top[h], m - A::TOP);  // what the weights are relative to
               const float sub = m == -pos_inf<float>() ? 0.f : m, shrink = t5_ex2(top[h] - sub);
               top[h] = m;
               float part = 0.f;

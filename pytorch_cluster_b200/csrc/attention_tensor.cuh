@@ -162,6 +162,9 @@ struct AtType<__nv_bfloat16> {
   static constexpr bool BF16 = true;
   static constexpr uint32_t EXP = 0x7fff7fffu, ONE = 0x00800080u;  // |w| + one step of the exponent overflows for inf, NaN
   static constexpr float SHIFT = 0.f;  // weights of the backward pass are kept times 2^SHIFT
+  // forward: weights are kept times 2^RAISED in tiles, where their sum over a step may grow to MOST, and times 2^TOP
+  // where none is above 1
+  static constexpr float RAISED = 0.f, MOST = 1024.f, TOP = 0.f;
   __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -176,6 +179,8 @@ struct AtType<__half> {
   static constexpr uint32_t EXP = 0x7fff7fffu, ONE = 0x04000400u;
   // probabilities below 2^-14 would lose bits in fp16: times 2^12 they keep them down to 2^-26
   static constexpr float SHIFT = 12.f;
+  // forward: below 2^-14 of a row's largest they would lose bits and vanish below 2^-25, however many they are
+  static constexpr float RAISED = 9.f, MOST = 32768.f, TOP = 15.f;
   __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

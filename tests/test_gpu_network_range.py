@@ -113,3 +113,32 @@ def test_forward_mode_derivatives_are_refused():
                         call(*mine)
         with fwAD.dual_level():
             call(*args)  # without tangents nothing is refused
+
+
+# ---- weights far below a row's largest -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("below", [21.86, 26.0])  # powers of two
+# tiles; tiles split over the keys; short examples; few queries
+@pytest.mark.parametrize("queries, keys, examples, channels, train", [
+    (300, 5000, 1, 64, True), (300, 5000, 1, 128, True), (200, 3000, 1, 64, False), (100, 120, 30, 32, True),
+    (1, 40000, 2, 64, False), (2, 3000, 4, 40, True), (1, 40000, 2, 7, False)])
+def test_attention_adds_up_small_weights(dtype, below, queries, keys, examples, channels, train):
+    """One key takes nearly all the weight and has the value zero: the result is what the others add."""
+    import pytorch_cluster_b200 as pc
+
+    g = gen(53)
+    m, n = queries * examples, keys * examples
+    q, k = torch.zeros(m, 1, channels, device="cuda"), torch.zeros(n, 1, channels, device="cuda")
+    q[..., 0], k[..., 0] = 4.0, -below * math.log(2) / 4
+    v = 1 + torch.rand(n, 1, channels, generator=g, device="cuda")
+    top = torch.arange(examples, device="cuda") * keys + keys // 3
+    k[top], v[top] = 0.0, 0.0
+    ts = [t.to(dtype).requires_grad_(train) for t in (q, k, v)]
+    lens_q, lens_k = [queries] * examples, [keys] * examples
+    out = pc.attention(*ts, ids(lens_q), ids(lens_k), scale=1.0, batch_size=examples)
+    o, tol = attention_plain(*(t.detach() for t in ts), lens_q, lens_k, scale=1.0)["out"]
+    if dtype == torch.float16:
+        # a weight is held in fp16 times 2^9 or more, of which 2^-25 is half the smallest step; v is below 2
+        tol = tol + keys * 2.0 ** -34 * 2
+    assert_close(out.detach(), o, tol, "out")
