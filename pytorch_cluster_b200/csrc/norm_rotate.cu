@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(NR_THREADS, 2) norm_rotate_backward_kernel(Nor
         sq = nr_sum<LP>(sq);
         tx = nr_sum<LP>(tx);
         const float inv = rsqrtf(fmaf(sq, mean, a.eps));
-        const float back = inv * inv * inv * (tx * mean);
+        // in an order in which rows of 1e16 and of 1e-14 pass (the cube of inv would leave the range of fp32)
+        const float back = inv * inv * (inv * tx * mean);
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
           const int c = (part + LP * i) * VL;

@@ -4,7 +4,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_network import DTYPES, assert_close, attention_plain, gen, ids, rand
+from test_gpu_network import DTYPES, assert_close, attention_plain, gen, ids, rand, rotate_plain
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +142,27 @@ def test_attention_adds_up_small_weights(dtype, below, queries, keys, examples, 
         # a weight is held in fp16 times 2^9 or more, of which 2^-25 is half the smallest step; v is below 2
         tol = tol + keys * 2.0 ** -34 * 2
     assert_close(out.detach(), o, tol, "out")
+
+
+# ---- rows far from unit size ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("channels", [64, 6])
+@pytest.mark.parametrize("size, eps", [(1e16, 1e-6), (1e-14, 1e-30)])
+def test_norm_rotate_gradients_of_large_and_small_rows(dtype, channels, size, eps):
+    import pytorch_cluster_b200 as pc
+
+    g = gen(54)
+    q, k = (rand(g, 100, 2, channels, dtype=dtype, scale=size).requires_grad_() for _ in range(2))
+    pos, freq = rand(g, 100, 2, dtype=torch.float32), rand(g, 2, channels // 2, dtype=torch.float32)
+    w = (1 + 0.2 * torch.randn(channels, generator=g, device="cuda")).requires_grad_()
+    dy = [rand(g, *q.shape, dtype=dtype) for _ in range(2)]
+    out = pc.norm_rotate(q, k, pos, pos, freq, w, w, eps=eps)
+    grads = torch.autograd.grad(out, (q, k, w), dy)
+    want_w, tol_w = 0.0, 0.0
+    for i, x in enumerate((q, k)):
+        y, ty, dx, tx, dw, tw = rotate_plain(x.detach(), pos, freq, w.detach(), eps, dy[i])
+        assert_close(out[i].detach(), y, ty, "y")
+        assert_close(grads[i], dx, tx, "dx")
+        want_w, tol_w = want_w + dw, tol_w + tw + 2.0 ** -24 * dw.abs()
+    assert_close(grads[2], want_w, tol_w + 2.0 ** -24 * want_w.abs(), "dw")
