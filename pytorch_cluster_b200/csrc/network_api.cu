@@ -1,4 +1,6 @@
 // extern "C" entry points of gather_rows, norm_rotate and attention: argument checks and kernel selection.
+#include <math.h>
+
 #include "attention.cuh"
 #include "common.cuh"
 #include "launchers.h"
@@ -10,6 +12,9 @@ int check_device();  // api.cu
 static bool is_network_type(int dtype) { return dtype == B200C_F32 || dtype == B200C_F16 || dtype == B200C_BF16; }
 static size_t elem_bytes(int dtype) { return dtype == B200C_F32 ? 4 : 2; }
 constexpr int64_t MOST_ROWS = 0x7fffffffLL;
+// Scores are divided by the cap and multiplied by it again.  Far beyond them a quotient would leave the normal numbers of
+// fp32 (a cap that large bends nothing), far below them the scaled queries would.
+constexpr float MOST_CAP = 1.2676506e30f;  // 2^100
 
 // what every workspace is carved from
 static bool aligned_workspace(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -76,7 +81,9 @@ static int check_attention(const b200c_attention_t *a) {
   B200C_CHECK_ARG(a->m == 0 || a->q, "null pointer");
   B200C_CHECK_ARG(a->n == 0 || (a->k && a->v), "null pointer");
   B200C_CHECK_ARG(a->dims == 0 || (a->slope && (a->m == 0 || a->pos_q) && (a->n == 0 || a->pos_k)), "null pointer");
-  B200C_CHECK_ARG(a->scale == a->scale && a->cap == a->cap, "scale and cap must be numbers");
+  B200C_CHECK_ARG(isfinite(a->scale) && isfinite(a->cap), "scale and cap must be finite numbers");
+  B200C_CHECK_ARG(!(a->cap > 0.f) || (a->cap <= MOST_CAP && fabsf(a->scale) <= MOST_CAP * a->cap),
+                  "cap must lie between 2^-100 of scale and 2^100");
   const uintptr_t mask = elem_bytes(a->dtype) - 1;
   B200C_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & mask) == 0, "misaligned pointer");
   return B200C_OK;

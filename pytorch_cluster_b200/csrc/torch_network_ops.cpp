@@ -7,6 +7,7 @@
 #include <torch/script.h>
 #include <nvtx3/nvToolsExt.h>
 
+#include <cmath>
 #include <tuple>
 #include <vector>
 
@@ -337,6 +338,8 @@ void prepare_attention(Attention &t, const torch::Tensor &q, const torch::Tensor
   a.m = q.size(0), a.n = k.size(0);
   a.heads = (int)q.size(1), a.groups = (int)k.size(1), a.channels = (int)q.size(2);
   a.scale = (float)scale, a.cap = (float)cap;
+  TORCH_CHECK(std::isfinite(a.scale) && std::isfinite(a.cap) && (cap > 0) == (a.cap > 0),
+              "scale and cap must be finite numbers of 32 bits");
   a.num_segments = 1;
   CHECK_INPUT(ptr_q.has_value() == ptr_k.has_value());
   if (ptr_q.has_value()) {

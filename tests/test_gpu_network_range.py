@@ -166,3 +166,23 @@ def test_norm_rotate_gradients_of_large_and_small_rows(dtype, channels, size, ep
         assert_close(grads[i], dx, tx, "dx")
         want_w, tol_w = want_w + dw, tol_w + tw + 2.0 ** -24 * dw.abs()
     assert_close(grads[2], want_w, tol_w + 2.0 ** -24 * want_w.abs(), "dw")
+
+
+# ---- caps and scales that 32 bits do not hold -----------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_caps_and_scales_beyond_32_bits_are_refused(dtype):
+    import pytorch_cluster_b200 as pc
+
+    h = rand(gen(56), 70, 2, 16, dtype=dtype)
+    for extra in (dict(cap=1e39), dict(cap=1e-50), dict(cap=1e-31, scale=1.0), dict(cap=1e31), dict(scale=math.inf), dict(scale=1e39),
+                  dict(scale=math.nan)):
+        with pytest.raises((RuntimeError, ValueError), match="cap|scale"):
+            pc.attention(h, h, h, **extra)
+    for cap in (math.inf, math.nan, 1e-50, 1e39, 1e31):
+        with pytest.raises(RuntimeError, match="cap"):
+            torch.ops.torch_cluster.attention(h, h, h, None, None, None, None, None, 1.0, cap)
+    # the largest and smallest that pass
+    for cap in (1e30, 1e-29):
+        got = pc.attention(h, h, h, cap=cap)
+        assert_close(got, *attention_plain(h, h, h, [70], [70], cap=cap)["out"], cap)

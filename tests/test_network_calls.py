@@ -1,6 +1,10 @@
 """Calls of gather_rows, norm_rotate and attention that are settled before any CUDA call."""
+import ctypes
+import math
+
 import pytest
 import torch
+from test_network_refusals import attention_args
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -25,3 +29,20 @@ def test_forward_mode_derivatives_are_refused():
                         call(*mine)
         with pytest.raises(RuntimeError, match="must be CUDA tensor"):
             call(*args)
+
+
+@pytest.mark.parametrize("changes, message", [
+    (dict(cap=math.inf), b"finite"), (dict(cap=-math.inf), b"finite"), (dict(cap=math.nan), b"finite"),
+    (dict(scale=math.inf), b"finite"), (dict(scale=-math.inf), b"finite"),
+    (dict(cap=1e31), b"cap"), (dict(cap=1e-31), b"cap"), (dict(cap=1e-31, scale=-1.0), b"cap"),
+])
+def test_attention_caps_and_scales_that_are_refused(changes, message):
+    from pytorch_cluster_b200 import _native
+
+    lib = _native.cabi()
+    a, p = attention_args(**changes), 1 << 20  # never followed
+    assert lib.b200c_attention_forward(ctypes.byref(a), p, None, None, None, 0, None) == 1
+    assert message in lib.b200c_last_error()
+    assert lib.b200c_attention_backward(ctypes.byref(a), p, None, p, p, p, p, p, None, 0, None) == 1
+    assert message in lib.b200c_last_error()
+    assert lib.b200c_attention_workspace_bytes(ctypes.byref(a)) == 0
