@@ -469,7 +469,7 @@ typedef struct {
   const void *q, *k, *v;           /* [m, heads, channels], [n, groups, channels] x 2; channels contiguous */
   int64_t q_row, q_head, k_row, k_head, v_row, v_head; /* strides in elements */
   const int64_t *ptr_q, *ptr_k;    /* [num_segments + 1], ascending; NULL: one segment */
-  int64_t num_segments;
+  int64_t num_segments;            /* at most 2^30 */
   const float *pos_q, *pos_k;      /* [m, dims], [n, dims]; used when dims > 0 */
   const float *slope;              /* [heads]; used when dims > 0 */
   int64_t m, n;

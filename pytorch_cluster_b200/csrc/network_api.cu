@@ -12,6 +12,7 @@ int check_device();  // api.cu
 static bool is_network_type(int dtype) { return dtype == B200C_F32 || dtype == B200C_F16 || dtype == B200C_BF16; }
 static size_t elem_bytes(int dtype) { return dtype == B200C_F32 ? 4 : 2; }
 constexpr int64_t MOST_ROWS = 0x7fffffffLL;
+constexpr int64_t MOST_SEGMENTS = 1ll << 30;  // segments are bisected with 32-bit numbers
 // Scores are divided by the cap and multiplied by it again.  Far beyond them a quotient would leave the normal numbers of
 // fp32 (a cap that large bends nothing), far below them the scaled queries would.
 constexpr float MOST_CAP = 1.2676506e30f;  // 2^100
@@ -76,8 +77,8 @@ static int check_attention(const b200c_attention_t *a) {
   B200C_CHECK_ARG(a->dims >= 0 && a->dims <= AT_MAX_DIMS, "0 to 8 coordinates are supported");
   B200C_CHECK_ARG(a->m * a->heads <= (1ll << 33), "more than 2^33 rows of all heads are not supported");
   B200C_CHECK_ARG((a->ptr_q == nullptr) == (a->ptr_k == nullptr), "Input mismatch");
-  B200C_CHECK_ARG(a->ptr_q == nullptr ? a->num_segments == 1 : (a->num_segments >= 1 && a->num_segments <= MOST_ROWS),
-                  "Input mismatch");
+  B200C_CHECK_ARG(a->ptr_q == nullptr ? a->num_segments == 1 : a->num_segments >= 1, "Input mismatch");
+  B200C_CHECK_ARG(a->num_segments <= MOST_SEGMENTS, "more than 2^30 segments are not supported");
   B200C_CHECK_ARG(a->m == 0 || a->q, "null pointer");
   B200C_CHECK_ARG(a->n == 0 || (a->k && a->v), "null pointer");
   B200C_CHECK_ARG(a->dims == 0 || (a->slope && (a->m == 0 || a->pos_q) && (a->n == 0 || a->pos_k)), "null pointer");

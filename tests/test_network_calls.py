@@ -46,3 +46,14 @@ def test_attention_caps_and_scales_that_are_refused(changes, message):
     assert lib.b200c_attention_backward(ctypes.byref(a), p, None, p, p, p, p, p, None, 0, None) == 1
     assert message in lib.b200c_last_error()
     assert lib.b200c_attention_workspace_bytes(ctypes.byref(a)) == 0
+
+
+def test_attention_of_more_segments_than_can_be_bisected_is_refused():
+    from pytorch_cluster_b200 import _native
+
+    lib = _native.cabi()
+    a, p = attention_args(ptr_q=1 << 20, ptr_k=1 << 20, num_segments=(1 << 30) + 1), 1 << 20
+    assert lib.b200c_attention_forward(ctypes.byref(a), p, None, None, None, 0, None) == 1
+    assert b"2^30 segments" in lib.b200c_last_error()
+    assert lib.b200c_attention_backward(ctypes.byref(a), p, None, p, p, p, p, p, None, 0, None) == 1
+    assert b"2^30 segments" in lib.b200c_last_error()
