@@ -484,8 +484,13 @@ typedef struct {
  * The backward pass takes out, rest, lse and the gradient dout [m, heads, channels] (contiguous) and writes dq [m, heads,
  * channels] and dk, dv [n, groups, channels] (contiguous; dq or both of dk and dv may be NULL).  Positions and slopes are
  * constants.  Sums take no atomics: the same bits every time.  The tensor-core kernels' waits are bounded; if one ever ran
- * out, its block's rows would be NaN. */
+ * out, all that its block writes would be NaN, and the word below would be set. */
 size_t b200c_attention_workspace_bytes(const b200c_attention_t *a);
+/* Where kernels launched from now on set a 1 if a wait of theirs runs out: a word of pinned host memory that every device in
+ * use can write (cudaHostAlloc, portable and mapped), which outlives them and the graphs they are captured into, or NULL,
+ * the default.  One word for the process; the torch operators set one of their own and raise at the next call. */
+void b200c_attention_set_report(int32_t *word);
+int32_t *b200c_attention_report(void);
 int b200c_attention_forward(const b200c_attention_t *a, void *out, void *rest, float *lse, void *workspace,
                             size_t workspace_bytes, b200c_stream_t stream);
 size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a);

@@ -137,6 +137,10 @@ def cabi() -> ctypes.CDLL:
     lib.b200c_norm_rotate_workspace_bytes.restype = sz
     lib.b200c_norm_rotate_backward.argtypes = [p, p, p, i32, i32, i32, i32, f32, i32, p, sz, p]
     lib.b200c_norm_rotate_backward.restype = i32
+    lib.b200c_attention_set_report.argtypes = [p]
+    lib.b200c_attention_set_report.restype = None
+    lib.b200c_attention_report.argtypes = []
+    lib.b200c_attention_report.restype = ctypes.POINTER(ctypes.c_int32)
     lib.b200c_attention_workspace_bytes.argtypes = [p]
     lib.b200c_attention_workspace_bytes.restype = sz
     lib.b200c_attention_forward.argtypes = [p, p, p, p, p, sz, p]

@@ -39,6 +39,7 @@ struct AttnArgs {
   // forward, split over the columns: [m, heads, splits, channels + 2] (maximum, sum, result)
   float *parts = nullptr;
   int splits = 1;
+  int *report = nullptr;         // host memory, set to 1 where a bounded wait ran out; may be null
   int *order = nullptr;          // place for the tiles' order (attention_tensor_ordered), queries' and keys' in turn
   cudaStream_t stream = nullptr;
 };

@@ -428,6 +428,7 @@ attention_backward_kernel(const __grid_constant__ AtBackwardMaps maps, const __g
       }
     }
   }
+  if (*failed && tid == 0) t5_report(a.report);
   if (*failed && warp == COPY) {
     at_drain(&r_full, 1, 1);
     at_drain(full, F::STAGES, issued);

@@ -449,9 +449,15 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
     a.parts[((row * p.heads + head) * a.splits + blockIdx.z) * (p.channels + 2) + 1] = __int_as_float(0x7fffffff);
   } else if (*failed && element && grp == 0 && row < tile.t1) {
     // a wait ran out: nothing of this block is to be trusted
-    T *dst = (T *)a.out + (row * p.heads + head) * p.channels;
-    for (int c = 0; c < p.channels; ++c) dst[c] = at_round<T>(__int_as_float(0x7fffffff));
+    const float nan = __int_as_float(0x7fffffff);
+    const int64_t at = (row * p.heads + head) * p.channels;
+    for (int c = 0; c < p.channels; ++c) {
+      ((T *)a.out)[at + c] = at_round<T>(nan);
+      if (rest) rest[at + c] = at_round<T>(nan);
+    }
+    if (a.lse) a.lse[(int64_t)head * p.m + row] = nan;
   }
+  if (*failed && tid == 0) t5_report(a.report);
   if (*failed && warp == COPY) {
     at_drain(&q_full, 1, 1);
     at_drain(full, F::STAGES, issued);

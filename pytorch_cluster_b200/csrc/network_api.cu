@@ -1,6 +1,8 @@
 // extern "C" entry points of gather_rows, norm_rotate and attention: argument checks and kernel selection.
 #include <math.h>
 
+#include <atomic>
+
 #include "attention.cuh"
 #include "common.cuh"
 #include "launchers.h"
@@ -16,6 +18,8 @@ constexpr int64_t MOST_SEGMENTS = 1ll << 30;  // segments are bisected with 32-b
 // Scores are divided by the cap and multiplied by it again.  Far beyond them a quotient would leave the normal numbers of
 // fp32 (a cap that large bends nothing), far below them the scaled queries would.
 constexpr float MOST_CAP = 1.2676506e30f;  // 2^100
+
+static std::atomic<int32_t *> attention_report{nullptr};
 
 // what every workspace is carved from
 static bool aligned_workspace(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -157,6 +161,9 @@ extern "C" int b200c_norm_rotate_backward(const b200c_norm_rotate_side_t *q, con
   return launch_norm_rotate(a, false, (float *)workspace);
 }
 
+extern "C" void b200c_attention_set_report(int32_t *word) { attention_report.store(word); }
+extern "C" int32_t *b200c_attention_report(void) { return attention_report.load(); }
+
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 extern "C" size_t b200c_attention_workspace_bytes(const b200c_attention_t *a) {
@@ -186,6 +193,7 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
   a.rest = rest;
   a.lse = lse;
   a.stream = (cudaStream_t)stream;
+  a.report = attention_report.load();
   const int splits = attention_few_splits(*p);
   if (splits > 0) return launch_attention_few(a, splits, workspace);
   if (attention_tensor_applicable(*p) && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0) {
@@ -231,6 +239,7 @@ extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *
   a.dk = dk;
   a.dv = dv;
   a.stream = (cudaStream_t)stream;
+  a.report = attention_report.load();
   float *norms = (float *)((char *)workspace + align256((size_t)p->m * p->heads * 4));
   a.norms = norms;
   if (attention_tensor_order_bytes(*p) > 0) a.order = (int *)((char *)norms + align256(attention_norms_bytes(*p) + 1));

@@ -84,6 +84,13 @@ __device__ __forceinline__ bool t5_mbar_wait_warp(uint64_t *bar, uint32_t parity
   return __all_sync(FULL_MASK, t5_mbar_wait(bar, parity, failed));
 }
 
+// tells the host that a wait of this block ran out
+__device__ __forceinline__ void t5_report(int *word) {
+  if (word == nullptr) return;
+  *(volatile int *)word = 1;
+  __threadfence_system();
+}
+
 // two barriers at once (the second only if `second`): where both are over already, one round trip instead of two
 __device__ __forceinline__ bool t5_mbar_wait_both(uint64_t *a, uint32_t pa, uint64_t *b, uint32_t pb, bool second,
                                                   volatile int *failed) {

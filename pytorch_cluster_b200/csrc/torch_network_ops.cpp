@@ -306,6 +306,29 @@ std::tuple<torch::Tensor, torch::Tensor> norm_rotate(torch::Tensor q, torch::Ten
 
 // ---- attention -----------------------------------------------------------------------------------------------------
 
+// The word in which a kernel says that a bounded wait of its ran out: read before each call, never waited for.  A caller
+// of the C ABI who has set one of their own keeps it.
+void check_waits() {
+  static int32_t *const word = [] {
+    int32_t *mine = b200c_attention_report();
+    if (mine != nullptr) return mine;
+    void *p = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // a first call may be a captured one
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t error = cudaHostAlloc(&p, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped);
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    C10_CUDA_CHECK(error);
+    mine = static_cast<int32_t *>(p);
+    *mine = 0;
+    b200c_attention_set_report(mine);
+    return mine;
+  }();
+  volatile int32_t *seen = word;
+  if (*seen == 0) return;
+  *seen = 0;
+  TORCH_CHECK(false, "b200_cluster: a bounded wait of an earlier attention call ran out; its rows are NaN");
+}
+
 struct Attention {
   torch::Tensor q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope;
   b200c_attention_t a{};
@@ -379,6 +402,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_forward(
   OpRange range("torch_cluster::attention_forward");
   CHECK_CUDA(q);
   c10::cuda::CUDAGuard guard(q.device());
+  check_waits();
   Attention t;
   prepare_attention(t, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap);
   auto out = torch::empty(q.sizes(), q.options());
@@ -402,6 +426,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> attention_backward(
   at::NoGradGuard no_grad;
   CHECK_CUDA(q);
   c10::cuda::CUDAGuard guard(q.device());
+  check_waits();
   Attention t;
   prepare_attention(t, q, k, v, ptr_q, ptr_k, pos_q, pos_k, slope, scale, cap);
   CHECK_INPUT(dout.sizes() == q.sizes() && out.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&

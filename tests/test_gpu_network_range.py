@@ -186,3 +186,31 @@ def test_caps_and_scales_beyond_32_bits_are_refused(dtype):
     for cap in (1e30, 1e-29):
         got = pc.attention(h, h, h, cap=cap)
         assert_close(got, *attention_plain(h, h, h, [70], [70], cap=cap)["out"], cap)
+
+
+# ---- waits that run out ----------------------------------------------------------------------------------------
+
+def test_a_wait_that_ran_out_is_reported_at_the_next_call():
+    """The kernels' part, setting the word, takes a hang; here the host sets it."""
+    import pytorch_cluster_b200 as pc
+    from pytorch_cluster_b200 import _native
+
+    h = rand(gen(60), 300, 2, 64, dtype=torch.bfloat16).requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    out = pc.attention(h, h, h)
+    word = _native.cabi().b200c_attention_report()
+    assert word and word[0] == 0
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="wait"):
+        pc.attention(h, h, h)
+    word[0] = 1
+    with pytest.raises(RuntimeError, match="wait"):
+        torch.autograd.grad(out.sum(), h, retain_graph=True)
+    # said once, and nothing else has changed
+    torch.autograd.grad(out.sum(), h)
+    with torch.no_grad():
+        want = pc.attention(h, h, h)
+        with torch.cuda.graph(graph):
+            again = pc.attention(h, h, h)
+    graph.replay()
+    assert torch.equal(again, want) and word[0] == 0

@@ -57,3 +57,15 @@ def test_attention_of_more_segments_than_can_be_bisected_is_refused():
     assert b"2^30 segments" in lib.b200c_last_error()
     assert lib.b200c_attention_backward(ctypes.byref(a), p, None, p, p, p, p, p, None, 0, None) == 1
     assert b"2^30 segments" in lib.b200c_last_error()
+
+
+def test_the_word_that_waits_report_to():
+    from pytorch_cluster_b200 import _native
+
+    lib = _native.cabi()
+    before = lib.b200c_attention_report()
+    word = ctypes.c_int32(0)
+    lib.b200c_attention_set_report(ctypes.byref(word))
+    assert ctypes.addressof(lib.b200c_attention_report().contents) == ctypes.addressof(word)
+    lib.b200c_attention_set_report(before)
+    assert bool(lib.b200c_attention_report()) == bool(before)
