@@ -13,14 +13,18 @@ def _segments(batch_q: Optional[torch.Tensor], batch_k: Optional[torch.Tensor], 
         return None, None
     assert batch_q is not None and batch_k is not None
     assert batch_q.numel() == rows_q and batch_k.numel() == rows_k
-    if batch_size is None:
-        batch_size = 1
-        for batch in (batch_q,) if batch_q is batch_k else (batch_q, batch_k):
-            if batch.numel() > 0:
-                batch_size = max(batch_size, torch.ops.torch_cluster.batch_info(batch)[0])
-    assert batch_size > 0
-    ptr_q = torch.ops.torch_cluster.segment_ptr(batch_q, batch_size)
-    return ptr_q, ptr_q if batch_q is batch_k else torch.ops.torch_cluster.segment_ptr(batch_k, batch_size)
+    same = batch_q is batch_k
+    examples = 1
+    if batch_size is not None:
+        examples = batch_size
+    else:
+        if batch_q.numel() > 0:
+            examples = max(examples, torch.ops.torch_cluster.batch_info(batch_q)[0])
+        if not same and batch_k.numel() > 0:
+            examples = max(examples, torch.ops.torch_cluster.batch_info(batch_k)[0])
+    assert examples > 0
+    ptr_q = torch.ops.torch_cluster.segment_ptr(batch_q, examples)
+    return ptr_q, ptr_q if same else torch.ops.torch_cluster.segment_ptr(batch_k, examples)
 
 
 def _places(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -71,7 +75,7 @@ def attention(
             raise RuntimeError("Input mismatch")
     if scale is None:
         scale = float(q.size(-1)) ** -0.5 if q.size(-1) > 0 else 1.0
-    if cap is not None and not 0 < cap < float("inf"):
+    if cap is not None and not (cap > 0.0 and cap < float("inf")):
         raise ValueError("`cap` needs to be positive and finite")
     if (pos_q is None) != (pos_k is None) or (pos_q is None) != (slope is None):
         raise ValueError("`pos_q`, `pos_k` and `slope` come together")

@@ -11,6 +11,15 @@ def _constant(name: str, t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _position(name: str, p: torch.Tensor) -> torch.Tensor:
+    p = _constant(name, p)
+    if not p.is_floating_point():
+        p = p.double()
+    elif p.dtype != torch.float32 and p.dtype != torch.float64:
+        p = p.float()
+    return p.view(-1, 1) if p.dim() == 1 else p
+
+
 def norm_rotate(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -43,22 +52,13 @@ def norm_rotate(
     if not q.is_cuda:
         raise RuntimeError("q must be CUDA tensor")
     same = pos_q is pos_k
-    pos = []
-    for name, p in (("pos_q", pos_q), ("pos_k", pos_k)):
-        p = _constant(name, p)
-        if not p.is_floating_point():
-            p = p.double()
-        elif p.dtype not in (torch.float32, torch.float64):
-            p = p.float()
-        pos.append(p.view(-1, 1) if p.dim() == 1 else p)
-        if same:
-            pos.append(pos[0])
-            break
-    if pos[0].dtype != pos[1].dtype:
-        pos = [p.double() for p in pos]
+    pos_q = _position("pos_q", pos_q)
+    pos_k = pos_q if same else _position("pos_k", pos_k)
+    if pos_q.dtype != pos_k.dtype:
+        pos_q, pos_k = pos_q.double(), pos_k.double()
     _constant("freq", freq)
     if weight_q is not None:
         weight_q = weight_q.float()
     if weight_k is not None:
         weight_k = weight_k.float()
-    return torch.ops.torch_cluster.norm_rotate(q, k, pos[0], pos[1], freq, weight_q, weight_k, float(eps))
+    return torch.ops.torch_cluster.norm_rotate(q, k, pos_q, pos_k, freq, weight_q, weight_k, float(eps))

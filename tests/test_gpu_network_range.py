@@ -214,3 +214,22 @@ def test_a_wait_that_ran_out_is_reported_at_the_next_call():
             again = pc.attention(h, h, h)
     graph.replay()
     assert torch.equal(again, want) and word[0] == 0
+
+
+# ---- scripted --------------------------------------------------------------------------------------------------
+
+def test_scripted_functions_give_the_same():
+    import pytorch_cluster_b200 as pc
+
+    g = gen(57)
+    h, b = rand(g, 50, 2, 32, dtype=torch.bfloat16), ids([20, 30])
+    pos, slope = rand(g, 50, 3, dtype=torch.float32), torch.tensor([1.0, 0.5], device="cuda")
+    freq = rand(g, 3, 16, dtype=torch.float32)
+    attention, rotate, gather = (torch.jit.script(f) for f in (pc.attention, pc.norm_rotate, pc.gather_rows))
+    assert torch.equal(attention(h, h, h, b, b, pos, pos, slope), pc.attention(h, h, h, b, b, pos, pos, slope))
+    assert torch.equal(attention(h, h, h, cap=3.0), pc.attention(h, h, h, cap=3.0))
+    for places in ((pos, pos), (pos, pos.double()), (pos[:, 0], pos[:, 0].clone())):
+        f = freq if places[0].dim() == 2 else freq[:1]
+        assert all(torch.equal(x, y) for x, y in zip(rotate(h, h, *places, f), pc.norm_rotate(h, h, *places, f)))
+    edges = torch.tensor([3, 1, 49], device="cuda")
+    assert torch.equal(gather(h[:, 0], edges, 2.0), pc.gather_rows(h[:, 0], edges, 2.0))

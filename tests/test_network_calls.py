@@ -69,3 +69,14 @@ def test_the_word_that_waits_report_to():
     assert ctypes.addressof(lib.b200c_attention_report().contents) == ctypes.addressof(word)
     lib.b200c_attention_set_report(before)
     assert bool(lib.b200c_attention_report()) == bool(before)
+
+
+def test_functions_can_be_scripted():
+    import pytorch_cluster_b200 as pc
+
+    h = torch.rand(4, 2, 8)
+    pos, freq = torch.rand(4, 2), torch.rand(2, 4)
+    for f, args in ((pc.gather_rows, (h[:, 0], torch.tensor([0]))), (pc.norm_rotate, (h, h, pos, pos, freq)),
+                    (pc.attention, (h, h, h))):
+        with pytest.raises(torch.jit.Error, match="must be CUDA tensor"):
+            torch.jit.script(f)(*args)
