@@ -9,11 +9,28 @@
 namespace b200c {
 
 // ---- segment pointers ----------------------------------------------------------------------------
-// ptr[i] = lower_bound(batch, i) (torch.bucketize(arange(B + 1), batch), torch_cluster/knn.py:77-79): a warp per
-// boundary looks at 32 places at a time, so that a million rows take four dependent loads instead of twenty (21 -> 12 us
-// for two vectors of 32 clouds, the larger of 1 M rows).
-__global__ void segment_ptr_kernel(const int64_t *__restrict__ batch, int64_t n, int64_t num_segments,
-                                   int64_t *__restrict__ ptr) {
+// ptr[i] = lower_bound(batch, i) (torch.bucketize(arange(B + 1), batch), torch_cluster/knn.py:77-79).  Up to
+// SEGMENT_PTR_WARPS examples a warp per boundary looks at 32 places at a time, so that a million rows take four dependent
+// loads instead of twenty; beyond that the threads cost more than the loads, and one bisects per boundary.  Measured on
+// 1000000 rows, thread / warp per boundary in us, from memory: 32 examples 16.4 / 9.2, 8192 16.4 / 10.3, 16384 16.4 / 12.5
+// (9.5 / 11.0 from the caches), 65536 16.4 / 24.6, 2000000 49 / 479.
+constexpr int64_t SEGMENT_PTR_WARPS = 16384;
+__global__ void segment_ptr_thread_kernel(const int64_t *__restrict__ batch, int64_t n, int64_t num_segments,
+                                          int64_t *__restrict__ ptr) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i > num_segments) return;
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (batch[mid] < i)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  ptr[i] = lo;
+}
+__global__ void segment_ptr_warp_kernel(const int64_t *__restrict__ batch, int64_t n, int64_t num_segments,
+                                        int64_t *__restrict__ ptr) {
   const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (i > num_segments) return;
@@ -327,8 +344,12 @@ extern "C" int b200c_segment_ptr(const int64_t *batch, int64_t n, int64_t num_se
   B200C_CHECK_ARG(ptr != nullptr && (batch != nullptr || n == 0), "null pointer");
   const int64_t total = num_segments + 1;
   const int threads = 128;
-  segment_ptr_kernel<<<(unsigned)((total * 32 + threads - 1) / threads), threads, 0, (cudaStream_t)stream>>>(
-      batch, n, num_segments, ptr);
+  if (num_segments <= SEGMENT_PTR_WARPS)
+    segment_ptr_warp_kernel<<<(unsigned)((total * 32 + threads - 1) / threads), threads, 0, (cudaStream_t)stream>>>(
+        batch, n, num_segments, ptr);
+  else
+    segment_ptr_thread_kernel<<<(unsigned)((total + threads - 1) / threads), threads, 0, (cudaStream_t)stream>>>(
+        batch, n, num_segments, ptr);
   B200C_LAUNCH_CHECK("segment_ptr_kernel");
   return B200C_OK;
 }

@@ -233,3 +233,16 @@ def test_scripted_functions_give_the_same():
         assert all(torch.equal(x, y) for x, y in zip(rotate(h, h, *places, f), pc.norm_rotate(h, h, *places, f)))
     edges = torch.tensor([3, 1, 49], device="cuda")
     assert torch.equal(gather(h[:, 0], edges, 2.0), pc.gather_rows(h[:, 0], edges, 2.0))
+
+
+# ---- segment pointers ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows, segments", [(0, 1), (1, 1), (33, 5), (1000, 4000), (100000, 7), (100000, 3000),
+                                            (70001, 200000), (1000003, 65536), (3000, 100000),
+                                            (50000, 16384), (50000, 16385)])
+def test_segment_pointers_of_few_and_many_examples(rows, segments):
+    g = gen(58)
+    batch = torch.randint(0, segments, (rows,), generator=g, device="cuda").sort().values
+    for shift in (0, -segments // 3, segments // 3):  # ids below zero and at or above the number of examples
+        got = torch.ops.torch_cluster.segment_ptr(batch + shift, segments)
+        assert torch.equal(got, torch.searchsorted(batch + shift, torch.arange(segments + 1, device="cuda")))
