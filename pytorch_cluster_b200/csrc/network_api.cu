@@ -14,6 +14,7 @@ int check_device();  // api.cu
 static bool is_network_type(int dtype) { return dtype == B200C_F32 || dtype == B200C_F16 || dtype == B200C_BF16; }
 static size_t elem_bytes(int dtype) { return dtype == B200C_F32 ? 4 : 2; }
 constexpr int64_t MOST_ROWS = 0x7fffffffLL;
+constexpr int64_t MOST_GATHER_CHANNELS = 65536;
 constexpr int64_t MOST_SEGMENTS = 1ll << 30;  // segments are bisected with 32-bit numbers
 // Scores are divided by the cap and multiplied by it again.  Far beyond them a quotient would leave the normal numbers of
 // fp32 (a cap that large bends nothing), far below them the scaled queries would.
@@ -29,7 +30,7 @@ static int check_gather(const void *in, const int64_t *index, int64_t rows, int6
   B200C_CHECK_ARG(is_network_type(dtype), "unsupported dtype");
   B200C_CHECK_ARG(rows >= 0 && edges >= 0 && channels >= 1, "Input mismatch");
   B200C_CHECK_ARG(rows <= MOST_ROWS && edges <= MOST_ROWS, "more than 2^31-1 rows or edges are not supported");
-  B200C_CHECK_ARG(channels <= 65536, "more than 65536 channels are not supported");
+  B200C_CHECK_ARG(channels <= MOST_GATHER_CHANNELS, "more than 65536 channels are not supported");
   B200C_CHECK_ARG((edges == 0 || index != nullptr) && (rows == 0 || edges == 0 || (in != nullptr && out != nullptr)),
                   "null pointer");
   const uintptr_t mask = elem_bytes(dtype) - 1;
@@ -107,6 +108,8 @@ extern "C" int b200c_gather_rows(const void *x, const int64_t *index, int64_t ro
 }
 
 extern "C" size_t b200c_gather_rows_workspace_bytes(int64_t rows, int64_t edges, int64_t channels) {
+  if (rows < 0 || edges <= 0 || channels < 1 || rows > MOST_ROWS || edges > MOST_ROWS || channels > MOST_GATHER_CHANNELS)
+    return 0;  // such calls are refused, or need none
   return gather_rows_workspace_bytes(rows, edges, channels);
 }
 
@@ -139,7 +142,9 @@ extern "C" int b200c_norm_rotate(const b200c_norm_rotate_side_t *q, const b200c_
   return launch_norm_rotate(a, true, nullptr);
 }
 
-extern "C" size_t b200c_norm_rotate_workspace_bytes(int channels) { return norm_rotate_workspace_bytes(channels); }
+extern "C" size_t b200c_norm_rotate_workspace_bytes(int channels) {
+  return channels < 2 || channels > 256 ? 0 : norm_rotate_workspace_bytes(channels);
+}
 
 extern "C" int b200c_norm_rotate_backward(const b200c_norm_rotate_side_t *q, const b200c_norm_rotate_side_t *k,
                                           const void *freq, int dims, int channels, int pos_f64, int freq_f64, float eps,

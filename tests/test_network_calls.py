@@ -80,3 +80,16 @@ def test_functions_can_be_scripted():
                     (pc.attention, (h, h, h))):
         with pytest.raises(torch.jit.Error, match="must be CUDA tensor"):
             torch.jit.script(f)(*args)
+
+
+def test_workspaces_of_sizes_that_are_refused_are_empty():
+    from pytorch_cluster_b200 import _native
+
+    lib = _native.cabi()
+    far = (1 << 63) - 1
+    for rows, edges, channels in ((far, 10, 8), (1 << 31, 10, 8), (-1, 10, 8), (10, -1, 8), (10, far, 8), (10, 1 << 31, 8),
+                                  (10, 10, 0), (10, 10, -8), (10, 10, 65537), (10, 0, 8)):
+        assert lib.b200c_gather_rows_workspace_bytes(rows, edges, channels) == 0, (rows, edges, channels)
+    assert lib.b200c_gather_rows_workspace_bytes(10, 10, 8) > 0
+    assert lib.b200c_norm_rotate_workspace_bytes(-2) == 0 and lib.b200c_norm_rotate_workspace_bytes(258) == 0
+    assert lib.b200c_norm_rotate_workspace_bytes(256) > 0
