@@ -422,8 +422,9 @@ int b200c_fps_large_segment(const void *src, int64_t seg_lo, int64_t seg_points,
                             int32_t *status, b200c_stream_t stream);
 
 /* ---- What a network does next with the same batch vectors, coordinates and edges -----------------------------
- * These have no counterpart in the reference.  Workspaces are 16-byte aligned.  Types: B200C_F32, B200C_F16, B200C_BF16; sums, softmax statistics
- * and norms are held in 32 bits and each result is rounded once. */
+ * These have no counterpart in the reference.  Workspaces are 16-byte aligned; the size of one for arguments that a call
+ * refuses is 0.  Types: B200C_F32, B200C_F16, B200C_BF16; sums, softmax statistics and norms are held in 32 bits and each
+ * result is rounded once. */
 
 /* Rows by index, scaled: out[e] = scale * x[index[e]] (x [rows, channels], out [edges, channels], contiguous).  An
  * index outside [0, rows) is padding, as the -1 of b200c_knn's padded form is: it gives a row of zeros. */

@@ -40,7 +40,7 @@ struct AttnArgs {
   float *parts = nullptr;
   int splits = 1;
   int *report = nullptr;         // host memory, set to 1 where a bounded wait ran out; may be null
-  int *order = nullptr;          // place for the tiles' order (attention_tensor_ordered), queries' and keys' in turn
+  int *order = nullptr;          // place for the tiles' order (attention_tensor_order_bytes), queries' and keys' in turn
   cudaStream_t stream = nullptr;
 };
 

@@ -234,7 +234,7 @@ __device__ __forceinline__ void at_clear(unsigned char *tile, int count, int tid
       reinterpret_cast<uint4 *>(tile + a * (AT_COLS * 128) + count * 128)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// Stages of a pass: `heads` walks over `count` columns.
+// Stages of one walk over `count` columns.
 __device__ __forceinline__ uint32_t at_stages(int64_t count) { return (uint32_t)((count + AT_COLS - 1) / AT_COLS); }
 
 // The place in a ring of stages, with the parity of its current round.
