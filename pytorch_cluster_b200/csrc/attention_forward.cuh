@@ -130,14 +130,18 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   bool by_example = false;
   int64_t next_row = tile.t0;
   AtPass pass = tile.all(shared_tile);
-  // this block's share of a pass's columns, in whole stages
+  // What of the pass lies in this block's share of the tile's columns (whole stages).  The share is that of the whole tile
+  // in a pass over one example too: each block decides by itself whether it goes example by example, and the others'
+  // columns must not depend on that.
   auto share = [&]() {
     if (a.splits <= 1) return;
+    const AtPass all = tile.all(shared_tile);
     const int64_t unit = (int64_t)a.splits * AT_COLS;
-    const int64_t each = (pass.c_hi - pass.c_lo + unit - 1) / unit * AT_COLS;
-    pass.c_lo += each * blockIdx.z;
-    if (pass.c_lo > pass.c_hi) pass.c_lo = pass.c_hi;
-    if (pass.c_lo + each < pass.c_hi) pass.c_hi = pass.c_lo + each;
+    const int64_t each = (all.c_hi - all.c_lo + unit - 1) / unit * AT_COLS;
+    const int64_t from = all.c_lo + each * blockIdx.z;
+    if (pass.c_lo < from) pass.c_lo = from;
+    if (pass.c_hi > from + each) pass.c_hi = from + each;
+    if (pass.c_hi < pass.c_lo) pass.c_hi = pass.c_lo;
   };
   share();
   const bool mixed = tile.b_first != tile.b_last;

@@ -246,3 +246,34 @@ def test_segment_pointers_of_few_and_many_examples(rows, segments):
     for shift in (0, -segments // 3, segments // 3):  # ids below zero and at or above the number of examples
         got = torch.ops.torch_cluster.segment_ptr(batch + shift, segments)
         assert torch.equal(got, torch.searchsorted(batch + shift, torch.arange(segments + 1, device="cuda")))
+
+
+# ---- small calls, split over the columns -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens_q, lens_k", [([300, 500, 400], [300, 500, 400]), ([40, 30, 50], [700, 900, 300]),
+                                            ([90, 0, 20], [400, 600, 800])])
+@pytest.mark.parametrize("channels, dims", [(64, 0), (128, 3)])
+def test_attention_split_over_columns_keeps_nan_in_its_example(dtype, lens_q, lens_k, channels, dims):
+    import pytorch_cluster_b200 as pc
+
+    g = gen(61)
+    after = 70  # rows of no example
+    bq, bk = ids([*lens_q, after]), ids([*lens_k, after])
+    m, n = sum(lens_q), sum(lens_k)
+    q, k, v = (rand(g, r + after, 2, channels, dtype=dtype) for r in (m, n, n))
+    extra = {}
+    if dims:
+        extra = dict(pos_q=rand(g, m + after, dims, dtype=torch.float32), pos_k=rand(g, n + after, dims, dtype=torch.float32),
+                     slope=torch.tensor([1.0, 0.3], device="cuda"))
+    rows = {name: t[:m] if name == "pos_q" else t[:n] if name == "pos_k" else t for name, t in extra.items()}
+    want, tol = attention_plain(q[:m], k[:n], v[:n], lens_q, lens_k, **rows)["out"]
+    for bad_example in (0, 1, 2, 3):
+        for value in (math.nan, math.inf):
+            v2, k2 = v.clone(), k.clone()
+            at = (bk == bad_example).nonzero().flatten()
+            v2[at[::50]], k2[at[::70]] = value, value
+            out = pc.attention(q, k2, v2, bq, bk, batch_size=3, **extra)
+            keep = (bq != bad_example)[:m]
+            assert_close(out[:m][keep], want[keep], tol[keep], (bad_example, value))
+            assert (out[m:] == 0).all()
