@@ -130,20 +130,18 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
   bool by_example = false;
   int64_t next_row = tile.t0;
   AtPass pass = tile.all(shared_tile);
-  // What of the pass lies in this block's share of the tile's columns (whole stages).  The share is that of the whole tile
-  // in a pass over one example too: each block decides by itself whether it goes example by example, and the others'
-  // columns must not depend on that.
-  auto share = [&]() {
-    if (a.splits <= 1) return;
-    const AtPass all = tile.all(shared_tile);
+  // This block's share of the tile's columns, in whole stages.  A pass over one example takes what of it lies in the share
+  // of the whole tile: each block decides by itself whether it goes example by example, and the others' columns must not
+  // depend on that.
+  __shared__ int64_t share_s[2];
+  if (a.splits > 1) {
     const int64_t unit = (int64_t)a.splits * AT_COLS;
-    const int64_t each = (all.c_hi - all.c_lo + unit - 1) / unit * AT_COLS;
-    const int64_t from = all.c_lo + each * blockIdx.z;
-    if (pass.c_lo < from) pass.c_lo = from;
-    if (pass.c_hi > from + each) pass.c_hi = from + each;
-    if (pass.c_hi < pass.c_lo) pass.c_hi = pass.c_lo;
-  };
-  share();
+    const int64_t each = (pass.c_hi - pass.c_lo + unit - 1) / unit * AT_COLS;
+    pass.c_lo += each * blockIdx.z;
+    if (pass.c_lo > pass.c_hi) pass.c_lo = pass.c_hi;
+    if (pass.c_lo + each < pass.c_hi) pass.c_hi = pass.c_lo + each;
+    if (tid == 0) share_s[0] = pass.c_lo, share_s[1] = pass.c_hi;  // read after a barrier, at the end of this pass
+  }
   const bool mixed = tile.b_first != tile.b_last;
   uint32_t stage0 = 0, passes = 0;  // stages, and passes with any, so far
   uint32_t issued = 0;              // copy warp: stages whose copies were issued
@@ -447,7 +445,11 @@ attention_forward_kernel(const __grid_constant__ AtForwardMaps maps, const __gri
       by_example = true;
     }
     if (!tile.next(next_row, pass)) break;
-    share();
+    if (a.splits > 1) {
+      if (pass.c_lo < share_s[0]) pass.c_lo = share_s[0];
+      if (pass.c_hi > share_s[1]) pass.c_hi = share_s[1];
+      if (pass.c_hi < pass.c_lo) pass.c_hi = pass.c_lo;
+    }
   }
   if (*failed && element && grp == 0 && row < tile.t1 && a.splits > 1) {
     a.parts[((row * p.heads + head) * a.splits + blockIdx.z) * (p.channels + 2) + 1] = __int_as_float(0x7fffffff);
