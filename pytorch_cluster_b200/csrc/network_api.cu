@@ -2,6 +2,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <initializer_list>
 
 #include "attention.cuh"
 #include "common.cuh"
@@ -24,6 +25,12 @@ static std::atomic<int32_t *> attention_report{nullptr};
 
 // what every workspace is carved from
 static bool aligned_workspace(const void *p) { return ((uintptr_t)p & 15) == 0; }
+// whether all pointers lie at multiples of their elements
+static bool aligned_to(size_t bytes, std::initializer_list<const void *> pointers) {
+  for (const void *p : pointers)
+    if ((uintptr_t)p & (bytes - 1)) return false;
+  return true;
+}
 
 static int check_gather(const void *in, const int64_t *index, int64_t rows, int64_t edges, int64_t channels, int dtype,
                         const void *out) {
@@ -33,9 +40,7 @@ static int check_gather(const void *in, const int64_t *index, int64_t rows, int6
   B200C_CHECK_ARG(channels <= MOST_GATHER_CHANNELS, "more than 65536 channels are not supported");
   B200C_CHECK_ARG((edges == 0 || index != nullptr) && (rows == 0 || edges == 0 || (in != nullptr && out != nullptr)),
                   "null pointer");
-  const uintptr_t mask = elem_bytes(dtype) - 1;
-  B200C_CHECK_ARG(((uintptr_t)in & mask) == 0 && ((uintptr_t)out & mask) == 0 && ((uintptr_t)index & 7) == 0,
-                  "misaligned pointer");
+  B200C_CHECK_ARG(aligned_to(elem_bytes(dtype), {in, out}) && aligned_to(8, {index}), "misaligned pointer");
   return check_device();
 }
 
@@ -46,6 +51,7 @@ static int check_rotate(const b200c_norm_rotate_side_t *q, const b200c_norm_rota
   B200C_CHECK_ARG(is_network_type(dtype), "unsupported dtype");
   B200C_CHECK_ARG(channels >= 2 && channels <= 256 && channels % 2 == 0, "channels must be even and at most 256");
   B200C_CHECK_ARG(dims >= 1 && dims <= 8, "1 to 8 coordinates are supported");
+  B200C_CHECK_ARG(aligned_to(freq_f64 ? 8 : 4, {freq}), "misaligned pointer");
   const b200c_norm_rotate_side_t *sides[2] = {q, k};
   for (int i = 0; i < 2; ++i) {
     const b200c_norm_rotate_side_t &s = *sides[i];
@@ -54,7 +60,11 @@ static int check_rotate(const b200c_norm_rotate_side_t *q, const b200c_norm_rota
     if (s.rows > 0) {
       B200C_CHECK_ARG(s.x && s.pos, "null pointer");
       B200C_CHECK_ARG(forward ? s.y != nullptr : (s.dy && s.dx), "null pointer");
+      B200C_CHECK_ARG(aligned_to(elem_bytes(dtype), {s.x, forward ? s.y : s.dx, forward ? nullptr : s.dy}) &&
+                          aligned_to(pos_f64 ? 8 : 4, {s.pos}),
+                      "misaligned pointer");
     }
+    B200C_CHECK_ARG(aligned_to(4, {s.weight, forward ? nullptr : s.dweight}), "misaligned pointer");
     a.side[i] = s;
     if (s.rows == 0) a.side[i].x = a.side[i].y = a.side[i].dx = nullptr, a.side[i].dy = nullptr;
     a.dweight[i] = forward ? nullptr : s.dweight;
@@ -90,8 +100,9 @@ static int check_attention(const b200c_attention_t *a) {
   B200C_CHECK_ARG(isfinite(a->scale) && isfinite(a->cap), "scale and cap must be finite numbers");
   B200C_CHECK_ARG(!(a->cap > 0.f) || (a->cap <= MOST_CAP && fabsf(a->scale) <= MOST_CAP * a->cap),
                   "cap must lie between 2^-100 of scale and 2^100");
-  const uintptr_t mask = elem_bytes(a->dtype) - 1;
-  B200C_CHECK_ARG((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & mask) == 0, "misaligned pointer");
+  B200C_CHECK_ARG(aligned_to(elem_bytes(a->dtype), {a->q, a->k, a->v}) && aligned_to(8, {a->ptr_q, a->ptr_k}) &&
+                      (a->dims == 0 || aligned_to(4, {a->pos_q, a->pos_k, a->slope})),
+                  "misaligned pointer");
   return B200C_OK;
 }
 
@@ -185,6 +196,7 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
   int st = check_attention(p);
   if (st != B200C_OK) return st;
   B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
+  B200C_CHECK_ARG(aligned_to(elem_bytes(p->dtype), {out, rest}) && aligned_to(4, {lse}), "misaligned pointer");
   if ((st = check_device()) != B200C_OK || p->m == 0) return st;
   B200C_CHECK_ARG(out != nullptr, "null output pointer");
   const size_t need = b200c_attention_workspace_bytes(p);
@@ -225,6 +237,8 @@ extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *
   int st = check_attention(p);
   if (st != B200C_OK) return st;
   B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
+  B200C_CHECK_ARG(aligned_to(elem_bytes(p->dtype), {out, rest, dout, dq, dk, dv}) && aligned_to(4, {lse}),
+                  "misaligned pointer");
   if ((st = check_device()) != B200C_OK) return st;
   B200C_CHECK_ARG(p->m == 0 || (out && lse && dout), "null pointer");
   B200C_CHECK_ARG((dk == nullptr) == (dv == nullptr), "dk and dv come together");

@@ -4,7 +4,7 @@ import math
 
 import pytest
 import torch
-from test_network_refusals import attention_args
+from test_network_refusals import Side, attention_args
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -93,3 +93,39 @@ def test_workspaces_of_sizes_that_are_refused_are_empty():
     assert lib.b200c_gather_rows_workspace_bytes(10, 10, 8) > 0
     assert lib.b200c_norm_rotate_workspace_bytes(-2) == 0 and lib.b200c_norm_rotate_workspace_bytes(258) == 0
     assert lib.b200c_norm_rotate_workspace_bytes(256) > 0
+
+
+@pytest.mark.parametrize("dtype", [0, 2, 3])  # fp32, fp16, bf16
+def test_pointers_between_two_elements_are_refused(dtype):
+    from pytorch_cluster_b200 import _native
+
+    lib = _native.cabi()
+    p, odd = 1 << 20, (1 << 20) + 1  # never followed
+
+    def refused(status):
+        assert status == 1 and b"misaligned" in lib.b200c_last_error()
+
+    for name in ("q", "k", "v", "ptr_q", "ptr_k", "pos_q", "pos_k", "slope"):
+        a = attention_args(**{**dict(dtype=dtype, dims=2, ptr_q=p, ptr_k=p, pos_q=p, pos_k=p, slope=p), name: odd})
+        refused(lib.b200c_attention_forward(ctypes.byref(a), p, None, None, None, 0, None))
+        refused(lib.b200c_attention_backward(ctypes.byref(a), p, None, p, p, p, p, p, None, 0, None))
+    a = ctypes.byref(attention_args(dtype=dtype))
+    for i in range(3):
+        refused(lib.b200c_attention_forward(a, *(odd if i == j else p for j in range(3)), None, 0, None))
+    for i in range(7):
+        refused(lib.b200c_attention_backward(a, *(odd if i == j else p for j in range(7)), None, 0, None))
+
+    def rotate(direction, side={}, freq=p, **flags):
+        s = Side(**{**dict(x=p, rows=4, row_stride=8, head_stride=8, heads=1, pos=p, weight=p, y=p, dy=p, dx=p, dweight=p),
+                    **side})
+        args = (ctypes.byref(s), ctypes.byref(s), freq, 1, 8, flags.get("pos_f64", 0), flags.get("freq_f64", 0), 1e-6, dtype)
+        return lib.b200c_norm_rotate(*args, None) if direction == "forward" else \
+            lib.b200c_norm_rotate_backward(*args, None, 0, None)
+
+    for direction, names in (("forward", ("x", "pos", "weight", "y")),
+                             ("backward", ("x", "pos", "weight", "dy", "dx", "dweight"))):
+        for name in names:
+            refused(rotate(direction, {name: odd}))
+        refused(rotate(direction, freq=odd))
+        refused(rotate(direction, {"pos": p + 4}, pos_f64=1))
+        refused(rotate(direction, freq=p + 4, freq_f64=1))
