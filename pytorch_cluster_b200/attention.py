@@ -63,7 +63,7 @@ def attention(
         scale: of the dot products, a finite number, ``C ** -0.5`` by default.
         cap: a positive number between ``2 ** -100`` of the scale's size and ``2 ** 100``, or None.
         batch_size: the number of examples; skips its inference and the host reads that takes (needed under stream
-            capture).  Rows with ids at or above it belong to no example.
+            capture).  Rows with ids at or above it belong to no example: zeros, without a gradient.
 
     Returns ``[M, H, C]``.  A query without keys gives zeros.  A few queries over many keys (pooling by a
     learned query, one new token) are split over the keys and joined.

@@ -7,7 +7,8 @@
 // P and dS enter the second products in the 16-bit type.  dq takes dS in two parts, rounded and what rounding left,
 // because the rows of dS sum to zero and a rounded one does not: dq's error was 1.5 times that of its own rounding, now
 // it is that (for dk and dv, 1.4 times, tensor memory has no room left).  In fp16, whose range is small, P is kept
-// times 2^12 and dS times a power of two of its example (at_sigma); both are taken out of the fp32 sums.
+// times 2^12 and dS times a power of two of its example (at_sigma); both are taken out of the fp32 sums.  What vanishes
+// there is below 2^-37 as a weight, and below 2^-39 of the largest value that dS can have in its example.
 #pragma once
 
 #include "attention_tensor.cuh"
