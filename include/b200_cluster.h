@@ -476,7 +476,7 @@ typedef struct {
   int64_t m, n;
   int heads, groups, channels;     /* heads a multiple of groups; channels 1 .. 128 */
   int dims;                        /* 0 .. 8 */
-  float scale, cap;                /* finite; cap <= 0: none, else between 2^-100 of |scale| and 2^100 */
+  float scale, cap;                /* finite; cap <= 0: none, else at least 2^-126, and scale / cap in range */
   int dtype;
 } b200c_attention_t;
 /* out [m, heads, channels] contiguous; rest (may be NULL): the same shape and type, what rounding took from out, which

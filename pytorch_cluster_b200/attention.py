@@ -61,7 +61,7 @@ def attention(
         pos_q, pos_k, slope: coordinates ``[M, D]`` and ``[N, D]`` (D at most 8, taken as fp32) and ``[H]``
             slopes of the bias by distance; all three or none.  They are constants: no gradient reaches them.
         scale: of the dot products, a finite number, ``C ** -0.5`` by default.
-        cap: a positive number between ``2 ** -100`` of the scale's size and ``2 ** 100``, or None.
+        cap: a positive number, or None; scale, cap and their quotient are numbers of 32 bits.
         batch_size: the number of examples; skips its inference and the host reads that takes (needed under stream
             capture).  Rows with ids at or above it belong to no example: zeros, without a gradient.
 

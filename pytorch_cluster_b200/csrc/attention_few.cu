@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_kernel(AttnArgs a, i
   const T *v = (const T *)p.v + group * p.v_head + part * VL;
   const int left = p.channels - part * VL;
   const bool bend = p.cap > 0.f;
-  const float pre = bend ? p.scale / p.cap : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E;
+  const float pre = bend ? p.scale : p.scale * AT_LOG2E, post = p.cap * AT_LOG2E, inv_cap = bend ? 1.f / p.cap : 0.f;
 
   for (int64_t r0 = 0; r0 < rows; r0 += QB) {
     float q[QB][VL], pos[QB][AT_MAX_DIMS], slope[QB], top[QB], sum[QB], o[QB][VL];
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(AF_THREADS) attention_few_kernel(AttnArgs a, i
           for (int c = 0; c < VL; ++c) t = fmaf(q[i][c], f[c], t);
 #pragma unroll
           for (int w = LPK / 2; w > 0; w >>= 1) t += __shfl_xor_sync(FULL_MASK, t, w);
-          if (bend) t = post * tanhf(t);
+          if (bend) t = post * tanhf(t * inv_cap);
           if (p.dims > 0) t = fmaf(-slope[i], sqrtf(dist[i]), t);
           s[u][i] = j < hi ? t : -pos_inf<float>();
         }

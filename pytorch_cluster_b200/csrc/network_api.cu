@@ -1,4 +1,5 @@
 // extern "C" entry points of gather_rows, norm_rotate and attention: argument checks and kernel selection.
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -17,9 +18,9 @@ static size_t elem_bytes(int dtype) { return dtype == B200C_F32 ? 4 : 2; }
 constexpr int64_t MOST_ROWS = 0x7fffffffLL;
 constexpr int64_t MOST_GATHER_CHANNELS = 65536;
 constexpr int64_t MOST_SEGMENTS = 1ll << 30;  // segments are bisected with 32-bit numbers
-// Scores are divided by the cap and multiplied by it again.  Far beyond them a quotient would leave the normal numbers of
-// fp32 (a cap that large bends nothing), far below them the scaled queries would.
-constexpr float MOST_CAP = 1.2676506e30f;  // 2^100
+// Scores are divided by a cap and multiplied by it again.  Above 2^100 it bends no score below 2^88, and those quotients
+// would leave the normal numbers of fp32: such a cap is none.
+constexpr float MOST_CAP = 1.2676506e30f;
 
 static std::atomic<int32_t *> attention_report{nullptr};
 
@@ -98,12 +99,18 @@ static int check_attention(const b200c_attention_t *a) {
   B200C_CHECK_ARG(a->n == 0 || (a->k && a->v), "null pointer");
   B200C_CHECK_ARG(a->dims == 0 || (a->slope && (a->m == 0 || a->pos_q) && (a->n == 0 || a->pos_k)), "null pointer");
   B200C_CHECK_ARG(isfinite(a->scale) && isfinite(a->cap), "scale and cap must be finite numbers");
-  B200C_CHECK_ARG(!(a->cap > 0.f) || (a->cap <= MOST_CAP && fabsf(a->scale) <= MOST_CAP * a->cap),
-                  "cap must lie between 2^-100 of scale and 2^100");
+  B200C_CHECK_ARG(!(a->cap > 0.f) || (a->cap >= FLT_MIN && isfinite(2.f * AT_LOG2E * fabsf(a->scale) / a->cap)),
+                  "cap must be at least 2^-126, and scale / cap a number of 32 bits");
   B200C_CHECK_ARG(aligned_to(elem_bytes(a->dtype), {a->q, a->k, a->v}) && aligned_to(8, {a->ptr_q, a->ptr_k}) &&
                       (a->dims == 0 || aligned_to(4, {a->pos_q, a->pos_k, a->slope})),
                   "misaligned pointer");
   return B200C_OK;
+}
+
+static b200c_attention_t without_idle_cap(const b200c_attention_t &a) {
+  b200c_attention_t p = a;
+  if (p.cap > MOST_CAP) p.cap = 0.f;
+  return p;
 }
 
 }  // namespace b200c
@@ -184,17 +191,19 @@ static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 extern "C" size_t b200c_attention_workspace_bytes(const b200c_attention_t *a) {
   if (check_attention(a) != B200C_OK) return 0;
-  const size_t few = attention_few_workspace_bytes(*a);
+  const b200c_attention_t p = without_idle_cap(*a);
+  const size_t few = attention_few_workspace_bytes(p);
   if (few > 0) return few;
-  const int splits = attention_tensor_splits(*a);
-  if (splits > 1) return (size_t)a->m * a->heads * splits * (a->channels + 2) * 4;
-  return attention_tensor_order_bytes(*a);
+  const int splits = attention_tensor_splits(p);
+  if (splits > 1) return (size_t)p.m * p.heads * splits * (p.channels + 2) * 4;
+  return attention_tensor_order_bytes(p);
 }
 
-extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, void *rest, float *lse, void *workspace,
+extern "C" int b200c_attention_forward(const b200c_attention_t *args, void *out, void *rest, float *lse, void *workspace,
                                        size_t workspace_bytes, b200c_stream_t stream) {
-  int st = check_attention(p);
+  int st = check_attention(args);
   if (st != B200C_OK) return st;
+  const b200c_attention_t effective = without_idle_cap(*args), *p = &effective;
   B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
   B200C_CHECK_ARG(aligned_to(elem_bytes(p->dtype), {out, rest}) && aligned_to(4, {lse}), "misaligned pointer");
   if ((st = check_device()) != B200C_OK || p->m == 0) return st;
@@ -228,14 +237,16 @@ extern "C" int b200c_attention_forward(const b200c_attention_t *p, void *out, vo
 extern "C" size_t b200c_attention_backward_workspace_bytes(const b200c_attention_t *a) {
   if (check_attention(a) != B200C_OK) return 0;
   // D, the largest norms, order; never 0
-  return align256((size_t)a->m * a->heads * 4) + align256(attention_norms_bytes(*a) + 1) + attention_tensor_order_bytes(*a);
+  return align256((size_t)a->m * a->heads * 4) + align256(attention_norms_bytes(*a) + 1) +
+         attention_tensor_order_bytes(without_idle_cap(*a));
 }
 
-extern "C" int b200c_attention_backward(const b200c_attention_t *p, const void *out, const void *rest, const float *lse,
-                                        const void *dout, void *dq, void *dk, void *dv, void *workspace,
+extern "C" int b200c_attention_backward(const b200c_attention_t *args, const void *out, const void *rest,
+                                        const float *lse, const void *dout, void *dq, void *dk, void *dv, void *workspace,
                                         size_t workspace_bytes, b200c_stream_t stream) {
-  int st = check_attention(p);
+  int st = check_attention(args);
   if (st != B200C_OK) return st;
+  const b200c_attention_t effective = without_idle_cap(*args), *p = &effective;
   B200C_CHECK_ARG(aligned_workspace(workspace), "misaligned workspace");
   B200C_CHECK_ARG(aligned_to(elem_bytes(p->dtype), {out, rest, dout, dq, dk, dv}) && aligned_to(4, {lse}),
                   "misaligned pointer");

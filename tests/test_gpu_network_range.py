@@ -175,17 +175,28 @@ def test_caps_and_scales_beyond_32_bits_are_refused(dtype):
     import pytorch_cluster_b200 as pc
 
     h = rand(gen(56), 70, 2, 16, dtype=dtype)
-    for extra in (dict(cap=1e39), dict(cap=1e-50), dict(cap=1e-31, scale=1.0), dict(cap=1e31), dict(scale=math.inf), dict(scale=1e39),
-                  dict(scale=math.nan)):
+    for extra in (dict(cap=1e39), dict(cap=1e-50), dict(cap=1e-39, scale=1.0), dict(cap=1.2e-38, scale=2.0),
+                  dict(scale=math.inf), dict(scale=1e39), dict(scale=math.nan)):
         with pytest.raises((RuntimeError, ValueError), match="cap|scale"):
             pc.attention(h, h, h, **extra)
-    for cap in (math.inf, math.nan, 1e-50, 1e39, 1e31):
+    for cap in (math.inf, math.nan, 1e-50, 1e39):
         with pytest.raises(RuntimeError, match="cap"):
             torch.ops.torch_cluster.attention(h, h, h, None, None, None, None, None, 1.0, cap)
-    # the largest and smallest that pass
-    for cap in (1e30, 1e-29):
-        got = pc.attention(h, h, h, cap=cap)
-        assert_close(got, *attention_plain(h, h, h, [70], [70], cap=cap)["out"], cap)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries, channels", [(70, 16), (300, 64), (70, 7), (1, 40), (1, 7)])
+def test_the_largest_and_smallest_caps(dtype, queries, channels):
+    g = gen(56)
+    ts = [rand(g, n, 2, channels, dtype=dtype) for n in (queries, 300, 300)]
+    ts[1][::3, :, ::2] = 0  # products that vanish
+    ts[1][::9] = 0
+    do = rand(g, queries, 2, channels, dtype=dtype)
+    for cap in (3e38, 1e35, 1e30, 1e25, 1e-29, 1e-37):
+        want = attention_plain(*ts, [queries], [300], cap=cap, scale=0.25, dout=do)
+        got = gradients(ts, do, cap=cap, scale=0.25)
+        for name, t in zip(("out", "dq", "dk", "dv"), got):
+            assert_close(t, *want[name], (cap, name))
 
 
 # ---- waits that run out ----------------------------------------------------------------------------------------

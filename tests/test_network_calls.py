@@ -34,7 +34,7 @@ def test_forward_mode_derivatives_are_refused():
 @pytest.mark.parametrize("changes, message", [
     (dict(cap=math.inf), b"finite"), (dict(cap=-math.inf), b"finite"), (dict(cap=math.nan), b"finite"),
     (dict(scale=math.inf), b"finite"), (dict(scale=-math.inf), b"finite"),
-    (dict(cap=1e31), b"cap"), (dict(cap=1e-31), b"cap"), (dict(cap=1e-31, scale=-1.0), b"cap"),
+    (dict(cap=1e-39), b"cap"), (dict(cap=1e-38, scale=-1.2), b"cap"), (dict(cap=1e-20, scale=1e20), b"cap"),
 ])
 def test_attention_caps_and_scales_that_are_refused(changes, message):
     from pytorch_cluster_b200 import _native
